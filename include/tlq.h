@@ -377,6 +377,46 @@ int tlq_quantize_sym4(const void* W, void* q_minus8, void* scales, int64_t N, in
  * Its outputs are the A / scale_a operands of tlq_gemm_w8a8. */
 int tlq_act_quant_i8(const void* X, void* Y, void* S, int64_t M, int64_t N, int in_dtype, int round_scale, void* stream);
 
+/* A mixture-of-experts layer on packed 4-bit weights: the router's choice, the experts' first product with its gated activation,
+ * the experts' second product with the weighted sum over a token's experts.  No counterpart in the reference, whose quantised
+ * products are dense (examples/dequantize_gemm); weights, scales and zero points are those of tlq_gemm_w4a16, one matrix per
+ * expert, back to back.
+ *
+ * tlq_moe_route: for each of M tokens the top_k of E experts, and their weights.
+ *   p = softmax(logits) (TLQ_MOE_SOFTMAX) or 1 / (1 + exp(-logits)) (TLQ_MOE_SIGMOID);  v = p + bias, p without a bias
+ *   n_group > 1: the E experts are n_group runs of E / n_group; a run's value is the sum of its two largest v, and only the
+ *   experts of the topk_group best runs may be chosen
+ *   ids = the top_k experts with the largest v, largest first;  weights = p[ids], divided by their sum with renormalize, times scaling
+ * Scores and what is compared are binary64, equal values go to the lowest index.  A logit or biased score of -infinity or NaN
+ * masks its expert (p = 0); where fewer than top_k experts are left, the remaining ids are -1 with weight 0.  Logits of
+ * +infinity share the softmax among them.  Where the chosen scores add up to 0 the renormalised weights are 0.
+ * logits [M, E] in_dtype (TLQ_F16, TLQ_BF16, TLQ_F32), bias fp32 [E] or NULL, weights fp32 [M, top_k], ids int32 [M, top_k].
+ * E <= 1024, top_k <= 64, n_group <= 64. */
+enum { TLQ_MOE_SOFTMAX = 0, TLQ_MOE_SIGMOID = 1 };
+int tlq_moe_route(const void* logits, const void* bias, void* weights, void* ids, int64_t M, int64_t E, int64_t top_k,
+                  int64_t n_group, int64_t topk_group, int scoring, int renormalize, float scaling, int in_dtype, void* stream);
+
+/* The experts' products.  ids int32 [M, top_k], as tlq_moe_route gives them; a value outside 0 .. E - 1 is a slot without an expert
+ * here (it is another GPU's, or empty); the same expert twice for a token is two slots like any others.
+ * tlq_moe_gate_up_w4a16:  H[t, j, n] = rn_T(silu(g) * u),  g = X[t] . W[e, n],  u = X[t] . W[e, N + n],  e = ids[t, j];
+ *   silu(g) = g / (1 + exp(-g)), g and u fp32;  0 for a slot without an expert.
+ *   X [M, K] dtype, w_packed [E, 2 N, K / 2], scales / zeros [E, 2 N, K / group], H [M, top_k, N] dtype.
+ * tlq_moe_down_w4a16:  Y[t, n] = rn_out( sum_j weights[t, j] * (H[t, j] . W[e, n]) ), fp32 sums; slots without an expert add nothing.
+ *   H [M, top_k, K] in_dtype, weights fp32 [M, top_k], w_packed [E, N, K / 2], scales / zeros [E, N, K / group], Y [M, N] out_dtype.
+ * W = rn_T(rn_T(T(u) - z) * s) as in tlq_dequant_w4 (scales NULL: 1; zeros NULL: zero_scalar); T = dtype: TLQ_F16 or TLQ_BF16.
+ * N % 16 == 0, K % 32 == 0, group a multiple of 32 that divides K, E <= 1024, top_k <= 64, M * top_k < 2^24.  X, H, Y and w_packed
+ * 16-byte aligned.  Results do not depend on timing: no floating-point sum is formed by atomic adds.
+ * The workspace (16-byte aligned, at least tlq_moe_*_workspace_bytes) holds nothing between calls; two calls that may run at the
+ * same time need one each. */
+int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k);
+int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N);
+int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void* w_packed, const void* scales, const void* zeros, void* H,
+                          void* workspace, int64_t workspace_bytes, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K,
+                          int64_t group, float zero_scalar, int dtype, void* stream);
+int tlq_moe_down_w4a16(const void* H, const void* ids, const void* weights, const void* w_packed, const void* scales,
+                       const void* zeros, void* Y, void* workspace, int64_t workspace_bytes, int64_t M, int64_t E, int64_t top_k,
+                       int64_t N, int64_t K, int64_t group, float zero_scalar, int in_dtype, int out_dtype, void* stream);
+
 /* The host-side self-checks of the kernels' address arithmetic (tlq_debug_*) and the tuning hooks that benchmark sweeps and
  * the autotuner use (tlq_tune_*) are exported by the same library and declared in tlq_debug.h: they are not part of the
  * operator boundary above. */

@@ -554,3 +554,88 @@ def quantize_sym4(W: torch.Tensor, group: int):
     quot = torch.where(torch.isnan(quot), torch.full_like(quot, -1e9), quot)
     q = torch.clamp(quot.to(torch.int64) + 8, 0, 16)
     return (q - 8).to(torch.int8).reshape(N, K), s.reshape(N, K // group).contiguous()
+
+
+# ------------------------------------------------------------------------------------------
+# mixture-of-experts layer (no counterpart in the reference: the definitions of include/tlq.h, in 64 bits)
+# ------------------------------------------------------------------------------------------
+def moe_route(logits, top_k, scoring="softmax", bias=None, n_group=1, topk_group=1, renormalize=True, scaling=1.0):
+    """-> (weights float64 [M, top_k], ids int64 [M, top_k]), one token and one expert at a time."""
+    x = logits.cpu().to(torch.float64).numpy()
+    M, E = x.shape
+    b = np.zeros(E) if bias is None else bias.cpu().to(torch.float64).numpy()
+    weights, ids = np.zeros((M, top_k)), np.full((M, top_k), -1, np.int64)
+    size = E // n_group
+    for m in range(M):
+        there = [e for e in range(E) if x[m, e] > -np.inf]  # (not a NaN either)
+        p = np.zeros(E)
+        if scoring == "sigmoid":
+            for e in there:
+                p[e] = 1 / (1 + np.exp(-x[m, e]))
+        elif there:
+            top = max(x[m, e] for e in there)
+            for e in there:
+                p[e] = 1.0 if x[m, e] == top else np.exp(x[m, e] - top)
+            p /= p.sum()
+        v = p + b
+        there = [e for e in there if v[e] > -np.inf]
+        if n_group > 1:
+            value = []
+            for g in range(n_group):
+                best = sorted((v[e] for e in there if e // size == g), reverse=True)[:2]
+                value.append(sum(best) if best else -np.inf)
+            kept = sorted(range(n_group), key=lambda g: (-value[g], g))[:topk_group]
+            there = [e for e in there if e // size in kept]
+        chosen = sorted(there, key=lambda e: (-v[e], e))[:top_k]
+        w = np.array([p[e] for e in chosen])
+        if renormalize and len(chosen):
+            w = w / w.sum() if w.sum() > 0 else w * 0
+        weights[m, : len(chosen)], ids[m, : len(chosen)] = w * scaling, chosen
+    return torch.from_numpy(weights), torch.from_numpy(ids)
+
+
+def _moe_products(rows, ids, B_packed, scales, zeros, group, dtype):
+    """(dots, sums of magnitudes) [M, top_k, N] float64: rows(t, j) times the matrix of expert ids[t, j]; 0 without one."""
+    E, N = B_packed.shape[:2]
+    M, k = ids.shape
+    dots, mags = torch.zeros(M, k, N, dtype=torch.float64), torch.zeros(M, k, N, dtype=torch.float64)
+    matrix = {}
+    for t in range(M):
+        for j in range(k):
+            e = int(ids[t, j])
+            if not 0 <= e < E:
+                continue
+            if e not in matrix:
+                z = zeros[e] if isinstance(zeros, torch.Tensor) else zeros
+                matrix[e] = dequant_w4(B_packed[e].cpu(), None if scales is None else scales[e], z, group, dtype).to(torch.float64)
+            x = rows(t, j).to(torch.float64)
+            dots[t, j] = matrix[e] @ x
+            mags[t, j] = matrix[e].abs() @ x.abs()
+    return dots, mags
+
+
+def moe_gate_up(X, ids, B_packed, scales=None, zeros=None, group=128):
+    """-> (H, what H may be off by before its rounding) float64 [M, top_k, N].
+
+    fp32 sums of K exact products: each is at most (K + 8) 2^-24 of the sum of magnitudes off (K additions, and a few for the
+    order inside a matrix instruction).  silu has slope at most 1.1; its exponential is computed in fp32 as 2^(-g log2 e):
+    (|g| + 4) 2^-22 of the value."""
+    X = X.cpu()
+    K = X.shape[1]
+    dots, mags = _moe_products(lambda t, j: X[t], ids.cpu(), B_packed, scales, zeros, group, X.dtype)
+    g, u = dots.chunk(2, 2)
+    dg, du = (mags * (K + 8) * 2.0**-24).chunk(2, 2)
+    act = g / (1 + torch.exp(-g))
+    h = act * u
+    return h, 1.1 * dg * (u.abs() + du) + act.abs() * du + (g.abs() + 4) * 2.0**-22 * h.abs()
+
+
+def moe_down(H, ids, weights, B_packed, scales=None, zeros=None, group=128):
+    """-> (Y, what Y may be off by before its rounding) float64 [M, N]: the sums as above, then one product and one addition per
+    slot."""
+    H, w = H.cpu(), weights.cpu().to(torch.float64)
+    k, K = H.shape[1:]
+    dots, mags = _moe_products(lambda t, j: H[t, j], ids.cpu(), B_packed, scales, zeros, group, H.dtype)
+    y = (dots * w[:, :, None]).sum(1)
+    off = mags * (K + 8) * 2.0**-24
+    return y, (w.abs()[:, :, None] * (off + (dots.abs() + off) * (k + 2) * 2.0**-24)).sum(1)

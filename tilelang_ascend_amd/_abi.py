@@ -19,6 +19,7 @@ F16, BF16, F32, I8, I32 = 0, 1, 2, 3, 4
 U4, S4_TWOS, S4_OFFSET8, S4_OFFSET7 = 0, 1, 2, 3
 B_KN, B_NK = 0, 1
 W_PLAIN, W_INTERLEAVED_F16 = 0, 1
+MOE_SOFTMAX, MOE_SIGMOID = 0, 1
 ALGO_AUTO, ALGO_GEMV, ALGO_MFMA, ALGO_SKINNY, ALGO_TWO_PASS, ALGO_STREAM, ALGO_DECODE, ALGO_PANEL, ALGO_PANEL256, ALGO_PANELM, ALGO_SMALL = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 11
 ABI_VERSION = 1
 
@@ -62,6 +63,11 @@ SIGNATURES = {
     "tlq_pack_int4": (_int, [_vp, _vp, _i64, _i64, _int, _vp]),
     "tlq_quantize_sym4": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
     "tlq_act_quant_i8": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "tlq_moe_route": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _int, _f32, _int, _vp]),
+    "tlq_moe_gate_up_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "tlq_moe_down_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "tlq_moe_gate_up_w4a16": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _vp]),
+    "tlq_moe_down_w4a16": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _vp]),
     "tlq_debug_check_gemm_addressing": (_int, [_int, _i64, _i64, _int, _int]),
     "tlq_debug_check_slots_schedule": (_int, [_int, _int]),
     "tlq_debug_check_ring_schedule": (_int, [_int, _int, _int]),

@@ -57,6 +57,8 @@ SOURCES = [
     "gemm_api.hip",
     "gemm_addr_check.hip",
     "gemm_w4a16_noalloc.hip",
+    "moe_route.hip",
+    "moe_w4a16.hip",
 ]
 # packed-fp32 VALU forms are disabled on purpose (some have produced silent wrong results on
 # this hardware pool); hipcc's host pass warns that it does not know the feature.

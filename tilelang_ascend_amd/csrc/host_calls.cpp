@@ -35,7 +35,8 @@ namespace {
   X(tlq_last_error) X(tlq_gemm_w4a16_layout_ws) X(tlq_w4a16_workspace_bytes_for) X(tlq_gemm_w8a8_ws) X(tlq_w8a8_workspace_bytes) \
   X(tlq_act_quant_i8) X(tlq_gemm_w4a8_ws) X(tlq_gemm_w4a8) X(tlq_gemm_i8) X(tlq_gemm_f16_ws) X(tlq_f16_workspace_bytes)          \
   X(tlq_gemm_f16_batched) X(tlq_gemv) X(tlq_gemm_f16_splitk) X(tlq_dequant_w4_layout) X(tlq_unpack_int4) X(tlq_pack_int4)        \
-  X(tlq_quantize_sym4)
+  X(tlq_quantize_sym4) X(tlq_moe_route) X(tlq_moe_gate_up_workspace_bytes) X(tlq_moe_down_workspace_bytes) X(tlq_moe_gate_up_w4a16)  \
+  X(tlq_moe_down_w4a16)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   TLQ_ENTRIES(X)
@@ -43,7 +44,7 @@ struct Entries {
 };
 Entries lib;
 
-enum Kind { kW4A16, kW8A8, kActQuant, kW4A8Ws, kW4A8, kI8, kF16, kF16Batched, kGemv, kSplitK };
+enum Kind { kW4A16, kW8A8, kActQuant, kW4A8Ws, kW4A8, kI8, kF16, kF16Batched, kGemv, kSplitK, kMoeRoute, kMoeGateUp, kMoeDown };
 struct KindName {
   const char* name;
   Kind kind;
@@ -51,7 +52,8 @@ struct KindName {
 };
 const KindName kKinds[] = {{"w4a16", kW4A16, 10, 3}, {"w8a8", kW8A8, 8, 4},  {"act_quant", kActQuant, 3, 3}, {"w4a8_ws", kW4A8Ws, 4, 4},
                            {"w4a8", kW4A8, 4, 3},    {"i8", kI8, 3, 3},      {"f16", kF16, 3, 3},            {"f16_batched", kF16Batched, 5, 3},
-                           {"gemv", kGemv, 3, 3},    {"splitk", kSplitK, 5, 3}};
+                           {"gemv", kGemv, 3, 3},    {"splitk", kSplitK, 5, 3},
+                           {"moe_route", kMoeRoute, 8, 3}, {"moe_gate_up", kMoeGateUp, 8, 4}, {"moe_down", kMoeDown, 9, 5}};
 
 const int kMaxDims = 4, kMaxParams = 8, kMaxSymbols = 4;
 enum Role { kInput, kOutput, kWorkspace };
@@ -118,6 +120,10 @@ int launch(const PlanObject& p, const at::Tensor* const* t, int device, hipStrea
     ws_bytes = lib.tlq_w8a8_workspace_bytes(v[0], v[1] < 0 ? t[0]->size(0) : v[1], v[2], v[3]);
   } else if (p.kind == kF16) {
     ws_bytes = lib.tlq_f16_workspace_bytes(1, v[0], v[1], v[2]);
+  } else if (p.kind == kMoeGateUp) {
+    ws_bytes = lib.tlq_moe_gate_up_workspace_bytes(t[0]->size(0), v[0], v[1]);
+  } else if (p.kind == kMoeDown) {
+    ws_bytes = lib.tlq_moe_down_workspace_bytes(t[0]->size(0), v[0], v[1], v[2]);
   }
   c10::DataPtr ws;  // the allocator's block alone: no tensor around it
   if (ws_bytes > 0) {
@@ -147,6 +153,27 @@ int launch(const PlanObject& p, const at::Tensor* const* t, int device, hipStrea
     case kF16: return lib.tlq_gemm_f16_ws(ptr(t[0]), ptr(t[1]), ptr(t[2]), w, ws_bytes, 1, v[0], v[1], v[2], TLQ_F16, TLQ_F16, TLQ_B_KN, stream);
     case kF16Batched: return lib.tlq_gemm_f16_batched(ptr(t[0]), ptr(t[1]), ptr(t[2]), v[0], v[1], v[2], v[3], (int)v[4], (int)v[4], TLQ_B_KN, stream);
     case kGemv: return lib.tlq_gemv(ptr(t[0]), ptr(t[1]), ptr(t[2]), v[0], v[1], (int)v[2], (int)v[2], stream);
+    // v: E, top_k, n_group, topk_group, scoring, renormalize, input type, with a bias; p.zero: the scaling
+    case kMoeRoute: {
+      const int i = v[7] ? 2 : 1;
+      return lib.tlq_moe_route(ptr(t[0]), v[7] ? ptr(t[1]) : nullptr, ptr(t[i]), ptr(t[i + 1]), t[0]->size(0), v[0], v[1], v[2], v[3], (int)v[4],
+                               (int)v[5], p.zero, (int)v[6], stream);
+    }
+    // v: E, top_k, N, K, group, type, with scales, with zeros (, output type)
+    case kMoeGateUp: {
+      int i = 3;
+      const at::Tensor* s = v[6] ? t[i++] : nullptr;
+      const at::Tensor* z = v[7] ? t[i++] : nullptr;
+      return lib.tlq_moe_gate_up_w4a16(ptr(t[0]), ptr(t[1]), ptr(t[2]), ptr(s), ptr(z), ptr(t[i]), w, ws_bytes, t[0]->size(0), v[0], v[1], v[2], v[3],
+                                       v[4], p.zero, (int)v[5], stream);
+    }
+    case kMoeDown: {
+      int i = 4;
+      const at::Tensor* s = v[6] ? t[i++] : nullptr;
+      const at::Tensor* z = v[7] ? t[i++] : nullptr;
+      return lib.tlq_moe_down_w4a16(ptr(t[0]), ptr(t[1]), ptr(t[2]), ptr(t[3]), ptr(s), ptr(z), ptr(t[i]), w, ws_bytes, t[0]->size(0), v[0], v[1], v[2],
+                                    v[3], v[4], p.zero, (int)v[5], (int)v[8], stream);
+    }
     case kSplitK: return lib.tlq_gemm_f16_splitk(ptr(t[0]), ptr(t[1]), ptr(t[2]), v[0], v[1], v[2], v[3], (int)v[4], TLQ_B_KN, stream);
   }
   return 1;
@@ -298,7 +325,8 @@ PyObject* plan_new(PyTypeObject* type, PyObject* args, PyObject*) {
   const Py_ssize_t n = PyTuple_GET_SIZE(params);
   int least = kn->tensors;
   if (kn->kind == kW4A16) least += (p->v[8] != 0) + (p->v[9] != 0);
-  if (kn->kind == kW8A8) least += p->v[7] != 0;
+  if (kn->kind == kW8A8 || kn->kind == kMoeRoute) least += p->v[7] != 0;
+  if (kn->kind == kMoeGateUp || kn->kind == kMoeDown) least += (p->v[6] != 0) + (p->v[7] != 0);
   if (n > kMaxParams || n < least) return bad("wrong number of parameters");
   p->n_params = (int)n;
   std::vector<std::string> names;
