@@ -435,7 +435,7 @@ def test_products_refuse():
         _rejected(f(ws=ODD), "workspace")
         assert f(M=0) == 0
     _rejected(up(n=lib.tlq_moe_gate_up_workspace_bytes(4, 8, 2) - 1), "workspace")
-    _rejected(down(n=lib.tlq_moe_down_workspace_bytes(4, 8, 2, 64) - 1), "workspace")
+    _rejected(down(n=lib.tlq_moe_down_workspace_bytes(4, 8, 2, 64, 128) - 1), "workspace")
     _rejected(down(weights=NULL), "null pointer")
     _rejected(down(weights=ODD), "aligned")
     _rejected(down(out=_abi.I32), "out_dtype")
@@ -444,10 +444,10 @@ def test_products_refuse():
 def test_workspace_sizes():
     lib = _abi.load()
     up, down = lib.tlq_moe_gate_up_workspace_bytes, lib.tlq_moe_down_workspace_bytes
-    assert up(0, 8, 2) == up(4, 0, 2) == up(4, 8, 0) == up(4, 2000, 2) == down(0, 8, 2, 64) == down(4, 8, 2, 0) == 0
+    assert up(0, 8, 2) == up(4, 0, 2) == up(4, 8, 0) == up(4, 2000, 2) == down(0, 8, 2, 64, 64) == down(4, 8, 2, 0, 64) == down(4, 8, 2, 64, 0) == 0
     for M in (1, 3, 64, 1000, 100000):
         assert 0 < up(M, 8, 2) and up(M, 8, 2) <= up(M + 1, 8, 2) and up(M, 8, 2) % 16 == 0
-        assert down(M, 8, 2, 64) >= up(M, 8, 2)
+        assert down(M, 8, 2, 64, 64) >= up(M, 8, 2)
 
 
 @pytest.mark.parametrize("kwargs,message", [

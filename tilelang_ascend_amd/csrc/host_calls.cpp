@@ -123,7 +123,7 @@ int launch(const PlanObject& p, const at::Tensor* const* t, int device, hipStrea
   } else if (p.kind == kMoeGateUp) {
     ws_bytes = lib.tlq_moe_gate_up_workspace_bytes(t[0]->size(0), v[0], v[1]);
   } else if (p.kind == kMoeDown) {
-    ws_bytes = lib.tlq_moe_down_workspace_bytes(t[0]->size(0), v[0], v[1], v[2]);
+    ws_bytes = lib.tlq_moe_down_workspace_bytes(t[0]->size(0), v[0], v[1], v[2], v[3]);
   }
   c10::DataPtr ws;  // the allocator's block alone: no tensor around it
   if (ws_bytes > 0) {

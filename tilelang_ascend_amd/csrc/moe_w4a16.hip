@@ -223,18 +223,19 @@ __global__ __launch_bounds__(256) void moe_w4a16_kernel(const ExpertArgs a) {
   }
 }
 
-// ---- few pairs: weights resident in registers -----------------------------------------------------------------------------
-// A wavefront asks for all its packed weights at once -- 16 weight rows x up to BPW blocks of 128 values of K, 1 KB a block -- and
-// keeps them while it multiplies them with the expert's pairs, `row_cap` of them a pass.  Every weight is read once whatever the
-// number of pairs, a CU has some 64 - 128 KB in flight, and no launch sorts the pairs first: a work-group looks its expert's pairs
-// up among all ids (at most kFewPairs).  The work-groups of an expert are those of the first pair that names it, or, where there
-// are more pairs than experts, those of the expert's number; one token's pairs are taken one by one.
-//   A tile is 16 weight rows: 16 outputs, or 8 gate rows and the 8 up rows that go with them.  A work-group has `tiles` of them side by
-// side, each shared by `splits` wavefronts that take a part of K each; their sums meet in LDS and are added in the order of K.
-//   Activations (a pass's rows, whole), scales and zero points of the tiles go global -> LDS ahead of the weights and are waited
-// for by count, with the weights still on their way.
+// ---- few pairs: every weight read once ---------------------------------------------------------------------------------------
+// For calls that are bound by reading the weights.  A work-group stages up to `row_cap` of its expert's activation rows in LDS, whole, with
+// the scales and zero points of its tiles, once; then every wavefront streams the packed weights of its own tiles through its registers,
+// with no barrier: the next kFewGroup blocks (1 KB each) are on their way while the last ones are expanded and multiplied with all rows.
+// No launch sorts the pairs first: a work-group looks its expert's pairs up among all ids (at most kFewPairs).  The work-groups of
+// an expert are those of the first pair that names it, or, where there are more pairs than experts, those of the expert's number; one
+// token's pairs are taken one by one.
+//   A tile is 16 weight rows: 16 outputs, or 8 gate rows and the 8 up rows that go with them.  A block is 128 values of K of a tile.
+// Where tiles are few, `splits` wavefronts share one, each with a part of K; their sums meet in LDS and are added in the order of K.
+// Long rows of the down product are cut into `chunks` work-groups too, whose sums moe_combine_kernel adds.
 constexpr int kFewPairs = 2048;
-enum { kFewByPair = 1, kFewOneToken = 2, kFewFold = 4 };
+constexpr int kFewGroup = 4;
+enum { kFewByPair = 1, kFewOneToken = 2, kFewFold = 4, kFewWide = 8 };
 
 struct FewArgs {
   const void* X;
@@ -245,10 +246,12 @@ struct FewArgs {
   const int32_t* ids;
   void* out;
   int pairs, E, top_k, N, K, groups;
-  uint32_t per_group;  // ceil(2^32 / (group / 32)), 0 for groups of 32
+  uint32_t per_group;    // ceil(2^32 / (group / 32)), 0 for groups of 32
   float zero_scalar;
-  int n_groups;                            // work-groups of an expert
-  uint32_t shape;                          // tiles | splits << 8 | row_cap << 16 | flags << 24 (kFewFold: the scalar zero point is a small integer)
+  int n_groups, units;   // work-groups of an expert side by side, and of all experts
+  uint32_t blocks;       // blocks of 128 values of K of a work-group | 16-byte pieces of a row's scales << 16
+  uint32_t shape;        // wavefronts | splits << 8 | row_cap << 16 | flags << 24 (kFewFold: the scalar zero point is a small integer)
+  int per_wave;          // tiles of a wavefront
 };
 
 __device__ __forceinline__ bool small_integer(float z) { return z == __builtin_rintf(z) && z >= -256.0f && z <= 256.0f; }
@@ -257,34 +260,65 @@ __device__ __forceinline__ bool small_integer(float z) { return z == __builtin_r
 __device__ __forceinline__ void direct16(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
-template <typename T, bool UP, int BPW>
-__global__ __launch_bounds__(512, 2) void moe_few_kernel(const FewArgs a) {
+__device__ __forceinline__ void direct4(const void* src, uint32_t lds) {  // 4 bytes per lane, lane l to lds + 4 l
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory");
+}
+
+// Four neighbouring sums of one pair: gate / up: outputs n .. n + 3 from the gates in q = 0, 1 and their ups 32 lanes on; down: the weighted row.
+template <typename T, bool UP, typename Args>
+__device__ __forceinline__ void moe_store(const Args& a, const float4_t& sum, bool live, int pair, float weight, int n, int q, int chunk) {
+  if constexpr (UP) {
+    float4_t up;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) up[i] = __shfl_xor(sum[i], 32);
+    if (q < 2 && live) {
+      T o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = from_float<T>(silu(sum[i]) * up[i]);
+      *(uint2_t*)((T*)a.out + (int64_t)pair * a.N + n) = bitcast<uint2_t>(o);
+    }
+  } else if (live) {
+    *(float4_t*)((float*)a.out + ((int64_t)chunk * a.pairs + pair) * a.N + n) = sum * weight;
+  }
+}
+
+template <typename T, bool UP, bool ZEROS>
+__global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
   typedef typename MmaOf<T>::type Mma;
   typedef __attribute__((address_space(3))) uint8_t* lptr_t;
   extern __shared__ __align__(16) uint8_t smem[];
-  const int tiles = a.shape & 255, splits = (a.shape >> 8) & 255, row_cap = (a.shape >> 16) & 255, flags = a.shape >> 24;
-  const int waves = tiles * splits, threads = waves * 64;
+  const int waves = a.shape & 255, splits = (a.shape >> 8) & 255, row_cap = (a.shape >> 16) & 255, flags = a.shape >> 24;
+  const int wg_blocks = a.blocks & 0xffff, pieces = a.blocks >> 16, threads = waves * 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q = lane >> 4;
-  const int who = (int)(blockIdx.x / (uint32_t)a.n_groups), group_no = (int)blockIdx.x - who * a.n_groups;
+  // neighbouring numbers go to different XCDs: those eight apart are the parts of K of one unit, which share its scales
+  const int chunks = ((a.K + 127) / 128 + wg_blocks - 1) / wg_blocks;
+  int unit = blockIdx.x, chunk = 0;
+  if (chunks > 1) {
+    const int i = unit >> 3, per8 = i / chunks;
+    chunk = i - per8 * chunks;
+    unit = per8 * 8 + (unit & 7);
+    if (unit >= a.units) return;
+  }
+  const int who = unit / a.n_groups, group_no = unit - who * a.n_groups;
   const bool by_pair = flags & kFewByPair, one_token = flags & kFewOneToken;
-  const int blocks = (a.K + 127) >> 7, groups = a.groups;
-  const int pitch = blocks * 256 + 16;  // bytes of an activation row: 16 more, so that the rows of an operand lie on different banks
-  // LDS: activation rows, scales, zero points, sums of the other wavefronts, the pairs
+  const int k0 = chunk * wg_blocks * 128, k_len = a.K - k0 < wg_blocks * 128 ? a.K - k0 : wg_blocks * 128;  // this work-group's part of K
+  const int pitch = wg_blocks * 256 + 16;  // bytes of an activation row: 16 more, so that the rows of an operand lie on different banks
+  constexpr int OUTS = UP ? 8 : 16;        // outputs of a tile
+  const int wg_tiles = waves / splits * a.per_wave, n_tiles = a.N / OUTS, tile0 = group_no * wg_tiles;
+  // LDS: activation rows, sums of the other wavefronts, scales, zero points, the rows' weights, the pairs
+  const int sums_at = row_cap * pitch, sc_at = sums_at + waves / splits * (splits - 1) * 1024, zp_at = sc_at + wg_tiles * 256 * pieces;
   uint8_t* const act = smem;
-  const uint32_t act_lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)smem);
-  const int sc_at = row_cap * pitch, zp_at = sc_at + (a.scales ? tiles * 32 * groups : 0), sums_at = zp_at + (a.zeros ? tiles * 32 * groups : 0);
-  float* const sums = (float*)(smem + sums_at);
-  int32_t* const head = (int32_t*)(sums + tiles * (splits - 1) * 256);  // [0] number of pairs, [1] an earlier pair has this expert
+  const int weights_at = zp_at + (ZEROS ? wg_tiles * 256 * pieces : 0);
+  int32_t* const head = (int32_t*)(smem + weights_at + (UP ? 0 : 64));  // [0] number of pairs, [1] an earlier pair has this expert
   uint16_t* const list = (uint16_t*)(head + 4);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)smem);
 
   const int e = by_pair ? __builtin_amdgcn_readfirstlane(a.ids[who]) : who;
   const bool none = (uint32_t)e >= (uint32_t)a.E;
-  constexpr int OUTS = UP ? 8 : 16;  // outputs of a tile
-  const int n_tiles = a.N / OUTS, tile0 = group_no * tiles;
   if (none && (!UP || by_pair)) {
     if (!UP) return;
     T* const h = (T*)a.out + (int64_t)who * a.N;
-    const int end = (tile0 + tiles) * OUTS;
+    const int end = (tile0 + wg_tiles) * OUTS;
     for (int n = tile0 * OUTS + tid; n < end && n < a.N; n += threads) h[n] = from_float<T>(0.0f);
     return;
   }
@@ -309,7 +343,7 @@ __global__ __launch_bounds__(512, 2) void moe_few_kernel(const FewArgs a) {
   }
   if (UP && none) {
     T* const h = (T*)a.out;
-    const int width = tiles * OUTS;
+    const int width = wg_tiles * OUTS;
     for (int i = tid; i < count * width; i += threads) {
       const int n = tile0 * OUTS + i % width;
       if (n < a.N) h[(int64_t)list[i / width] * a.N + n] = from_float<T>(0.0f);
@@ -317,151 +351,177 @@ __global__ __launch_bounds__(512, 2) void moe_few_kernel(const FewArgs a) {
     return;
   }
 
-  // a pass's rows -> LDS; and zeros up to the end of the last block
-  auto load_rows = [&](int row0, int rows) __attribute__((always_inline)) {
-    for (int r = wave; r < rows; r += waves) {
-      const int pair = one_token ? who : __builtin_amdgcn_readfirstlane((int)list[row0 + r]);
-      const uint8_t* const x = (const uint8_t*)((const T*)a.X + (int64_t)(UP ? pair / a.top_k : pair) * a.K);
-      for (int at = 0; at < a.K * 2; at += 1024)
-        if (at + lane * 16 < a.K * 2) direct16(x + at + lane * 16, act_lds + r * pitch + at);
-      if (a.K * 2 + lane * 16 < blocks * 256) *(uint4_t*)(act + r * pitch + a.K * 2 + lane * 16) = uint4_t{0, 0, 0, 0};
-    }
-  };
-  // scales and zero points: half tiles of 8 rows, back to back in memory and in LDS (16 * groups bytes each)
-  const int chunks = tiles * 2 * groups;
-  auto group_values = [&](int c) -> int64_t {  // where the eight values of chunk c lie in their tensors
-    const int half = c / groups, at = c - half * groups;
-    int t = tile0 + (half >> 1);
+  // the row of W that row r of tile t is
+  auto weight_row = [&](int t, int r) __attribute__((always_inline)) -> int64_t {
     t = t < n_tiles ? t : n_tiles - 1;
-    const int64_t row = UP ? (int64_t)e * 2 * a.N + (half & 1) * a.N + t * 8 : (int64_t)e * a.N + t * 16 + (half & 1) * 8;
-    return row * groups + at * 8;
+    return UP ? (int64_t)e * 2 * a.N + (r >> 3) * a.N + t * 8 + (r & 7) : (int64_t)e * a.N + t * 16 + r;
   };
-  // (nothing is on its way here or behind the loop below; said so, because the compiler would wait once more, for the direct loads)
-  const auto nothing_on_its_way = []() __attribute__((always_inline)) { __builtin_amdgcn_s_waitcnt(0x0f70); };
-  nothing_on_its_way();
-  if ((((uintptr_t)a.scales | (uintptr_t)a.zeros) & 15) == 0) {
-    load_rows(0, count < row_cap ? count : row_cap);
-    for (int c0 = wave * 64; c0 < chunks; c0 += threads) {
-      if (c0 + lane >= chunks) continue;
-      const int64_t off = group_values(c0 + lane);
-      if (a.scales) direct16((const T*)a.scales + off, act_lds + sc_at + c0 * 16);
-      if (a.zeros) direct16((const T*)a.zeros + off, act_lds + zp_at + c0 * 16);
+  auto group_of = [&](int u) __attribute__((always_inline)) -> int {  // the group of the u-th 32 values of a row
+    return a.per_group ? (int)__umulhi((uint32_t)u, a.per_group) : u;
+  };
+  // a pass's rows -> LDS, 1 KB an instruction; and zeros up to the end of the last block
+  auto load_rows = [&](int row0, int rows) __attribute__((always_inline)) {
+    const int per_row = (k_len + 511) >> 9;
+    if (!UP && wave == 0 && lane < rows) direct4(a.weights + (one_token ? who : (int)list[row0 + lane]), lds0 + weights_at);
+    for (int i = wave; i < rows * per_row; i += waves) {
+      const int r = i / per_row, at = (i - r * per_row) * 1024;
+      const int pair = one_token ? who : __builtin_amdgcn_readfirstlane((int)list[row0 + r]);
+      const uint8_t* const x = (const uint8_t*)((const T*)a.X + (int64_t)(UP ? pair / a.top_k : pair) * a.K + k0);
+      if (at + lane * 16 < k_len * 2) direct16(x + at + lane * 16, lds0 + r * pitch + at);
+      else if (at + lane * 16 < ((k_len + 127) & ~127) * 2) *(uint4_t*)(act + r * pitch + at + lane * 16) = uint4_t{0, 0, 0, 0};
     }
-  } else {  // value by value; ahead of the rows, because loads into registers wait for everything before them
-    for (int i = tid; i < chunks * 8; i += threads) {
-      const int64_t off = group_values(i >> 3) + (i & 7);
-      if (a.scales) ((T*)(smem + sc_at))[i] = ((const T*)a.scales)[off];
-      if (a.zeros) ((T*)(smem + zp_at))[i] = ((const T*)a.zeros)[off];
-    }
-    nothing_on_its_way();
-    load_rows(0, count < row_cap ? count : row_cap);
-  }
-  // the weights: lane (r16, q) takes the 32 values 32 q .. of every block of row r16
-  const int my_tile = wave / splits, split = wave - my_tile * splits;
-  const int tile = tile0 + my_tile < n_tiles ? tile0 + my_tile : n_tiles - 1;
-  const int per = (blocks + splits - 1) / splits, block0 = split * per;
-  const int mine = blocks - block0 < per ? (blocks - block0 < 0 ? 0 : blocks - block0) : per;
-  uint4_t w[BPW];
+  };
+  // Scales and zero points of the work-group's tiles and part of K: for each of 16 rows a tile the `pieces` 16-byte pieces that hold them.
+  // A row's first value lies (row * groups + g0) % 8 values into its first piece; the tensors' sizes are multiples of 16 bytes, so that
+  // no piece reaches past their ends.
+  const int g0 = group_of(k0 / 32);
   {
-    const int64_t row = UP ? (int64_t)e * 2 * a.N + (r16 >> 3) * a.N + tile * 8 + (r16 & 7) : (int64_t)e * a.N + tile * 16 + r16;
-    // BPW loads whatever there is to load, so that they can be counted: past the end, an address of the row that is asked for anyway
-    // (behind K the rows in LDS are zeros)
-    const uint8_t* const src = a.Wp + row * (a.K / 2);
-    const int off = (mine > 0 ? block0 : 0) * 64 + q * 16, last = a.K / 2 - 16;
-#pragma unroll
-    for (int b = 0; b < BPW; ++b) {
-      const int at = b < mine ? off + b * 64 : off;
-      w[b] = __builtin_nontemporal_load((const uint4_t*)(src + (at < last ? at : last)));
+    const int all = wg_tiles * 16 * pieces;
+    const int64_t end = (int64_t)a.E * (UP ? 2 : 1) * a.N * a.groups;
+    if (flags & kFewWide) {
+      for (int c0 = wave * 64; c0 < all; c0 += threads) {
+        const int c = c0 + lane;
+        if (c >= all) continue;
+        const int r = c / pieces, at = c - r * pieces;
+        int64_t off = (weight_row(tile0 + (r >> 4), r & 15) * a.groups + g0) / 8 * 8 + at * 8;
+        off = off < end ? off : end - 8;
+        if (a.scales) direct16((const T*)a.scales + off, lds0 + sc_at + c0 * 16);
+        if (ZEROS) direct16((const T*)a.zeros + off, lds0 + zp_at + c0 * 16);
+      }
+    } else {  // a tensor that is aligned to its type only: value by value, to the same places
+      for (int i = tid; i < all * 8; i += threads) {
+        const int r = i / (pieces * 8), at = i - r * pieces * 8;
+        int64_t off = (weight_row(tile0 + (r >> 4), r & 15) * a.groups + g0) / 8 * 8 + at;
+        off = off < end ? off : end - 1;
+        if (a.scales) ((T*)(smem + sc_at))[i] = ((const T*)a.scales)[off];
+        if (ZEROS) ((T*)(smem + zp_at))[i] = ((const T*)a.zeros)[off];
+      }
     }
   }
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BPW) : "memory");  // all but the weights
-  __syncthreads();
 
-  const NibbleMagic mg = make_nibble_magic();
+  // this wavefront's part of K and tiles
+  const int lane_tile = wave / splits, split = wave - lane_tile * splits, my_tile0 = lane_tile * a.per_wave;
+  const int blocks = (k_len + 127) >> 7, per = (wg_blocks + splits - 1) / splits, block0 = split * per;
+  const int mine = blocks - block0 < per ? (blocks - block0 < 0 ? 0 : blocks - block0) : per;
+  int my_tiles = n_tiles - tile0 - my_tile0;
+  my_tiles = my_tiles < 0 ? 0 : my_tiles < a.per_wave ? my_tiles : a.per_wave;
+  const int total = my_tiles * mine;
+  // lane (r16, q) loads the 32 values 32 q .. of each block of row r16; past the end of a row its last ones (behind K the activation rows
+  // in LDS are zeros)
+  const uint8_t* const w_first = a.Wp + weight_row(tile0 + my_tile0, r16) * (a.K / 2);
+  const int64_t tile_stride = (int64_t)OUTS * (a.K / 2);
+  const int off_first = k0 / 2 + block0 * 64 + q * 16, off_last = a.K / 2 - 16;
   const T one = from_float<T>(1.0f), zs = from_float<T>(a.zero_scalar);
-  const T* const my_sc = (const T*)(smem + sc_at) + (my_tile * 16 + r16) * groups;
-  const T* const my_zp = (const T*)(smem + zp_at) + (my_tile * 16 + r16) * groups;
-  bool fold = flags & kFewFold;
-  if (a.zeros) {  // are this tile's zero points small integers?
-    bool ok = true;
-    for (int c = lane; c < 2 * groups; c += 64) {
-      const uint4_t v = *(const uint4_t*)(smem + zp_at + (my_tile * 2 * groups + c) * 16);
-      const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ok = ok && small_integer(to_float(bitcast<T>((uint16_t)x[i]))) && small_integer(to_float(bitcast<T>((uint16_t)(x[i] >> 16))));
-    }
-    fold = __builtin_amdgcn_ballot_w64(ok) == ~0ull;
-  }
+  const NibbleMagic mg = make_nibble_magic();
+  const int u_last = a.K / 32 - 1;
 
-  auto pass = [&](int row0, int rows) __attribute__((always_inline)) {
-    float4_t acc[2] = {float4_t{0, 0, 0, 0}, float4_t{0, 0, 0, 0}};
-    const uint8_t* const my_act = act + (r16 < rows ? r16 : rows - 1) * pitch + q * 64 + block0 * 256;
-    auto multiply = [&](auto fold_tag) __attribute__((always_inline)) {
-      constexpr bool FOLD = decltype(fold_tag)::value;
+  for (int row0 = 0; row0 < count; row0 += row_cap) {
+    const int rows = count - row0 < row_cap ? count - row0 : row_cap;
+    if (row0) __syncthreads();  // (the last pass's rows have been read, its sums added up)
+    load_rows(row0, rows);
+    // the first group, and how to go on from there: loads into registers behind the direct ones
+    uint4_t next[kFewGroup];
+    const uint8_t* src = w_first;
+    int load_block = 0, load_tile = 0;
+    auto load_group = [&]() __attribute__((always_inline)) {  // always kFewGroup loads, past the last tile of its last block
 #pragma unroll
-      for (int b = 0; b < BPW; ++b) {
-        if (b >= mine) break;
-        const uint32_t u = (uint32_t)((block0 + b) * 4 + q), at = a.per_group ? __umulhi(u, a.per_group) : u;
-        const uint32_t g = (int)at < groups ? at : groups - 1;  // (behind K, where the rows hold zeros)
-        const Expand8<T, FOLD> ex(a.scales ? my_sc[g] : one, a.zeros ? my_zp[g] : zs, mg);
-        // (opaque: the expanded weights are the same in every pass, and would be kept, four times as many registers as there are)
-        asm volatile("" : "+v"(w[b].x), "+v"(w[b].y), "+v"(w[b].z), "+v"(w[b].w));
-        const uint32_t words[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j & 1] = Mma::mma(ex(words[j]), *(const uint4_t*)(my_act + b * 256 + j * 16), acc[j & 1]);
+      for (int i = 0; i < kFewGroup; ++i) {
+        const int off = off_first + load_block * 64;
+        next[i] = __builtin_nontemporal_load((const uint4_t*)(src + (off < off_last ? off : off_last)));
+        if (load_block + 1 < mine) ++load_block;
+        else if (load_tile + 1 < my_tiles) load_block = 0, ++load_tile, src += tile_stride;
       }
     };
-    if (fold) multiply(std::true_type{});
-    else multiply(std::false_type{});
-    float4_t sum = acc[0] + acc[1];
-    if (splits > 1) {
-      if (split) *(float4_t*)(sums + ((my_tile * (splits - 1) + split - 1) * 64 + lane) * 4) = sum;
-      __syncthreads();
-      if (split) return;
-      for (int i = 1; i < splits; ++i) sum += *(const float4_t*)(sums + ((my_tile * (splits - 1) + i - 1) * 64 + lane) * 4);
+    // wait for the rows and, ahead of the first pass, the scales
+    if (total > 0) {
+      load_group();
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kFewGroup) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    // lane (r16, q): outputs 4 q .. 4 q + 3 of pair r16; gate / up: gates in q = 0, 1, their ups 32 lanes on
-    const bool live = r16 < rows && tile0 + my_tile < n_tiles;
-    if constexpr (UP) {
-      float4_t up;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) up[i] = __shfl_xor(sum[i], 32);
-      if (q < 2 && live) {
-        T o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = from_float<T>(silu(sum[i]) * up[i]);
-        *(uint2_t*)((T*)a.out + (int64_t)list[row0 + r16] * a.N + tile * 8 + q * 4) = bitcast<uint2_t>(o);
-      }
-    } else if (live) {
-      const int pair = list[row0 + r16];
-      *(float4_t*)((float*)a.out + (int64_t)pair * a.N + tile * 16 + q * 4) = sum * a.weights[pair];
-    }
-  };
-  // (the first pass apart from the loop: ahead of a loop the compiler waits for all weights, and here they are to be waited for one by one)
-  pass(0, count < row_cap ? count : row_cap);
-  for (int row0 = row_cap; row0 < count; row0 += row_cap) {
-    const int rows = count - row0 < row_cap ? count - row0 : row_cap;
-    __syncthreads();  // (the last pass's rows have been read, its sums added up)
-    load_rows(row0, rows);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    pass(row0, rows);
+
+    const int my_row = r16 < rows ? r16 : rows - 1, my_pair = list[row0 + my_row];
+    const float my_weight = UP ? 0.0f : *(const float*)(smem + weights_at + my_row * 4);
+    const uint8_t* const my_act = act + my_row * pitch + q * 64 + block0 * 256;
+    float4_t acc[2] = {float4_t{0, 0, 0, 0}, float4_t{0, 0, 0, 0}};
+    int tile = 0, block = 0, sc0 = 0;
+    for (int s = 0; s < total; s += kFewGroup) {
+      uint4_t w[kFewGroup];
+#pragma unroll
+      for (int i = 0; i < kFewGroup; ++i) {
+        w[i] = next[i];
+        asm volatile("" : "+v"(w[i].x), "+v"(w[i].y), "+v"(w[i].z), "+v"(w[i].w));
+      }
+      if (s + kFewGroup < total) load_group();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kFewGroup; ++i) {
+        if (s + i >= total) break;
+        if (block == 0)  // this lane's scales in LDS: that of group g lies at sc0 + g
+          sc0 = ((my_tile0 + tile) * 16 + r16) * pieces * 8 + (int)((weight_row(tile0 + my_tile0 + tile, r16) * a.groups + g0) & 7) - g0;
+        const int u = k0 / 32 + (block0 + block) * 4 + q, at = sc0 + group_of(u < u_last ? u : u_last);
+        const T sv = a.scales ? ((const T*)(smem + sc_at))[at] : one, zv = ZEROS ? ((const T*)(smem + zp_at))[at] : zs;
+        const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        const uint8_t* const x = my_act + block * 256;
+        auto multiply = [&](auto fold_tag) __attribute__((always_inline)) {
+          const Expand8<T, decltype(fold_tag)::value> ex(sv, zv, mg);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j & 1] = Mma::mma(ex(words[j]), *(const uint4_t*)(x + j * 16), acc[j & 1]);
+        };
+        // zero points that are small integers fold into the unpacking's bias
+        const bool fold = ZEROS ? __builtin_amdgcn_ballot_w64(small_integer(to_float(zv))) == ~0ull : (flags & kFewFold) != 0;
+        if (__builtin_expect(fold, 1)) multiply(std::true_type{});
+        else multiply(std::false_type{});
+        if (++block < mine) continue;
+        block = 0;
+        if (splits == 1) {
+          moe_store<T, UP>(a, acc[0] + acc[1], r16 < rows, my_pair, my_weight, (tile0 + my_tile0 + tile) * OUTS + q * 4, q, chunk);
+          acc[0] = acc[1] = float4_t{0, 0, 0, 0};
+        }
+        ++tile;
+      }
+    }
+    if (splits > 1) {  // (one tile a wavefront) the sums of the others
+      float4_t sum = acc[0] + acc[1];
+      float* const sums = (float*)(smem + sums_at) + (lane_tile * (splits - 1) * 64 + lane) * 4;
+      if (split) *(float4_t*)(sums + (split - 1) * 256) = sum;
+      __syncthreads();
+      if (split == 0 && my_tiles > 0) {
+        for (int i = 1; i < splits; ++i) sum += *(const float4_t*)(sums + (i - 1) * 256);
+        moe_store<T, UP>(a, sum, r16 < rows, my_pair, my_weight, (tile0 + my_tile0) * OUTS + q * 4, q, chunk);
+      }
+    }
   }
 }
 
-// y[t] = the sum of token t's rows, slot by slot
+// y[t] = the sum of token t's rows, slot by slot, each over the parts of K it was cut into; four slots' rows are asked for at once.  A
+// work-group has 256 x 4 values of one token.
 __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restrict__ rows, const int32_t* __restrict__ ids, void* __restrict__ Y,
-                                                         int64_t quads, int N4, int top_k, int E, int out_dtype) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= quads) return;
-  const int64_t t = i / N4;
-  const int n = (int)(i - t * N4) * 4;
+                                                         int N, int n_groups, int top_k, int E, int out_dtype, int chunks, int64_t chunk_stride) {
+  const int64_t t = blockIdx.x / (uint32_t)n_groups;
+  const int n = ((int)(blockIdx.x - (uint32_t)t * n_groups) * 256 + (int)threadIdx.x) * 4;
+  if (n >= N) return;
+  const int32_t* const my_ids = ids + t * top_k;
+  const float* const mine = rows + t * top_k * N + n;
   float4_t sum{0, 0, 0, 0};
-  for (int j = 0; j < top_k; ++j) {
-    if ((uint32_t)ids[t * top_k + j] >= (uint32_t)E) continue;  // (no row was written for it)
-    sum += *(const float4_t*)(rows + (t * top_k + j) * (int64_t)N4 * 4 + n);
+  for (int j = 0; j < top_k; j += 4) {
+    float4_t v[4];
+    bool there[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      there[i] = j + i < top_k && (uint32_t)my_ids[j + i] < (uint32_t)E;  // (otherwise no row was written)
+      v[i] = there[i] ? *(const float4_t*)(mine + (int64_t)(j + i) * N) : float4_t{0, 0, 0, 0};
+    }
+    for (int c = 1; c < chunks; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (there[i]) v[i] += *(const float4_t*)(mine + c * chunk_stride + (int64_t)(j + i) * N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (there[i]) sum += v[i];
   }
-  const int64_t o = t * N4 * 4 + n;
+  const int64_t o = t * N + n;
   if (out_dtype == TLQ_F32) {
     *(float4_t*)((float*)Y + o) = sum;
   } else if (out_dtype == TLQ_F16) {
@@ -495,43 +555,55 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // How moe_few_kernel is launched.  ok: it takes the call.
 struct FewPlan {
   bool ok;
-  int tiles, splits, bpw, row_cap, n_groups;
+  int waves, splits, per_wave, row_cap, n_groups, chunks, blocks, pieces;
   bool by_pair;
-  int64_t lds, blocks;
+  int64_t lds, units, grid;
 };
-FewPlan few_plan(bool up, int64_t pairs, int64_t E, int64_t N, int64_t K, int64_t group, bool scales, bool zeros) {
+int64_t down_chunks(int64_t pairs, int64_t K) { return pairs > 256 ? 1 : ceil_div(ceil_div(K, (int64_t)128), (int64_t)32); }
+FewPlan few_plan(bool up, int64_t pairs, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, bool zeros) {
   FewPlan p{};
-  const int64_t blocks = ceil_div(K, (int64_t)128), n_tiles = N / (up ? 8 : 16), groups = K / group;
+  const int64_t all = ceil_div(K, (int64_t)128), n_tiles = N / (up ? 8 : 16);
   const int64_t experts = pairs < E ? pairs : E;
-  if (pairs > kFewPairs || pairs > experts * 8 || blocks > 8 * 16) return p;
+  if (pairs > kFewPairs || pairs > experts * 8 || K > 65536) return p;
+  p.chunks = up ? 1 : (int)down_chunks(pairs, K);
+  const int64_t blocks = ceil_div(all, (int64_t)p.chunks);
+  p.chunks = (int)ceil_div(all, blocks);
+  p.blocks = (int)blocks;
+  p.waves = 4;
   p.splits = 1;
-  while (ceil_div(blocks, (int64_t)p.splits) > 16) p.splits *= 2;
-  while (p.splits < 8 && p.splits * 2 <= blocks && experts * n_tiles * p.splits < 2048) p.splits *= 2;
-  const int64_t per = ceil_div(blocks, (int64_t)p.splits);
-  p.bpw = per <= 4 ? 4 : per <= 8 ? 8 : 16;
-  p.tiles = p.splits >= 4 ? 1 : 4 / p.splits;
+  while (p.splits < 4 && p.splits * 4 <= blocks && experts * n_tiles * p.chunks * p.splits < 2048) p.splits *= 2;
+  p.per_wave = 1;
+  // tiles of a wavefront: as many as leave every CU several work-groups
+  if (p.splits == 1)
+    while (p.per_wave < 8 && experts * ceil_div(n_tiles, (int64_t)p.waves * p.per_wave * 2) * p.chunks >= 1536) p.per_wave *= 2;
   p.by_pair = pairs <= E;
-  // rows of a pass: twice what an expert has on average, while they leave LDS for two work-groups
-  const int64_t pitch = blocks * 256 + 16, average = ceil_div(pairs, experts);
+  // the scales of a part of K: its groups, the first of them anywhere in its piece; parts need not begin with a group
+  const int64_t part_groups = p.chunks == 1 ? K / group : (blocks * 128 + group - 1) / group + 1;
+  p.pieces = (int)((part_groups + 7 + 7) / 8);
+  // rows of a pass: sixteen (an operand's columns), while they leave LDS for two work-groups
+  const int64_t pitch = blocks * 256 + 16;
   p.row_cap = 16;
-  while (p.row_cap > 1 && (p.row_cap >= 4 * average || p.row_cap * pitch > 60 * 1024)) p.row_cap /= 2;
-  p.n_groups = (int)ceil_div(n_tiles, (int64_t)p.tiles);
-  p.lds = p.row_cap * pitch + (int64_t)((scales ? 1 : 0) + (zeros ? 1 : 0)) * p.tiles * 16 * groups * 2 + (int64_t)p.tiles * (p.splits - 1) * 1024 + 16 + ceil_div(pairs, (int64_t)8) * 16;
-  p.blocks = (p.by_pair ? pairs : E + (up ? 1 : 0)) * p.n_groups;
-  p.ok = p.lds <= 160 * 1024 && p.blocks < ((int64_t)1 << 31);
+  while (p.row_cap > 1 && (p.row_cap > pairs || p.row_cap * pitch > 36 * 1024)) p.row_cap /= 2;
+  if (p.by_pair && pairs == top_k) p.row_cap = 1;
+  const int64_t wg_tiles = p.waves / p.splits * p.per_wave;
+  p.n_groups = (int)ceil_div(n_tiles, wg_tiles);
+  p.lds = p.row_cap * pitch + p.waves / p.splits * (p.splits - 1) * 1024 + (zeros ? 2 : 1) * wg_tiles * 256 * (int64_t)p.pieces + 64 + 16 + ceil_div(pairs, (int64_t)8) * 16;
+  p.units = (p.by_pair ? pairs : E + (up ? 1 : 0)) * p.n_groups;
+  p.grid = p.chunks == 1 ? p.units : ceil_div(p.units, (int64_t)8) * 8 * p.chunks;
+  p.ok = p.lds <= 160 * 1024 && p.grid < ((int64_t)1 << 31);
   return p;
 }
 
-template <typename T, bool UP, int BPW>
+template <typename T, bool UP, bool ZEROS>
 int launch_few(const char* what, const FewArgs& a, const FewPlan& p, hipStream_t st) {
-  auto kern = moe_few_kernel<T, UP, BPW>;
+  auto kern = moe_few_kernel<T, UP, ZEROS>;
   static bool attr_set = false;
   if (!attr_set) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     TLQ_REQUIRE(e == hipSuccess, "%s: cannot reserve LDS: %s", what, hipGetErrorString(e));
     attr_set = true;
   }
-  kern<<<(unsigned)p.blocks, p.tiles * p.splits * 64, (size_t)p.lds, st>>>(a);
+  kern<<<(unsigned)p.grid, p.waves * 64, (size_t)p.lds, st>>>(a);
   return check_launch(what, "moe_few_kernel") ? 0 : 1;
 }
 
@@ -539,18 +611,19 @@ template <bool UP>
 int run_few(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, const FewPlan& p, hipStream_t st) {
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32;
-  const int flags = (p.by_pair ? kFewByPair : 0) | (p.by_pair && pairs == x.top_k ? kFewOneToken : 0) | (whole ? kFewFold : 0);
+  const int flags = (p.by_pair ? kFewByPair : 0) | (p.by_pair && pairs == x.top_k ? kFewOneToken : 0) | (whole ? kFewFold : 0) |
+                    (aligned16(x.scales) && aligned16(x.zeros) ? kFewWide : 0);
   const FewArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, (const int32_t*)ids, x.out, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
-                  units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, p.n_groups,
-                  (uint32_t)(p.tiles | p.splits << 8 | p.row_cap << 16 | flags << 24)};
-#define TLQ_FEW(BPW) (dtype == TLQ_F16 ? launch_few<half_t, UP, BPW>(what, a, p, st) : launch_few<bf16_t, UP, BPW>(what, a, p, st))
-  return p.bpw == 4 ? TLQ_FEW(4) : p.bpw == 8 ? TLQ_FEW(8) : TLQ_FEW(16);
+                  units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, p.n_groups, (int)p.units,
+                  (uint32_t)(p.blocks | p.pieces << 16), (uint32_t)(p.waves | p.splits << 8 | p.row_cap << 16 | flags << 24), p.per_wave};
+#define TLQ_FEW(T) (x.zeros ? launch_few<T, UP, true>(what, a, p, st) : launch_few<T, UP, false>(what, a, p, st))
+  return dtype == TLQ_F16 ? TLQ_FEW(half_t) : TLQ_FEW(bf16_t);
 #undef TLQ_FEW
 }
 
 template <bool UP>
 int run_experts(const char* what, ExpertArgs a, const void* ids, int64_t pairs, int dtype, void* ws, hipStream_t st) {
-  const FewPlan few = few_plan(UP, pairs, a.E, a.N, a.K, a.group, a.scales != nullptr, a.zeros != nullptr);
+  const FewPlan few = few_plan(UP, pairs, a.E, a.top_k, a.N, a.K, a.group, a.zeros != nullptr);
   if (few.ok) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
   const PlanPtrs p = plan_at(ws, a.E);
   a.begin = p.begin, a.tiles = p.tiles, a.order = p.order;
@@ -576,10 +649,10 @@ extern "C" int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t
   return plan_bytes(E, M * top_k);
 }
 
-extern "C" int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N) {
+extern "C" int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
   const int64_t plan = tlq_moe_gate_up_workspace_bytes(M, E, top_k);
-  if (plan == 0 || N < 1 || N >= ((int64_t)1 << 24)) return 0;
-  return plan + M * top_k * N * 4;
+  if (plan == 0 || N < 1 || N >= ((int64_t)1 << 24) || K < 1 || K >= ((int64_t)1 << 24)) return 0;
+  return plan + down_chunks(M * top_k, K) * M * top_k * N * 4;
 }
 
 extern "C" int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void* w_packed, const void* scales, const void* zeros, void* H,
@@ -608,7 +681,7 @@ extern "C" int tlq_moe_down_w4a16(const void* H, const void* ids, const void* we
   TLQ_REQUIRE(H && ids && weights && w_packed && Y, "%s: null pointer", what);
   TLQ_REQUIRE(aligned16(H) && aligned16(w_packed) && aligned16(Y) && (((uintptr_t)ids | (uintptr_t)weights) & 3) == 0 && (((uintptr_t)scales | (uintptr_t)zeros) & 1) == 0,
               "%s: H, w_packed and Y must be 16-byte aligned, the others to their type", what);
-  const int64_t want = tlq_moe_down_workspace_bytes(M, E, top_k, N);
+  const int64_t want = tlq_moe_down_workspace_bytes(M, E, top_k, N, K);
   TLQ_REQUIRE(workspace && workspace_bytes >= want && aligned16(workspace), "%s: a 16-byte aligned workspace of %lld bytes is wanted (got %lld)", what,
               (long long)want, (long long)(workspace ? workspace_bytes : 0));
   const int64_t pairs = M * top_k;
@@ -616,7 +689,10 @@ extern "C" int tlq_moe_down_w4a16(const void* H, const void* ids, const void* we
   ExpertArgs a{H, (const uint8_t*)w_packed, scales, zeros, (const float*)weights, rows, nullptr, nullptr, nullptr, (int)E, (int)top_k, (int)N, (int)K, (int)group, 0, zero_scalar};
   hipStream_t st = (hipStream_t)stream;
   if (run_experts<false>(what, a, ids, pairs, in_dtype, workspace, st)) return 1;
-  const int64_t quads = M * (N / 4);
-  moe_combine_kernel<<<(unsigned)ceil_div(quads, (int64_t)256), 256, 0, st>>>(rows, (const int32_t*)ids, Y, quads, (int)(N / 4), (int)top_k, (int)E, out_dtype);
+  const int64_t n_groups = ceil_div(N, (int64_t)1024);
+  const FewPlan few = few_plan(false, pairs, E, top_k, N, K, group, zeros != nullptr);
+  TLQ_REQUIRE(M * n_groups < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)(M * n_groups));
+  moe_combine_kernel<<<(unsigned)(M * n_groups), 256, 0, st>>>(rows, (const int32_t*)ids, Y, (int)N, (int)n_groups, (int)top_k, (int)E, out_dtype,
+                                                                 few.ok ? few.chunks : 1, pairs * N);
   return check_launch(what, "moe_combine_kernel") ? 0 : 1;
 }
