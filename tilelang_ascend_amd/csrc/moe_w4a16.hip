@@ -19,23 +19,24 @@ constexpr int kPlanThreads = 1024;
 constexpr int kMaxExperts = 1024;
 
 // What a call works out of its ids, in the workspace:
-//   begin[E + 2]  where the pairs of expert e begin in `order`; entry E: those without an expert, entry E + 1: the number of pairs
-//   tiles[E + 2]  the same for tiles of `rows` pairs
 //   order[P]      pairs by expert
-struct PlanPtrs {
-  int32_t *begin, *tiles, *order;
+//   tiles[]       {expert, first entry of `order`, pairs} of every tile of at most `rows` pairs; tiles behind the last one: no pairs
+struct PlanTile {
+  int32_t expert, first, pairs, unused;
 };
-__host__ __device__ inline int64_t plan_bytes(int64_t E, int64_t pairs) { return (((E + 2) * 2 + pairs) * 4 + 255) / 256 * 256; }
-inline PlanPtrs plan_at(void* ws, int64_t E) {
-  int32_t* p = (int32_t*)ws;
-  return {p, p + (E + 2), p + 2 * (E + 2)};
+// tiles of `rows` pairs that E experts and the pairs without one can need at most
+inline int64_t most_tiles(int64_t pairs, int64_t E, int64_t rows) {
+  const int64_t some = pairs < E + 1 ? pairs : E + 1;
+  return some + (pairs - some) / rows;
 }
+constexpr int kLeastRows = 16;  // of a tile
+inline int64_t order_bytes(int64_t pairs) { return (pairs * 4 + 255) / 256 * 256; }
+inline int64_t plan_bytes(int64_t E, int64_t pairs) { return order_bytes(pairs) + (most_tiles(pairs, E, kLeastRows) * 16 + 255) / 256 * 256; }
 
 // One work-group per expert, and one more for the pairs without one: each counts all pairs (LDS histogram; whole numbers, so the
 // order of the atomic adds does not matter) and writes down its own.
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ begin,
-                                                               int32_t* __restrict__ tiles, int32_t* __restrict__ order, int pairs,
-                                                               int E, int rows) {
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, PlanTile* __restrict__ tiles,
+                                                               int32_t* __restrict__ order, int pairs, int E, int rows, int all_tiles) {
   __shared__ int32_t count[kMaxExperts + 1];
   __shared__ int32_t part[kPlanThreads / 64][2];
   __shared__ int32_t of_wave[kPlanThreads / 64];
@@ -73,10 +74,13 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
     before += part[i][0], tiles_before += part[i][1];
     at += i < wave ? of_wave[i] : 0;
   }
-  if (tid == 0) {
-    begin[e] = before, tiles[e] = tiles_before;
-    if (e == E) begin[E + 1] = pairs, tiles[E + 1] = tiles_before + (count[E] + rows - 1) / rows;
+  const int my_count = count[e], my_tiles = (my_count + rows - 1) / rows;
+  for (int i = tid; i < my_tiles; i += kPlanThreads) {
+    const int left = my_count - i * rows;
+    tiles[tiles_before + i] = PlanTile{e, before + i * rows, left < rows ? left : rows, 0};
   }
+  if (e == E)
+    for (int i = tiles_before + my_tiles + tid; i < all_tiles; i += kPlanThreads) tiles[i] = PlanTile{0, 0, 0, 0};
   at += before;
   for (int s = 0; s < steps; ++s) {
     const int p = first + s * 64 + lane;
@@ -109,158 +113,21 @@ struct ExpertArgs {
   const void* zeros;     // the same, or null
   const float* weights;  // down: [pairs]
   void* out;             // gate / up: h [pairs, N]; down: fp32 [pairs, N]
-  const int32_t *begin, *tiles, *order;
-  int E, top_k, N, K, group, n_blocks;
+  int E, top_k, N, K, group;
   float zero_scalar;
 };
 
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
-
-// Tiles of 64 pairs x 64 outputs; a wavefront has 16 outputs (gate / up: 16 gate and 16 up rows).  Per step of 128 values of K the
-// activations pass through LDS, the packed weights go from memory to the operand registers: lane (row r16, q) takes the 16 bytes
-// with the values 32 q .. 32 q + 31 of the step of its weight row, and at MFMA k-step j the word 4 q + j; the activation operand
-// of lane (m = r16, q) holds the same eight k.  K % 32 == 0: such 16 bytes lie inside a row or behind it.
-constexpr int kRows = 64, kOuts = 64, kPitch = 128 + 8;
-
-template <typename T, bool UP>
-__global__ __launch_bounds__(256) void moe_w4a16_kernel(const ExpertArgs a) {
-  typedef typename MmaOf<T>::type Mma;
-  constexpr int MT = kRows / 16, NP = UP ? 2 : 1;
-  __shared__ __align__(16) T tile[kRows][kPitch];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q = lane >> 4;
-  const int t = (int)(blockIdx.x / (uint32_t)a.n_blocks);
-  if (t >= a.tiles[a.E + (UP ? 1 : 0)]) return;
-  int e = 0;
-  {
-    int lo = 0, hi = a.E;  // the last expert whose tiles begin at or before t
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.tiles[mid] <= t) lo = mid; else hi = mid - 1;
-    }
-    e = lo;
-  }
-  const int row0 = a.begin[e] + (t - a.tiles[e]) * kRows;
-  const int left = a.begin[e + 1] - row0, rows = left < kRows ? left : kRows;
-  const int n0 = (int)(blockIdx.x % (uint32_t)a.n_blocks) * kOuts;
-  if (UP && e == a.E) {  // pairs without an expert
-    T* const h = (T*)a.out;
-    for (int i = tid; i < rows * kOuts; i += 256) {
-      const int n = n0 + i % kOuts;
-      if (n < a.N) h[(int64_t)a.order[row0 + i / kOuts] * a.N + n] = from_float<T>(0.0f);
-    }
-    return;
-  }
-  const int groups = a.K / a.group;
-  const int n = n0 + wave * 16 + r16;  // this lane's weight row (gate / up: its gate row)
-  const int nc = n < a.N ? n : a.N - 1;
-  int64_t w_row[NP];
-#pragma unroll
-  for (int i = 0; i < NP; ++i) w_row[i] = (int64_t)e * (NP * a.N) + (int64_t)i * a.N + nc;
-  // activation rows: thread tid copies 16-byte chunk tid % 16 of rows tid / 16 + 16 i
-  const T* src[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int r = i * 16 + (tid >> 4);
-    const int pair = a.order[row0 + (r < rows ? r : 0)];
-    src[i] = (const T*)a.X + (int64_t)(UP ? pair / a.top_k : pair) * a.K;
-  }
-  const NibbleMagic mg = make_nibble_magic();
-  const T one = from_float<T>(1.0f), zs = from_float<T>(a.zero_scalar);
-  float4_t acc[NP][MT];
-#pragma unroll
-  for (int i = 0; i < NP; ++i)
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) acc[i][mt] = float4_t{0, 0, 0, 0};
-
-  for (int k0 = 0; k0 < a.K; k0 += 128) {
-    const int ka = k0 + (tid & 15) * 8;
-    uint4_t v[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) v[i] = ka < a.K ? *(const uint4_t*)(src[i] + ka) : uint4_t{0, 0, 0, 0};
-    const int kw = k0 + 32 * q;
-    const bool in = kw < a.K;
-    uint4_t w[NP];
-    T s[NP], z[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      w[i] = in ? *(const uint4_t*)(a.Wp + w_row[i] * (a.K / 2) + kw / 2) : uint4_t{0, 0, 0, 0};
-      const int64_t g = w_row[i] * groups + (in ? kw / a.group : 0);
-      s[i] = !in ? from_float<T>(0.0f) : a.scales ? ((const T*)a.scales)[g] : one;
-      z[i] = !in ? from_float<T>(0.0f) : a.zeros ? ((const T*)a.zeros)[g] : zs;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < MT; ++i) *(uint4_t*)&tile[i * 16 + (tid >> 4)][(tid & 15) * 8] = v[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const Expand8<T, false> ex(s[i], z[i], mg);
-      const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4_t wo = ex(words[j]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[i][mt] = Mma::mma(wo, *(const uint4_t*)&tile[mt * 16 + r16][32 * q + 8 * j], acc[i][mt]);
-      }
-    }
-  }
-  // lane (r16, q) holds rows m = 16 mt + r16, outputs 4 q .. 4 q + 3 of the wavefront's 16 (N % 16 == 0: all inside or all outside)
-  const int no = n0 + wave * 16 + 4 * q;
-  if (no >= a.N) return;
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = mt * 16 + r16;
-    if (r >= rows) continue;
-    const int pair = a.order[row0 + r];
-    if (UP) {
-      T o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = from_float<T>(silu(acc[0][mt][i]) * acc[NP - 1][mt][i]);
-      *(uint2_t*)((T*)a.out + (int64_t)pair * a.N + no) = bitcast<uint2_t>(o);
-    } else {
-      *(float4_t*)((float*)a.out + (int64_t)pair * a.N + no) = acc[0][mt] * a.weights[pair];
-    }
-  }
-}
-
-// ---- few pairs: every weight read once ---------------------------------------------------------------------------------------
-// For calls that are bound by reading the weights.  A work-group stages up to `row_cap` of its expert's activation rows in LDS, whole, with
-// the scales and zero points of its tiles, once; then every wavefront streams the packed weights of its own tiles through its registers,
-// with no barrier: the next kFewGroup blocks (1 KB each) are on their way while the last ones are expanded and multiplied with all rows.
-// No launch sorts the pairs first: a work-group looks its expert's pairs up among all ids (at most kFewPairs).  The work-groups of
-// an expert are those of the first pair that names it, or, where there are more pairs than experts, those of the expert's number; one
-// token's pairs are taken one by one.
-//   A tile is 16 weight rows: 16 outputs, or 8 gate rows and the 8 up rows that go with them.  A block is 128 values of K of a tile.
-// Where tiles are few, `splits` wavefronts share one, each with a part of K; their sums meet in LDS and are added in the order of K.
-// Long rows of the down product are cut into `chunks` work-groups too, whose sums moe_combine_kernel adds.
-constexpr int kFewPairs = 2048;
-constexpr int kFewGroup = 4;
-enum { kFewByPair = 1, kFewOneToken = 2, kFewFold = 4, kFewWide = 8 };
-
-struct FewArgs {
-  const void* X;
-  const uint8_t* Wp;
-  const void* scales;
-  const void* zeros;
-  const float* weights;
-  const int32_t* ids;
-  void* out;
-  int pairs, E, top_k, N, K, groups;
-  uint32_t per_group;    // ceil(2^32 / (group / 32)), 0 for groups of 32
-  float zero_scalar;
-  int n_groups, units;   // work-groups of an expert side by side, and of all experts
-  uint32_t blocks;       // blocks of 128 values of K of a work-group | 16-byte pieces of a row's scales << 16
-  uint32_t shape;        // wavefronts | splits << 8 | row_cap << 16 | flags << 24 (kFewFold: the scalar zero point is a small integer)
-  int per_wave;          // tiles of a wavefront
-};
-
 __device__ __forceinline__ bool small_integer(float z) { return z == __builtin_rintf(z) && z >= -256.0f && z <= 256.0f; }
 
-// 16 bytes per lane, global -> LDS: lane l to lds + 16 l (lanes that are switched off: nothing)
+// Global -> LDS without registers: 16 or 4 bytes per lane, lane l to lds + 16 l or 4 l (lanes that are switched off: nothing).
 __device__ __forceinline__ void direct16(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
-__device__ __forceinline__ void direct4(const void* src, uint32_t lds) {  // 4 bytes per lane, lane l to lds + 4 l
+__device__ __forceinline__ void direct16_at(uint32_t off, const uint8_t* base, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void direct4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 
@@ -282,7 +149,272 @@ __device__ __forceinline__ void moe_store(const Args& a, const float4_t& sum, bo
   }
 }
 
-template <typename T, bool UP, bool ZEROS>
+// ---- tiles of many pairs ----------------------------------------------------------------------------------------------------
+// Up to 16 MAXMT pairs of one expert x NT tiles of 16 weight rows for each of four wavefronts (a tile: 16 outputs, or 8 gate rows and the 8
+// up rows that go with them).  K goes by in steps of KSB blocks of 128 values: the activation rows are gathered global -> LDS into
+// two buffers a step ahead, the packed weights go straight into operand registers a step ahead -- lane (r16, q) has the 32 values 32 q ..
+// of each block of row r16, at MFMA k-step j the eight of word 4 q + j --, are expanded there and multiplied with all rows: a weight
+// is expanded once per 16 MAXMT pairs, an activation operand read once per NT tiles.  One barrier a step.
+//   Scales and zero points come through LDS in windows of eight groups (whole steps: 8 groups are 256 (group / 32) values), loaded a window
+// ahead as the two 16-byte pieces of a row that hold them.  ANY: zero points that need not be small integers, which are folded into the
+// unpacking's bias (a tensor, looked at block by block, or such a scalar).
+struct TileArgs {
+  const void* X;
+  const uint8_t* Wp;
+  const void* scales;
+  const void* zeros;
+  const float* weights;
+  void* out;
+  const PlanTile* tiles;
+  const int32_t* order;
+  int pairs, E, top_k, N, K, groups;
+  uint32_t per_group;  // ceil(2^32 / (group / 32)), 0 for groups of 32
+  float zero_scalar;
+  int n_groups;        // work-groups side by side
+  int window;          // steps of a window
+  int chunk_steps;     // steps of a work-group: those of a part of K (down product with few tiles), whose sums moe_combine_kernel adds
+};
+
+template <int MAXMT, int NT, int KSB>
+struct TileCfg {
+  static constexpr int ROWS = 16 * MAXMT, ROW_BYTES = KSB * 256, ACT = ROWS * ROW_BYTES;
+  static constexpr int TILES = 4 * NT, WINDOW = TILES * 16 * 32;          // scales of a window: 32 bytes a row
+  static constexpr int RPI = 1024 / ROW_BYTES, LOADS = ROWS / RPI / 4;    // rows of a load instruction, loads of a wavefront and step
+  static_assert(ROWS % (RPI * 4) == 0, "the rows split over the wavefronts");
+  static constexpr int lds(bool zeros) { return 2 * ACT + 2 * WINDOW * (zeros ? 2 : 1) + ROWS * 8; }
+};
+
+template <typename T, bool UP, bool ANY, int MAXMT, int NT, int KSB>
+__global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_kernel(const TileArgs a) {
+  typedef typename MmaOf<T>::type Mma;
+  typedef TileCfg<MAXMT, NT, KSB> Cfg;
+  typedef __attribute__((address_space(3))) uint8_t* lptr_t;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q = lane >> 4;
+  // Work-groups of one tile's neighbours side by side on one XCD (numbers go to the XCDs in turn): they share its activation rows, and the
+  // tiles of an expert, which follow each other, its weights.
+  const int all_steps = (a.K + KSB * 128 - 1) / (KSB * 128), chunks = (all_steps + a.chunk_steps - 1) / a.chunk_steps;
+  const int part = (int)(blockIdx.x / (uint32_t)a.n_groups), group_no = (int)blockIdx.x - part * a.n_groups;
+  const int tile_no = part / chunks, chunk = part - tile_no * chunks;
+  const PlanTile pt = a.tiles[tile_no];
+  const int e = __builtin_amdgcn_readfirstlane(pt.expert), first = __builtin_amdgcn_readfirstlane(pt.first), rows = __builtin_amdgcn_readfirstlane(pt.pairs);
+  if (rows == 0) return;
+  constexpr int OUTS = UP ? 8 : 16;
+  const int n_tiles = a.N / OUTS, tile0 = group_no * Cfg::TILES;
+  if (e == a.E) {  // pairs without an expert
+    if constexpr (UP) {
+      T* const h = (T*)a.out;
+      constexpr int width = Cfg::TILES * OUTS;
+      for (int i = tid; i < rows * width; i += 256) {
+        const int n = tile0 * OUTS + i % width;
+        if (n < a.N) h[(int64_t)a.order[first + i / width] * a.N + n] = from_float<T>(0.0f);
+      }
+    }
+    return;
+  }
+  uint8_t* const sc = smem + 2 * Cfg::ACT;
+  uint8_t* const zp = sc + 2 * Cfg::WINDOW;
+  int32_t* const list = (int32_t*)(zp + (ANY ? 2 * Cfg::WINDOW : 0));
+  float* const row_weight = (float*)(list + Cfg::ROWS);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)smem);
+  if (tid < Cfg::ROWS) {
+    const int pair = a.order[first + (tid < rows ? tid : rows - 1)];
+    list[tid] = pair;
+    if (!UP) row_weight[tid] = a.weights[pair];
+  }
+  __syncthreads();
+
+  // Activation rows: lane l of load i of a wavefront brings a 16-byte piece of row (4 i + wave) RPI + l / (64 / RPI); its place in the row is
+  // swapped with its neighbours' by the row (xor), so that eight rows' operand reads meet every bank once.
+  constexpr int LPR = 64 / Cfg::RPI;  // lanes (16-byte pieces) of a row
+  const uint8_t* act_src[Cfg::LOADS];
+  const int act_k = ((lane % LPR) ^ ((wave * Cfg::RPI + lane / LPR) & 7)) * 8;  // (the rows of a wavefront's loads are multiples of eight apart)
+  static_assert(4 * Cfg::RPI % 8 == 0, "the same place in every load's rows");
+#pragma unroll
+  for (int i = 0; i < Cfg::LOADS; ++i) {
+    const int pair = list[(4 * i + wave) * Cfg::RPI + lane / LPR];
+    act_src[i] = (const uint8_t*)((const T*)a.X + (int64_t)(UP ? pair / a.top_k : pair) * a.K + act_k);
+  }
+  const int s_begin = chunk * a.chunk_steps, s_end = s_begin + a.chunk_steps < all_steps ? s_begin + a.chunk_steps : all_steps;
+  auto load_act = [&](int s) __attribute__((always_inline)) {
+    const int k = s * (KSB * 128);
+    const uint32_t buf = lds0 + (uint32_t)((s & 1) * Cfg::ACT);
+#pragma unroll
+    for (int i = 0; i < Cfg::LOADS; ++i) {
+      if ((4 * i + wave) * Cfg::RPI >= rows) break;  // (uniform)
+      const uint32_t at = (uint32_t)((4 * i + wave) * 1024);
+      if (k + act_k < a.K) direct16(act_src[i] + k * 2, buf + at);
+      else *(uint4_t*)(smem + (s & 1) * Cfg::ACT + at + lane * 16) = uint4_t{0, 0, 0, 0};
+    }
+  };
+  // weights
+  auto weight_row = [&](int t, int r) __attribute__((always_inline)) -> int64_t {
+    t = tile0 + t < n_tiles ? tile0 + t : n_tiles - 1;
+    return UP ? (int64_t)e * 2 * a.N + (r >> 3) * a.N + t * 8 + (r & 7) : (int64_t)e * a.N + t * 16 + r;
+  };
+  const uint8_t* const w_base = uniform_ptr(a.Wp + (int64_t)e * (UP ? 2 : 1) * a.N * (a.K / 2));
+  uint32_t w_off[NT];  // (an expert's matrix is below 4 GiB)
+#pragma unroll
+  for (int t = 0; t < NT; ++t) w_off[t] = (uint32_t)((weight_row(wave * NT + t, r16) - (int64_t)e * (UP ? 2 : 1) * a.N) * (a.K / 2)) + q * 16;
+  const int w_last = a.K / 2 - 16 - q * 16;
+  uint4_t next[KSB][NT];
+  auto load_weights = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < KSB; ++b) {
+      const int at = (s * KSB + b) * 64;
+      const uint32_t off = (uint32_t)(at < w_last ? at : w_last);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) next[b][t] = *(const uint4_t*)(w_base + (w_off[t] + off));
+    }
+  };
+  // scales of window v: pieces (row * groups) / 8 + v and the next one of every row (the tensors' sizes are multiples of 16 bytes, so that
+  // no piece reaches past their ends)
+  auto group_of = [&](int u) __attribute__((always_inline)) -> int { return a.per_group ? (int)__umulhi((uint32_t)u, a.per_group) : u; };
+  const int window = a.window;
+  const int64_t sc_e = (int64_t)e * (UP ? 2 : 1) * a.N * a.groups;  // the expert's first value: a multiple of eight
+  const uint32_t sc_last = (uint32_t)((UP ? 2 : 1) * a.N * a.groups / 8 - 1) * 16;
+  constexpr int SC_LOADS = Cfg::TILES * 32 / 256;
+  uint32_t sc_off[SC_LOADS];
+#pragma unroll
+  for (int i = 0; i < SC_LOADS; ++i) {
+    const int c = (i * 4 + wave) * 64 + lane, r = c >> 1;
+    sc_off[i] = (uint32_t)((weight_row(r >> 4, r & 15) * a.groups - sc_e) / 8 + (c & 1)) * 16;
+  }
+  const uint8_t* const sc_base = uniform_ptr((const uint8_t*)((const T*)a.scales + (a.scales ? sc_e : 0)));
+  const uint8_t* const zp_base = uniform_ptr((const uint8_t*)((const T*)a.zeros + (a.zeros ? sc_e : 0)));
+  auto load_scales = [&](int v) __attribute__((always_inline)) {
+    const uint32_t buf = lds0 + 2 * Cfg::ACT + (uint32_t)((v & 1) * Cfg::WINDOW);
+#pragma unroll
+    for (int i = 0; i < SC_LOADS; ++i) {
+      uint32_t off = sc_off[i] + (uint32_t)v * 16;
+      off = off < sc_last ? off : sc_last;
+      if (a.scales) direct16_at(off, sc_base, buf + (i * 4 + wave) * 1024);
+      if (ANY && a.zeros) direct16_at(off, zp_base, buf + 2 * Cfg::WINDOW + (i * 4 + wave) * 1024);
+    }
+  };
+  int sc_at[NT];  // where this lane's first scale of a window lies in it (in values); the first of window v is group 8 v
+#pragma unroll
+  for (int t = 0; t < NT; ++t) sc_at[t] = ((wave * NT + t) * 16 + r16) * 16 + (int)((weight_row(wave * NT + t, r16) * a.groups) & 7);
+  const T one = from_float<T>(1.0f), zs = from_float<T>(a.zero_scalar);
+  const NibbleMagic mg = make_nibble_magic();
+  const int u_last = a.K / 32 - 1;
+
+  auto run = [&](auto mt_tag) __attribute__((always_inline)) {
+    constexpr int MT = decltype(mt_tag)::value;
+    float4_t acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[t][m] = float4_t{0, 0, 0, 0};
+    int v = s_begin / window, in_window = s_begin - v * window;
+    for (int s = s_begin; s < s_end; ++s) {
+      uint4_t w[KSB][NT];
+#pragma unroll
+      for (int b = 0; b < KSB; ++b)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          w[b][t] = next[b][t];
+          asm volatile("" : "+v"(w[b][t].x), "+v"(w[b][t].y), "+v"(w[b][t].z), "+v"(w[b][t].w));
+        }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();  // this step's rows are there, and nobody reads the last step's any more
+      if (s + 1 < s_end) {
+        load_act(s + 1);
+        if ((in_window == 0 || s == s_begin) && (v + 1) * window < s_end) load_scales(v + 1);
+        load_weights(s + 1);
+      }
+      const uint8_t* const x0 = smem + (s & 1) * Cfg::ACT + r16 * Cfg::ROW_BYTES;
+      const int buf = (v & 1) * (Cfg::WINDOW / 2);
+#pragma unroll
+      for (int b = 0; b < KSB; ++b) {
+        const int u = (s * KSB + b) * 4 + q, g = group_of(u < u_last ? u : u_last) - 8 * v + buf;
+        T sv[NT], zv[NT];
+        bool whole = true;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          sv[t] = a.scales ? ((const T*)sc)[sc_at[t] + g] : one;
+          zv[t] = ANY && a.zeros ? ((const T*)zp)[sc_at[t] + g] : zs;
+          if (ANY) whole = whole && small_integer(to_float(zv[t]));
+        }
+        auto multiply = [&](auto fold_tag) __attribute__((always_inline)) {
+          typedef Expand8<T, decltype(fold_tag)::value> Ex;
+          Ex ex[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) ex[t] = Ex(sv[t], zv[t], mg);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            uint4_t x[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) x[m] = *(const uint4_t*)(x0 + m * 16 * Cfg::ROW_BYTES + (((b * 16 + 4 * q + j) ^ (r16 & 7)) * 16));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              const uint32_t word = j == 0 ? w[b][t].x : j == 1 ? w[b][t].y : j == 2 ? w[b][t].z : w[b][t].w;
+              if constexpr (!decltype(fold_tag)::value) __builtin_amdgcn_sched_barrier(0);  // (few registers rather than fast)
+              const uint4_t wo = ex[t](word);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) acc[t][m] = Mma::mma(wo, x[m], acc[t][m]);
+            }
+          }
+        };
+        if constexpr (ANY) {
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(whole) == ~0ull, 1)) multiply(std::true_type{});
+          else multiply(std::false_type{});
+        } else {
+          multiply(std::true_type{});
+        }
+      }
+      if (++in_window == window) in_window = 0, ++v;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = (tile0 + wave * NT + t) * OUTS + q * 4;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int r = m * 16 + r16;
+        moe_store<T, UP>(a, acc[t][m], r < rows && tile0 + wave * NT + t < n_tiles, list[r], UP ? 0.0f : row_weight[r], n, q, chunk);
+      }
+    }
+  };
+  load_scales(s_begin / window);
+  load_act(s_begin);
+  load_weights(s_begin);
+  if (rows > Cfg::ROWS / 2) run(std::integral_constant<int, MAXMT>{});
+  else run(std::integral_constant<int, MAXMT / 2>{});
+}
+
+// ---- few pairs: every weight read once ---------------------------------------------------------------------------------------
+// For calls that are bound by reading the weights.  A work-group stages up to `row_cap` of its expert's activation rows in LDS, whole, with
+// the scales and zero points of its tiles, once; then every wavefront streams the packed weights of its own tiles through its registers,
+// with no barrier: the next kFewGroup blocks (1 KB each) are on their way while the last ones are expanded and multiplied with all rows.
+// No launch sorts the pairs first: a work-group looks its expert's pairs up among all ids (at most kFewPairs).  The work-groups of
+// an expert are those of the first pair that names it, or, where there are more pairs than experts, those of the expert's number; one
+// token's pairs are taken one by one.
+//   A tile is 16 weight rows: 16 outputs, or 8 gate rows and the 8 up rows that go with them.  A block is 128 values of K of a tile.
+// Where tiles are few, `splits` wavefronts share one, each with a part of K; their sums meet in LDS and are added in the order of K.
+// Long rows of the down product are cut into `chunks` work-groups too, whose sums moe_combine_kernel adds.
+constexpr int kFewPairs = 2048;
+constexpr int kFewGroup = 4;
+enum { kFewByPair = 1, kFewOneToken = 2 };
+
+struct FewArgs {
+  const void* X;
+  const uint8_t* Wp;
+  const void* scales;
+  const void* zeros;
+  const float* weights;
+  const int32_t* ids;
+  void* out;
+  int pairs, E, top_k, N, K, groups;
+  uint32_t per_group;    // ceil(2^32 / (group / 32)), 0 for groups of 32
+  float zero_scalar;
+  int n_groups, units;   // work-groups of an expert side by side, and of all experts
+  uint32_t blocks;       // blocks of 128 values of K of a work-group | 16-byte pieces of a row's scales << 16
+  uint32_t shape;        // wavefronts | splits << 8 | row_cap << 16 | flags << 24
+  int per_wave;          // tiles of a wavefront
+};
+
+template <typename T, bool UP, bool ANY>
 __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
   typedef typename MmaOf<T>::type Mma;
   typedef __attribute__((address_space(3))) uint8_t* lptr_t;
@@ -308,7 +440,7 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
   // LDS: activation rows, sums of the other wavefronts, scales, zero points, the rows' weights, the pairs
   const int sums_at = row_cap * pitch, sc_at = sums_at + waves / splits * (splits - 1) * 1024, zp_at = sc_at + wg_tiles * 256 * pieces;
   uint8_t* const act = smem;
-  const int weights_at = zp_at + (ZEROS ? wg_tiles * 256 * pieces : 0);
+  const int weights_at = zp_at + (ANY ? wg_tiles * 256 * pieces : 0);
   int32_t* const head = (int32_t*)(smem + weights_at + (UP ? 0 : 64));  // [0] number of pairs, [1] an earlier pair has this expert
   uint16_t* const list = (uint16_t*)(head + 4);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)smem);
@@ -378,24 +510,17 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
   {
     const int all = wg_tiles * 16 * pieces;
     const int64_t end = (int64_t)a.E * (UP ? 2 : 1) * a.N * a.groups;
-    if (flags & kFewWide) {
-      for (int c0 = wave * 64; c0 < all; c0 += threads) {
-        const int c = c0 + lane;
-        if (c >= all) continue;
-        const int r = c / pieces, at = c - r * pieces;
-        int64_t off = (weight_row(tile0 + (r >> 4), r & 15) * a.groups + g0) / 8 * 8 + at * 8;
-        off = off < end ? off : end - 8;
-        if (a.scales) direct16((const T*)a.scales + off, lds0 + sc_at + c0 * 16);
-        if (ZEROS) direct16((const T*)a.zeros + off, lds0 + zp_at + c0 * 16);
-      }
-    } else {  // a tensor that is aligned to its type only: value by value, to the same places
-      for (int i = tid; i < all * 8; i += threads) {
-        const int r = i / (pieces * 8), at = i - r * pieces * 8;
-        int64_t off = (weight_row(tile0 + (r >> 4), r & 15) * a.groups + g0) / 8 * 8 + at;
-        off = off < end ? off : end - 1;
-        if (a.scales) ((T*)(smem + sc_at))[i] = ((const T*)a.scales)[off];
-        if (ZEROS) ((T*)(smem + zp_at))[i] = ((const T*)a.zeros)[off];
-      }
+    // (no load into registers is on its way here; said so, because the compiler would wait for one ahead of the weights, and so for the
+    // direct loads)
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    for (int c0 = wave * 64; c0 < all; c0 += threads) {
+      const int c = c0 + lane;
+      if (c >= all) continue;
+      const int r = c / pieces, at = c - r * pieces;
+      int64_t off = (weight_row(tile0 + (r >> 4), r & 15) * a.groups + g0) / 8 * 8 + at * 8;
+      off = off < end ? off : end - 8;
+      if (a.scales) direct16((const T*)a.scales + off, lds0 + sc_at + c0 * 16);
+      if (ANY && a.zeros) direct16((const T*)a.zeros + off, lds0 + zp_at + c0 * 16);
     }
   }
 
@@ -461,7 +586,7 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
         if (block == 0)  // this lane's scales in LDS: that of group g lies at sc0 + g
           sc0 = ((my_tile0 + tile) * 16 + r16) * pieces * 8 + (int)((weight_row(tile0 + my_tile0 + tile, r16) * a.groups + g0) & 7) - g0;
         const int u = k0 / 32 + (block0 + block) * 4 + q, at = sc0 + group_of(u < u_last ? u : u_last);
-        const T sv = a.scales ? ((const T*)(smem + sc_at))[at] : one, zv = ZEROS ? ((const T*)(smem + zp_at))[at] : zs;
+        const T sv = a.scales ? ((const T*)(smem + sc_at))[at] : one, zv = ANY && a.zeros ? ((const T*)(smem + zp_at))[at] : zs;
         const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
         const uint8_t* const x = my_act + block * 256;
         auto multiply = [&](auto fold_tag) __attribute__((always_inline)) {
@@ -469,10 +594,12 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[j & 1] = Mma::mma(ex(words[j]), *(const uint4_t*)(x + j * 16), acc[j & 1]);
         };
-        // zero points that are small integers fold into the unpacking's bias
-        const bool fold = ZEROS ? __builtin_amdgcn_ballot_w64(small_integer(to_float(zv))) == ~0ull : (flags & kFewFold) != 0;
-        if (__builtin_expect(fold, 1)) multiply(std::true_type{});
-        else multiply(std::false_type{});
+        if constexpr (ANY) {
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(small_integer(to_float(zv))) == ~0ull, 1)) multiply(std::true_type{});
+          else multiply(std::false_type{});
+        } else {
+          multiply(std::true_type{});
+        }
         if (++block < mine) continue;
         block = 0;
         if (splits == 1) {
@@ -532,12 +659,6 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
   }
 }
 
-// tiles of `rows` pairs that E experts (and the pairs without one) can need at most
-int64_t most_tiles(int64_t pairs, int64_t E, int64_t rows) {
-  const int64_t some = pairs < E + 1 ? pairs : E + 1;
-  return some + (pairs - some) / rows;
-}
-
 int check_experts(const char* what, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, int dtype) {
   TLQ_REQUIRE(M >= 0 && E >= 1 && E <= kMaxExperts && top_k >= 1 && top_k <= 64, "%s: bad shape M=%lld E=%lld top_k=%lld (at most 1024 experts, 64 of them for a token)",
               what, (long long)M, (long long)E, (long long)top_k);
@@ -546,6 +667,7 @@ int check_experts(const char* what, int64_t M, int64_t E, int64_t top_k, int64_t
   TLQ_REQUIRE(K >= 32 && K % 32 == 0 && K < ((int64_t)1 << 24), "%s: K=%lld must be a multiple of 32", what, (long long)K);
   TLQ_REQUIRE(group >= 32 && group % 32 == 0 && K % group == 0, "%s: group=%lld must be a multiple of 32 that divides K=%lld", what,
               (long long)group, (long long)K);
+  TLQ_REQUIRE(2 * N * (K / 2) < ((int64_t)1 << 32), "%s: N=%lld x K=%lld is too large a matrix for one expert", what, (long long)N, (long long)K);
   TLQ_REQUIRE(dtype == TLQ_F16 || dtype == TLQ_BF16, "%s: in_dtype must be float16 or bfloat16 (got %d)", what, dtype);
   return 0;
 }
@@ -559,13 +681,13 @@ struct FewPlan {
   bool by_pair;
   int64_t lds, units, grid;
 };
-int64_t down_chunks(int64_t pairs, int64_t K) { return pairs > 256 ? 1 : ceil_div(ceil_div(K, (int64_t)128), (int64_t)32); }
+int64_t few_chunks(int64_t K) { return ceil_div(ceil_div(K, (int64_t)128), (int64_t)32); }
 FewPlan few_plan(bool up, int64_t pairs, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, bool zeros) {
   FewPlan p{};
   const int64_t all = ceil_div(K, (int64_t)128), n_tiles = N / (up ? 8 : 16);
   const int64_t experts = pairs < E ? pairs : E;
-  if (pairs > kFewPairs || pairs > experts * 8 || K > 65536) return p;
-  p.chunks = up ? 1 : (int)down_chunks(pairs, K);
+  if (pairs > kFewPairs || K > 65536) return p;
+  p.chunks = up ? 1 : (int)few_chunks(K);
   const int64_t blocks = ceil_div(all, (int64_t)p.chunks);
   p.chunks = (int)ceil_div(all, blocks);
   p.blocks = (int)blocks;
@@ -611,32 +733,91 @@ template <bool UP>
 int run_few(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, const FewPlan& p, hipStream_t st) {
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32;
-  const int flags = (p.by_pair ? kFewByPair : 0) | (p.by_pair && pairs == x.top_k ? kFewOneToken : 0) | (whole ? kFewFold : 0) |
-                    (aligned16(x.scales) && aligned16(x.zeros) ? kFewWide : 0);
+  const int flags = (p.by_pair ? kFewByPair : 0) | (p.by_pair && pairs == x.top_k ? kFewOneToken : 0);
   const FewArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, (const int32_t*)ids, x.out, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
                   units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, p.n_groups, (int)p.units,
                   (uint32_t)(p.blocks | p.pieces << 16), (uint32_t)(p.waves | p.splits << 8 | p.row_cap << 16 | flags << 24), p.per_wave};
-#define TLQ_FEW(T) (x.zeros ? launch_few<T, UP, true>(what, a, p, st) : launch_few<T, UP, false>(what, a, p, st))
+#define TLQ_FEW(T) (x.zeros || !whole ? launch_few<T, UP, true>(what, a, p, st) : launch_few<T, UP, false>(what, a, p, st))
   return dtype == TLQ_F16 ? TLQ_FEW(half_t) : TLQ_FEW(bf16_t);
 #undef TLQ_FEW
 }
 
-template <bool UP>
-int run_experts(const char* what, ExpertArgs a, const void* ids, int64_t pairs, int dtype, void* ws, hipStream_t st) {
-  const FewPlan few = few_plan(UP, pairs, a.E, a.top_k, a.N, a.K, a.group, a.zeros != nullptr);
-  if (few.ok) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
-  const PlanPtrs p = plan_at(ws, a.E);
-  a.begin = p.begin, a.tiles = p.tiles, a.order = p.order;
-  moe_plan_kernel<<<a.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, p.begin, p.tiles, p.order, (int)pairs, a.E, kRows);
-  if (!check_launch(what, "moe_plan_kernel")) return 1;
-  a.n_blocks = (int)ceil_div((int64_t)a.N, (int64_t)kOuts);
-  const int64_t grid = most_tiles(pairs, a.E, kRows) * a.n_blocks;
+template <typename T, bool UP, bool ZEROS, int MAXMT, int NT, int KSB>
+int launch_tiles(const char* what, const TileArgs& a, int64_t grid, hipStream_t st) {
+  auto kern = moe_tile_kernel<T, UP, ZEROS, MAXMT, NT, KSB>;
+  constexpr int lds = TileCfg<MAXMT, NT, KSB>::lds(ZEROS);
+  static bool attr_set = false;
+  if (!attr_set) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    TLQ_REQUIRE(e == hipSuccess, "%s: cannot reserve LDS: %s", what, hipGetErrorString(e));
+    attr_set = true;
+  }
+  kern<<<(unsigned)grid, 256, (size_t)lds, st>>>(a);
+  return check_launch(what, "moe_tile_kernel") ? 0 : 1;
+}
+
+// Work-groups of moe_tile_kernel side by side, and the parts that K of the down product is cut into where there are too few of them
+// to keep four on every CU (eight experts of 4096 x 14336 and 16 tokens: 106 us whole).  `tiles`: about how many tiles of pairs there are.
+template <bool UP, int NT>
+int64_t tile_groups(int64_t N) {
+  return ceil_div(N, (int64_t)(4 * NT * (UP ? 8 : 16)));
+}
+int64_t tile_chunks(int64_t tiles, int64_t n_groups, int64_t K) {
+  int64_t chunks = 1;
+  while (chunks < 8 && tiles * n_groups * chunks * 2 <= 1024 && K / (chunks * 2) >= 1024) chunks *= 2;
+  return chunks;
+}
+int64_t about_tiles(int64_t pairs, int64_t E, int64_t rows) { return (pairs < E ? pairs : E) + pairs / rows; }
+
+// The plan, then the products on tiles of 16 MAXMT pairs.  chunks: the parts of K of the down product.
+template <bool UP, int MAXMT, int NT, int KSB>
+int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st) {
+  constexpr int rows = 16 * MAXMT;
+  static_assert(rows >= kLeastRows, "the workspace holds the tiles");
+  int32_t* const order = (int32_t*)ws;
+  PlanTile* const tiles = (PlanTile*)((uint8_t*)ws + order_bytes(pairs));
+  const int64_t all_tiles = most_tiles(pairs, x.E, rows), n_groups = tile_groups<UP, NT>(x.N), steps = ceil_div((int64_t)x.K, (int64_t)(KSB * 128));
+  const int64_t chunk_steps = UP ? steps : ceil_div(steps, tile_chunks(about_tiles(pairs, x.E, rows), n_groups, x.K));
+  *chunks = ceil_div(steps, chunk_steps);
+  const int64_t grid = all_tiles * n_groups * *chunks;
   TLQ_REQUIRE(grid < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
-  if (dtype == TLQ_F16)
-    moe_w4a16_kernel<half_t, UP><<<(unsigned)grid, 256, 0, st>>>(a);
-  else
-    moe_w4a16_kernel<bf16_t, UP><<<(unsigned)grid, 256, 0, st>>>(a);
-  return check_launch(what, "moe_w4a16_kernel") ? 0 : 1;
+  moe_plan_kernel<<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, tiles, order, (int)pairs, x.E, rows, (int)all_tiles);
+  if (!check_launch(what, "moe_plan_kernel")) return 1;
+  const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
+  const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
+  const TileArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, x.out, tiles, order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
+                   units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};
+#define TLQ_TILES(T) (x.zeros || !whole ? launch_tiles<T, UP, true, MAXMT, NT, KSB>(what, a, grid, st) : launch_tiles<T, UP, false, MAXMT, NT, KSB>(what, a, grid, st))
+  return dtype == TLQ_F16 ? TLQ_TILES(half_t) : TLQ_TILES(bf16_t);
+#undef TLQ_TILES
+}
+
+// Which kernel: the one without a plan while an expert has two pairs at most on average and the tiles' work-groups would not fill the machine
+// (MoE layers of 8 to 256 experts, bf16, group 128, zero points, this kernel / tiles of 32: 4 tokens on 6 of 64 experts of 1408 x 2048 21.3 / 24.2 us, 8 tokens
+// 30.3 / 30.0; 1 token on 2 of 8 experts, down, 4096 x 14336 25.6 / 95.8; 16 tokens on 4 of 16 experts of 2048 x 2048 28.3 / 24.5).
+bool few_pairs(bool up, int64_t pairs, int64_t E, int64_t N) {
+  const int64_t experts = pairs < E ? pairs : E, groups = up ? tile_groups<true, 2>(N) : tile_groups<false, 2>(N);
+  return pairs <= 2 * experts && experts * groups <= 1024;
+}
+constexpr int64_t kSmallTiles = 12;  // pairs of an expert on average from which tiles of 64 pairs are taken
+
+template <bool UP>
+int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st) {
+  if (few_pairs(UP, pairs, a.E, a.N)) {
+    const FewPlan few = few_plan(UP, pairs, a.E, a.top_k, a.N, a.K, a.group, a.zeros != nullptr);
+    *chunks = few.chunks;
+    if (few.ok) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
+  }
+  if (pairs / a.E < kSmallTiles) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
+  return run_tiles<UP, 4, 4, 1>(what, a, ids, pairs, dtype, ws, chunks, st);
+}
+
+// the most that any of them cuts K of the down product into
+int64_t down_chunks(int64_t pairs, int64_t E, int64_t N, int64_t K) {
+  int64_t c = few_pairs(false, pairs, E, N) ? few_chunks(K) : 1;
+  const int64_t small = tile_chunks(about_tiles(pairs, E, 32), tile_groups<false, 2>(N), K), large = tile_chunks(about_tiles(pairs, E, 64), tile_groups<false, 4>(N), K);
+  c = c > small ? c : small;
+  return c > large ? c : large;
 }
 
 }  // namespace
@@ -652,7 +833,7 @@ extern "C" int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t
 extern "C" int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
   const int64_t plan = tlq_moe_gate_up_workspace_bytes(M, E, top_k);
   if (plan == 0 || N < 1 || N >= ((int64_t)1 << 24) || K < 1 || K >= ((int64_t)1 << 24)) return 0;
-  return plan + down_chunks(M * top_k, K) * M * top_k * N * 4;
+  return plan + down_chunks(M * top_k, E, N, K) * M * top_k * N * 4;
 }
 
 extern "C" int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void* w_packed, const void* scales, const void* zeros, void* H,
@@ -662,13 +843,14 @@ extern "C" int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void*
   if (check_experts(what, M, E, top_k, N, K, group, dtype)) return 1;
   if (M == 0) return 0;
   TLQ_REQUIRE(X && ids && w_packed && H, "%s: null pointer", what);
-  TLQ_REQUIRE(aligned16(X) && aligned16(w_packed) && aligned16(H) && ((uintptr_t)ids & 3) == 0 && (((uintptr_t)scales | (uintptr_t)zeros) & 1) == 0,
-              "%s: X, w_packed and H must be 16-byte aligned, the others to their type", what);
+  TLQ_REQUIRE(aligned16(X) && aligned16(w_packed) && aligned16(H) && aligned16(scales) && aligned16(zeros) && ((uintptr_t)ids & 3) == 0,
+              "%s: X, w_packed, scales, zeros and H must be 16-byte aligned, ids to their type", what);
   const int64_t want = tlq_moe_gate_up_workspace_bytes(M, E, top_k);
   TLQ_REQUIRE(workspace && workspace_bytes >= want && aligned16(workspace), "%s: a 16-byte aligned workspace of %lld bytes is wanted (got %lld)", what,
               (long long)want, (long long)(workspace ? workspace_bytes : 0));
-  ExpertArgs a{X, (const uint8_t*)w_packed, scales, zeros, nullptr, H, nullptr, nullptr, nullptr, (int)E, (int)top_k, (int)N, (int)K, (int)group, 0, zero_scalar};
-  return run_experts<true>(what, a, ids, M * top_k, dtype, workspace, (hipStream_t)stream);
+  ExpertArgs a{X, (const uint8_t*)w_packed, scales, zeros, nullptr, H, (int)E, (int)top_k, (int)N, (int)K, (int)group, zero_scalar};
+  int64_t chunks = 1;
+  return run_experts<true>(what, a, ids, M * top_k, dtype, workspace, &chunks, (hipStream_t)stream);
 }
 
 extern "C" int tlq_moe_down_w4a16(const void* H, const void* ids, const void* weights, const void* w_packed, const void* scales,
@@ -679,20 +861,20 @@ extern "C" int tlq_moe_down_w4a16(const void* H, const void* ids, const void* we
   TLQ_REQUIRE(out_dtype == TLQ_F16 || out_dtype == TLQ_BF16 || out_dtype == TLQ_F32, "%s: out_dtype must be float16, bfloat16 or float32 (got %d)", what, out_dtype);
   if (M == 0) return 0;
   TLQ_REQUIRE(H && ids && weights && w_packed && Y, "%s: null pointer", what);
-  TLQ_REQUIRE(aligned16(H) && aligned16(w_packed) && aligned16(Y) && (((uintptr_t)ids | (uintptr_t)weights) & 3) == 0 && (((uintptr_t)scales | (uintptr_t)zeros) & 1) == 0,
-              "%s: H, w_packed and Y must be 16-byte aligned, the others to their type", what);
+  TLQ_REQUIRE(aligned16(H) && aligned16(w_packed) && aligned16(Y) && aligned16(scales) && aligned16(zeros) && (((uintptr_t)ids | (uintptr_t)weights) & 3) == 0,
+              "%s: H, w_packed, scales, zeros and Y must be 16-byte aligned, ids and weights to their type", what);
   const int64_t want = tlq_moe_down_workspace_bytes(M, E, top_k, N, K);
   TLQ_REQUIRE(workspace && workspace_bytes >= want && aligned16(workspace), "%s: a 16-byte aligned workspace of %lld bytes is wanted (got %lld)", what,
               (long long)want, (long long)(workspace ? workspace_bytes : 0));
   const int64_t pairs = M * top_k;
   float* const rows = (float*)((uint8_t*)workspace + plan_bytes(E, pairs));
-  ExpertArgs a{H, (const uint8_t*)w_packed, scales, zeros, (const float*)weights, rows, nullptr, nullptr, nullptr, (int)E, (int)top_k, (int)N, (int)K, (int)group, 0, zero_scalar};
+  ExpertArgs a{H, (const uint8_t*)w_packed, scales, zeros, (const float*)weights, rows, (int)E, (int)top_k, (int)N, (int)K, (int)group, zero_scalar};
   hipStream_t st = (hipStream_t)stream;
-  if (run_experts<false>(what, a, ids, pairs, in_dtype, workspace, st)) return 1;
+  int64_t chunks = 1;
+  if (run_experts<false>(what, a, ids, pairs, in_dtype, workspace, &chunks, st)) return 1;
   const int64_t n_groups = ceil_div(N, (int64_t)1024);
-  const FewPlan few = few_plan(false, pairs, E, top_k, N, K, group, zeros != nullptr);
   TLQ_REQUIRE(M * n_groups < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)(M * n_groups));
   moe_combine_kernel<<<(unsigned)(M * n_groups), 256, 0, st>>>(rows, (const int32_t*)ids, Y, (int)N, (int)n_groups, (int)top_k, (int)E, out_dtype,
-                                                                 few.ok ? few.chunks : 1, pairs * N);
+                                                                 (int)chunks, pairs * N);
   return check_launch(what, "moe_combine_kernel") ? 0 : 1;
 }
