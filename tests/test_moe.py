@@ -153,6 +153,12 @@ SHAPES = [
     (12, 4, 2, 48, 2208, 96, "bfloat16", "frac", "holes"),
     (20, 4, 2, 32, 2208, 736, "float16", 8, "spread"),
     (64, 2, 2, 16, 8192, 64, "bfloat16", 3.25, "one"),
+    # (tiles of 256 pairs, and what is left of an expert's pairs)
+    (700, 3, 2, 272, 384, 64, "bfloat16", "frac", "holes"),
+    (1100, 2, 1, 144, 128, 32, "float16", None, "one"),
+    (515, 4, 2, 160, 256, 128, "bfloat16", 8, "spread"),
+    (641, 2, 1, 48, 512, 256, "float16", "int", "spread"),
+    (450, 2, 2, 16, 640, 128, "float16", 7.5, "twice"),
 ]
 
 

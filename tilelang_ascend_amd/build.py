@@ -59,6 +59,7 @@ SOURCES = [
     "gemm_w4a16_noalloc.hip",
     "moe_route.hip",
     "moe_w4a16.hip",
+    "moe_w4a16_panel.hip",
 ]
 # packed-fp32 VALU forms are disabled on purpose (some have produced silent wrong results on
 # this hardware pool); hipcc's host pass warns that it does not know the feature.

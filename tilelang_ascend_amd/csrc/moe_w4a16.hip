@@ -7,10 +7,11 @@
 // Pairs are sorted by expert first (moe_plan_kernel: counts, where each expert's pairs begin, the pairs in order -- a pair keeps
 // its place among those of its expert, so nothing depends on timing), then every expert's rows are cut into tiles of activation
 // rows, which work-groups find by their number.
+#include <stdlib.h>
+
 #include <type_traits>
 
-#include "expand8.h"
-#include "gemm_core.h"
+#include "moe.h"
 
 namespace tlq {
 namespace {
@@ -18,81 +19,110 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxExperts = 1024;
 
-// What a call works out of its ids, in the workspace:
-//   order[P]      pairs by expert
-//   tiles[]       {expert, first entry of `order`, pairs} of every tile of at most `rows` pairs; tiles behind the last one: no pairs
-struct PlanTile {
-  int32_t expert, first, pairs, unused;
-};
-// tiles of `rows` pairs that E experts and the pairs without one can need at most
+// The plan in the workspace: totals, the pairs by expert, tiles of few pairs, tiles of 256 pairs.
+// Tiles of `rows` pairs that E experts and the pairs without one can need at most.
 inline int64_t most_tiles(int64_t pairs, int64_t E, int64_t rows) {
   const int64_t some = pairs < E + 1 ? pairs : E + 1;
   return some + (pairs - some) / rows;
 }
-constexpr int kLeastRows = 16;  // of a tile
-inline int64_t order_bytes(int64_t pairs) { return (pairs * 4 + 255) / 256 * 256; }
-inline int64_t plan_bytes(int64_t E, int64_t pairs) { return order_bytes(pairs) + (most_tiles(pairs, E, kLeastRows) * 16 + 255) / 256 * 256; }
+constexpr int kLeastRows = 32;  // of a tile of few pairs
+// With tiles of 256 pairs (`large`): an expert's last tile is one of them if it has more than 128 pairs, so that it has 129 at least, and
+// tiles of few pairs take what is left.
+__host__ __device__ inline int64_t large_tiles(int64_t pairs) { return (pairs + kLargeRows / 2 - 1) / kLargeRows; }
+inline int64_t most_large_tiles(int64_t pairs) { return pairs / (kLargeRows / 2 + 1); }
+inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+inline int64_t plan_bytes(int64_t E, int64_t pairs) {
+  return 256 + align256(pairs * 4) + align256(most_tiles(pairs, E, kLeastRows) * 16) + align256(most_large_tiles(pairs) * 16);
+}
+struct PlanPtrs {
+  int32_t *totals, *order;
+  PlanTile *small, *large;
+};
+inline PlanPtrs plan_at(void* ws, int64_t E, int64_t pairs) {
+  uint8_t* const p = (uint8_t*)ws + 256;
+  uint8_t* const small = p + align256(pairs * 4);
+  return {(int32_t*)ws, (int32_t*)p, (PlanTile*)small, (PlanTile*)(small + align256(most_tiles(pairs, E, kLeastRows) * 16))};
+}
 
 // One work-group per expert, and one more for the pairs without one: each counts all pairs (LDS histogram; whole numbers, so the
-// order of the atomic adds does not matter) and writes down its own.
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, PlanTile* __restrict__ tiles,
-                                                               int32_t* __restrict__ order, int pairs, int E, int rows, int all_tiles) {
+// order of the atomic adds does not matter) and writes down its own.  A wavefront takes a run of pairs, so that a pair's place is that of its
+// wavefront, its step and its lane; eight steps' ids are asked for at once (65536 pairs of 64 experts: one by one 40 us).
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ totals,
+                                                               int32_t* __restrict__ order, PlanTile* __restrict__ small,
+                                                               PlanTile* __restrict__ large, int pairs, int E, int rows, int with_large) {
   __shared__ int32_t count[kMaxExperts + 1];
-  __shared__ int32_t part[kPlanThreads / 64][2];
+  __shared__ int32_t part[kPlanThreads / 64][3];
   __shared__ int32_t of_wave[kPlanThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = blockIdx.x;
-  constexpr int waves = kPlanThreads / 64;
+  constexpr int waves = kPlanThreads / 64, AHEAD = 8;
   for (int i = tid; i <= E; i += kPlanThreads) count[i] = 0;
   __syncthreads();
-  // every wavefront takes a run of pairs, so that a pair's place is that of its wavefront, its step and its lane
   const int steps = (pairs + kPlanThreads - 1) / kPlanThreads;
   const int first = wave * steps * 64;
-  int mine = 0;
-  for (int s = 0; s < steps; ++s) {
-    const int p = first + s * 64 + lane;
-    if (p < pairs) {
-      const int id = ids[p];
-      const int at = (uint32_t)id < (uint32_t)E ? id : E;
-      atomicAdd(&count[at], 1);
-      mine += at == e;
+  // f(the pair, its expert or E, whether there is one) for every step of this wavefront
+  auto each = [&](auto&& f) __attribute__((always_inline)) {
+    for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+      int id[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int p = first + (s0 + i) * 64 + lane;
+        id[i] = s0 + i < steps && p < pairs ? ids[p] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int p = first + (s0 + i) * 64 + lane;
+        f(p, (uint32_t)id[i] < (uint32_t)E ? id[i] : E, s0 + i < steps && p < pairs);
+      }
     }
-  }
-  // pairs of this expert in the wavefront's run
-  for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
+  };
+  int mine = 0;  // pairs of this expert in the wavefront's run
+  each([&](int, int at, bool there) {
+    if (there) atomicAdd(&count[at], 1);
+    mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && at == e));
+  });
   if (lane == 0) of_wave[wave] = mine;
   __syncthreads();
+  auto large_of = [&](int i) { return with_large && i < E ? (int)large_tiles(count[i]) : 0; };
+  auto small_of = [&](int i, int l) {
+    const int left = count[i] - l * kLargeRows;
+    return left > 0 ? (left + rows - 1) / rows : 0;
+  };
   // pairs and tiles of the experts before this one
-  int before = 0, tiles_before = 0;
-  for (int i = tid; i < e; i += kPlanThreads) before += count[i], tiles_before += (count[i] + rows - 1) / rows;
-  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o), tiles_before += __shfl_xor(tiles_before, o);
-  if (lane == 0) part[wave][0] = before, part[wave][1] = tiles_before;
+  int before[3] = {0, 0, 0};
+  for (int i = tid; i < e; i += kPlanThreads) {
+    const int l = large_of(i);
+    before[0] += count[i], before[1] += small_of(i, l), before[2] += l;
+  }
+#pragma unroll
+  for (int c = 0; c < 3; ++c) {
+    for (int o = 32; o > 0; o >>= 1) before[c] += __shfl_xor(before[c], o);
+    if (lane == 0) part[wave][c] = before[c];
+    before[c] = 0;
+  }
   __syncthreads();
-  before = tiles_before = 0;
   int at = 0;
 #pragma unroll
   for (int i = 0; i < waves; ++i) {
-    before += part[i][0], tiles_before += part[i][1];
+#pragma unroll
+    for (int c = 0; c < 3; ++c) before[c] += part[i][c];
     at += i < wave ? of_wave[i] : 0;
   }
-  const int my_count = count[e], my_tiles = (my_count + rows - 1) / rows;
-  for (int i = tid; i < my_tiles; i += kPlanThreads) {
-    const int left = my_count - i * rows;
-    tiles[tiles_before + i] = PlanTile{e, before + i * rows, left < rows ? left : rows, 0};
+  const int my_count = count[e], my_large = large_of(e), my_small = small_of(e, my_large);
+  for (int i = tid; i < my_large; i += kPlanThreads) {
+    const int left = my_count - i * kLargeRows;
+    large[before[2] + i] = PlanTile{e, before[0] + i * kLargeRows, left < kLargeRows ? left : kLargeRows, 0};
   }
-  if (e == E)
-    for (int i = tiles_before + my_tiles + tid; i < all_tiles; i += kPlanThreads) tiles[i] = PlanTile{0, 0, 0, 0};
-  at += before;
-  for (int s = 0; s < steps; ++s) {
-    const int p = first + s * 64 + lane;
-    bool hit = false;
-    if (p < pairs) {
-      const int id = ids[p];
-      hit = ((uint32_t)id < (uint32_t)E ? id : E) == e;
-    }
-    const uint64_t hits = __builtin_amdgcn_ballot_w64(hit);
-    if (hit) order[at + __builtin_popcountll(hits & (((uint64_t)1 << lane) - 1))] = p;
+  for (int i = tid; i < my_small; i += kPlanThreads) {
+    const int from = my_large * kLargeRows + i * rows, left = my_count - from;
+    small[before[1] + i] = PlanTile{e, before[0] + from, left < rows ? left : rows, 0};
+  }
+  if (e == E && tid == 0) totals[0] = before[1] + my_small, totals[1] = before[2];
+  at += before[0];
+  each([&](int p, int expert, bool there) {
+    const uint64_t hits = __builtin_amdgcn_ballot_w64(there && expert == e);
+    if (there && expert == e) order[at + __builtin_popcountll(hits & (((uint64_t)1 << lane) - 1))] = p;
     at += __builtin_popcountll(hits);
-  }
+  });
 }
 
 template <typename T>
@@ -106,20 +136,6 @@ struct MmaOf<bf16_t> {
   typedef MmaBF16 type;
 };
 
-struct ExpertArgs {
-  const void* X;         // activations: [M, K] (gate / up) or [pairs, K] (down)
-  const uint8_t* Wp;     // [E, rows of an expert, K / 2]
-  const void* scales;    // [E, rows of an expert, K / group] or null
-  const void* zeros;     // the same, or null
-  const float* weights;  // down: [pairs]
-  void* out;             // gate / up: h [pairs, N]; down: fp32 [pairs, N]
-  int E, top_k, N, K, group;
-  float zero_scalar;
-};
-
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
-__device__ __forceinline__ bool small_integer(float z) { return z == __builtin_rintf(z) && z >= -256.0f && z <= 256.0f; }
-
 // Global -> LDS without registers: 16 or 4 bytes per lane, lane l to lds + 16 l or 4 l (lanes that are switched off: nothing).
 __device__ __forceinline__ void direct16(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
@@ -129,24 +145,6 @@ __device__ __forceinline__ void direct16_at(uint32_t off, const uint8_t* base, u
 }
 __device__ __forceinline__ void direct4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory");
-}
-
-// Four neighbouring sums of one pair: gate / up: outputs n .. n + 3 from the gates in q = 0, 1 and their ups 32 lanes on; down: the weighted row.
-template <typename T, bool UP, typename Args>
-__device__ __forceinline__ void moe_store(const Args& a, const float4_t& sum, bool live, int pair, float weight, int n, int q, int chunk) {
-  if constexpr (UP) {
-    float4_t up;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) up[i] = __shfl_xor(sum[i], 32);
-    if (q < 2 && live) {
-      T o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = from_float<T>(silu(sum[i]) * up[i]);
-      *(uint2_t*)((T*)a.out + (int64_t)pair * a.N + n) = bitcast<uint2_t>(o);
-    }
-  } else if (live) {
-    *(float4_t*)((float*)a.out + ((int64_t)chunk * a.pairs + pair) * a.N + n) = sum * weight;
-  }
 }
 
 // ---- tiles of many pairs ----------------------------------------------------------------------------------------------------
@@ -166,7 +164,7 @@ struct TileArgs {
   const float* weights;
   void* out;
   const PlanTile* tiles;
-  const int32_t* order;
+  const int32_t* order;  // (how many tiles there are: at order[-64])
   int pairs, E, top_k, N, K, groups;
   uint32_t per_group;  // ceil(2^32 / (group / 32)), 0 for groups of 32
   float zero_scalar;
@@ -191,14 +189,16 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
   typedef __attribute__((address_space(3))) uint8_t* lptr_t;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q = lane >> 4;
-  // Work-groups of one tile's neighbours side by side on one XCD (numbers go to the XCDs in turn): they share its activation rows, and the
-  // tiles of an expert, which follow each other, its weights.
+  // Work-groups of a tile, and tiles of an expert, which follow each other, on one XCD (numbers go to the XCDs in turn): they share
+  // activation rows and weights.
   const int all_steps = (a.K + KSB * 128 - 1) / (KSB * 128), chunks = (all_steps + a.chunk_steps - 1) / a.chunk_steps;
-  const int part = (int)(blockIdx.x / (uint32_t)a.n_groups), group_no = (int)blockIdx.x - part * a.n_groups;
+  const int live = a.order[-64] * chunks * a.n_groups;
+  if ((int)blockIdx.x >= live) return;
+  const int no = addr::xcd_order(blockIdx.x, live);
+  const int part = (int)((uint32_t)no / (uint32_t)a.n_groups), group_no = no - part * a.n_groups;
   const int tile_no = part / chunks, chunk = part - tile_no * chunks;
   const PlanTile pt = a.tiles[tile_no];
   const int e = __builtin_amdgcn_readfirstlane(pt.expert), first = __builtin_amdgcn_readfirstlane(pt.first), rows = __builtin_amdgcn_readfirstlane(pt.pairs);
-  if (rows == 0) return;
   constexpr int OUTS = UP ? 8 : 16;
   const int n_tiles = a.N / OUTS, tile0 = group_no * Cfg::TILES;
   if (e == a.E) {  // pairs without an expert
@@ -771,21 +771,28 @@ int64_t about_tiles(int64_t pairs, int64_t E, int64_t rows) { return (pairs < E 
 
 // The plan, then the products on tiles of 16 MAXMT pairs.  chunks: the parts of K of the down product.
 template <bool UP, int MAXMT, int NT, int KSB>
-int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st) {
+int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st, bool large = false) {
   constexpr int rows = 16 * MAXMT;
   static_assert(rows >= kLeastRows, "the workspace holds the tiles");
-  int32_t* const order = (int32_t*)ws;
-  PlanTile* const tiles = (PlanTile*)((uint8_t*)ws + order_bytes(pairs));
-  const int64_t all_tiles = most_tiles(pairs, x.E, rows), n_groups = tile_groups<UP, NT>(x.N), steps = ceil_div((int64_t)x.K, (int64_t)(KSB * 128));
-  const int64_t chunk_steps = UP ? steps : ceil_div(steps, tile_chunks(about_tiles(pairs, x.E, rows), n_groups, x.K));
+  const PlanPtrs p = plan_at(ws, x.E, pairs);
+  // (beside tiles of 256 pairs an expert has two at most, and those of the pairs without one)
+  const int64_t beside = 2 * (int64_t)x.E + pairs / rows + 1;
+  int64_t all_tiles = most_tiles(pairs, x.E, rows);
+  if (large && beside < all_tiles) all_tiles = beside;
+  const int64_t n_groups = tile_groups<UP, NT>(x.N), steps = ceil_div((int64_t)x.K, (int64_t)(KSB * 128));
+  const int64_t chunk_steps = UP || large ? steps : ceil_div(steps, tile_chunks(about_tiles(pairs, x.E, rows), n_groups, x.K));
   *chunks = ceil_div(steps, chunk_steps);
   const int64_t grid = all_tiles * n_groups * *chunks;
   TLQ_REQUIRE(grid < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
-  moe_plan_kernel<<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, tiles, order, (int)pairs, x.E, rows, (int)all_tiles);
+  moe_plan_kernel<<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, large);
   if (!check_launch(what, "moe_plan_kernel")) return 1;
+  if (large && most_large_tiles(pairs) > 0) {
+    const Plan plan{p.order, p.small, p.large, p.totals};
+    if (moe_panel(what, x, plan, most_large_tiles(pairs), dtype, UP, st)) return 1;
+  }
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
-  const TileArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, x.out, tiles, order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
+  const TileArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
                    units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};
 #define TLQ_TILES(T) (x.zeros || !whole ? launch_tiles<T, UP, true, MAXMT, NT, KSB>(what, a, grid, st) : launch_tiles<T, UP, false, MAXMT, NT, KSB>(what, a, grid, st))
   return dtype == TLQ_F16 ? TLQ_TILES(half_t) : TLQ_TILES(bf16_t);
@@ -799,6 +806,7 @@ bool few_pairs(bool up, int64_t pairs, int64_t E, int64_t N) {
   const int64_t experts = pairs < E ? pairs : E, groups = up ? tile_groups<true, 2>(N) : tile_groups<false, 2>(N);
   return pairs <= 2 * experts && experts * groups <= 1024;
 }
+int g_large = getenv("MOE_LARGE") ? atoi(getenv("MOE_LARGE")) : 96;
 constexpr int64_t kSmallTiles = 12;  // pairs of an expert on average from which tiles of 64 pairs are taken
 
 template <bool UP>
@@ -809,7 +817,8 @@ int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t 
     if (few.ok) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
   }
   if (pairs / a.E < kSmallTiles) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
-  return run_tiles<UP, 4, 4, 1>(what, a, ids, pairs, dtype, ws, chunks, st);
+  const bool large = pairs / a.E >= g_large && moe_panel_takes(a, pairs, UP);
+  return run_tiles<UP, 4, 4, 1>(what, a, ids, pairs, dtype, ws, chunks, st, large);
 }
 
 // the most that any of them cuts K of the down product into
