@@ -28,11 +28,13 @@ struct ExpertArgs {
   float zero_scalar;
 };
 
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
+// (the reciprocal to an ulp; where the exponential overflows it is 0)
+__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 __device__ __forceinline__ bool small_integer(float z) { return z == __builtin_rintf(z) && z >= -256.0f && z <= 256.0f; }
 
 // Gate / up (up = true) or down product of the tiles of 256 pairs (moe_w4a16_panel.hip).
 bool moe_panel_takes(const ExpertArgs& a, int64_t pairs, bool up);
+int64_t moe_panel_groups(int64_t N, bool up);  // work-groups of a tile
 int moe_panel(const char* what, const ExpertArgs& a, const Plan& plan, int64_t most_tiles, int dtype, bool up, hipStream_t st);
 
 // Four neighbouring sums of one pair: gate / up: outputs n .. n + 3 from the gates in q = 0, 1 and their ups 32 lanes on; down: the weighted row.

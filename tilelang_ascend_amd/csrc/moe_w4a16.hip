@@ -7,8 +7,6 @@
 // Pairs are sorted by expert first (moe_plan_kernel: counts, where each expert's pairs begin, the pairs in order -- a pair keeps
 // its place among those of its expert, so nothing depends on timing), then every expert's rows are cut into tiles of activation
 // rows, which work-groups find by their number.
-#include <stdlib.h>
-
 #include <type_traits>
 
 #include "moe.h"
@@ -19,54 +17,79 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxExperts = 1024;
 
-// The plan in the workspace: totals, the pairs by expert, tiles of few pairs, tiles of 256 pairs.
-// Tiles of `rows` pairs that E experts and the pairs without one can need at most.
-inline int64_t most_tiles(int64_t pairs, int64_t E, int64_t rows) {
+// The plan in the workspace: how many tiles there are, the pairs by expert, tiles of few pairs, tiles of 256 pairs.  With tiles of 256 pairs
+// (with_large: the work-groups of one of them, 0: none) an expert's last tile is one of them if it has `from` pairs, and tiles of 64 pairs take
+// what is left otherwise.
+//   Up to kCompactPairs pairs the work-groups of the plan know the counts of all experts.  Tiles follow each other, and `from` is chosen for
+// the fewest rounds of work-groups (choose_from).  With more pairs a tile's place goes by the pairs before it alone -- tiles of `rows` pairs of
+// expert e begin at place (pairs before e) / rows + e, what is left beside large tiles at e --, which leaves at most one place an expert empty;
+// `from` is 65, and beside large tiles the pairs without an expert are cut into kNoneTiles tiles at most (places for all pairs in tiles of 64
+// would be work-groups that find nothing to do).
+constexpr int kCompactPairs = 4096, kNoneTiles = 64, kLargeFrom = 65;
+__host__ __device__ inline int large_tiles(int pairs, int from) { return pairs + kLargeRows <= from ? 0 : (pairs + kLargeRows - from) / kLargeRows; }
+struct PlanSizes {
+  int64_t small, large;  // places for tiles
+};
+inline PlanSizes plan_sizes(int64_t E, int64_t pairs, int64_t rows, bool large) {
   const int64_t some = pairs < E + 1 ? pairs : E + 1;
-  return some + (pairs - some) / rows;
+  PlanSizes z;
+  z.small = pairs > kCompactPairs ? pairs / rows + E + 1 : some + (pairs - some) / rows;
+  if (large && pairs > kCompactPairs) z.small = E + kNoneTiles;
+  z.large = !large ? 0 : pairs > kCompactPairs ? pairs / kLargeRows + E : pairs / kLargeFrom;
+  return z;
 }
-constexpr int kLeastRows = 32;  // of a tile of few pairs
-// With tiles of 256 pairs (`large`): an expert's last tile is one of them if it has more than 128 pairs, so that it has 129 at least, and
-// tiles of few pairs take what is left.
-__host__ __device__ inline int64_t large_tiles(int64_t pairs) { return (pairs + kLargeRows / 2 - 1) / kLargeRows; }
-inline int64_t most_large_tiles(int64_t pairs) { return pairs / (kLargeRows / 2 + 1); }
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-inline int64_t plan_bytes(int64_t E, int64_t pairs) {
-  return 256 + align256(pairs * 4) + align256(most_tiles(pairs, E, kLeastRows) * 16) + align256(most_large_tiles(pairs) * 16);
-}
 struct PlanPtrs {
   int32_t *totals, *order;
   PlanTile *small, *large;
 };
-inline PlanPtrs plan_at(void* ws, int64_t E, int64_t pairs) {
+inline PlanPtrs plan_at(void* ws, int64_t pairs, const PlanSizes& z) {
   uint8_t* const p = (uint8_t*)ws + 256;
   uint8_t* const small = p + align256(pairs * 4);
-  return {(int32_t*)ws, (int32_t*)p, (PlanTile*)small, (PlanTile*)(small + align256(most_tiles(pairs, E, kLeastRows) * 16))};
+  return {(int32_t*)ws, (int32_t*)p, (PlanTile*)small, (PlanTile*)(small + align256(z.small * 16))};
+}
+inline int64_t plan_bytes_of(int64_t E, int64_t pairs, int64_t rows, bool large) {
+  const PlanSizes z = plan_sizes(E, pairs, rows, large);
+  return 256 + align256(pairs * 4) + align256(z.small * 16) + align256(z.large * 16);
+}
+inline int64_t plan_bytes(int64_t E, int64_t pairs) {
+  const int64_t a = plan_bytes_of(E, pairs, 32, false), b = plan_bytes_of(E, pairs, 64, false), c = plan_bytes_of(E, pairs, 64, true);
+  return a > b ? (a > c ? a : c) : (b > c ? b : c);
 }
 
-// One work-group per expert, and one more for the pairs without one: each counts all pairs (LDS histogram; whole numbers, so the
-// order of the atomic adds does not matter) and writes down its own.  A wavefront takes a run of pairs, so that a pair's place is that of its
-// wavefront, its step and its lane; eight steps' ids are asked for at once (65536 pairs of 64 experts: one by one 40 us).
+// Candidates for `from`: 65, 129, 193, 257 (whole tiles only), and more pairs than there are (none).  A round of large tiles is 256 work-groups,
+// one a CU, one of tiles of 64 pairs 512, which take 5 / 8 of its time (gate / up, 16 experts of 2048 x 4096: 98 and 61 us).
+constexpr int kFromChoices = 5;
+__device__ __forceinline__ int from_choice(int i) { return i < 4 ? 64 * i + 65 : 1 << 24; }
+__device__ __forceinline__ int rounds_of(int large, int small, int groups) { return 8 * ((large * groups + 255) / 256) + 5 * ((small * groups + 511) / 512); }
+
+// One work-group per expert, and one more for the pairs without one: each looks at all pairs and writes down its own.  A wavefront takes
+// a run of pairs, so that a pair's place is that of its wavefront, its step and its lane; sixteen steps' ids are asked for at once (65536 pairs of 64
+// experts: one by one, with an LDS histogram of all experts, 44 us).
+template <bool COMPACT>
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ totals,
                                                                int32_t* __restrict__ order, PlanTile* __restrict__ small,
                                                                PlanTile* __restrict__ large, int pairs, int E, int rows, int with_large) {
-  __shared__ int32_t count[kMaxExperts + 1];
-  __shared__ int32_t part[kPlanThreads / 64][3];
-  __shared__ int32_t of_wave[kPlanThreads / 64];
+  constexpr int waves = kPlanThreads / 64, AHEAD = COMPACT ? kCompactPairs / kPlanThreads : 16;
+  __shared__ int32_t count[COMPACT ? kMaxExperts + 1 : 1];
+  __shared__ int32_t part[waves][4];
+  __shared__ int32_t tiles_of[kFromChoices][2];  // large and small tiles that each choice makes
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = blockIdx.x;
-  constexpr int waves = kPlanThreads / 64, AHEAD = 8;
-  for (int i = tid; i <= E; i += kPlanThreads) count[i] = 0;
-  __syncthreads();
+  if (COMPACT) {
+    for (int i = tid; i <= E; i += kPlanThreads) count[i] = 0;
+    if (tid < 2 * kFromChoices) tiles_of[tid >> 1][tid & 1] = 0;
+    __syncthreads();
+  }
   const int steps = (pairs + kPlanThreads - 1) / kPlanThreads;
   const int first = wave * steps * 64;
-  // f(the pair, its expert or E, whether there is one) for every step of this wavefront
+  // f(a pair, its expert or E, whether there is one) for every step of this wavefront
   auto each = [&](auto&& f) __attribute__((always_inline)) {
     for (int s0 = 0; s0 < steps; s0 += AHEAD) {
       int id[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int p = first + (s0 + i) * 64 + lane;
-        id[i] = s0 + i < steps && p < pairs ? ids[p] : -1;
+        id[i] = ids[s0 + i < steps && p < pairs ? p : 0];
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
@@ -75,50 +98,73 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
       }
     }
   };
-  int mine = 0;  // pairs of this expert in the wavefront's run
-  each([&](int, int at, bool there) {
-    if (there) atomicAdd(&count[at], 1);
-    mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && at == e));
+  int own = 0, fewer = 0;  // pairs of this expert, and of those before it, in the wavefront's run
+  each([&](int, int at, bool there) __attribute__((always_inline)) {
+    if (COMPACT) {
+      if (there) atomicAdd(&count[at], 1);  // (whole numbers: in any order)
+    } else {
+      fewer += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && at < e));
+    }
+    own += __builtin_popcountll(__builtin_amdgcn_ballot_w64(there && at == e));
   });
-  if (lane == 0) of_wave[wave] = mine;
-  __syncthreads();
-  auto large_of = [&](int i) { return with_large && i < E ? (int)large_tiles(count[i]) : 0; };
-  auto small_of = [&](int i, int l) {
-    const int left = count[i] - l * kLargeRows;
-    return left > 0 ? (left + rows - 1) / rows : 0;
-  };
-  // pairs and tiles of the experts before this one
-  int before[3] = {0, 0, 0};
-  for (int i = tid; i < e; i += kPlanThreads) {
-    const int l = large_of(i);
-    before[0] += count[i], before[1] += small_of(i, l), before[2] += l;
+  int small_before = 0, large_before = 0, from = kLargeFrom;
+  if (COMPACT) {
+    __syncthreads();
+    if (with_large) {  // (the same in every work-group)
+      for (int c = 0; c < kFromChoices; ++c) {
+        int l = 0, m = 0;
+        for (int i = tid; i < E; i += kPlanThreads) {
+          const int n = large_tiles(count[i], from_choice(c)), left = count[i] - n * kLargeRows;
+          l += n, m += left > 0 ? (left + rows - 1) / rows : 0;
+        }
+        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o), m += __shfl_xor(m, o);
+        if (lane == 0 && (l | m)) atomicAdd(&tiles_of[c][0], l), atomicAdd(&tiles_of[c][1], m);
+      }
+      __syncthreads();
+      int best = 0x7fffffff;
+      for (int c = 0; c < kFromChoices; ++c) {
+        const int rounds = rounds_of(tiles_of[c][0], tiles_of[c][1], with_large);
+        if (rounds < best) best = rounds, from = from_choice(c);
+      }
+    }
+    for (int i = tid; i < e; i += kPlanThreads) {
+      const int l = with_large ? large_tiles(count[i], from) : 0, left = count[i] - l * kLargeRows;
+      fewer += count[i], large_before += l, small_before += left > 0 ? (left + rows - 1) / rows : 0;
+    }
+    for (int o = 32; o > 0; o >>= 1) fewer += __shfl_xor(fewer, o), small_before += __shfl_xor(small_before, o), large_before += __shfl_xor(large_before, o);
   }
-#pragma unroll
-  for (int c = 0; c < 3; ++c) {
-    for (int o = 32; o > 0; o >>= 1) before[c] += __shfl_xor(before[c], o);
-    if (lane == 0) part[wave][c] = before[c];
-    before[c] = 0;
-  }
+  if (lane == 0) part[wave][0] = own, part[wave][1] = fewer, part[wave][2] = small_before, part[wave][3] = large_before;
   __syncthreads();
-  int at = 0;
+  int at = 0, mine = 0;
+  fewer = small_before = large_before = 0;
 #pragma unroll
   for (int i = 0; i < waves; ++i) {
-#pragma unroll
-    for (int c = 0; c < 3; ++c) before[c] += part[i][c];
-    at += i < wave ? of_wave[i] : 0;
+    at += i < wave ? part[i][0] : 0;
+    mine += part[i][0], fewer += part[i][1], small_before += part[i][2], large_before += part[i][3];
   }
-  const int my_count = count[e], my_large = large_of(e), my_small = small_of(e, my_large);
-  for (int i = tid; i < my_large; i += kPlanThreads) {
-    const int left = my_count - i * kLargeRows;
-    large[before[2] + i] = PlanTile{e, before[0] + i * kLargeRows, left < kLargeRows ? left : kLargeRows, 0};
+  const int my_large = with_large && e < E ? large_tiles(mine, from) : 0, left = mine - my_large * kLargeRows;
+  if (!COMPACT && with_large && e == E && rows < (pairs + kNoneTiles - 1) / kNoneTiles) rows = (pairs + kNoneTiles - 1) / kNoneTiles;
+  const int my_small = left > 0 ? (left + rows - 1) / rows : 0;
+  int small_end = small_before + my_small, large_end = large_before + my_large;
+  if (!COMPACT) {
+    small_before = with_large ? e : fewer / rows + e;
+    small_end = with_large ? (e < E ? e + 1 : E + my_small) : (fewer + mine) / rows + e + 1;
+    large_before = fewer / kLargeRows + e;
+    large_end = e < E ? (fewer + mine) / kLargeRows + e + 1 : large_before;
   }
-  for (int i = tid; i < my_small; i += kPlanThreads) {
-    const int from = my_large * kLargeRows + i * rows, left = my_count - from;
-    small[before[1] + i] = PlanTile{e, before[0] + from, left < rows ? left : rows, 0};
+  if (with_large) {
+    for (int i = tid; i < large_end - large_before; i += kPlanThreads) {
+      const int at = i * kLargeRows, n = i < my_large ? (mine - at < kLargeRows ? mine - at : kLargeRows) : 0;
+      large[large_before + i] = PlanTile{e, fewer + at, n, 0};
+    }
   }
-  if (e == E && tid == 0) totals[0] = before[1] + my_small, totals[1] = before[2];
-  at += before[0];
-  each([&](int p, int expert, bool there) {
+  for (int i = tid; i < small_end - small_before; i += kPlanThreads) {
+    const int at = my_large * kLargeRows + i * rows, n = i < my_small ? (mine - at < rows ? mine - at : rows) : 0;
+    small[small_before + i] = PlanTile{e, fewer + at, n, 0};
+  }
+  if (e == E && tid == 0) totals[0] = small_end, totals[1] = large_end;
+  at += fewer;
+  each([&](int p, int expert, bool there) __attribute__((always_inline)) {
     const uint64_t hits = __builtin_amdgcn_ballot_w64(there && expert == e);
     if (there && expert == e) order[at + __builtin_popcountll(hits & (((uint64_t)1 << lane) - 1))] = p;
     at += __builtin_popcountll(hits);
@@ -154,7 +200,7 @@ __device__ __forceinline__ void direct4(const void* src, uint32_t lds) {
 // of each block of row r16, at MFMA k-step j the eight of word 4 q + j --, are expanded there and multiplied with all rows: a weight
 // is expanded once per 16 MAXMT pairs, an activation operand read once per NT tiles.  One barrier a step.
 //   Scales and zero points come through LDS in windows of eight groups (whole steps: 8 groups are 256 (group / 32) values), loaded a window
-// ahead as the two 16-byte pieces of a row that hold them.  ANY: zero points that need not be small integers, which are folded into the
+// ahead as the 16-byte pieces of a row that hold them (two, unless rows are whole pieces).  ANY: zero points that need not be small integers, which are folded into the
 // unpacking's bias (a tensor, looked at block by block, or such a scalar).
 struct TileArgs {
   const void* X;
@@ -176,10 +222,10 @@ struct TileArgs {
 template <int MAXMT, int NT, int KSB>
 struct TileCfg {
   static constexpr int ROWS = 16 * MAXMT, ROW_BYTES = KSB * 256, ACT = ROWS * ROW_BYTES;
-  static constexpr int TILES = 4 * NT, WINDOW = TILES * 16 * 32;          // scales of a window: 32 bytes a row
+  static constexpr int TILES = 4 * NT, WINDOW = TILES * 16 * 16;          // scales of a window: a piece of every row, or two
   static constexpr int RPI = 1024 / ROW_BYTES, LOADS = ROWS / RPI / 4;    // rows of a load instruction, loads of a wavefront and step
   static_assert(ROWS % (RPI * 4) == 0, "the rows split over the wavefronts");
-  static constexpr int lds(bool zeros) { return 2 * ACT + 2 * WINDOW * (zeros ? 2 : 1) + ROWS * 8; }
+  static constexpr int lds(int pieces, bool zeros) { return 2 * ACT + 2 * WINDOW * pieces * (zeros ? 2 : 1); }
 };
 
 template <typename T, bool UP, bool ANY, int MAXMT, int NT, int KSB>
@@ -199,6 +245,7 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
   const int tile_no = part / chunks, chunk = part - tile_no * chunks;
   const PlanTile pt = a.tiles[tile_no];
   const int e = __builtin_amdgcn_readfirstlane(pt.expert), first = __builtin_amdgcn_readfirstlane(pt.first), rows = __builtin_amdgcn_readfirstlane(pt.pairs);
+  if (rows == 0) return;
   constexpr int OUTS = UP ? 8 : 16;
   const int n_tiles = a.N / OUTS, tile0 = group_no * Cfg::TILES;
   if (e == a.E) {  // pairs without an expert
@@ -212,17 +259,11 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
     }
     return;
   }
+  const int pieces = a.groups % 8 == 0 ? 1 : 2, window_bytes = Cfg::WINDOW * pieces;
   uint8_t* const sc = smem + 2 * Cfg::ACT;
-  uint8_t* const zp = sc + 2 * Cfg::WINDOW;
-  int32_t* const list = (int32_t*)(zp + (ANY ? 2 * Cfg::WINDOW : 0));
-  float* const row_weight = (float*)(list + Cfg::ROWS);
+  uint8_t* const zp = sc + 2 * window_bytes;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)smem);
-  if (tid < Cfg::ROWS) {
-    const int pair = a.order[first + (tid < rows ? tid : rows - 1)];
-    list[tid] = pair;
-    if (!UP) row_weight[tid] = a.weights[pair];
-  }
-  __syncthreads();
+  const int32_t* const mine = a.order + first;
 
   // Activation rows: lane l of load i of a wavefront brings a 16-byte piece of row (4 i + wave) RPI + l / (64 / RPI); its place in the row is
   // swapped with its neighbours' by the row (xor), so that eight rows' operand reads meet every bank once.
@@ -232,7 +273,7 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
   static_assert(4 * Cfg::RPI % 8 == 0, "the same place in every load's rows");
 #pragma unroll
   for (int i = 0; i < Cfg::LOADS; ++i) {
-    const int pair = list[(4 * i + wave) * Cfg::RPI + lane / LPR];
+    const int r = (4 * i + wave) * Cfg::RPI + lane / LPR, pair = mine[r < rows ? r : rows - 1];
     act_src[i] = (const uint8_t*)((const T*)a.X + (int64_t)(UP ? pair / a.top_k : pair) * a.K + act_k);
   }
   const int s_begin = chunk * a.chunk_steps, s_end = s_begin + a.chunk_steps < all_steps ? s_begin + a.chunk_steps : all_steps;
@@ -257,6 +298,8 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
 #pragma unroll
   for (int t = 0; t < NT; ++t) w_off[t] = (uint32_t)((weight_row(wave * NT + t, r16) - (int64_t)e * (UP ? 2 : 1) * a.N) * (a.K / 2)) + q * 16;
   const int w_last = a.K / 2 - 16 - q * 16;
+  // (global, not flat: a flat load counts as an LDS access too, and the operand reads would wait for it)
+  typedef __attribute__((address_space(1))) const uint4_t* global16_t;
   uint4_t next[KSB][NT];
   auto load_weights = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
@@ -264,7 +307,7 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
       const int at = (s * KSB + b) * 64;
       const uint32_t off = (uint32_t)(at < w_last ? at : w_last);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) next[b][t] = *(const uint4_t*)(w_base + (w_off[t] + off));
+      for (int t = 0; t < NT; ++t) next[b][t] = *(global16_t)(uintptr_t)(w_base + (w_off[t] + off));
     }
   };
   // scales of window v: pieces (row * groups) / 8 + v and the next one of every row (the tensors' sizes are multiples of 16 bytes, so that
@@ -273,28 +316,29 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
   const int window = a.window;
   const int64_t sc_e = (int64_t)e * (UP ? 2 : 1) * a.N * a.groups;  // the expert's first value: a multiple of eight
   const uint32_t sc_last = (uint32_t)((UP ? 2 : 1) * a.N * a.groups / 8 - 1) * 16;
-  constexpr int SC_LOADS = Cfg::TILES * 32 / 256;
+  constexpr int SC_LOADS = Cfg::TILES * 32 / 256;  // (with two pieces)
   uint32_t sc_off[SC_LOADS];
 #pragma unroll
   for (int i = 0; i < SC_LOADS; ++i) {
-    const int c = (i * 4 + wave) * 64 + lane, r = c >> 1;
-    sc_off[i] = (uint32_t)((weight_row(r >> 4, r & 15) * a.groups - sc_e) / 8 + (c & 1)) * 16;
+    const int c = (i * 4 + wave) * 64 + lane, r = c >> (pieces - 1);
+    sc_off[i] = (uint32_t)((weight_row(r >> 4, r & 15) * a.groups - sc_e) / 8 + (pieces == 2 ? c & 1 : 0)) * 16;
   }
   const uint8_t* const sc_base = uniform_ptr((const uint8_t*)((const T*)a.scales + (a.scales ? sc_e : 0)));
   const uint8_t* const zp_base = uniform_ptr((const uint8_t*)((const T*)a.zeros + (a.zeros ? sc_e : 0)));
   auto load_scales = [&](int v) __attribute__((always_inline)) {
-    const uint32_t buf = lds0 + 2 * Cfg::ACT + (uint32_t)((v & 1) * Cfg::WINDOW);
+    const uint32_t buf = lds0 + 2 * Cfg::ACT + (uint32_t)((v & 1) * window_bytes);
 #pragma unroll
     for (int i = 0; i < SC_LOADS; ++i) {
+      if ((i * 4 + wave) * 1024 >= window_bytes) break;  // (uniform)
       uint32_t off = sc_off[i] + (uint32_t)v * 16;
       off = off < sc_last ? off : sc_last;
       if (a.scales) direct16_at(off, sc_base, buf + (i * 4 + wave) * 1024);
-      if (ANY && a.zeros) direct16_at(off, zp_base, buf + 2 * Cfg::WINDOW + (i * 4 + wave) * 1024);
+      if (ANY && a.zeros) direct16_at(off, zp_base, buf + 2 * window_bytes + (i * 4 + wave) * 1024);
     }
   };
   int sc_at[NT];  // where this lane's first scale of a window lies in it (in values); the first of window v is group 8 v
 #pragma unroll
-  for (int t = 0; t < NT; ++t) sc_at[t] = ((wave * NT + t) * 16 + r16) * 16 + (int)((weight_row(wave * NT + t, r16) * a.groups) & 7);
+  for (int t = 0; t < NT; ++t) sc_at[t] = ((wave * NT + t) * 16 + r16) * 8 * pieces + (int)((weight_row(wave * NT + t, r16) * a.groups) & 7);
   const T one = from_float<T>(1.0f), zs = from_float<T>(a.zero_scalar);
   const NibbleMagic mg = make_nibble_magic();
   const int u_last = a.K / 32 - 1;
@@ -324,7 +368,7 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
         load_weights(s + 1);
       }
       const uint8_t* const x0 = smem + (s & 1) * Cfg::ACT + r16 * Cfg::ROW_BYTES;
-      const int buf = (v & 1) * (Cfg::WINDOW / 2);
+      const int buf = (v & 1) * (window_bytes / 2);
 #pragma unroll
       for (int b = 0; b < KSB; ++b) {
         const int u = (s * KSB + b) * 4 + q, g = group_of(u < u_last ? u : u_last) - 8 * v + buf;
@@ -366,13 +410,19 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
       }
       if (++in_window == window) in_window = 0, ++v;
     }
+    int pair[MT];
+    float weight[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      pair[m] = mine[m * 16 + r16 < rows ? m * 16 + r16 : rows - 1];
+      weight[m] = UP ? 0.0f : a.weights[pair[m]];
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int n = (tile0 + wave * NT + t) * OUTS + q * 4;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const int r = m * 16 + r16;
-        moe_store<T, UP>(a, acc[t][m], r < rows && tile0 + wave * NT + t < n_tiles, list[r], UP ? 0.0f : row_weight[r], n, q, chunk);
+        moe_store<T, UP>(a, acc[t][m], m * 16 + r16 < rows && tile0 + wave * NT + t < n_tiles, pair[m], weight[m], n, q, chunk);
       }
     }
   };
@@ -745,10 +795,10 @@ int run_few(const char* what, const ExpertArgs& x, const void* ids, int64_t pair
 template <typename T, bool UP, bool ZEROS, int MAXMT, int NT, int KSB>
 int launch_tiles(const char* what, const TileArgs& a, int64_t grid, hipStream_t st) {
   auto kern = moe_tile_kernel<T, UP, ZEROS, MAXMT, NT, KSB>;
-  constexpr int lds = TileCfg<MAXMT, NT, KSB>::lds(ZEROS);
+  const int lds = TileCfg<MAXMT, NT, KSB>::lds(a.groups % 8 == 0 ? 1 : 2, a.zeros != nullptr);
   static bool attr_set = false;
   if (!attr_set) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, TileCfg<MAXMT, NT, KSB>::lds(2, true));
     TLQ_REQUIRE(e == hipSuccess, "%s: cannot reserve LDS: %s", what, hipGetErrorString(e));
     attr_set = true;
   }
@@ -773,22 +823,22 @@ int64_t about_tiles(int64_t pairs, int64_t E, int64_t rows) { return (pairs < E 
 template <bool UP, int MAXMT, int NT, int KSB>
 int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st, bool large = false) {
   constexpr int rows = 16 * MAXMT;
-  static_assert(rows >= kLeastRows, "the workspace holds the tiles");
-  const PlanPtrs p = plan_at(ws, x.E, pairs);
-  // (beside tiles of 256 pairs an expert has two at most, and those of the pairs without one)
-  const int64_t beside = 2 * (int64_t)x.E + pairs / rows + 1;
-  int64_t all_tiles = most_tiles(pairs, x.E, rows);
-  if (large && beside < all_tiles) all_tiles = beside;
+  static_assert(rows == 32 || rows == 64, "sizes that the workspace holds the plan of");
+  const PlanSizes z = plan_sizes(x.E, pairs, rows, large);
+  const PlanPtrs p = plan_at(ws, pairs, z);
   const int64_t n_groups = tile_groups<UP, NT>(x.N), steps = ceil_div((int64_t)x.K, (int64_t)(KSB * 128));
   const int64_t chunk_steps = UP || large ? steps : ceil_div(steps, tile_chunks(about_tiles(pairs, x.E, rows), n_groups, x.K));
   *chunks = ceil_div(steps, chunk_steps);
-  const int64_t grid = all_tiles * n_groups * *chunks;
+  const int64_t grid = z.small * n_groups * *chunks;
   TLQ_REQUIRE(grid < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
-  moe_plan_kernel<<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, large);
+  if (pairs > kCompactPairs)
+    moe_plan_kernel<false><<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, large ? (int)moe_panel_groups(x.N, UP) : 0);
+  else
+    moe_plan_kernel<true><<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, large ? (int)moe_panel_groups(x.N, UP) : 0);
   if (!check_launch(what, "moe_plan_kernel")) return 1;
-  if (large && most_large_tiles(pairs) > 0) {
+  if (z.large > 0) {
     const Plan plan{p.order, p.small, p.large, p.totals};
-    if (moe_panel(what, x, plan, most_large_tiles(pairs), dtype, UP, st)) return 1;
+    if (moe_panel(what, x, plan, z.large, dtype, UP, st)) return 1;
   }
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
@@ -806,8 +856,14 @@ bool few_pairs(bool up, int64_t pairs, int64_t E, int64_t N) {
   const int64_t experts = pairs < E ? pairs : E, groups = up ? tile_groups<true, 2>(N) : tile_groups<false, 2>(N);
   return pairs <= 2 * experts && experts * groups <= 1024;
 }
-int g_large = getenv("MOE_LARGE") ? atoi(getenv("MOE_LARGE")) : 96;
-constexpr int64_t kSmallTiles = 12;  // pairs of an expert on average from which tiles of 64 pairs are taken
+
+// Tiles of 32 pairs, 64 or 256, by the pairs of an expert on average.
+//   64 rather than 32 (us, bf16, zero points; 32 / 64): gate / up of 64 experts of 1408 x 2048, 24 pairs each 74 / 87, 40 95 / 99, 64 135 / 131,
+// 192 304 / 248; 8 of 14336 x 4096, 24 187 / 208, 64 362 / 304; down of 8 of 4096 x 14336, 24 116 / 109, 64 204 / 187.
+//   256 beside 64: where the plan can count what they make (choose by rounds, above), or with long enough rows and many pairs.  (64 / 256) gate / up of 64 experts of 1408 x 2048, 192 pairs each
+// 248 / 274, 384 433 / 390, 768 803 / 625; 128 of 4096 x 4096, 64 1214 / 1274, 256 3566 / 3069; 32 of 2816 x 5120, 256 821 / 764; down of 64 of
+// 2048 x 1408, 256 215 / 243, 768 529 / 538; 128 of 2048 x 768, 384 390 / 430; 32 of 5120 x 2816, 256 451 / 469, 512 827 / 718.
+constexpr int kTilesOf64 = 48, kTilesOf256 = 256;
 
 template <bool UP>
 int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st) {
@@ -816,8 +872,9 @@ int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t 
     *chunks = few.chunks;
     if (few.ok) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
   }
-  if (pairs / a.E < kSmallTiles) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
-  const bool large = pairs / a.E >= g_large && moe_panel_takes(a, pairs, UP);
+  if (pairs / a.E < kTilesOf64) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
+  const int64_t large_groups = pairs / kLargeRows * moe_panel_groups(a.N, UP);
+  const bool large = (pairs > kCompactPairs ? a.K >= 2048 && pairs / a.E >= kTilesOf256 && large_groups >= 512 : large_groups >= 192) && moe_panel_takes(a, pairs, UP);
   return run_tiles<UP, 4, 4, 1>(what, a, ids, pairs, dtype, ws, chunks, st, large);
 }
 

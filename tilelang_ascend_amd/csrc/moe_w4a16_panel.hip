@@ -36,6 +36,7 @@ __global__ __launch_bounds__(256, 1) void moe_panel_kernel(const PanelArgs a) {
   const int tile_no = (int)((uint32_t)no / (uint32_t)a.n_groups), group_no = no - tile_no * a.n_groups;
   const PlanTile pt = a.tiles[tile_no];
   const int e = __builtin_amdgcn_readfirstlane(pt.expert), rows = __builtin_amdgcn_readfirstlane(pt.pairs);
+  if (rows == 0) return;
   const int32_t* const mine = a.order + __builtin_amdgcn_readfirstlane(pt.first);
   const int groups = a.K >> a.gshift;
   const int64_t row0 = (int64_t)e * (UP ? 2 : 1) * a.N;  // of the expert's matrix
@@ -116,10 +117,12 @@ bool moe_panel_takes(const ExpertArgs& a, int64_t pairs, bool up) {
   return a.K % 128 == 0 && (a.group & (a.group - 1)) == 0 && x_rows * a.K * 2 < reach && (up ? 2 : 1) * (int64_t)a.N * (a.K / 2) < reach;
 }
 
+int64_t moe_panel_groups(int64_t N, bool up) { return ceil_div(N, (int64_t)(up ? Panel2Cfg::BN / 2 : Panel2Cfg::BN)); }
+
 int moe_panel(const char* what, const ExpertArgs& x, const Plan& plan, int64_t most_tiles, int dtype, bool up, hipStream_t st) {
   int gshift = 0;
   while ((1 << gshift) < x.group) ++gshift;
-  const int64_t n_groups = ceil_div((int64_t)x.N, (int64_t)(up ? Panel2Cfg::BN / 2 : Panel2Cfg::BN)), grid = most_tiles * n_groups;
+  const int64_t n_groups = moe_panel_groups(x.N, up), grid = most_tiles * n_groups;
   TLQ_REQUIRE(grid < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
   const PanelArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, x.out, plan.order, plan.large, plan.totals + 1, x.top_k, x.N, x.K, gshift, (int)n_groups, x.zero_scalar};
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
