@@ -78,6 +78,28 @@ def test_route(M, E, k, n_group, topk_group, scoring, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("M,E,k,n_group,topk_group", [(5, 16, 4, 16, 5), (3, 64, 7, 64, 7), (3, 60, 3, 12, 4), (5, 96, 9, 3, 2), (2, 45, 4, 15, 4), (7, 130, 5, 2, 1)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_groups_of_one_expert_and_of_odd_sizes(scoring, M, E, k, n_group, topk_group):
+    logits = torch.randn(M, E, generator=gen(M + E)) * 2
+    check_route(logits, k, scoring=scoring, n_group=n_group, topk_group=topk_group)
+    check_route(logits - 705.0, k, scoring=scoring, n_group=n_group, topk_group=topk_group)  # sigmoid: where 64 bits run out
+
+
+@gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_near_ties_are_told_apart_in_64_bits(scoring):
+    x = torch.full((3, 256), 1.0)
+    x[0, 77], x[0, 200], x[0, 3] = 1.0 + 2.0**-23, 1.0 + 2.0**-22, 1.0 - 2.0**-24
+    x[1] = 20.0
+    x[1, ::7] = 20.0 + 2.0**-19
+    x[2] = 1e-12
+    x[2, 5], x[2, 250] = 2e-12, 3e-12
+    check_route(x, 20, scoring=scoring)
+    check_route(x, 20, scoring=scoring, n_group=8, topk_group=4)
+
+
+@gpu
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 def test_route_ties_go_to_the_lowest_index(scoring):
     x = torch.zeros(4, 192)

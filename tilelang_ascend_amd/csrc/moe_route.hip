@@ -29,6 +29,9 @@ struct RouteArgs {
   int E, top_k, n_group, topk_group;
   int sigmoid, renormalize;
   float scaling;
+  int lanes_shift;  // 2^lanes_shift lanes for a group
+  int group_size;
+  uint32_t per_size;  // ceil(2^32 / group_size), for the group of an expert; 0 for groups of one
 };
 
 __device__ __forceinline__ double from_halves(uint32_t lo, uint32_t hi) { return bitcast<double>(((uint64_t)hi << 32) | lo); }
@@ -64,6 +67,35 @@ __device__ __forceinline__ double wave_all(double v, Op op) {
   return v;
 }
 
+// The largest of the 64 lanes' values.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#define TLQ_DPP_MAX(ctrl)                                                                             \
+  {                                                                                                   \
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true);        \
+    v = v > o ? v : o;                                                                                \
+  }
+  TLQ_DPP_MAX(0xb1)
+  TLQ_DPP_MAX(0x4e)
+  TLQ_DPP_MAX(0x141)
+  TLQ_DPP_MAX(0x140)
+#undef TLQ_DPP_MAX
+  const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16), c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  const uint32_t ab = a > b ? a : b, cd = c > d ? c : d;
+  return ab > cd ? ab : cd;
+}
+// Whole numbers in the order of the values (no NaN, no -0); 0 is free for an expert that is not to be had.
+__device__ __forceinline__ uint64_t key_of(double v) {
+  const uint64_t b = bitcast<uint64_t>(v);
+  return b ^ ((uint64_t)((int64_t)b >> 63) | ((uint64_t)1 << 63));
+}
+
+// 1 / x to about an ulp, x from 1 to 1e300: two of Newton's steps
+__device__ __forceinline__ double reciprocal(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+  return __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+}
+
 template <typename T, int EPL>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const RouteArgs a) {
   __shared__ double scores[kRouteWaves][64 * EPL];
@@ -72,7 +104,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
   const int64_t m = (int64_t)blockIdx.x * kRouteWaves + wave;
   if (m >= a.M) return;  // (a wavefront shares nothing with the others: no barrier below)
   const double inf = __builtin_huge_val();
-  const auto larger = [](double x, double y) { return __builtin_fmax(x, y); };
+  const auto larger = [](double x, double y) { return x > y ? x : y; };
   const auto plus = [](double x, double y) { return x + y; };
   double* const my_scores = scores[wave];
   double* const my_values = values[wave];
@@ -89,7 +121,19 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
   }
   if (a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) p[i] = masked[i] ? 0.0 : 1.0 / (1.0 + exp(-v[i]));
+    for (int i = 0; i < EPL; ++i) p[i] = 1.0 + exp(masked[i] ? 0.0 : -v[i]);  // (all of them, so that they share their constants)
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) far = far || p[i] > 1e300;
+    if (__builtin_amdgcn_ballot_w64(far)) {  // (the steps below would lose what is left of such a reciprocal)
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) p[i] = 1.0 / p[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) p[i] = reciprocal(p[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) p[i] = masked[i] ? 0.0 : p[i];
   } else {
     double top = v[0];
 #pragma unroll
@@ -98,7 +142,9 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      p[i] = masked[i] ? 0.0 : v[i] == top ? 1.0 : exp(v[i] - top);  // (equal: also where both are +infinity)
+      const bool is_top = v[i] == top;  // (also where both are +infinity)
+      p[i] = exp(is_top ? 0.0 : v[i] - top);
+      p[i] = masked[i] ? 0.0 : p[i];
       sum += p[i];
     }
     sum = wave_all(sum, plus);
@@ -119,50 +165,62 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
 #pragma unroll
     for (int i = 0; i < EPL; ++i) my_values[lane * EPL + i] = v[i];
     __builtin_amdgcn_wave_barrier();
-    const int size = a.E / a.n_group;
+    // 64 / n_group lanes (a power of two) scan a group in turn, then join their two largest
+    const int size = a.group_size, shift = a.lanes_shift, mine = lane >> shift, per = 1 << shift;
     double first = -inf, second = -inf;
-    if (lane < a.n_group) {
-      int at = lane % size;  // (every lane starts elsewhere: the groups are whole multiples of the banks apart)
-      for (int i = 0; i < size; ++i) {
-        const double y = my_values[lane * size + at];
-        at = at + 1 == size ? 0 : at + 1;
-        second = larger(second, __builtin_fmin(first, y));
-        first = larger(first, y);
+    if (mine < a.n_group) {
+      for (int i = lane & (per - 1); i < size; i += per) {
+        const double y = my_values[mine * size + i];
+        second = y > first ? first : y > second ? y : second;
+        first = y > first ? y : first;
       }
+    }
+    for (int o = 1; o < per; o <<= 1) {
+      const double f = __shfl_xor(first, o), t = __shfl_xor(second, o);
+      const double less = f > first ? first : f, more = t > second ? t : second;
+      first = f > first ? f : first;
+      second = less > more ? less : more;
     }
     // a group with one expert to be had counts with that one
     const double of_group = second > -inf ? first + second : first;
     int rank = 0;
     const uint64_t bits = bitcast<uint64_t>(of_group);
     for (int g = 0; g < a.n_group; ++g) {
-      const double other = from_halves(__builtin_amdgcn_readlane((uint32_t)bits, g), __builtin_amdgcn_readlane((uint32_t)(bits >> 32), g));
-      rank += (other > of_group || (other == of_group && g < lane)) ? 1 : 0;
+      const double other = from_halves(__builtin_amdgcn_readlane((uint32_t)bits, g << shift), __builtin_amdgcn_readlane((uint32_t)(bits >> 32), g << shift));
+      rank += (other > of_group || (other == of_group && g < mine)) ? 1 : 0;
     }
-    const uint64_t kept = __builtin_amdgcn_ballot_w64(lane < a.n_group && rank < a.topk_group);
+    const uint64_t kept = __builtin_amdgcn_ballot_w64(mine < a.n_group && rank < a.topk_group);  // group g: bit g << shift
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       const int e = lane * EPL + i;
-      if (e < a.E && !((kept >> (e / size)) & 1)) v[i] = -inf;
+      if (e < a.E && !((kept >> ((a.per_size ? __umulhi((uint32_t)e, a.per_size) : (uint32_t)e) << shift)) & 1)) v[i] = -inf;
     }
   }
 
+  // The largest by the upper halves of the keys, which nearly always one lane alone has; otherwise by the lower halves among those that do.
+  uint64_t key[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) key[i] = v[i] > -inf ? key_of(v[i]) : 0;
   int id = -1;  // lane j: the j-th expert
   for (int j = 0; j < a.top_k; ++j) {
-    double mine = v[0];
+    uint64_t mine = key[0];
     int at = 0;
 #pragma unroll
     for (int i = 1; i < EPL; ++i)
-      if (v[i] > mine) mine = v[i], at = i;
-    const double best = wave_all(mine, larger);
-    if (!(best > -inf)) break;  // nothing left: the remaining slots stay empty
-    const int winner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(mine == best));
+      if (key[i] > mine) mine = key[i], at = i;
+    const uint32_t upper = (uint32_t)(mine >> 32), best = wave_max(upper);
+    if (best == 0) break;  // nothing left: the remaining slots stay empty
+    uint64_t have = __builtin_amdgcn_ballot_w64(upper == best);
+    if (have & (have - 1)) {
+      const uint32_t lower = upper == best ? (uint32_t)mine : 0, best_lower = wave_max(lower);
+      have = __builtin_amdgcn_ballot_w64(upper == best && lower == best_lower);
+    }
+    const int winner = __builtin_ctzll(have);
     const int e = winner * EPL + __builtin_amdgcn_readlane(at, winner);
     if (lane == j) id = e;
-    if (lane == winner) {
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (i == at) v[i] = -inf;
-    }
+    for (int i = 0; i < EPL; ++i)
+      if (lane == winner && i == at) key[i] = 0;
   }
   __builtin_amdgcn_wave_barrier();
   double w = id >= 0 ? my_scores[id] : 0.0;
@@ -213,8 +271,11 @@ extern "C" int tlq_moe_route(const void* logits, const void* bias, void* weights
   TLQ_REQUIRE(logits && weights && ids, "tlq_moe_route: null pointer");
   TLQ_REQUIRE((((uintptr_t)weights | (uintptr_t)ids | (uintptr_t)bias) & 3) == 0 && ((uintptr_t)logits & (in_dtype == TLQ_F32 ? 3 : 1)) == 0,
               "tlq_moe_route: misaligned pointer");
+  int shift = 6;
+  while ((n_group << shift) > 64) --shift;
   const RouteArgs a{logits, (const float*)bias, (float*)weights, (int32_t*)ids, M, (int)E, (int)top_k, (int)n_group, (int)topk_group,
-                    scoring == TLQ_MOE_SIGMOID, renormalize != 0, scaling};
+                    scoring == TLQ_MOE_SIGMOID, renormalize != 0, scaling, shift,
+                    (int)(E / n_group), E == n_group ? 0u : (uint32_t)ceil_div((int64_t)1 << 32, E / n_group)};
   hipStream_t st = (hipStream_t)stream;
   if (in_dtype == TLQ_F16) return run_route<half_t>(a, st);
   if (in_dtype == TLQ_BF16) return run_route<bf16_t>(a, st);
