@@ -58,7 +58,7 @@ inline int64_t plan_bytes(int64_t E, int64_t pairs) {
 }
 
 // Candidates for `from`: 65, 129, 193, 257 (whole tiles only), and more pairs than there are (none).  A round of large tiles is 256 work-groups,
-// one a CU, one of tiles of 64 pairs 512, which take 5 / 8 of its time (gate / up, 16 experts of 2048 x 4096: 98 and 61 us).
+// one a CU; of tiles of 64 pairs as wide as those 512 go at once and take 5 / 8 of its time (gate / up, 16 experts of 2048 x 4096: 98 and 61 us).
 constexpr int kFromChoices = 5;
 __device__ __forceinline__ int from_choice(int i) { return i < 4 ? 64 * i + 65 : 1 << 24; }
 __device__ __forceinline__ int rounds_of(int large, int small, int groups) { return 8 * ((large * groups + 255) / 256) + 5 * ((small * groups + 511) / 512); }
@@ -858,12 +858,12 @@ bool few_pairs(bool up, int64_t pairs, int64_t E, int64_t N) {
 }
 
 // Tiles of 32 pairs, 64 or 256, by the pairs of an expert on average.
-//   64 rather than 32 (us, bf16, zero points; 32 / 64): gate / up of 64 experts of 1408 x 2048, 24 pairs each 74 / 87, 40 95 / 99, 64 135 / 131,
-// 192 304 / 248; 8 of 14336 x 4096, 24 187 / 208, 64 362 / 304; down of 8 of 4096 x 14336, 24 116 / 109, 64 204 / 187.
-//   256 beside 64: where the plan can count what they make (choose by rounds, above), or with long enough rows and many pairs.  (64 / 256) gate / up of 64 experts of 1408 x 2048, 192 pairs each
-// 248 / 274, 384 433 / 390, 768 803 / 625; 128 of 4096 x 4096, 64 1214 / 1274, 256 3566 / 3069; 32 of 2816 x 5120, 256 821 / 764; down of 64 of
-// 2048 x 1408, 256 215 / 243, 768 529 / 538; 128 of 2048 x 768, 384 390 / 430; 32 of 5120 x 2816, 256 451 / 469, 512 827 / 718.
-constexpr int kTilesOf64 = 48, kTilesOf256 = 256;
+//   64 rather than 32 (us, bf16, zero points; 32 / 64): gate / up of 64 experts of 1408 x 2048, 12 pairs each 58.7 / 62.2, 24 75.4 / 75.1, 40 96.5 / 92.4;
+// 8 of 14336 x 4096, 12 155 / 163, 24 188 / 184, 40 268 / 221; down of 8 of 4096 x 14336, 12 94 / 97, 24 117 / 105; 16 of 2048 x 4096, 24 38.3 / 41.5, 40 50.7 / 44.5.
+//   256 beside 64: where the plan can count what they make (choose by rounds, above), or with long enough rows and many pairs.  (64 / 256) gate / up of
+// 64 experts of 1408 x 2048, 192 pairs each 235 / 266, 256 305 / 303, 768 791 / 615; 128 of 768 x 2048, 256 325 / 318, 768 871 / 659; down of 64 of
+// 2048 x 1408, 256 193 / 224, 768 514 / 525; 128 of 2048 x 768, 768 750 / 796; 16 of 2048 x 4096, 768 326 / 325.
+constexpr int kTilesOf64 = 24, kTilesOf256 = 256;
 
 template <bool UP>
 int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st) {
@@ -875,13 +875,13 @@ int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t 
   if (pairs / a.E < kTilesOf64) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
   const int64_t large_groups = pairs / kLargeRows * moe_panel_groups(a.N, UP);
   const bool large = (pairs > kCompactPairs ? a.K >= 2048 && pairs / a.E >= kTilesOf256 && large_groups >= 512 : large_groups >= 192) && moe_panel_takes(a, pairs, UP);
-  return run_tiles<UP, 4, 4, 1>(what, a, ids, pairs, dtype, ws, chunks, st, large);
+  return run_tiles<UP, 4, 2, 1>(what, a, ids, pairs, dtype, ws, chunks, st, large);
 }
 
 // the most that any of them cuts K of the down product into
 int64_t down_chunks(int64_t pairs, int64_t E, int64_t N, int64_t K) {
   int64_t c = few_pairs(false, pairs, E, N) ? few_chunks(K) : 1;
-  const int64_t small = tile_chunks(about_tiles(pairs, E, 32), tile_groups<false, 2>(N), K), large = tile_chunks(about_tiles(pairs, E, 64), tile_groups<false, 4>(N), K);
+  const int64_t small = tile_chunks(about_tiles(pairs, E, 32), tile_groups<false, 2>(N), K), large = tile_chunks(about_tiles(pairs, E, 64), tile_groups<false, 2>(N), K);
   c = c > small ? c : small;
   return c > large ? c : large;
 }
