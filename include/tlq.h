@@ -404,7 +404,7 @@ int tlq_moe_route(const void* logits, const void* bias, void* weights, void* ids
  * tlq_moe_down_w4a16:  Y[t, n] = rn_out( sum_j weights[t, j] * (H[t, j] . W[e, n]) ), fp32 sums; slots without an expert add nothing.
  *   H [M, top_k, K] in_dtype, weights fp32 [M, top_k], w_packed [E, N, K / 2], scales / zeros [E, N, K / group], Y [M, N] out_dtype.
  * W = rn_T(rn_T(T(u) - z) * s) as in tlq_dequant_w4 (scales NULL: 1; zeros NULL: zero_scalar); T = dtype: TLQ_F16 or TLQ_BF16.
- * N % 16 == 0, K % 32 == 0, group a multiple of 32 that divides K, E <= 1024, top_k <= 64, M * top_k < 2^24.  X, H, Y, w_packed,
+ * N % 16 == 0, K % 32 == 0, N * K < 2^32, group a multiple of 32 that divides K, E <= 1024, top_k <= 64, M * top_k < 2^24.  X, H, Y, w_packed,
  * scales and zeros 16-byte aligned.  Results do not depend on timing: no floating-point sum is formed by atomic adds.
  * The workspace (16-byte aligned, at least tlq_moe_*_workspace_bytes) holds nothing between calls; two calls that may run at the
  * same time need one each. */

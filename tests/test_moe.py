@@ -232,6 +232,78 @@ def test_down(M, E, k, N, K, group, dtype, zeros, kind, out):
     assert_close64(got, want, off, f"down {M, E, k, N, K}")
 
 
+# M, E, top_k, N, K, group, type, zeros, how ids are spread: tiles of 256 pairs beside tiles of 64 where the counts of all experts are known
+# (up to 4096 pairs) and where they are not, and tiles of 32 and 64 of many pairs
+MANY = [
+    (2048, 5, 2, 3104, 256, 128, "bfloat16", "frac", "spread"),
+    (2047, 4, 2, 3104, 128, 32, "float16", 8, "holes"),
+    (1365, 3, 3, 4112, 256, 64, "float16", "int", "twice"),
+    (4096, 2, 1, 3104, 128, 128, "bfloat16", 7.5, "one"),
+    (4100, 7, 2, 4112, 2048, 128, "bfloat16", "frac", "holes"),
+    (4200, 6, 2, 4112, 2048, 2048, "float16", 7.5, "spread"),
+    (8200, 3, 1, 4112, 2048, 64, "float16", "int", "one"),
+    (2100, 9, 2, 48, 96, 96, "bfloat16", "int", "holes"),
+    (1100, 300, 4, 32, 64, 32, "float16", "frac", "spread"),
+    (2500, 4, 2, 80, 448, 64, "float16", 8, "one"),
+]
+
+
+def some_tokens(M):
+    return torch.cat([torch.tensor([0, 1, M - 2, M - 1]), torch.randint(0, M, (60,), generator=gen(M))])
+
+
+@gpu
+@pytest.mark.parametrize("M,E,k,N,K,group,dtype,zeros,kind", MANY)
+def test_gate_up_of_many_pairs(M, E, k, N, K, group, dtype, zeros, kind):
+    T = DT[dtype]
+    X = torch.randn(M, K, generator=gen(7)).to(T)
+    ids = make_ids(M, E, k, kind, 11)
+    Wp, s, z = make_experts(E, 2 * N, K, group, T, zeros, 13)
+    got = ops.moe_gate_up_w4a16(E, k, N, K, group, dtype, zeros=kernel_zeros(z))(*operands(X, ids, Wp, s, z)).cpu()
+    some = some_tokens(M)
+    want, off = ref.moe_gate_up(X[some], ids[some], Wp, s, z, group)
+    assert_close64(got[some], want, off, f"gate_up {M, E, k, N, K}")
+    empty = (ids < 0) | (ids >= E)
+    assert (got[empty] == 0).all() and torch.isfinite(got).all()
+    assert (got[~empty].abs().amax(-1) > 0).all()  # every row was written
+
+
+@gpu
+@pytest.mark.parametrize("M,E,k,N,K,group,dtype,zeros,kind", MANY)
+def test_down_of_many_pairs(M, E, k, N, K, group, dtype, zeros, kind):
+    T = DT[dtype]
+    H = torch.randn(M, k, K, generator=gen(7)).to(T)
+    ids = make_ids(M, E, k, kind, 11)
+    weights = torch.rand(M, k, generator=gen(5)) + 0.25
+    Wp, s, z = make_experts(E, N, K, group, T, zeros, 13)
+    got = ops.moe_down_w4a16(E, k, N, K, group, dtype, "float32", zeros=kernel_zeros(z))(*operands(H, ids, weights, Wp, s, z)).cpu()
+    some = some_tokens(M)
+    want, off = ref.moe_down(H[some], ids[some], weights[some], Wp, s, z, group)
+    assert_close64(got[some], want, off, f"down {M, E, k, N, K}")
+    empty = ((ids < 0) | (ids >= E)).all(1)
+    assert (got[empty] == 0).all() and torch.isfinite(got).all()
+    assert (got[~empty].abs().amax(-1) > 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 9, 40, 300])
+def test_weights_that_overflow_at_the_end_of_a_row_that_is_no_multiple_of_128(M):
+    """15 * 6000 is infinite in binary16: with positive activations so is every sum, and nothing behind the end of a row makes it NaN."""
+    E, k, N, K = 4, 2, 32, 160
+    ids = make_ids(M, E, k, "spread", 3)
+    for zeros in (None, "tensor"):
+        z = None if zeros is None else torch.zeros(E, 2 * N, K // 32, dtype=torch.float16)
+        Wp = torch.full((E, 2 * N, K // 2), 0xFF, dtype=torch.uint8)
+        s = torch.full((E, 2 * N, K // 32), 2.0**-10, dtype=torch.float16)
+        s[..., -1] = 6000.0
+        X = torch.rand(M, K, generator=gen(1)).half() + 0.5
+        got = ops.moe_gate_up_w4a16(E, k, N, K, 32, "float16", zeros=zeros)(*operands(X, ids, Wp, s, z))
+        assert (got == float("inf")).all()
+        H = torch.rand(M, k, K, generator=gen(2)).half() + 0.5
+        got = ops.moe_down_w4a16(E, k, 2 * N, K, 32, "float16", "float32", zeros=zeros)(*operands(H, ids, torch.ones(M, k), Wp, s, z))
+        assert (got == float("inf")).all()
+
+
 @gpu
 def test_products_without_scales_and_without_any_expert():
     E, k, N, K = 4, 2, 32, 64

@@ -380,6 +380,13 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
           zv[t] = ANY && a.zeros ? ((const T*)zp)[sc_at[t] + g] : zs;
           if (ANY) whole = whole && small_integer(to_float(zv[t]));
         }
+        if ((s * KSB + b) * 128 + 128 > a.K) {  // (uniform) behind K: zeros, not an infinite weight times zero
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            sv[t] = u > u_last ? from_float<T>(0.0f) : sv[t];
+            zv[t] = u > u_last ? from_float<T>(0.0f) : zv[t];
+          }
+        }
         auto multiply = [&](auto fold_tag) __attribute__((always_inline)) {
           typedef Expand8<T, decltype(fold_tag)::value> Ex;
           Ex ex[NT];
@@ -636,7 +643,8 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
         if (block == 0)  // this lane's scales in LDS: that of group g lies at sc0 + g
           sc0 = ((my_tile0 + tile) * 16 + r16) * pieces * 8 + (int)((weight_row(tile0 + my_tile0 + tile, r16) * a.groups + g0) & 7) - g0;
         const int u = k0 / 32 + (block0 + block) * 4 + q, at = sc0 + group_of(u < u_last ? u : u_last);
-        const T sv = a.scales ? ((const T*)(smem + sc_at))[at] : one, zv = ANY && a.zeros ? ((const T*)(smem + zp_at))[at] : zs;
+        T sv = a.scales ? ((const T*)(smem + sc_at))[at] : one, zv = ANY && a.zeros ? ((const T*)(smem + zp_at))[at] : zs;
+        if (u > u_last) sv = zv = from_float<T>(0.0f);  // (behind K: zeros, not an infinite weight times zero)
         const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
         const uint8_t* const x = my_act + block * 256;
         auto multiply = [&](auto fold_tag) __attribute__((always_inline)) {
@@ -710,7 +718,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 }
 
 int check_experts(const char* what, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, int dtype) {
-  TLQ_REQUIRE(M >= 0 && E >= 1 && E <= kMaxExperts && top_k >= 1 && top_k <= 64, "%s: bad shape M=%lld E=%lld top_k=%lld (at most 1024 experts, 64 of them for a token)",
+  TLQ_REQUIRE(M >= 0 && M < ((int64_t)1 << 32) && E >= 1 && E <= kMaxExperts && top_k >= 1 && top_k <= 64, "%s: bad shape M=%lld E=%lld top_k=%lld (at most 1024 experts, 64 of them for a token)",
               what, (long long)M, (long long)E, (long long)top_k);
   TLQ_REQUIRE(M * top_k < ((int64_t)1 << 24), "%s: M * top_k = %lld is 2^24 or more: call it for fewer tokens at once", what, (long long)(M * top_k));
   TLQ_REQUIRE(N >= 16 && N % 16 == 0 && N < ((int64_t)1 << 24), "%s: N=%lld must be a multiple of 16", what, (long long)N);
