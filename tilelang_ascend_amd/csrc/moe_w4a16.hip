@@ -199,6 +199,11 @@ __device__ __forceinline__ void direct4(const void* src, uint32_t lds) {
 // two buffers a step ahead, the packed weights go straight into operand registers a step ahead -- lane (r16, q) has the 32 values 32 q ..
 // of each block of row r16, at MFMA k-step j the eight of word 4 q + j --, are expanded there and multiplied with all rows: a weight
 // is expanded once per 16 MAXMT pairs, an activation operand read once per NT tiles.  One barrier a step.
+//   64 pairs: fp16, zero points, 211 tokens on 2 of 8 experts of 14336 x 4096 (gate / up): 222 - 250 us, of the vector units' time 57 % (13
+// instructions expand eight weights), of the matrix units' 26 %; the rest is the trip of a step's loads.  With 64 rows of W a wavefront in the
+// place of 32 (NT = 4) 5 - 10 % slower -- fewer work-groups on a CU, coarser rounds --; with 128 pairs level where experts have 192 pairs and more, 10 - 30 % slower
+// below; tiles of an expert side by side on the same weight rows 3 - 6 % faster on matrices of 58 MB, 2 - 8 % slower on small ones.
+//   32 pairs: bf16, 48 tokens on 8 of 128 experts of 768 x 2048 (gate / up): 35 - 40 us for 199 MB, the rate of a large copy.
 //   Scales and zero points come through LDS in windows of eight groups (whole steps: 8 groups are 256 (group / 32) values), loaded a window
 // ahead as the 16-byte pieces of a row that hold them (two, unless rows are whole pieces).  ANY: zero points that need not be small integers, which are folded into the
 // unpacking's bias (a tensor, looked at block by block, or such a scalar).
@@ -450,6 +455,9 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
 //   A tile is 16 weight rows: 16 outputs, or 8 gate rows and the 8 up rows that go with them.  A block is 128 values of K of a tile.
 // Where tiles are few, `splits` wavefronts share one, each with a part of K; their sums meet in LDS and are added in the order of K.
 // Long rows of the down product are cut into `chunks` work-groups too, whose sums moe_combine_kernel adds.
+//   fp16, zero points: one token, 6 of 64 experts of 1408 x 2048, gate / up 11 us (18 MB), down 9.4; 2 of 8 of 4096 x 14336, down 24 us + 4 for the sums
+// (66 MB, 13.4 us at the rate of a large copy).  What is left is latency: ids, then rows and scales, then 28 KB of weights a wavefront, 4 KB at a time.  With
+// eight blocks asked for at once the kernel spills and takes 25 - 40 % more.
 constexpr int kFewPairs = 2048;
 constexpr int kFewGroup = 4;
 enum { kFewByPair = 1, kFewOneToken = 2 };
@@ -680,7 +688,7 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
   }
 }
 
-// y[t] = the sum of token t's rows, slot by slot, each over the parts of K it was cut into; four slots' rows are asked for at once.  A
+// (down of 4099 tokens, 6 slots of 2048: 32 us for 218 MB, 6.9 TB/s.)  y[t] = the sum of token t's rows, slot by slot, each over the parts of K it was cut into; four slots' rows are asked for at once.  A
 // work-group has 256 x 4 values of one token.
 __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restrict__ rows, const int32_t* __restrict__ ids, void* __restrict__ Y,
                                                          int N, int n_groups, int top_k, int E, int out_dtype, int chunks, int64_t chunk_stride) {
