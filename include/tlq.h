@@ -408,7 +408,7 @@ int tlq_moe_route(const void* logits, const void* bias, void* weights, void* ids
  * scales and zeros 16-byte aligned.  Results do not depend on timing: no floating-point sum is formed by atomic adds.
  * The workspace (16-byte aligned, at least tlq_moe_*_workspace_bytes) holds nothing between calls; two calls that may run at the
  * same time need one each. */
-int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k);
+int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K);
 int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K);
 int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void* w_packed, const void* scales, const void* zeros, void* H,
                           void* workspace, int64_t workspace_bytes, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K,

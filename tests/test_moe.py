@@ -175,6 +175,10 @@ SHAPES = [
     (12, 4, 2, 48, 2208, 96, "bfloat16", "frac", "holes"),
     (20, 4, 2, 32, 2208, 736, "float16", 8, "spread"),
     (64, 2, 2, 16, 8192, 64, "bfloat16", 3.25, "one"),
+    # (gate / up in parts of K, with outputs and pairs left over)
+    (40, 3, 2, 80, 8224, 32, "float16", "frac", "holes"),
+    (90, 2, 1, 176, 10240, 128, "bfloat16", 8, "spread"),
+    (70, 2, 2, 1040, 2048, 64, "bfloat16", "int", "twice"),
     # (tiles of 256 pairs, and what is left of an expert's pairs)
     (700, 3, 2, 272, 384, 64, "bfloat16", "frac", "holes"),
     (1100, 2, 1, 144, 128, 32, "float16", None, "one"),
@@ -523,7 +527,7 @@ def test_products_refuse():
         _rejected(f(ws=NULL), "workspace")
         _rejected(f(ws=ODD), "workspace")
         assert f(M=0) == 0
-    _rejected(up(n=lib.tlq_moe_gate_up_workspace_bytes(4, 8, 2) - 1), "workspace")
+    _rejected(up(n=lib.tlq_moe_gate_up_workspace_bytes(4, 8, 2, 64, 128) - 1), "workspace")
     _rejected(down(n=lib.tlq_moe_down_workspace_bytes(4, 8, 2, 64, 128) - 1), "workspace")
     _rejected(down(weights=NULL), "null pointer")
     _rejected(down(weights=ODD), "aligned")
@@ -533,10 +537,12 @@ def test_products_refuse():
 def test_workspace_sizes():
     lib = _abi.load()
     up, down = lib.tlq_moe_gate_up_workspace_bytes, lib.tlq_moe_down_workspace_bytes
-    assert up(0, 8, 2) == up(4, 0, 2) == up(4, 8, 0) == up(4, 2000, 2) == down(0, 8, 2, 64, 64) == down(4, 8, 2, 0, 64) == down(4, 8, 2, 64, 0) == 0
+    assert up(0, 8, 2, 64, 64) == up(4, 0, 2, 64, 64) == up(4, 8, 0, 64, 64) == up(4, 2000, 2, 64, 64) == up(4, 8, 2, 0, 64) == up(4, 8, 2, 64, 0) == 0
+    assert down(0, 8, 2, 64, 64) == down(4, 8, 2, 0, 64) == down(4, 8, 2, 64, 0) == 0
     for M in (1, 3, 64, 1000, 100000):
-        assert 0 < up(M, 8, 2) and up(M, 8, 2) <= up(M + 1, 8, 2) and up(M, 8, 2) % 16 == 0
-        assert down(M, 8, 2, 64, 64) >= up(M, 8, 2)
+        assert 0 < up(M, 8, 2, 64, 64) and up(M, 8, 2, 64, 64) <= up(M + 1, 8, 2, 64, 64) and up(M, 8, 2, 64, 64) % 16 == 0
+        assert down(M, 8, 2, 64, 64) >= up(M, 8, 2, 64, 64)
+    assert up(16, 8, 2, 64, 8192) >= up(16, 8, 2, 64, 64) + 2 * 32 * 128 * 4  # parts of K
 
 
 @pytest.mark.parametrize("kwargs,message", [

@@ -64,7 +64,7 @@ SIGNATURES = {
     "tlq_quantize_sym4": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
     "tlq_act_quant_i8": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
     "tlq_moe_route": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _int, _f32, _int, _vp]),
-    "tlq_moe_gate_up_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "tlq_moe_gate_up_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "tlq_moe_down_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "tlq_moe_gate_up_w4a16": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _vp]),
     "tlq_moe_down_w4a16": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _vp]),

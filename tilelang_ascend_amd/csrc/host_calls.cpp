@@ -121,7 +121,7 @@ int launch(const PlanObject& p, const at::Tensor* const* t, int device, hipStrea
   } else if (p.kind == kF16) {
     ws_bytes = lib.tlq_f16_workspace_bytes(1, v[0], v[1], v[2]);
   } else if (p.kind == kMoeGateUp) {
-    ws_bytes = lib.tlq_moe_gate_up_workspace_bytes(t[0]->size(0), v[0], v[1]);
+    ws_bytes = lib.tlq_moe_gate_up_workspace_bytes(t[0]->size(0), v[0], v[1], v[2], v[3]);
   } else if (p.kind == kMoeDown) {
     ws_bytes = lib.tlq_moe_down_workspace_bytes(t[0]->size(0), v[0], v[1], v[2], v[3]);
   }

@@ -221,7 +221,8 @@ struct TileArgs {
   float zero_scalar;
   int n_groups;        // work-groups side by side
   int window;          // steps of a window
-  int chunk_steps;     // steps of a work-group: those of a part of K (down product with few tiles), whose sums moe_combine_kernel adds
+  int chunk_steps;     // steps of a work-group: those of a part of K (few tiles), whose sums moe_combine_kernel or moe_gate_kernel adds
+  float* parts;        // gate / up in parts of K: the sums [part][pair][2 N], else null
 };
 
 template <int MAXMT, int NT, int KSB>
@@ -255,6 +256,7 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
   const int n_tiles = a.N / OUTS, tile0 = group_no * Cfg::TILES;
   if (e == a.E) {  // pairs without an expert
     if constexpr (UP) {
+      if (a.parts) return;  // (moe_gate_kernel writes their zeros)
       T* const h = (T*)a.out;
       constexpr int width = Cfg::TILES * OUTS;
       for (int i = tid; i < rows * width; i += 256) {
@@ -434,6 +436,11 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
       const int n = (tile0 + wave * NT + t) * OUTS + q * 4;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
+        if (UP && a.parts) {  // this lane's four gates (q = 0, 1) or ups
+          if (m * 16 + r16 < rows && tile0 + wave * NT + t < n_tiles)
+            *(float4_t*)(a.parts + ((int64_t)chunk * a.pairs + pair[m]) * (2 * (int64_t)a.N) + (q >= 2 ? a.N - 8 : 0) + n) = acc[t][m];
+          continue;
+        }
         moe_store<T, UP>(a, acc[t][m], m * 16 + r16 < rows && tile0 + wave * NT + t < n_tiles, pair[m], weight[m], n, q, chunk);
       }
     }
@@ -725,6 +732,27 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
   }
 }
 
+// h of the gate / up product from its sums over parts of K.  A work-group has 256 x 4 values of one pair.
+template <typename T>
+__global__ __launch_bounds__(256) void moe_gate_kernel(const float* __restrict__ parts, const int32_t* __restrict__ ids, T* __restrict__ H, int N,
+                                                      int n_groups, int E, int chunks, int64_t chunk_stride) {
+  const int64_t pair = blockIdx.x / (uint32_t)n_groups;
+  const int n = ((int)(blockIdx.x - (uint32_t)pair * n_groups) * 256 + (int)threadIdx.x) * 4;
+  if (n >= N) return;
+  T o[4];
+  if ((uint32_t)ids[pair] < (uint32_t)E) {
+    const float* const mine = parts + pair * 2 * N + n;
+    float4_t g = *(const float4_t*)mine, u = *(const float4_t*)(mine + N);
+    for (int c = 1; c < chunks; ++c) g += *(const float4_t*)(mine + c * chunk_stride), u += *(const float4_t*)(mine + c * chunk_stride + N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = from_float<T>(silu(g[i]) * u[i]);
+  } else {  // (no row was written)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = from_float<T>(0.0f);
+  }
+  *(uint2_t*)(H + pair * N + n) = bitcast<uint2_t>(o);
+}
+
 int check_experts(const char* what, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, int dtype) {
   TLQ_REQUIRE(M >= 0 && M < ((int64_t)1 << 32) && E >= 1 && E <= kMaxExperts && top_k >= 1 && top_k <= 64, "%s: bad shape M=%lld E=%lld top_k=%lld (at most 1024 experts, 64 of them for a token)",
               what, (long long)M, (long long)E, (long long)top_k);
@@ -822,8 +850,8 @@ int launch_tiles(const char* what, const TileArgs& a, int64_t grid, hipStream_t 
   return check_launch(what, "moe_tile_kernel") ? 0 : 1;
 }
 
-// Work-groups of moe_tile_kernel side by side, and the parts that K of the down product is cut into where there are too few of them
-// to keep four on every CU (eight experts of 4096 x 14336 and 16 tokens: 106 us whole).  `tiles`: about how many tiles of pairs there are.
+// Work-groups of moe_tile_kernel side by side, and the parts that K is cut into where there are too few of them
+// to keep four on every CU (down of eight experts of 4096 x 14336 and 16 tokens: 106 us whole).  `tiles`: about how many tiles of pairs there are.
 template <bool UP, int NT>
 int64_t tile_groups(int64_t N) {
   return ceil_div(N, (int64_t)(4 * NT * (UP ? 8 : 16)));
@@ -835,7 +863,7 @@ int64_t tile_chunks(int64_t tiles, int64_t n_groups, int64_t K) {
 }
 int64_t about_tiles(int64_t pairs, int64_t E, int64_t rows) { return (pairs < E ? pairs : E) + pairs / rows; }
 
-// The plan, then the products on tiles of 16 MAXMT pairs.  chunks: the parts of K of the down product.
+// The plan, then the products on tiles of 16 MAXMT pairs.  chunks: the parts of K.
 template <bool UP, int MAXMT, int NT, int KSB>
 int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st, bool large = false) {
   constexpr int rows = 16 * MAXMT;
@@ -843,8 +871,9 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
   const PlanSizes z = plan_sizes(x.E, pairs, rows, large);
   const PlanPtrs p = plan_at(ws, pairs, z);
   const int64_t n_groups = tile_groups<UP, NT>(x.N), steps = ceil_div((int64_t)x.K, (int64_t)(KSB * 128));
-  const int64_t chunk_steps = UP || large ? steps : ceil_div(steps, tile_chunks(about_tiles(pairs, x.E, rows), n_groups, x.K));
+  const int64_t chunk_steps = large ? steps : ceil_div(steps, tile_chunks(about_tiles(pairs, x.E, rows), n_groups, x.K));
   *chunks = ceil_div(steps, chunk_steps);
+  float* const parts = UP && *chunks > 1 ? (float*)((uint8_t*)ws + plan_bytes(x.E, pairs)) : nullptr;
   const int64_t grid = z.small * n_groups * *chunks;
   TLQ_REQUIRE(grid < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
   if (pairs > kCompactPairs)
@@ -859,15 +888,26 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
   const TileArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
-                   units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};
+                   units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps, parts};
 #define TLQ_TILES(T) (x.zeros || !whole ? launch_tiles<T, UP, true, MAXMT, NT, KSB>(what, a, grid, st) : launch_tiles<T, UP, false, MAXMT, NT, KSB>(what, a, grid, st))
-  return dtype == TLQ_F16 ? TLQ_TILES(half_t) : TLQ_TILES(bf16_t);
+  if (dtype == TLQ_F16 ? TLQ_TILES(half_t) : TLQ_TILES(bf16_t)) return 1;
 #undef TLQ_TILES
+  if (!parts) return 0;
+  const int64_t groups = ceil_div((int64_t)x.N, (int64_t)1024), stride = pairs * 2 * x.N;  // (few work-groups: K was cut because tiles are few)
+  const dim3 g((unsigned)(pairs * groups));
+  if (dtype == TLQ_F16)
+    moe_gate_kernel<half_t><<<g, 256, 0, st>>>(parts, (const int32_t*)ids, (half_t*)x.out, x.N, (int)groups, x.E, (int)*chunks, stride);
+  else
+    moe_gate_kernel<bf16_t><<<g, 256, 0, st>>>(parts, (const int32_t*)ids, (bf16_t*)x.out, x.N, (int)groups, x.E, (int)*chunks, stride);
+  return check_launch(what, "moe_gate_kernel") ? 0 : 1;
 }
 
 // Which kernel: the one without a plan while an expert has two pairs at most on average and the tiles' work-groups would not fill the machine
 // (MoE layers of 8 to 256 experts, bf16, group 128, zero points, this kernel / tiles of 32: 4 tokens on 6 of 64 experts of 1408 x 2048 21.3 / 24.2 us, 8 tokens
 // 30.3 / 30.0; 1 token on 2 of 8 experts, down, 4096 x 14336 25.6 / 95.8; 16 tokens on 4 of 16 experts of 2048 x 2048 28.3 / 24.5).
+//   And while the passes of its `row_cap` rows stay few, each of which reads the expert's weights again: up to twice as many tokens, or pairs on few of
+// the experts (groups of 32; gate / up of 256 experts of 320 x 6016, two rows a pass, 16 tokens on 2 each 30 / 54, 32 tokens 126 / 56; down of 32 of
+// 640 x 10240, four rows, 4 tokens on 4 each 23 / 30, 16 tokens 61 / 36).
 bool few_pairs(bool up, int64_t pairs, int64_t E, int64_t N) {
   const int64_t experts = pairs < E ? pairs : E, groups = up ? tile_groups<true, 2>(N) : tile_groups<false, 2>(N);
   return pairs <= 2 * experts && experts * groups <= 1024;
@@ -886,7 +926,7 @@ int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t 
   if (few_pairs(UP, pairs, a.E, a.N)) {
     const FewPlan few = few_plan(UP, pairs, a.E, a.top_k, a.N, a.K, a.group, a.zeros != nullptr);
     *chunks = few.chunks;
-    if (few.ok) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
+    if (few.ok && (pairs <= 2 * few.row_cap * a.top_k || pairs * 16 <= (int64_t)a.E * few.row_cap)) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
   }
   if (pairs / a.E < kTilesOf64) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
   const int64_t large_groups = pairs / kLargeRows * moe_panel_groups(a.N, UP);
@@ -894,12 +934,19 @@ int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t 
   return run_tiles<UP, 4, 2, 1>(what, a, ids, pairs, dtype, ws, chunks, st, large);
 }
 
-// the most that any of them cuts K of the down product into
-int64_t down_chunks(int64_t pairs, int64_t E, int64_t N, int64_t K) {
-  int64_t c = few_pairs(false, pairs, E, N) ? few_chunks(K) : 1;
-  const int64_t small = tile_chunks(about_tiles(pairs, E, 32), tile_groups<false, 2>(N), K), large = tile_chunks(about_tiles(pairs, E, 64), tile_groups<false, 2>(N), K);
+// the most that any of them cuts K into
+template <bool UP>
+int64_t most_chunks(int64_t pairs, int64_t E, int64_t N, int64_t K) {
+  int64_t c = !UP && few_pairs(UP, pairs, E, N) ? few_chunks(K) : 1;
+  const int64_t small = tile_chunks(about_tiles(pairs, E, 32), tile_groups<UP, 2>(N), K), large = tile_chunks(about_tiles(pairs, E, 64), tile_groups<UP, 2>(N), K);
   c = c > small ? c : small;
   return c > large ? c : large;
+}
+// of the plan alone; 0: sizes that no call takes
+int64_t plan_workspace(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
+  if (M <= 0 || E < 1 || top_k < 1 || E > kMaxExperts || top_k > 64 || M >= ((int64_t)1 << 24) || N < 1 || N >= ((int64_t)1 << 24) || K < 1 || K >= ((int64_t)1 << 24))
+    return 0;
+  return plan_bytes(E, M * top_k);
 }
 
 }  // namespace
@@ -907,15 +954,14 @@ int64_t down_chunks(int64_t pairs, int64_t E, int64_t N, int64_t K) {
 
 using namespace tlq;
 
-extern "C" int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k) {
-  if (M <= 0 || E < 1 || top_k < 1 || E > kMaxExperts || top_k > 64 || M >= ((int64_t)1 << 24)) return 0;
-  return plan_bytes(E, M * top_k);
+extern "C" int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
+  const int64_t plan = plan_workspace(M, E, top_k, N, K), chunks = plan ? most_chunks<true>(M * top_k, E, N, K) : 0;
+  return plan + (chunks > 1 ? chunks * M * top_k * 2 * N * 4 : 0);
 }
 
 extern "C" int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
-  const int64_t plan = tlq_moe_gate_up_workspace_bytes(M, E, top_k);
-  if (plan == 0 || N < 1 || N >= ((int64_t)1 << 24) || K < 1 || K >= ((int64_t)1 << 24)) return 0;
-  return plan + down_chunks(M * top_k, E, N, K) * M * top_k * N * 4;
+  const int64_t plan = plan_workspace(M, E, top_k, N, K);
+  return plan + (plan ? most_chunks<false>(M * top_k, E, N, K) * M * top_k * N * 4 : 0);
 }
 
 extern "C" int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void* w_packed, const void* scales, const void* zeros, void* H,
@@ -927,7 +973,7 @@ extern "C" int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void*
   TLQ_REQUIRE(X && ids && w_packed && H, "%s: null pointer", what);
   TLQ_REQUIRE(aligned16(X) && aligned16(w_packed) && aligned16(H) && aligned16(scales) && aligned16(zeros) && ((uintptr_t)ids & 3) == 0,
               "%s: X, w_packed, scales, zeros and H must be 16-byte aligned, ids to their type", what);
-  const int64_t want = tlq_moe_gate_up_workspace_bytes(M, E, top_k);
+  const int64_t want = tlq_moe_gate_up_workspace_bytes(M, E, top_k, N, K);
   TLQ_REQUIRE(workspace && workspace_bytes >= want && aligned16(workspace), "%s: a 16-byte aligned workspace of %lld bytes is wanted (got %lld)", what,
               (long long)want, (long long)(workspace ? workspace_bytes : 0));
   ExpertArgs a{X, (const uint8_t*)w_packed, scales, zeros, nullptr, H, (int)E, (int)top_k, (int)N, (int)K, (int)group, zero_scalar};
