@@ -65,22 +65,23 @@ __device__ __forceinline__ int rounds_of(int large, int small, int groups) { ret
 
 // One work-group per expert, and one more for the pairs without one: each looks at all pairs and writes down its own.  A wavefront takes
 // a run of pairs, so that a pair's place is that of its wavefront, its step and its lane; sixteen steps' ids are asked for at once (65536 pairs of 64
-// experts: one by one, with an LDS histogram of all experts, 44 us).
-template <bool COMPACT>
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ totals,
+// experts: one by one, with an LDS histogram of all experts, 44 us).  Up to 1024 pairs 256 threads, which come and go faster (layer of 16 tokens on 8 of
+// 256 experts of 1024 x 4096: 180 -> 174 us for two plans; 128 tokens on 8 of 512 of 512 x 1024, gate / up 50 -> 45).
+template <bool COMPACT, int THREADS>
+__global__ __launch_bounds__(THREADS) void moe_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ totals,
                                                                int32_t* __restrict__ order, PlanTile* __restrict__ small,
                                                                PlanTile* __restrict__ large, int pairs, int E, int rows, int with_large) {
-  constexpr int waves = kPlanThreads / 64, AHEAD = COMPACT ? kCompactPairs / kPlanThreads : 16;
+  constexpr int waves = THREADS / 64, AHEAD = COMPACT ? 4 : 16;
   __shared__ int32_t count[COMPACT ? kMaxExperts + 1 : 1];
   __shared__ int32_t part[waves][4];
   __shared__ int32_t tiles_of[kFromChoices][2];  // large and small tiles that each choice makes
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = blockIdx.x;
   if (COMPACT) {
-    for (int i = tid; i <= E; i += kPlanThreads) count[i] = 0;
+    for (int i = tid; i <= E; i += THREADS) count[i] = 0;
     if (tid < 2 * kFromChoices) tiles_of[tid >> 1][tid & 1] = 0;
     __syncthreads();
   }
-  const int steps = (pairs + kPlanThreads - 1) / kPlanThreads;
+  const int steps = (pairs + THREADS - 1) / THREADS;
   const int first = wave * steps * 64;
   // f(a pair, its expert or E, whether there is one) for every step of this wavefront
   auto each = [&](auto&& f) __attribute__((always_inline)) {
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
     if (with_large) {  // (the same in every work-group)
       for (int c = 0; c < kFromChoices; ++c) {
         int l = 0, m = 0;
-        for (int i = tid; i < E; i += kPlanThreads) {
+        for (int i = tid; i < E; i += THREADS) {
           const int n = large_tiles(count[i], from_choice(c)), left = count[i] - n * kLargeRows;
           l += n, m += left > 0 ? (left + rows - 1) / rows : 0;
         }
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
         if (rounds < best) best = rounds, from = from_choice(c);
       }
     }
-    for (int i = tid; i < e; i += kPlanThreads) {
+    for (int i = tid; i < e; i += THREADS) {
       const int l = with_large ? large_tiles(count[i], from) : 0, left = count[i] - l * kLargeRows;
       fewer += count[i], large_before += l, small_before += left > 0 ? (left + rows - 1) / rows : 0;
     }
@@ -153,12 +154,12 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
     large_end = e < E ? (fewer + mine) / kLargeRows + e + 1 : large_before;
   }
   if (with_large) {
-    for (int i = tid; i < large_end - large_before; i += kPlanThreads) {
+    for (int i = tid; i < large_end - large_before; i += THREADS) {
       const int at = i * kLargeRows, n = i < my_large ? (mine - at < kLargeRows ? mine - at : kLargeRows) : 0;
       large[large_before + i] = PlanTile{e, fewer + at, n, 0};
     }
   }
-  for (int i = tid; i < small_end - small_before; i += kPlanThreads) {
+  for (int i = tid; i < small_end - small_before; i += THREADS) {
     const int at = my_large * kLargeRows + i * rows, n = i < my_small ? (mine - at < rows ? mine - at : rows) : 0;
     small[small_before + i] = PlanTile{e, fewer + at, n, 0};
   }
@@ -876,10 +877,13 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
   float* const parts = UP && *chunks > 1 ? (float*)((uint8_t*)ws + plan_bytes(x.E, pairs)) : nullptr;
   const int64_t grid = z.small * n_groups * *chunks;
   TLQ_REQUIRE(grid < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
-  if (pairs > kCompactPairs)
-    moe_plan_kernel<false><<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, large ? (int)moe_panel_groups(x.N, UP) : 0);
-  else
-    moe_plan_kernel<true><<<x.E + 1, kPlanThreads, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, large ? (int)moe_panel_groups(x.N, UP) : 0);
+#define TLQ_PLAN(COMPACT, THREADS)                                                                                                          \
+  moe_plan_kernel<COMPACT, THREADS><<<x.E + 1, THREADS, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, \
+                                                                 large ? (int)moe_panel_groups(x.N, UP) : 0)
+  if (pairs > kCompactPairs) TLQ_PLAN(false, kPlanThreads);
+  else if (pairs > kCompactPairs / 4) TLQ_PLAN(true, kPlanThreads);
+  else TLQ_PLAN(true, kPlanThreads / 4);
+#undef TLQ_PLAN
   if (!check_launch(what, "moe_plan_kernel")) return 1;
   if (z.large > 0) {
     const Plan plan{p.order, p.small, p.large, p.totals};
@@ -918,8 +922,9 @@ bool few_pairs(bool up, int64_t pairs, int64_t E, int64_t N) {
 // 8 of 14336 x 4096, 12 155 / 163, 24 188 / 184, 40 268 / 221; down of 8 of 4096 x 14336, 12 94 / 97, 24 117 / 105; 16 of 2048 x 4096, 24 38.3 / 41.5, 40 50.7 / 44.5.
 //   256 beside 64: where the plan can count what they make (choose by rounds, above), or with long enough rows and many pairs.  (64 / 256) gate / up of
 // 64 experts of 1408 x 2048, 192 pairs each 235 / 266, 256 305 / 303, 768 791 / 615; 128 of 768 x 2048, 256 325 / 318, 768 871 / 659; down of 64 of
-// 2048 x 1408, 256 193 / 224, 768 514 / 525; 128 of 2048 x 768, 768 750 / 796; 16 of 2048 x 4096, 768 326 / 325.
-constexpr int kTilesOf64 = 24, kTilesOf256 = 256;
+// 2048 x 1408, 256 193 / 224, 768 514 / 525; 128 of 2048 x 768, 768 750 / 796; 16 of 2048 x 4096, 768 326 / 325; gate / up with shorter rows, 64 of
+// 1984 x 1536, 300 375 / 343, 640 737 / 579; 32 of 4096 x 1024, 300 284 / 302, 640 548 / 457; 64 of 2048 x 512, 300 165 / 178, 640 320 / 296.
+constexpr int kTilesOf64 = 24, kTilesOf256 = 256, kTilesOf256Short = 448;
 
 template <bool UP>
 int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st) {
@@ -930,7 +935,8 @@ int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t 
   }
   if (pairs / a.E < kTilesOf64) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
   const int64_t large_groups = pairs / kLargeRows * moe_panel_groups(a.N, UP);
-  const bool large = (pairs > kCompactPairs ? a.K >= 2048 && pairs / a.E >= kTilesOf256 && large_groups >= 512 : large_groups >= 192) && moe_panel_takes(a, pairs, UP);
+  const bool long_rows = a.K >= (UP ? 1536 : 2048), many = UP && a.K >= 512 && !long_rows ? pairs / a.E >= kTilesOf256Short : long_rows && pairs / a.E >= kTilesOf256;
+  const bool large = (pairs > kCompactPairs ? many && large_groups >= 512 : large_groups >= 192) && moe_panel_takes(a, pairs, UP);
   return run_tiles<UP, 4, 2, 1>(what, a, ids, pairs, dtype, ws, chunks, st, large);
 }
 
