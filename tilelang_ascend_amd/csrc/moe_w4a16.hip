@@ -194,20 +194,26 @@ __device__ __forceinline__ void direct4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 
+// A zero point that is a small integer can be folded into the unpacking's bias.  In bfloat16 that is worth it (gate / up of 64 experts of 1408 x 2048,
+// 400 tokens on 6: 75 us, 98 the other way) and a tensor of zero points is looked at block by block; binary16 subtracts two values in one instruction
+// and takes the other way always: 80 -> 73 us, with no look at the zero points and registers for four work-groups on a CU.
+template <typename T>
+constexpr bool kFolds = !std::is_same<T, half_t>::value;
+
 // ---- tiles of many pairs ----------------------------------------------------------------------------------------------------
 // Up to 16 MAXMT pairs of one expert x NT tiles of 16 weight rows for each of four wavefronts (a tile: 16 outputs, or 8 gate rows and the 8
 // up rows that go with them).  K goes by in steps of KSB blocks of 128 values: the activation rows are gathered global -> LDS into
 // two buffers a step ahead, the packed weights go straight into operand registers a step ahead -- lane (r16, q) has the 32 values 32 q ..
 // of each block of row r16, at MFMA k-step j the eight of word 4 q + j --, are expanded there and multiplied with all rows: a weight
 // is expanded once per 16 MAXMT pairs, an activation operand read once per NT tiles.  One barrier a step.
-//   64 pairs: fp16, zero points, 211 tokens on 2 of 8 experts of 14336 x 4096 (gate / up): 222 - 250 us, of the vector units' time 57 % (13
-// instructions expand eight weights), of the matrix units' 26 %; the rest is the trip of a step's loads.  With 64 rows of W a wavefront in the
+//   64 pairs: fp16, zero points, 211 tokens on 2 of 8 experts of 14336 x 4096 (gate / up): 246 us; the vector units were busy for
+// 57 % of it, the matrix units for 26 %; the rest is the trip of a step's loads.  With 64 rows of W a wavefront in the
 // place of 32 (NT = 4) 5 - 10 % slower -- fewer work-groups on a CU, coarser rounds --; with 128 pairs level where experts have 192 pairs and more, 10 - 30 % slower
 // below; tiles of an expert side by side on the same weight rows 3 - 6 % faster on matrices of 58 MB, 2 - 8 % slower on small ones.
 //   32 pairs: bf16, 48 tokens on 8 of 128 experts of 768 x 2048 (gate / up): 35 - 40 us for 199 MB, the rate of a large copy.
 //   Scales and zero points come through LDS in windows of eight groups (whole steps: 8 groups are 256 (group / 32) values), loaded a window
-// ahead as the 16-byte pieces of a row that hold them (two, unless rows are whole pieces).  ANY: zero points that need not be small integers, which are folded into the
-// unpacking's bias (a tensor, looked at block by block, or such a scalar).
+// ahead as the 16-byte pieces of a row that hold them (two, unless rows are whole pieces).  ANY: zero points that need not be small integers (a tensor, or
+// such a scalar).
 struct TileArgs {
   const void* X;
   const uint8_t* Wp;
@@ -236,7 +242,7 @@ struct TileCfg {
 };
 
 template <typename T, bool UP, bool ANY, int MAXMT, int NT, int KSB>
-__global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_kernel(const TileArgs a) {
+__global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel(const TileArgs a) {
   typedef typename MmaOf<T>::type Mma;
   typedef TileCfg<MAXMT, NT, KSB> Cfg;
   typedef __attribute__((address_space(3))) uint8_t* lptr_t;
@@ -386,7 +392,7 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
         for (int t = 0; t < NT; ++t) {
           sv[t] = a.scales ? ((const T*)sc)[sc_at[t] + g] : one;
           zv[t] = ANY && a.zeros ? ((const T*)zp)[sc_at[t] + g] : zs;
-          if (ANY) whole = whole && small_integer(to_float(zv[t]));
+          if (ANY && kFolds<T>) whole = whole && small_integer(to_float(zv[t]));
         }
         if ((s * KSB + b) * 128 + 128 > a.K) {  // (uniform) behind K: zeros, not an infinite weight times zero
 #pragma unroll
@@ -409,14 +415,16 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               const uint32_t word = j == 0 ? w[b][t].x : j == 1 ? w[b][t].y : j == 2 ? w[b][t].z : w[b][t].w;
-              if constexpr (!decltype(fold_tag)::value) __builtin_amdgcn_sched_barrier(0);  // (few registers rather than fast)
+              if constexpr (kFolds<T> && !decltype(fold_tag)::value) __builtin_amdgcn_sched_barrier(0);  // (few registers rather than fast)
               const uint4_t wo = ex[t](word);
 #pragma unroll
               for (int m = 0; m < MT; ++m) acc[t][m] = Mma::mma(wo, x[m], acc[t][m]);
             }
           }
         };
-        if constexpr (ANY) {
+        if constexpr (!kFolds<T>) {
+          multiply(std::false_type{});
+        } else if constexpr (ANY) {
           if (__builtin_expect(__builtin_amdgcn_ballot_w64(whole) == ~0ull, 1)) multiply(std::true_type{});
           else multiply(std::false_type{});
         } else {
@@ -463,7 +471,7 @@ __global__ __launch_bounds__(256, MAXMT >= 4 ? 2 : ANY ? 3 : 4) void moe_tile_ke
 //   A tile is 16 weight rows: 16 outputs, or 8 gate rows and the 8 up rows that go with them.  A block is 128 values of K of a tile.
 // Where tiles are few, `splits` wavefronts share one, each with a part of K; their sums meet in LDS and are added in the order of K.
 // Long rows of the down product are cut into `chunks` work-groups too, whose sums moe_combine_kernel adds.
-//   fp16, zero points: one token, 6 of 64 experts of 1408 x 2048, gate / up 11 us (18 MB), down 9.4; 2 of 8 of 4096 x 14336, down 24 us + 4 for the sums
+//   fp16, zero points: one token, 6 of 64 experts of 1408 x 2048, gate / up 10.3 us (18 MB), down 9.3; 2 of 8 of 4096 x 14336, down 21 us + 4 for the sums
 // (66 MB, 13.4 us at the rate of a large copy).  What is left is latency: ids, then rows and scales, then 28 KB of weights a wavefront, 4 KB at a time.  With
 // eight blocks asked for at once the kernel spills and takes 25 - 40 % more.
 constexpr int kFewPairs = 2048;
@@ -668,7 +676,9 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[j & 1] = Mma::mma(ex(words[j]), *(const uint4_t*)(x + j * 16), acc[j & 1]);
         };
-        if constexpr (ANY) {
+        if constexpr (!kFolds<T>) {
+          multiply(std::false_type{});
+        } else if constexpr (ANY) {
           if (__builtin_expect(__builtin_amdgcn_ballot_w64(small_integer(to_float(zv))) == ~0ull, 1)) multiply(std::true_type{});
           else multiply(std::false_type{});
         } else {
