@@ -219,7 +219,7 @@ struct TileArgs {
   const uint8_t* Wp;
   const void* scales;
   const void* zeros;
-  const float* weights;
+  float* weights;  // down: of the pairs; gate / up in parts of K: the sums to write, [part][pair][2 N], otherwise null
   void* out;
   const PlanTile* tiles;
   const int32_t* order;  // (how many tiles there are: at order[-64])
@@ -229,7 +229,6 @@ struct TileArgs {
   int n_groups;        // work-groups side by side
   int window;          // steps of a window
   int chunk_steps;     // steps of a work-group: those of a part of K (few tiles), whose sums moe_combine_kernel or moe_gate_kernel adds
-  float* parts;        // gate / up in parts of K: the sums [part][pair][2 N], else null
 };
 
 template <int MAXMT, int NT, int KSB>
@@ -263,7 +262,7 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
   const int n_tiles = a.N / OUTS, tile0 = group_no * Cfg::TILES;
   if (e == a.E) {  // pairs without an expert
     if constexpr (UP) {
-      if (a.parts) return;  // (moe_gate_kernel writes their zeros)
+      if (a.weights) return;  // (moe_gate_kernel writes their zeros)
       T* const h = (T*)a.out;
       constexpr int width = Cfg::TILES * OUTS;
       for (int i = tid; i < rows * width; i += 256) {
@@ -445,9 +444,9 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
       const int n = (tile0 + wave * NT + t) * OUTS + q * 4;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        if (UP && a.parts) {  // this lane's four gates (q = 0, 1) or ups
+        if (UP && a.weights) {  // this lane's four gates (q = 0, 1) or ups
           if (m * 16 + r16 < rows && tile0 + wave * NT + t < n_tiles)
-            *(float4_t*)(a.parts + ((int64_t)chunk * a.pairs + pair[m]) * (2 * (int64_t)a.N) + (q >= 2 ? a.N - 8 : 0) + n) = acc[t][m];
+            *(float4_t*)(a.weights + ((int64_t)chunk * a.pairs + pair[m]) * (2 * (int64_t)a.N) + (q >= 2 ? a.N - 8 : 0) + n) = acc[t][m];
           continue;
         }
         moe_store<T, UP>(a, acc[t][m], m * 16 + r16 < rows && tile0 + wave * NT + t < n_tiles, pair[m], weight[m], n, q, chunk);
@@ -901,8 +900,8 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
   }
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
-  const TileArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
-                   units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps, parts};
+  const TileArgs a{x.X, x.Wp, x.scales, x.zeros, UP ? parts : const_cast<float*>(x.weights), x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
+                   units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};
 #define TLQ_TILES(T) (x.zeros || !whole ? launch_tiles<T, UP, true, MAXMT, NT, KSB>(what, a, grid, st) : launch_tiles<T, UP, false, MAXMT, NT, KSB>(what, a, grid, st))
   if (dtype == TLQ_F16 ? TLQ_TILES(half_t) : TLQ_TILES(bf16_t)) return 1;
 #undef TLQ_TILES
