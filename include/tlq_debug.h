@@ -111,6 +111,11 @@ int tlq_debug_gemv_rows_plan(int64_t batch, int64_t N, int64_t K, int64_t group,
 int tlq_debug_gemm_tile(int64_t batch, int64_t M, int64_t N, int fused);
 int tlq_debug_gemv_ring_plan(int64_t M, int64_t N, int64_t K, int64_t group, int cus, void* plan_out);
 int tlq_debug_check_gemv_ring_addressing(int64_t M, int64_t N, int64_t K, int64_t group, int rows_per_block, int waves, int depth);
+/* The kernel that a product of the experts (up: gate / up, otherwise down) runs on: 1 few pairs, without a plan; 2 tiles of 32 pairs; 3 tiles of 64; 4 tiles
+ * of 256 with tiles of 64 for what is left.  zeros: with a tensor of zero points.  For 1 plan_out, optional, receives int64 rows of a pass, wavefronts
+ * that share a tile, tiles of a wavefront, parts of K, bytes of LDS that the launch asks for, those that the kernel uses, work-groups of an expert.  0: sizes
+ * that no call takes. */
+int tlq_debug_moe_choice(int up, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, int zeros, void* plan_out);
 
 /* Tuning hooks for benchmark sweeps and the autotuner (each sets a value of the CALLING THREAD, read by that thread's
  * later launches; other threads keep the automatic choice; 0 = automatic choice).

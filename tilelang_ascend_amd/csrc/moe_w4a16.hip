@@ -494,6 +494,22 @@ struct FewArgs {
   int per_wave;          // tiles of a wavefront
 };
 
+// Where what lies in LDS, for the kernel and for the launch: activation rows, sums of the other wavefronts, scales, zero points (with a tensor of them; one
+// that is a number takes no room, whole or not), the rows' weights (down), two words (number of pairs, an earlier pair has this expert), the pairs.
+struct FewLds {
+  int sums, scales, zeros, weights, head, list;
+};
+__host__ __device__ inline FewLds few_lds(bool up, bool zeros, int waves, int splits, int wg_tiles, int row_cap, int pitch, int pieces) {
+  FewLds l;
+  l.sums = row_cap * pitch;
+  l.scales = l.sums + waves / splits * (splits - 1) * 1024;
+  l.zeros = l.scales + wg_tiles * 256 * pieces;
+  l.weights = l.zeros + (zeros ? wg_tiles * 256 * pieces : 0);
+  l.head = l.weights + (up ? 0 : 64);
+  l.list = l.head + 16;
+  return l;
+}
+
 template <typename T, bool UP, bool ANY>
 __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
   typedef typename MmaOf<T>::type Mma;
@@ -517,12 +533,11 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
   const int pitch = wg_blocks * 256 + 16;  // bytes of an activation row: 16 more, so that the rows of an operand lie on different banks
   constexpr int OUTS = UP ? 8 : 16;        // outputs of a tile
   const int wg_tiles = waves / splits * a.per_wave, n_tiles = a.N / OUTS, tile0 = group_no * wg_tiles;
-  // LDS: activation rows, sums of the other wavefronts, scales, zero points, the rows' weights, the pairs
-  const int sums_at = row_cap * pitch, sc_at = sums_at + waves / splits * (splits - 1) * 1024, zp_at = sc_at + wg_tiles * 256 * pieces;
+  const FewLds at_lds = few_lds(UP, ANY && a.zeros, waves, splits, wg_tiles, row_cap, pitch, pieces);
+  const int sums_at = at_lds.sums, sc_at = at_lds.scales, zp_at = at_lds.zeros, weights_at = at_lds.weights;
   uint8_t* const act = smem;
-  const int weights_at = zp_at + (ANY ? wg_tiles * 256 * pieces : 0);
-  int32_t* const head = (int32_t*)(smem + weights_at + (UP ? 0 : 64));  // [0] number of pairs, [1] an earlier pair has this expert
-  uint16_t* const list = (uint16_t*)(head + 4);
+  int32_t* const head = (int32_t*)(smem + at_lds.head);  // [0] number of pairs, [1] an earlier pair has this expert
+  uint16_t* const list = (uint16_t*)(smem + at_lds.list);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)smem);
 
   const int e = by_pair ? __builtin_amdgcn_readfirstlane(a.ids[who]) : who;
@@ -813,7 +828,7 @@ FewPlan few_plan(bool up, int64_t pairs, int64_t E, int64_t top_k, int64_t N, in
   if (p.by_pair && pairs == top_k) p.row_cap = 1;
   const int64_t wg_tiles = p.waves / p.splits * p.per_wave;
   p.n_groups = (int)ceil_div(n_tiles, wg_tiles);
-  p.lds = p.row_cap * pitch + p.waves / p.splits * (p.splits - 1) * 1024 + (zeros ? 2 : 1) * wg_tiles * 256 * (int64_t)p.pieces + 64 + 16 + ceil_div(pairs, (int64_t)8) * 16;
+  p.lds = few_lds(up, zeros, p.waves, p.splits, (int)wg_tiles, p.row_cap, (int)pitch, p.pieces).list + ceil_div(pairs, (int64_t)8) * 16;
   p.units = (p.by_pair ? pairs : E + (up ? 1 : 0)) * p.n_groups;
   p.grid = p.chunks == 1 ? p.units : ceil_div(p.units, (int64_t)8) * 8 * p.chunks;
   p.ok = p.lds <= 160 * 1024 && p.grid < ((int64_t)1 << 31);
@@ -935,18 +950,28 @@ bool few_pairs(bool up, int64_t pairs, int64_t E, int64_t N) {
 // 1984 x 1536, 300 375 / 343, 640 737 / 579; 32 of 4096 x 1024, 300 284 / 302, 640 548 / 457; 64 of 2048 x 512, 300 165 / 178, 640 320 / 296.
 constexpr int kTilesOf64 = 24, kTilesOf256 = 256, kTilesOf256Short = 448;
 
+enum { kMoeFew = 1, kMoeTiles32 = 2, kMoeTiles64 = 3, kMoeTiles256 = 4 };
+int choose_kernel(bool up, const ExpertArgs& a, int64_t pairs, FewPlan* few) {
+  if (few_pairs(up, pairs, a.E, a.N)) {
+    *few = few_plan(up, pairs, a.E, a.top_k, a.N, a.K, a.group, a.zeros != nullptr);
+    if (few->ok && (pairs <= 2 * few->row_cap * a.top_k || pairs * 16 <= (int64_t)a.E * few->row_cap)) return kMoeFew;
+  }
+  if (pairs / a.E < kTilesOf64) return kMoeTiles32;
+  const int64_t large_groups = pairs / kLargeRows * moe_panel_groups(a.N, up);
+  const bool long_rows = a.K >= (up ? 1536 : 2048), many = up && a.K >= 512 && !long_rows ? pairs / a.E >= kTilesOf256Short : long_rows && pairs / a.E >= kTilesOf256;
+  return (pairs > kCompactPairs ? many && large_groups >= 512 : large_groups >= 192) && moe_panel_takes(a, pairs, up) ? kMoeTiles256 : kMoeTiles64;
+}
+
 template <bool UP>
 int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t pairs, int dtype, void* ws, int64_t* chunks, hipStream_t st) {
-  if (few_pairs(UP, pairs, a.E, a.N)) {
-    const FewPlan few = few_plan(UP, pairs, a.E, a.top_k, a.N, a.K, a.group, a.zeros != nullptr);
+  FewPlan few;
+  const int kernel = choose_kernel(UP, a, pairs, &few);
+  if (kernel == kMoeFew) {
     *chunks = few.chunks;
-    if (few.ok && (pairs <= 2 * few.row_cap * a.top_k || pairs * 16 <= (int64_t)a.E * few.row_cap)) return run_few<UP>(what, a, ids, pairs, dtype, few, st);
+    return run_few<UP>(what, a, ids, pairs, dtype, few, st);
   }
-  if (pairs / a.E < kTilesOf64) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
-  const int64_t large_groups = pairs / kLargeRows * moe_panel_groups(a.N, UP);
-  const bool long_rows = a.K >= (UP ? 1536 : 2048), many = UP && a.K >= 512 && !long_rows ? pairs / a.E >= kTilesOf256Short : long_rows && pairs / a.E >= kTilesOf256;
-  const bool large = (pairs > kCompactPairs ? many && large_groups >= 512 : large_groups >= 192) && moe_panel_takes(a, pairs, UP);
-  return run_tiles<UP, 4, 2, 1>(what, a, ids, pairs, dtype, ws, chunks, st, large);
+  if (kernel == kMoeTiles32) return run_tiles<UP, 2, 2, 2>(what, a, ids, pairs, dtype, ws, chunks, st);
+  return run_tiles<UP, 4, 2, 1>(what, a, ids, pairs, dtype, ws, chunks, st, kernel == kMoeTiles256);
 }
 
 // the most that any of them cuts K into
@@ -1020,4 +1045,18 @@ extern "C" int tlq_moe_down_w4a16(const void* H, const void* ids, const void* we
   moe_combine_kernel<<<(unsigned)(M * n_groups), 256, 0, st>>>(rows, (const int32_t*)ids, Y, (int)N, (int)n_groups, (int)top_k, (int)E, out_dtype,
                                                                  (int)chunks, pairs * N);
   return check_launch(what, "moe_combine_kernel") ? 0 : 1;
+}
+
+extern "C" int tlq_debug_moe_choice(int up, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, int zeros, void* plan_out) {
+  if (check_experts("tlq_debug_moe_choice", M, E, top_k, N, K, group, TLQ_F16) || M == 0) return 0;
+  const ExpertArgs a{nullptr, nullptr, nullptr, zeros ? (const void*)16 : nullptr, nullptr, nullptr, (int)E, (int)top_k, (int)N, (int)K, (int)group, 0.0f};
+  FewPlan few;
+  const int kernel = choose_kernel(up != 0, a, M * top_k, &few);
+  if (plan_out && kernel == kMoeFew) {
+    const int wg_tiles = few.waves / few.splits * few.per_wave;
+    const FewLds l = few_lds(up != 0, zeros != 0, few.waves, few.splits, wg_tiles, few.row_cap, few.blocks * 256 + 16, few.pieces);
+    const int64_t plan[7] = {few.row_cap, few.splits, few.per_wave, few.chunks, few.lds, l.list + M * top_k * 2, few.n_groups};
+    for (int i = 0; i < 7; ++i) ((int64_t*)plan_out)[i] = plan[i];
+  }
+  return kernel;
 }
