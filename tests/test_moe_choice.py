@@ -61,3 +61,46 @@ def test_few_pairs_use_no_more_lds_than_they_ask_for(M, E, k, N, K, group, up):
 @pytest.mark.parametrize("M,E,k,N,K,group", FRACTIONAL)
 def test_few_pairs_with_a_zero_point_that_does_not_fold(M, E, k, N, K, group, zeros, dtype, up):
     run_both(up, M, E, k, N, K, group, dtype, zeros, "spread")
+
+
+# ---- groups of millions of values -----------------------------------------------------------------------------------------------
+def test_the_group_of_a_value_for_groups_of_any_size():
+    group_of = _abi.load().tlq_debug_moe_group
+    longest = (1 << 24) // 32
+    for units in [*range(1, 70), 127, 128, 4096, 5461, 65535, 65536, 65537, 65538, 98304, 131071, 131073, 262143, longest - 1]:
+        edges = {u for q in {1, 2, 3, longest // units - 1, longest // units} for u in (q * units - 1, q * units, q * units + 1)}
+        for u in sorted({0, 1, longest - 1, *edges}):
+            if 0 <= u < longest:
+                assert group_of(units * 32, u) == u // units, (units, u)
+
+
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("K,group", [(2097184, 2097184), (6291456, 3145728)])
+def test_scales_of_groups_of_millions_of_values(K, group, up):
+    """Activations other than 0 at both ends of each group alone, so that the bound of the sums (which counts K additions) is a part of these
+    few products; neighbouring rows' scales are eight times apart."""
+    E, N = 2, 16
+    rows = 2 * N if up else N
+    g = gen(41)
+    Wp = torch.randint(0, 256, (E, rows, K // 2), dtype=torch.uint8, generator=g)
+    s = (2.0 ** -(4 + 3 * (torch.arange(E * rows * (K // group)) % 2)).view(E, rows, K // group)).half()
+    x = torch.zeros(1, K)
+    for at in range(0, K, group):
+        x[0, at:at + 32] = 1.0
+        x[0, at + group - 32:at + group] = torch.rand(32, generator=g) + 0.5
+    x, ids = x.half(), torch.tensor([[1]], dtype=torch.int32)
+    small = (x[0] != 0).nonzero()[:, 0]
+    d = ref.dequant_w4(Wp[1], s[1], 0, group, torch.float16)[:, small].double() @ x[0, small].double()  # (no weight is negative: the sum of magnitudes too)
+    # the zeros add nothing and lose nothing: as many additions as there are other values
+    off = d * (len(small) + 8) * 2.0**-24
+    if up:
+        got = ops.moe_gate_up_w4a16(E, 1, N, K, group)(*operands(x, ids, Wp, s))[0, 0]
+        gate, u = d.chunk(2)
+        dg, du = off.chunk(2)
+        want = gate / (1 + torch.exp(-gate)) * u
+        allowed = 1.1 * dg * (u + du) + gate * du + (gate + 4) * 2.0**-22 * want
+    else:
+        got = ops.moe_down_w4a16(E, 1, N, K, group, out_dtype="float32")(*operands(x[:, None], ids, torch.ones(1, 1), Wp, s))[0]
+        want, allowed = d, off + (d + off) * 3 * 2.0**-24
+    assert_close64(got, want, allowed, f"K={K} group={group} up={up}")

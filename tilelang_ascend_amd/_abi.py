@@ -106,6 +106,7 @@ SIGNATURES = {
     "tlq_tune_gemm_slots": (None, [_int]),
     "tlq_tune_gemm_tile": (None, [_int]),
     "tlq_debug_moe_choice": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp]),
+    "tlq_debug_moe_group": (_i64, [_i64, _i64]),
     "tlq_debug_gemm_tile": (_int, [_i64, _i64, _i64, _int]),
     "tlq_tune_w4a16_stream": (None, [_int]),
     "tlq_tune_w4a16_stream_slice": (None, [_int]),

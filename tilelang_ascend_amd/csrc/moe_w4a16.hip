@@ -214,6 +214,21 @@ constexpr bool kFolds = !std::is_same<T, half_t>::value;
 //   Scales and zero points come through LDS in windows of eight groups (whole steps: 8 groups are 256 (group / 32) values), loaded a window
 // ahead as the 16-byte pieces of a row that hold them (two, unless rows are whole pieces).  ANY: zero points that need not be small integers (a tensor, or
 // such a scalar).
+// u / units for u below 2^30: with 2^shift <= units < 2^(shift + 1) and mul = ceil(2^(31 + shift) / units), mul * units is at most units - 1 < 2^(shift + 1)
+// more than 2^(31 + shift), so that u * mul / 2^(31 + shift) is less than 2 u / 2^31 / units <= 1 / units above u / units: the same whole number below.
+// (One multiplication and one shift, a power of two or not; a reciprocal of 32 bits alone, ceil(2^32 / units), is wrong from units of 65537 on.)
+struct GroupOf {
+  uint32_t mul;
+  int32_t shift;
+  __host__ __device__ __forceinline__ int operator()(int u) const { return (int)((uint32_t)(((uint64_t)((uint32_t)u * 2) * mul) >> 32) >> shift); }
+};
+inline GroupOf make_group_of(int units) {
+  GroupOf g{0, 0};
+  while ((units >> g.shift) > 1) ++g.shift;
+  g.mul = (uint32_t)((((uint64_t)1 << (31 + g.shift)) + units - 1) / units);
+  return g;
+}
+
 struct TileArgs {
   const void* X;
   const uint8_t* Wp;
@@ -224,7 +239,7 @@ struct TileArgs {
   const PlanTile* tiles;
   const int32_t* order;  // (how many tiles there are: at order[-64])
   int pairs, E, top_k, N, K, groups;
-  uint32_t per_group;  // ceil(2^32 / (group / 32)), 0 for groups of 32
+  GroupOf group_of;    // of the u-th 32 values of a row
   float zero_scalar;
   int n_groups;        // work-groups side by side
   int window;          // steps of a window
@@ -325,7 +340,6 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
   };
   // scales of window v: pieces (row * groups) / 8 + v and the next one of every row (the tensors' sizes are multiples of 16 bytes, so that
   // no piece reaches past their ends)
-  auto group_of = [&](int u) __attribute__((always_inline)) -> int { return a.per_group ? (int)__umulhi((uint32_t)u, a.per_group) : u; };
   const int window = a.window;
   const int64_t sc_e = (int64_t)e * (UP ? 2 : 1) * a.N * a.groups;  // the expert's first value: a multiple of eight
   const uint32_t sc_last = (uint32_t)((UP ? 2 : 1) * a.N * a.groups / 8 - 1) * 16;
@@ -384,7 +398,7 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
       const int buf = (v & 1) * (window_bytes / 2);
 #pragma unroll
       for (int b = 0; b < KSB; ++b) {
-        const int u = (s * KSB + b) * 4 + q, g = group_of(u < u_last ? u : u_last) - 8 * v + buf;
+        const int u = (s * KSB + b) * 4 + q, g = a.group_of(u < u_last ? u : u_last) - 8 * v + buf;
         T sv[NT], zv[NT];
         bool whole = true;
 #pragma unroll
@@ -486,7 +500,7 @@ struct FewArgs {
   const int32_t* ids;
   void* out;
   int pairs, E, top_k, N, K, groups;
-  uint32_t per_group;    // ceil(2^32 / (group / 32)), 0 for groups of 32
+  uint32_t per_group;    // ceil(2^32 / (group / 32)), 0 for groups of 32 (rows of at most 65536 values: exact)
   float zero_scalar;
   int n_groups, units;   // work-groups of an expert side by side, and of all experts
   uint32_t blocks;       // blocks of 128 values of K of a work-group | 16-byte pieces of a row's scales << 16
@@ -916,7 +930,7 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
   const TileArgs a{x.X, x.Wp, x.scales, x.zeros, UP ? parts : const_cast<float*>(x.weights), x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
-                   units == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + units - 1) / units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};
+                   make_group_of(units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};
 #define TLQ_TILES(T) (x.zeros || !whole ? launch_tiles<T, UP, true, MAXMT, NT, KSB>(what, a, grid, st) : launch_tiles<T, UP, false, MAXMT, NT, KSB>(what, a, grid, st))
   if (dtype == TLQ_F16 ? TLQ_TILES(half_t) : TLQ_TILES(bf16_t)) return 1;
 #undef TLQ_TILES
@@ -1060,3 +1074,5 @@ extern "C" int tlq_debug_moe_choice(int up, int64_t M, int64_t E, int64_t top_k,
   }
   return kernel;
 }
+
+extern "C" int64_t tlq_debug_moe_group(int64_t group, int64_t u) { return make_group_of((int)(group / 32))((int)u); }
