@@ -407,7 +407,7 @@ int tlq_moe_route(const void* logits, const void* bias, void* weights, void* ids
  * N % 16 == 0, K % 32 == 0, N * K < 2^32, group a multiple of 32 that divides K, E <= 1024, top_k <= 64, M * top_k < 2^24.  X, H, Y, w_packed,
  * scales and zeros 16-byte aligned.  Results do not depend on timing: no floating-point sum is formed by atomic adds.
  * The workspace (16-byte aligned, at least tlq_moe_*_workspace_bytes) holds nothing between calls; two calls that may run at the
- * same time need one each. */
+ * same time need one each.  The size does not fall as M grows: that of a program's largest call does for its others of the same sizes. */
 int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K);
 int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K);
 int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void* w_packed, const void* scales, const void* zeros, void* H,

@@ -104,3 +104,43 @@ def test_scales_of_groups_of_millions_of_values(K, group, up):
         got = ops.moe_down_w4a16(E, 1, N, K, group, out_dtype="float32")(*operands(x[:, None], ids, torch.ones(1, 1), Wp, s))[0]
         want, allowed = d, off + (d + off) * 3 * 2.0**-24
     assert_close64(got, want, allowed, f"K={K} group={group} up={up}")
+
+
+# ---- one workspace for a program's calls ------------------------------------------------------------------------------------------
+WORKSPACES = [(8, 2, 4096, 14336), (8, 2, 1024, 4096), (64, 1, 4096, 14336), (128, 8, 1408, 2048), (256, 8, 512, 7168), (3, 2, 16, 64), (1, 1, 16, 8192), (1024, 5, 96, 32)]
+
+
+@pytest.mark.parametrize("E,k,N,K", WORKSPACES)
+def test_a_workspace_for_many_tokens_does_for_fewer(E, k, N, K):
+    lib = _abi.load()
+    for size in (lib.tlq_moe_gate_up_workspace_bytes, lib.tlq_moe_down_workspace_bytes):
+        sizes = [size(M, E, k, N, K) for M in sorted({*range(1, 700), *range(700, 5000, 7), *range(max(1, 4096 // k - 2), 4096 // k + 3), 8192, 100000})]
+        assert sizes == sorted(sizes) and sizes[0] > 0
+
+
+@gpu
+@pytest.mark.parametrize("E,k,N,K", [(8, 2, 256, 8192), (4, 2, 1024, 4096), (64, 1, 64, 14336)])
+def test_calls_of_every_size_in_the_workspace_of_the_largest(E, k, N, K):
+    """M from 1 to the largest in one workspace of the largest one's size, in both products: the rows of the definition, and nothing behind them."""
+    lib, P, most = _abi.load(), _abi.ptr, 300
+    st = torch.cuda.current_stream().cuda_stream
+    T = torch.float16
+    w1, s1, _ = make_experts(E, 2 * N, K, 64, T, 8, 61)
+    X, ids = torch.randn(most, K, generator=gen(62)).to(T), make_ids(most, E, k, "spread", 63)
+    g1 = operands(X, ids, w1, s1)
+    size = lib.tlq_moe_gate_up_workspace_bytes(most, E, k, N, K), lib.tlq_moe_down_workspace_bytes(most, E, k, 2 * N, K)
+    ws = torch.zeros(max(size), dtype=torch.uint8, device="cuda")
+    H = torch.randn(most, k, K, generator=gen(64)).to(T)
+    weights = torch.softmax(torch.randn(most, k, generator=gen(65)), 1)
+    g2 = operands(H, weights)
+    for M in (1, 2, 3, 5, 16, 31, 32, 33, 70, 140, 287, 288, 300):
+        h = torch.full((most, k, N), float("nan"), dtype=T, device="cuda")
+        _abi.check(lib.tlq_moe_gate_up_w4a16(P(g1[0]), P(g1[1]), P(g1[2]), P(g1[3]), None, P(h), P(ws), size[0], M, E, k, N, K, 64, 8.0, _abi.F16, st))
+        some = torch.tensor(sorted({0, M // 2, M - 1}))
+        assert_close64(h[some.cuda()], *ref.moe_gate_up(X[some], ids[some], w1, s1, 8, 64), f"gate_up M={M}")
+        assert not bool(h[:M].isnan().any()) and bool(h[M:].isnan().all())
+        y = torch.full((most, 2 * N), float("nan"), device="cuda")
+        _abi.check(lib.tlq_moe_down_w4a16(P(g2[0]), P(g1[1]), P(g2[1]), P(g1[2]), P(g1[3]), None, P(y), P(ws), size[1], M, E, k, 2 * N, K, 64, 8.0, _abi.F16,
+                                          _abi.F32, st))
+        assert_close64(y[some.cuda()], *ref.moe_down(H[some], ids[some], weights[some], w1, s1, 8, 64), f"down M={M}")
+        assert not bool(y[:M].isnan().any()) and bool(y[M:].isnan().all())

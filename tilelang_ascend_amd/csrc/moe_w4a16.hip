@@ -52,9 +52,10 @@ inline int64_t plan_bytes_of(int64_t E, int64_t pairs, int64_t rows, bool large)
   const PlanSizes z = plan_sizes(E, pairs, rows, large);
   return 256 + align256(pairs * 4) + align256(z.small * 16) + align256(z.large * 16);
 }
-inline int64_t plan_bytes(int64_t E, int64_t pairs) {
+inline int64_t plan_bytes(int64_t E, int64_t pairs) {  // of these pairs and of fewer
   const int64_t a = plan_bytes_of(E, pairs, 32, false), b = plan_bytes_of(E, pairs, 64, false), c = plan_bytes_of(E, pairs, 64, true);
-  return a > b ? (a > c ? a : c) : (b > c ? b : c);
+  const int64_t most = a > b ? (a > c ? a : c) : (b > c ? b : c), fewer = pairs > kCompactPairs ? plan_bytes(E, kCompactPairs) : 0;
+  return most > fewer ? most : fewer;
 }
 
 // Candidates for `from`: 65, 129, 193, 257 (whole tiles only), and more pairs than there are (none).  A round of large tiles is 256 work-groups,
@@ -988,13 +989,24 @@ int run_experts(const char* what, const ExpertArgs& a, const void* ids, int64_t 
   return run_tiles<UP, 4, 2, 1>(what, a, ids, pairs, dtype, ws, chunks, st, kernel == kMoeTiles256);
 }
 
-// the most that any of them cuts K into
+// The most parts of K times pairs that a product of these pairs or of fewer has sums for: fewer pairs can make more of them (tile_chunks, few_pairs), and a
+// workspace for a program's largest call has to do for the others.  0: no sums of parts (gate / up alone).
 template <bool UP>
-int64_t most_chunks(int64_t pairs, int64_t E, int64_t N, int64_t K) {
-  int64_t c = !UP && few_pairs(UP, pairs, E, N) ? few_chunks(K) : 1;
-  const int64_t small = tile_chunks(about_tiles(pairs, E, 32), tile_groups<UP, 2>(N), K), large = tile_chunks(about_tiles(pairs, E, 64), tile_groups<UP, 2>(N), K);
-  c = c > small ? c : small;
-  return c > large ? c : large;
+int64_t most_rows(int64_t pairs, int64_t E, int64_t top_k, int64_t N, int64_t K) {
+  const int64_t groups = tile_groups<UP, 2>(N);
+  int64_t most = UP ? 0 : pairs;
+  const auto take = [&](int64_t chunks, int64_t up_to) {
+    const int64_t rows = chunks * ((up_to < pairs ? up_to : pairs) / top_k * top_k);
+    most = rows > most ? rows : most;
+  };
+  if (!UP) take(few_chunks(K), E * groups <= 1024 ? 2 * E : 1024 / groups);
+  for (int64_t chunks = 2; chunks <= 8 && K / chunks >= 1024; chunks *= 2) {
+    const int64_t tiles = 1024 / (groups * chunks);  // about_tiles at most
+    if (tiles == 0) break;
+    for (int64_t rows = 32; rows <= 64; rows *= 2)
+      take(chunks, tiles < E ? tiles - (tiles + 1) / (rows + 1) : (tiles - E + 1) * rows - 1 > E ? (tiles - E + 1) * rows - 1 : E);
+  }
+  return most;
 }
 // of the plan alone; 0: sizes that no call takes
 int64_t plan_workspace(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
@@ -1009,13 +1021,13 @@ int64_t plan_workspace(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K
 using namespace tlq;
 
 extern "C" int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
-  const int64_t plan = plan_workspace(M, E, top_k, N, K), chunks = plan ? most_chunks<true>(M * top_k, E, N, K) : 0;
-  return plan + (chunks > 1 ? chunks * M * top_k * 2 * N * 4 : 0);
+  const int64_t plan = plan_workspace(M, E, top_k, N, K);
+  return plan + (plan ? most_rows<true>(M * top_k, E, top_k, N, K) * 2 * N * 4 : 0);
 }
 
 extern "C" int64_t tlq_moe_down_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K) {
   const int64_t plan = plan_workspace(M, E, top_k, N, K);
-  return plan + (plan ? most_chunks<false>(M * top_k, E, N, K) * M * top_k * N * 4 : 0);
+  return plan + (plan ? most_rows<false>(M * top_k, E, top_k, N, K) * N * 4 : 0);
 }
 
 extern "C" int tlq_moe_gate_up_w4a16(const void* X, const void* ids, const void* w_packed, const void* scales, const void* zeros, void* H,
