@@ -144,3 +144,50 @@ def test_calls_of_every_size_in_the_workspace_of_the_largest(E, k, N, K):
                                           _abi.F32, st))
         assert_close64(y[some.cuda()], *ref.moe_down(H[some], ids[some], weights[some], w1, s1, 8, 64), f"down M={M}")
         assert not bool(y[:M].isnan().any()) and bool(y[M:].isnan().all())
+
+
+# ---- more tokens than threads of one launch -----------------------------------------------------------------------------------------
+@gpu
+def test_route_of_more_tokens_than_one_launch_takes():
+    """2^26 tokens are 2^32 threads."""
+    M = (1 << 26) + 5
+    x = torch.rand(M, 2, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").bfloat16()
+    weights, ids = ops.moe_route(2, 1, renormalize=False, in_dtype="bfloat16")(x)
+    assert bool((ids[:, 0] == (x[:, 1] > x[:, 0])).all())  # (ties go to the lower index)
+    for part in (slice(0, 9), slice(M // 2, M // 2 + 9), slice((1 << 26) - 9, M)):
+        want, _ = ref.moe_route(x[part], 1, renormalize=False)
+        assert bool(((weights[part].cpu().double() - want).abs() <= want * (2.0**-24 + 2.0**-40)).all())
+    assert bool((weights >= 0.5).all()) and bool((weights < 1).all())
+    del x, weights, ids
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_down_of_more_rows_than_one_launch_adds():
+    """2^23 tokens of 1040 outputs are 2^32 threads of the kernel that adds a token's rows (36 GB of them)."""
+    E, N, K, M = 2, 1040, 32, (1 << 23) + 3
+    lib, P = _abi.load(), _abi.ptr
+    g = torch.Generator(device="cuda").manual_seed(2)
+    Wp, s, _ = make_experts(E, N, K, 32, torch.float16, 8, 71)
+    H = torch.randn(M, 1, K, generator=g, device="cuda").half()
+    ids = torch.randint(0, E, (M, 1), generator=g, device="cuda", dtype=torch.int32)
+    weights = torch.rand(M, 1, generator=g, device="cuda") + 0.5
+    Y = torch.full((M, N), float("nan"), dtype=torch.float16, device="cuda")
+    ws = torch.empty(lib.tlq_moe_down_workspace_bytes(M, E, 1, N, K), dtype=torch.uint8, device="cuda")
+    w, sc = operands(Wp, s)
+    _abi.check(lib.tlq_moe_down_w4a16(P(H), P(ids), P(weights), P(w), P(sc), None, P(Y), P(ws), ws.numel(), M, E, 1, N, K, 32, 8.0, _abi.F16, _abi.F16,
+                                      torch.cuda.current_stream().cuda_stream))
+    some = torch.cat([torch.arange(0, M, M // 40), torch.arange((1 << 23) - 4, M)])
+    take = some.cuda()
+    want, off = ref.moe_down(H[take], ids[take], weights[take], Wp, s, 8, 32)
+    assert_close64(Y[take], want, off, "down")
+    assert not any(bool(part.isnan().any()) for part in Y.split(1 << 20))
+    del H, Y, ws
+    torch.cuda.empty_cache()
+
+
+def test_gate_up_of_more_work_groups_than_one_launch_takes_is_refused():
+    lib, p = _abi.load(), ctypes.c_void_p(0x1000)
+    M, k, N, K = (1 << 24) - 1, 1, 8192, 32
+    rc = lib.tlq_moe_gate_up_w4a16(p, p, p, p, None, p, p, 1 << 50, M, 8, k, N, K, 32, 0.0, _abi.F16, None)
+    assert rc != 0 and "fewer tokens" in _abi.last_error(), _abi.last_error()

@@ -16,6 +16,7 @@ struct Plan {
   const int32_t* totals;  // [0] small, [1] large
 };
 constexpr int kLargeRows = 256;
+constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;  // work-groups of 256 threads of a launch, which has fewer than 2^32 threads
 
 struct ExpertArgs {
   const void* X;         // activations: [M, K] (gate / up) or [pairs, K] (down)

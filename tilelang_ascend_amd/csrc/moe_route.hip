@@ -237,17 +237,27 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
   }
 }
 
+// (a launch has fewer than 2^32 threads: 2^26 tokens less a work-group's)
+constexpr int64_t kRouteTokens = (((int64_t)1 << 24) - 1) * kRouteWaves;
+
 template <typename T>
-int run_route(const RouteArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)ceil_div(a.M, (int64_t)kRouteWaves));
+int run_route(const RouteArgs& all, hipStream_t st) {
+  for (int64_t m = 0; m < all.M; m += kRouteTokens) {
+    RouteArgs a = all;
+    a.logits = (const T*)all.logits + m * all.E;
+    a.weights += m * all.top_k, a.ids += m * all.top_k;
+    a.M = all.M - m < kRouteTokens ? all.M - m : kRouteTokens;
+    const dim3 grid((unsigned)ceil_div(a.M, (int64_t)kRouteWaves));
 #define TLQ_ROUTE(EPL) moe_route_kernel<T, EPL><<<grid, 64 * kRouteWaves, 0, st>>>(a)
-  if (a.E <= 64) TLQ_ROUTE(1);
-  else if (a.E <= 128) TLQ_ROUTE(2);
-  else if (a.E <= 256) TLQ_ROUTE(4);
-  else if (a.E <= 512) TLQ_ROUTE(8);
-  else TLQ_ROUTE(16);
+    if (a.E <= 64) TLQ_ROUTE(1);
+    else if (a.E <= 128) TLQ_ROUTE(2);
+    else if (a.E <= 256) TLQ_ROUTE(4);
+    else if (a.E <= 512) TLQ_ROUTE(8);
+    else TLQ_ROUTE(16);
 #undef TLQ_ROUTE
-  return check_launch("tlq_moe_route", "moe_route_kernel") ? 0 : 1;
+    if (!check_launch("tlq_moe_route", "moe_route_kernel")) return 1;
+  }
+  return 0;
 }
 
 }  // namespace

@@ -846,7 +846,7 @@ FewPlan few_plan(bool up, int64_t pairs, int64_t E, int64_t top_k, int64_t N, in
   p.lds = few_lds(up, zeros, p.waves, p.splits, (int)wg_tiles, p.row_cap, (int)pitch, p.pieces).list + ceil_div(pairs, (int64_t)8) * 16;
   p.units = (p.by_pair ? pairs : E + (up ? 1 : 0)) * p.n_groups;
   p.grid = p.chunks == 1 ? p.units : ceil_div(p.units, (int64_t)8) * 8 * p.chunks;
-  p.ok = p.lds <= 160 * 1024 && p.grid < ((int64_t)1 << 31);
+  p.ok = p.lds <= 160 * 1024 && p.grid <= kMostGroups;
   return p;
 }
 
@@ -915,7 +915,7 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
   *chunks = ceil_div(steps, chunk_steps);
   float* const parts = UP && *chunks > 1 ? (float*)((uint8_t*)ws + plan_bytes(x.E, pairs)) : nullptr;
   const int64_t grid = z.small * n_groups * *chunks;
-  TLQ_REQUIRE(grid < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
+  TLQ_REQUIRE(grid <= kMostGroups, "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
 #define TLQ_PLAN(COMPACT, THREADS)                                                                                                          \
   moe_plan_kernel<COMPACT, THREADS><<<x.E + 1, THREADS, 0, st>>>((const int32_t*)ids, p.totals, p.order, p.small, p.large, (int)pairs, x.E, rows, \
                                                                  large ? (int)moe_panel_groups(x.N, UP) : 0)
@@ -1067,10 +1067,15 @@ extern "C" int tlq_moe_down_w4a16(const void* H, const void* ids, const void* we
   int64_t chunks = 1;
   if (run_experts<false>(what, a, ids, pairs, in_dtype, workspace, &chunks, st)) return 1;
   const int64_t n_groups = ceil_div(N, (int64_t)1024);
-  TLQ_REQUIRE(M * n_groups < ((int64_t)1 << 31), "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)(M * n_groups));
-  moe_combine_kernel<<<(unsigned)(M * n_groups), 256, 0, st>>>(rows, (const int32_t*)ids, Y, (int)N, (int)n_groups, (int)top_k, (int)E, out_dtype,
-                                                                 (int)chunks, pairs * N);
-  return check_launch(what, "moe_combine_kernel") ? 0 : 1;
+  const int64_t most = kMostGroups / n_groups;  // tokens of a launch
+  for (int64_t t = 0; t < M; t += most) {
+    const int64_t tokens = M - t < most ? M - t : most;
+    moe_combine_kernel<<<(unsigned)(tokens * n_groups), 256, 0, st>>>(rows + t * top_k * N, (const int32_t*)ids + t * top_k,
+                                                                      (uint8_t*)Y + t * N * (out_dtype == TLQ_F32 ? 4 : 2), (int)N, (int)n_groups, (int)top_k,
+                                                                      (int)E, out_dtype, (int)chunks, pairs * N);
+    if (!check_launch(what, "moe_combine_kernel")) return 1;
+  }
+  return 0;
 }
 
 extern "C" int tlq_debug_moe_choice(int up, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, int zeros, void* plan_out) {
