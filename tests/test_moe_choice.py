@@ -191,3 +191,51 @@ def test_gate_up_of_more_work_groups_than_one_launch_takes_is_refused():
     M, k, N, K = (1 << 24) - 1, 1, 8192, 32
     rc = lib.tlq_moe_gate_up_w4a16(p, p, p, p, None, p, p, 1 << 50, M, 8, k, N, K, 32, 0.0, _abi.F16, None)
     assert rc != 0 and "fewer tokens" in _abi.last_error(), _abi.last_error()
+
+
+# ---- gates far from 0 --------------------------------------------------------------------------------------------------------------
+# M, E, N, K: every kernel that applies silu (few pairs; tiles of 32; of 64; of 256; the sums of parts of K)
+GATES = [(64, 64, 16, 128, FEW), (40, 2, 48, 64, TILES32), (200, 2, 16, 64, TILES64), (4096, 1, 3104, 128, TILES256), (40, 2, 16, 4096, TILES32)]
+
+
+@pytest.mark.parametrize("M,E,N,K,kernel", GATES)
+def test_gates_far_from_zero_reach_every_kernel(M, E, N, K, kernel):
+    assert choice(True, M, E, 1, N, K, K, None)[0] == kernel
+
+
+@gpu
+@pytest.mark.parametrize("M,E,N,K,kernel", GATES)
+def test_gates_far_from_zero(M, E, N, K, kernel):
+    """silu(g) * u of exact sums g and u, for g from -94 to 100 and u = 300: bfloat16 holds all of them as normal numbers, also where exp(-g) is more than
+    fp32 holds or silu(g) less.  (|g| + 4) 2^-22 of the value as in the oracle, and the rounding."""
+    Wp = torch.zeros(E, 2 * N, K // 2, dtype=torch.uint8)
+    Wp[:, :N, 0], Wp[:, N:, 0] = 0x01, 0x10  # gate = x[0], up = x[1]
+    s = torch.ones(E, 2 * N, 1, dtype=torch.bfloat16)
+    X = torch.zeros(M, K, dtype=torch.bfloat16)
+    X[:, 0] = torch.linspace(-94, 100, M).bfloat16()
+    X[:, 1] = 300
+    ids = (torch.arange(M) % E).int()[:, None]
+    got = ops.moe_gate_up_w4a16(E, 1, N, K, K, "bfloat16")(*operands(X, ids, Wp, s))[:, 0].cpu()
+    g = X[:, :1].double()
+    want = (g / (1 + torch.exp(-g)) * 300).expand(M, N)
+    assert float(want.abs().min()) > 2.0**-126
+    assert_close64(got, want, (g.abs() + 4) * 2.0**-22 * want.abs(), "far gates")
+
+
+@gpu
+def test_a_far_gate_beside_one_that_is_no_number():
+    """Outputs are independent of each other: a NaN beside a gate of -90 leaves its product as it is."""
+    N, K = 16, 64
+    Wp = torch.zeros(1, 2 * N, K // 2, dtype=torch.uint8)
+    Wp[:, :N, 0], Wp[:, N:, 0] = 0x01, 0x10
+    X = torch.zeros(1, K, dtype=torch.bfloat16)
+    X[0, 0], X[0, 1] = -90, 300
+    ids = torch.zeros(1, 1, dtype=torch.int32)
+    for at in range(4):
+        s = torch.ones(1, 2 * N, 1, dtype=torch.bfloat16)
+        s[0, at] = float("nan")
+        got = ops.moe_gate_up_w4a16(1, 1, N, K, K, "bfloat16")(*operands(X, ids, Wp, s))[0, 0].cpu()
+        assert bool(got[at].isnan())
+        rest = torch.arange(N) != at
+        want = torch.full((N - 1,), -90 / (1 + torch.exp(torch.tensor(90.0, dtype=torch.float64))).item() * 300, dtype=torch.float64)
+        assert_close64(got[rest], want, 94 * 2.0**-22 * want.abs(), f"beside {at}")

@@ -784,8 +784,9 @@ __global__ __launch_bounds__(256) void moe_gate_kernel(const float* __restrict__
     const float* const mine = parts + pair * 2 * N + n;
     float4_t g = *(const float4_t*)mine, u = *(const float4_t*)(mine + N);
     for (int c = 1; c < chunks; ++c) g += *(const float4_t*)(mine + c * chunk_stride), u += *(const float4_t*)(mine + c * chunk_stride + N);
+    const float4_t y = silu_times(g, u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = from_float<T>(silu(g[i]) * u[i]);
+    for (int i = 0; i < 4; ++i) o[i] = from_float<T>(y[i]);
   } else {  // (no row was written)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = from_float<T>(0.0f);

@@ -79,9 +79,10 @@ __global__ __launch_bounds__(256, 1) void moe_panel_kernel(const PanelArgs a) {
         float4_t g = acc[t][tm], u = acc[t + 2][tm];
         asm volatile("" : "+v"(g), "+v"(u));  // (moved out of the accumulation registers here, not all of them ahead)
         const int n = n_of(t) + q * 4;
+        const float4_t y = silu_times(g, u);
         T o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = from_float<T>(silu(g[i]) * u[i]);
+        for (int i = 0; i < 4; ++i) o[i] = from_float<T>(y[i]);
         if (live_row && n < a.N) *(uint2_t*)(h + n) = bitcast<uint2_t>(o);
       }
     } else {
