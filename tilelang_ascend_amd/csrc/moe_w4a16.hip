@@ -235,8 +235,8 @@ struct TileArgs {
   const uint8_t* Wp;
   const void* scales;
   const void* zeros;
-  float* weights;  // down: of the pairs; gate / up in parts of K: the sums to write, [part][pair][2 N], otherwise null
-  void* out;
+  const float* weights;  // down: of the pairs
+  void* out;             // gate / up: h [pairs, N], or with K in parts fp32 sums [part][pair][2 N]; down: weighted fp32 rows [part][pair][N]
   const PlanTile* tiles;
   const int32_t* order;  // (how many tiles there are: at order[-64])
   int pairs, E, top_k, N, K, groups;
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
   const int n_tiles = a.N / OUTS, tile0 = group_no * Cfg::TILES;
   if (e == a.E) {  // pairs without an expert
     if constexpr (UP) {
-      if (a.weights) return;  // (moe_gate_kernel writes their zeros)
+      if (chunks > 1) return;  // (moe_gate_kernel writes their zeros)
       T* const h = (T*)a.out;
       constexpr int width = Cfg::TILES * OUTS;
       for (int i = tid; i < rows * width; i += 256) {
@@ -459,9 +459,9 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
       const int n = (tile0 + wave * NT + t) * OUTS + q * 4;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        if (UP && a.weights) {  // this lane's four gates (q = 0, 1) or ups
+        if (UP && chunks > 1) {  // this lane's four gates (q = 0, 1) or ups
           if (m * 16 + r16 < rows && tile0 + wave * NT + t < n_tiles)
-            *(float4_t*)(a.weights + ((int64_t)chunk * a.pairs + pair[m]) * (2 * (int64_t)a.N) + (q >= 2 ? a.N - 8 : 0) + n) = acc[t][m];
+            *(float4_t*)((float*)a.out + ((int64_t)chunk * a.pairs + pair[m]) * (2 * (int64_t)a.N) + (q >= 2 ? a.N - 8 : 0) + n) = acc[t][m];
           continue;
         }
         moe_store<T, UP>(a, acc[t][m], m * 16 + r16 < rows && tile0 + wave * NT + t < n_tiles, pair[m], weight[m], n, q, chunk);
@@ -931,7 +931,7 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
   }
   const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
   const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
-  const TileArgs a{x.X, x.Wp, x.scales, x.zeros, UP ? parts : const_cast<float*>(x.weights), x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
+  const TileArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, parts ? (void*)parts : x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
                    make_group_of(units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};
 #define TLQ_TILES(T) (x.zeros || !whole ? launch_tiles<T, UP, true, MAXMT, NT, KSB>(what, a, grid, st) : launch_tiles<T, UP, false, MAXMT, NT, KSB>(what, a, grid, st))
   if (dtype == TLQ_F16 ? TLQ_TILES(half_t) : TLQ_TILES(bf16_t)) return 1;
