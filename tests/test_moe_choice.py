@@ -239,3 +239,35 @@ def test_a_far_gate_beside_one_that_is_no_number():
         rest = torch.arange(N) != at
         want = torch.full((N - 1,), -90 / (1 + torch.exp(torch.tensor(90.0, dtype=torch.float64))).item() * 300, dtype=torch.float64)
         assert_close64(got[rest], want, 94 * 2.0**-22 * want.abs(), f"beside {at}")
+
+
+# ---- tiles of 256 pairs --------------------------------------------------------------------------------------------------------------
+# the pairs of each expert, and those of none: whole tiles, one more and one fewer, what is left at every candidate for a last tile of 256
+COUNTS = [([256, 200], 0), ([512, 256, 768], 0), ([255, 257, 513], 7), ([256, 64, 65, 320, 321], 0), ([128, 129, 192, 193, 448, 449], 3), ([1, 0, 1024, 0, 2], 500),
+          ([256] * 16, 0), ([40] * 40 + [2496], 0)]
+
+
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("counts,none", COUNTS)
+def test_tiles_of_256_pairs_by_count(counts, none, up):
+    E, K = len(counts), 128
+    M = sum(counts) + none
+    N = (-(-192 // (M // 256)) - 1) * (128 if up else 256) + 16  # the fewest work-groups that the rule wants, the last of them with 16 outputs
+    assert choice(up, M, E, 1, N, K, 128, None)[0] == TILES256
+    ids = torch.cat([torch.full((n,), e) for e, n in enumerate(counts)] + [torch.full((none,), -1)]).int()
+    ids = ids[torch.randperm(len(ids), generator=gen(81))][:, None]
+    Wp, s, _ = make_experts(E, 2 * N if up else N, K, 128, torch.bfloat16, 8, 82)
+    some = torch.tensor(sorted({int((ids[:, 0] == e).nonzero()[i, 0]) for e in range(E) for i in {0, counts[e] // 2, counts[e] - 1} if counts[e]}))[:24]
+    if up:
+        X = torch.randn(M, K, generator=gen(83)).bfloat16()
+        got = ops.moe_gate_up_w4a16(E, 1, N, K, 128, "bfloat16", zeros=8)(*operands(X, ids, Wp, s))
+        want, off = ref.moe_gate_up(X[some], ids[some], Wp, s, 8, 128)
+    else:
+        H, w = torch.randn(M, 1, K, generator=gen(83)).bfloat16(), torch.ones(M, 1)
+        got = ops.moe_down_w4a16(E, 1, N, K, 128, "bfloat16", "bfloat16", zeros=8)(*operands(H, ids, w, Wp, s))
+        want, off = ref.moe_down(H[some], ids[some], w[some], Wp, s, 8, 128)
+    assert_close64(got[some.cuda()], want, off, f"{counts} {up}")
+    got = got.view(M, N)
+    live = (ids[:, 0] >= 0).cuda()
+    assert bool(torch.isfinite(got).all()) and bool((got[~live] == 0).all()) and bool((got[live].abs().amax(1) > 0).all())

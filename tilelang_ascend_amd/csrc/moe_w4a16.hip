@@ -58,10 +58,10 @@ inline int64_t plan_bytes(int64_t E, int64_t pairs) {  // of these pairs and of 
   return most > fewer ? most : fewer;
 }
 
-// Candidates for `from`: 65, 129, 193, 257 (whole tiles only), and more pairs than there are (none).  A round of large tiles is 256 work-groups,
+// Candidates for `from`: 65, 129, 193, 256 (whole tiles only), and more pairs than there are (none).  A round of large tiles is 256 work-groups,
 // one a CU; of tiles of 64 pairs as wide as those 512 go at once and take 5 / 8 of its time (gate / up, 16 experts of 2048 x 4096: 98 and 61 us).
 constexpr int kFromChoices = 5;
-__device__ __forceinline__ int from_choice(int i) { return i < 4 ? 64 * i + 65 : 1 << 24; }
+__device__ __forceinline__ int from_choice(int i) { return i < 3 ? 64 * i + 65 : i == 3 ? kLargeRows : 1 << 24; }
 __device__ __forceinline__ int rounds_of(int large, int small, int groups) { return 8 * ((large * groups + 255) / 256) + 5 * ((small * groups + 511) / 512); }
 
 // One work-group per expert, and one more for the pairs without one: each looks at all pairs and writes down its own.  A wavefront takes
