@@ -830,8 +830,8 @@ FewPlan few_plan(bool up, int64_t pairs, int64_t E, int64_t top_k, int64_t N, in
   p.splits = 1;
   while (p.splits < 4 && p.splits * 4 <= blocks && experts * n_tiles * p.chunks * p.splits < 2048) p.splits *= 2;
   p.per_wave = 1;
-  // tiles of a wavefront: as many as leave every CU several work-groups
-  if (p.splits == 1)
+  // tiles of a wavefront: as many as leave every CU several work-groups (gate / up is on tiles of pairs where there are that many, few_pairs)
+  if (!up && p.splits == 1)
     while (p.per_wave < 8 && experts * ceil_div(n_tiles, (int64_t)p.waves * p.per_wave * 2) * p.chunks >= 1536) p.per_wave *= 2;
   p.by_pair = pairs <= E;
   // the scales of a part of K: its groups, the first of them anywhere in its piece; parts need not begin with a group
