@@ -7,7 +7,7 @@ import ctypes
 import pytest
 import torch
 
-from helpers import DT, gen
+from helpers import DT, assert_bit_equal, gen
 from oracle import ref
 from tilelang_ascend_amd import _abi, ops
 from test_moe import assert_close64, kernel_zeros, make_experts, make_ids, operands
@@ -24,21 +24,23 @@ def choice(up, M, E, k, N, K, group, zeros):
     return kernel, dict(zip(names, plan)) if kernel == FEW else None
 
 
-def run_both(up, M, E, k, N, K, group, dtype, zeros, kind, out="float32", seed=20):
-    """One product against the oracle; returns the output on the CPU."""
+def run_both(up, M, E, k, N, K, group, dtype, zeros, kind, out="float32", seed=20, some=None):
+    """One product against the oracle (in the rows `some`, or all); returns the output on the CPU."""
     T = DT[dtype]
     ids = make_ids(M, E, k, kind, seed)
     Wp, s, z = make_experts(E, 2 * N if up else N, K, group, T, zeros, seed + 1)
+    at = torch.arange(M) if some is None else torch.tensor(some)
     if up:
         X = torch.randn(M, K, generator=gen(seed + 2)).to(T)
         got = ops.moe_gate_up_w4a16(E, k, N, K, group, dtype, zeros=kernel_zeros(z))(*operands(X, ids, Wp, s, z))
-        want, off = ref.moe_gate_up(X, ids, Wp, s, z, group)
+        want, off = ref.moe_gate_up(X[at], ids[at], Wp, s, z, group)
     else:
         H = torch.randn(M, k, K, generator=gen(seed + 2)).to(T)
         weights = torch.softmax(torch.randn(M, k, generator=gen(seed + 3)), 1)
         got = ops.moe_down_w4a16(E, k, N, K, group, dtype, out, zeros=kernel_zeros(z))(*operands(H, ids, weights, Wp, s, z))
-        want, off = ref.moe_down(H, ids, weights, Wp, s, z, group)
-    assert_close64(got, want, off, f"{'gate_up' if up else 'down'} {M, E, k, N, K, group, dtype, zeros, kind}")
+        want, off = ref.moe_down(H[at], ids[at], weights[at], Wp, s, z, group)
+    assert_close64(got.cpu()[at], want, off, f"{'gate_up' if up else 'down'} {M, E, k, N, K, group, dtype, zeros, kind}")
+    assert bool(torch.isfinite(got).all())
     return got.cpu()
 
 
@@ -271,3 +273,182 @@ def test_tiles_of_256_pairs_by_count(counts, none, up):
     got = got.view(M, N)
     live = (ids[:, 0] >= 0).cuda()
     assert bool(torch.isfinite(got).all()) and bool((got[~live] == 0).all()) and bool((got[live].abs().amax(1) > 0).all())
+
+
+# ---- few pairs: several passes over an expert's rows, several tiles of a wavefront ---------------------------------------------------
+# up, M, E, top_k, N, K, group, type, zeros, what the plan has to be; all pairs on one expert ("one"): more of them than rows of a pass, the last pass not full
+PASSES = [
+    (True, 35, 64, 1, 48, 256, 64, "float16", "int", dict(rows=16, splits=1)),
+    (False, 35, 64, 1, 48, 256, 64, "bfloat16", "frac", dict(rows=16, splits=1)),
+    (True, 35, 64, 1, 48, 1024, 64, "bfloat16", "frac", dict(rows=16, splits=4)),
+    (False, 35, 64, 1, 48, 1024, 64, "float16", "int", dict(rows=16, splits=4)),
+    (True, 7, 64, 3, 48, 4128, 32, "float16", "frac", dict(rows=4, splits=4)),
+    (True, 5, 8, 3, 48, 4128, 96, "bfloat16", 8, dict(rows=4, splits=4)),
+    (False, 7, 8, 2, 48, 6016, 32, "bfloat16", "int", dict(rows=4, splits=4, parts=2)),
+    (False, 5, 64, 3, 80, 4128, 32, "float16", 7.5, dict(rows=8, splits=4, parts=2)),
+    (False, 7, 16, 3, 32, 8224, 32, "float16", "frac", dict(rows=4, splits=4, parts=3)),
+    (False, 8, 64, 8, 1808, 4256, 32, "float16", "int", dict(rows=8, splits=1, tiles=2, parts=2)),
+    (False, 8, 64, 8, 1808, 14336, 128, "bfloat16", "frac", dict(rows=4, splits=1, tiles=4, parts=4)),
+]
+
+
+@pytest.mark.parametrize("up,M,E,k,N,K,group,dtype,zeros,plan", PASSES)
+def test_plans_of_several_passes(up, M, E, k, N, K, group, dtype, zeros, plan):
+    kernel, got = choice(up, M, E, k, N, K, group, zeros if isinstance(zeros, str) else None)
+    assert kernel == FEW and {key: got[key] for key in plan} == plan, got
+    assert M * k > got["rows"] and M * k % got["rows"] or got["tiles"] > 1
+
+
+@gpu
+@pytest.mark.parametrize("up,M,E,k,N,K,group,dtype,zeros,plan", PASSES)
+def test_few_pairs_in_several_passes(up, M, E, k, N, K, group, dtype, zeros, plan):
+    run_both(up, M, E, k, N, K, group, dtype, zeros, "one")
+    run_both(up, M, E, k, N, K, group, dtype, zeros, "spread", some=[0, M - 1])
+
+
+# ---- which kernel -------------------------------------------------------------------------------------------------------------------
+# tiles of 256 pairs with few outputs: wavefronts and 16-row tiles behind the last output
+FEW_OUTPUTS = [(True, 16384, 8, 8, 16, 1536), (True, 16390, 4, 8, 144, 1536), (True, 16384, 3, 8, 48, 1664), (False, 16384, 8, 8, 16, 2048), (False, 8200, 4, 16, 272, 2048)]
+
+
+@pytest.mark.parametrize("up,M,E,k,N,K", FEW_OUTPUTS)
+def test_few_outputs_are_on_tiles_of_256_pairs(up, M, E, k, N, K):
+    assert choice(up, M, E, k, N, K, 128, "tensor")[0] == TILES256
+
+
+def big_call(up, M, E, k, N, K, group, T, ids, Wp, s, z, seed):
+    """A product of tensors made on the GPU -> (output, what the oracle takes for the tokens `some`, with their experts alone)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    name = {v: n for n, v in DT.items()}[T]
+    extra = [z] if isinstance(z, torch.Tensor) else []
+    if up:
+        x = torch.randn(M, K, generator=g, device="cuda").to(T)
+        got = ops.moe_gate_up_w4a16(E, k, N, K, group, name, zeros=kernel_zeros(z))(x, ids, Wp, s, *extra)
+    else:
+        x = torch.randn(M, k, K, generator=g, device="cuda").to(T)
+        weights = torch.rand(M, k, generator=g, device="cuda") + 0.25
+        got = ops.moe_down_w4a16(E, k, N, K, group, name, "float32", zeros=kernel_zeros(z))(x, ids, weights, Wp, s, *extra)
+
+    def check(some):
+        at = torch.tensor(some, device="cuda")
+        mine = ids[at]
+        used = torch.unique(mine[(mine >= 0) & (mine < E)]).long()
+        to = torch.full((E,), -1, dtype=torch.int32, device="cuda")
+        to[used] = torch.arange(len(used), dtype=torch.int32, device="cuda")
+        local = torch.where((mine >= 0) & (mine < E), to[mine.clamp(0, E - 1).long()], -1).cpu()
+        part = (Wp[used].cpu(), s[used].cpu(), z[used].cpu() if isinstance(z, torch.Tensor) else z, group)
+        if up:
+            want, off = ref.moe_gate_up(x[at].cpu(), local, *part)
+        else:
+            want, off = ref.moe_down(x[at].cpu(), local, weights[at].cpu(), *part)
+        assert_close64(got[at], want, off, f"{up, M, E, k, N, K}")
+
+    return got, check
+
+
+def gpu_experts(E, rows, K, group, T, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    words = torch.randint(-(2**63), 2**63 - 1, (E, rows, K // 16), generator=g, device="cuda", dtype=torch.int64)
+    s = (torch.rand(E, rows, K // group, generator=g, device="cuda") * 0.015 + 0.005).to(T)
+    return words.view(torch.uint8), s, torch.randint(6, 10, s.shape, generator=g, device="cuda").to(T)
+
+
+@gpu
+@pytest.mark.parametrize("up,M,E,k,N,K", FEW_OUTPUTS)
+def test_few_outputs_on_tiles_of_256_pairs(up, M, E, k, N, K):
+    T = torch.bfloat16 if up else torch.float16
+    g = torch.Generator(device="cuda").manual_seed(91)
+    ids = torch.randint(-1, E, (M, k), generator=g, device="cuda", dtype=torch.int32)
+    Wp, s, z = gpu_experts(E, 2 * N if up else N, K, 128, T, 92)
+    got, check = big_call(up, M, E, k, N, K, 128, T, ids, Wp, s, z, 93)
+    check([0, 1, M // 2, M - 2, M - 1])
+    assert bool(torch.isfinite(got).all())
+    if up:
+        assert bool((got[ids < 0] == 0).all()) and bool((got[ids >= 0].abs().amax(1) > 0).all())
+    else:
+        assert bool((got[(ids >= 0).any(1)].abs().amax(1) > 0).all())
+
+
+# ---- weights of more than 4 GiB, a thousand experts, sixty-four of them a token -------------------------------------------------------
+# M and top_k: few pairs, tiles of 32, of 64, of 256
+THOUSAND = [(4, 2, FEW), (200, 8, TILES32), (4096, 8, TILES64), (32768, 8, TILES256)]
+
+
+@pytest.mark.parametrize("M,k,kernel", THOUSAND)
+@pytest.mark.parametrize("up", [True, False])
+def test_a_thousand_experts_reach_every_kernel(M, k, kernel, up):
+    assert choice(up, M, 1024, k, 1024 if up else 2048, 4224, 128, "tensor")[0] == kernel
+
+
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+def test_weights_of_more_than_4_gib(up):
+    """1024 experts of 2048 rows of 4224 values, 4.4e9 bytes: the first, the last and those behind 2^31 and 2^32 bytes."""
+    E, rows, K, T = 1024, 2048, 4224, torch.bfloat16
+    Wp, s, z = gpu_experts(E, rows, K, 128, T, 95)
+    assert Wp.numel() > 2**32
+    N = rows // 2 if up else rows
+    for M, k, _ in THOUSAND:
+        g = torch.Generator(device="cuda").manual_seed(96)
+        ids = torch.randint(0, E, (M, k), generator=g, device="cuda", dtype=torch.int32)
+        ids[0, 0], ids[0, 1], ids[1, 0], ids[1, 1], ids[M - 1, 0], ids[M - 1, 1] = 0, E - 1, 496, 497, 993, 994
+        got, check = big_call(up, M, E, k, N, K, 128, T, ids, Wp, s, z, 97)
+        check([0, 1, M - 1])
+        assert bool(torch.isfinite(got).all())
+        del got, check
+    del Wp, s, z
+    torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("M,E,k", [(1, 100, 64), (5, 64, 64), (70, 1024, 64)])
+def test_sixty_four_experts_a_token(M, E, k, up):
+    run_both(up, M, E, k, 32, 160, 32, "bfloat16", "int", "spread", some=[0, M - 1])
+
+
+# ---- slots that are mostly empty -----------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("M,E,k,N,K,kernel", [(16384, 8, 8, 272, 2048, TILES256), (512, 8, 8, 3088, 128, TILES256), (300, 8, 8, 80, 256, TILES64), (20, 16, 8, 80, 256, TILES32)])
+def test_slots_that_are_mostly_empty(M, E, k, N, K, kernel, up):
+    """One slot in eight has an expert here, and then with none at all."""
+    assert choice(up, M, E, k, N, K, 128, "tensor")[0] == kernel
+    T = torch.float16
+    Wp, s, z = gpu_experts(E, 2 * N if up else N, K, 128, T, 101)
+    g = torch.Generator(device="cuda").manual_seed(102)
+    ids = torch.randint(0, 8 * E, (M, k), generator=g, device="cuda", dtype=torch.int32)
+    ids[M - 1, k - 1] = E - 1
+    for round_ids in (ids, torch.full_like(ids, -1)):
+        got, check = big_call(up, M, E, k, N, K, 128, T, round_ids, Wp, s, z, 103)
+        check([0, 1, 2, M // 2, M - 1])
+        here = (round_ids >= 0) & (round_ids < E)
+        assert bool(torch.isfinite(got).all())
+        if up:
+            assert bool((got[~here] == 0).all()) and bool((got[here].abs().amax(1) > 0).all() if bool(here.any()) else True)
+        else:
+            assert bool((got[~here.any(1)] == 0).all())
+
+
+# ---- a token beside others -----------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("M", [1, 4, 12, 70, 200])
+def test_a_token_gets_the_same_bits_beside_other_tokens(M):  # (few pairs, tiles of 32, of 64)
+    """As many tokens, the others' inputs and experts changed: the first and the last keep their bits (below the sizes of tiles of 256 pairs, where
+    the counts of all experts decide which of two kernels a pair is on)."""
+    E, k, N, K = 8, 2, 96, 256
+    w1, s1, z1 = operands(*make_experts(E, 2 * N, K, 64, torch.bfloat16, "int", 111))
+    w2, s2, z2 = operands(*make_experts(E, K, N, 96, torch.bfloat16, "frac", 112))
+    up, down = ops.moe_gate_up_w4a16(E, k, N, K, 64, "bfloat16", zeros="tensor"), ops.moe_down_w4a16(E, k, K, N, 96, "bfloat16", "float32", zeros="tensor")
+    kept = sorted({0, M - 1})
+    x0, ids0, weights = torch.randn(M, K, generator=gen(1)).bfloat16(), make_ids(M, E, k, "spread", 2), torch.softmax(torch.randn(M, k, generator=gen(3)), 1).cuda()
+    first = None
+    for other in range(4):
+        x, ids = torch.randn(M, K, generator=gen(10 + other)).bfloat16(), make_ids(M, E, k, ["spread", "one", "holes", "twice"][other], 20 + other)
+        x[kept], ids[kept] = x0[kept], ids0[kept]
+        h = up(x.cuda(), ids.cuda(), w1, s1, z1)
+        y = down(h, ids.cuda(), weights, w2, s2, z2)
+        mine = h[kept].cpu(), y[kept].cpu()
+        first = first or mine
+        assert_bit_equal(mine[0], first[0], "hidden")
+        assert_bit_equal(mine[1], first[1], "y")
