@@ -416,8 +416,7 @@ static int dispatch_skinny(const W4Args& a) {
 
 int gemm_w4a16_skinny(const void* A, const void* Wp, const void* scales, const void* zeros, void* C, int64_t M, int64_t N,
                       int64_t K, int64_t group, float zero_scalar, int in_dtype, int out_dtype, hipStream_t st) {
-  const bool fold = zeros == nullptr && zero_scalar == (float)(int)zero_scalar && zero_scalar >= -256.0f &&
-                    zero_scalar <= 256.0f;
+  const bool fold = zeros == nullptr && zero_folds(zero_scalar);
   const W4Args a{A, Wp, scales, zeros, C, M, N, K, group, zero_scalar, out_dtype, st};
   if (in_dtype == TLQ_F16) return fold ? dispatch_skinny<half_t, true>(a) : dispatch_skinny<half_t, false>(a);
   return fold ? dispatch_skinny<bf16_t, true>(a) : dispatch_skinny<bf16_t, false>(a);
@@ -490,8 +489,7 @@ void launch_splitk_reduce(const float* partial, void* C, int64_t M, int64_t N, i
 int gemm_w4a16_mfma_splitk(const void* A, const void* Wp, const void* scales, const void* zeros, void* C, int64_t M,
                            int64_t N, int64_t K, int64_t group, float zero_scalar, int in_dtype, int out_dtype,
                            int64_t split, float* partial, hipStream_t st) {
-  const bool fold = zeros == nullptr && zero_scalar == (float)(int)zero_scalar && zero_scalar >= -256.0f &&
-                    zero_scalar <= 256.0f;
+  const bool fold = zeros == nullptr && zero_folds(zero_scalar);
   W4Args a{A, Wp, scales, zeros, C, M, N, K, group, zero_scalar, out_dtype, st};
   a.split = split;
   a.partial = partial;
@@ -512,8 +510,7 @@ int gemm_w4a16_mfma(const void* A, const void* Wp, const void* scales, const voi
     return 1;
   }
   // An integer zero point shared by the whole matrix folds exactly into the unpack bias.
-  const bool fold = zeros == nullptr && zero_scalar == (float)(int)zero_scalar && zero_scalar >= -256.0f &&
-                    zero_scalar <= 256.0f;
+  const bool fold = zeros == nullptr && zero_folds(zero_scalar);
   const W4Args a{A, Wp, scales, zeros, C, M, N, K, group, zero_scalar, out_dtype, st};
   if (in_dtype == TLQ_F16) return fold ? dispatch_w4a16<half_t, true>(a) : dispatch_w4a16<half_t, false>(a);
   return fold ? dispatch_w4a16<bf16_t, true>(a) : dispatch_w4a16<bf16_t, false>(a);

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(1024) void w4a16_decode_kernel(const T* __restrict_
           sv[kb] = has_s ? bitcast<T>((uint16_t)(sdw[kb] >> rd_half[kb])) : one;
           zv[kb] = has_z ? bitcast<T>((uint16_t)(zdw[kb] >> rd_half[kb])) : zs;
           const float zf = to_float(zv[kb]);
-          ok = ok && zf == __builtin_rintf(zf) && zf >= -256.0f && zf <= 256.0f;
+          ok = ok && zero_folds(zf);
         }
         typename Mma::acc_t acc2[2] = {typename Mma::acc_t{0, 0, 0, 0}, typename Mma::acc_t{0, 0, 0, 0}};
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(ok) == ~0ull, 1)) {  // integer zero points fold into the unpack bias (exact)
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(1024) void w4a16_decode_kernel(const T* __restrict_
           const T sv = has_s ? bitcast<T>((uint16_t)(sdw >> rd_half[kb])) : one;
           const T zv = has_z ? bitcast<T>((uint16_t)(zdw >> rd_half[kb])) : zs;
           const float zf = to_float(zv);
-          const bool ok = zf == __builtin_rintf(zf) && zf >= -256.0f && zf <= 256.0f;
+          const bool ok = zero_folds(zf);
           const uint32_t w[4] = {wf.x, wf.y, wf.z, wf.w};
           if (__builtin_expect(__builtin_amdgcn_ballot_w64(ok) == ~0ull, 1)) {
             const Expand8<T, true, 1> ex(sv, zv, mg);

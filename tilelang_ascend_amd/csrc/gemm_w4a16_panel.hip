@@ -246,7 +246,7 @@ __global__ __launch_bounds__(512, 1) void w4a16_panel_kernel(const T* __restrict
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float zf = to_float(bitcast<T>((uint16_t)(x[i] >> (16 * e))));
-        integral = integral && zf == __builtin_rintf(zf) && zf >= -256.0f && zf <= 256.0f;
+        integral = integral && zf == __builtin_rintf(zf) && zf >= -kFoldsWithin && zf <= kFoldsWithin;
       }
     return __builtin_amdgcn_ballot_w64(integral) == ~0ull;
   };
@@ -411,7 +411,7 @@ int gemm_w4a16_panel(const void* A, const void* Wp, const void* scales, const vo
   int gshift = 0;
   while (((int64_t)1 << gshift) < group) ++gshift;
   const int band = g_gemm_band_rows > 0 ? g_gemm_band_rows : 4;
-  const bool fold_scalar = zero_scalar == (float)(int)zero_scalar && zero_scalar >= -256.0f && zero_scalar <= 256.0f;
+  const bool fold_scalar = zero_folds(zero_scalar);
   static std::atomic<uint32_t> epochs{0x5eed0001u};
   const uint32_t epoch = zeros != nullptr ? epochs.fetch_add(1, std::memory_order_relaxed) : 0u;
   int rc;

@@ -154,7 +154,7 @@ int gemm_w4a16_panel256(const void* A, const void* Wp, const void* scales, const
   int gshift = 0;
   while (((int64_t)1 << gshift) < group) ++gshift;
   const int band = g_gemm_band_rows > 0 ? g_gemm_band_rows : 4;
-  const bool fold_scalar = zero_scalar == (float)(int)zero_scalar && zero_scalar >= -256.0f && zero_scalar <= 256.0f;
+  const bool fold_scalar = zero_folds(zero_scalar);
   int rc;
 #define TLQ_PANEL3(T, LAY, ZM) launch_panel256<T, LAY, ZM>(A, Wp, scales, zeros, C, partial, M, N, K, gshift, zero_scalar, out_dtype, p, band, st)
 #define TLQ_PANEL2(T, ZM) (w_layout == TLQ_W_INTERLEAVED_F16 ? TLQ_PANEL3(T, 1, ZM) : TLQ_PANEL3(T, 0, ZM))

@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256, 1) void w4a16_panelm_kernel(const T* __restric
         fract_bits |= bitcast<uint32_t>(__builtin_amdgcn_fractf(zf));
         max_abs = __builtin_fmaxf(max_abs, __builtin_fabsf(zf));
       }
-    return __builtin_amdgcn_ballot_w64(fract_bits == 0 && max_abs <= 256.0f) == ~0ull;
+    return __builtin_amdgcn_ballot_w64(fract_bits == 0 && max_abs <= kFoldsWithin) == ~0ull;
   };
 
   // ---- state of the pipeline that runs across steps
@@ -466,7 +466,7 @@ int gemm_w4a16_panelm(const void* A, const void* Wp, const void* scales, const v
   int gshift = 0;
   while (((int64_t)1 << gshift) < group) ++gshift;
   const int band = g_gemm_band_rows > 0 ? g_gemm_band_rows : 4;
-  const bool fold_scalar = zero_scalar == (float)(int)zero_scalar && zero_scalar >= -256.0f && zero_scalar <= 256.0f;
+  const bool fold_scalar = zero_folds(zero_scalar);
   int rc;
 #define TLQ_PANELM3(T, TM, ZM) launch_panelm<T, TM, ZM>(A, Wp, scales, zeros, C, partial, M, N, K, gshift, zero_scalar, out_dtype, p, band, st)
 #define TLQ_PANELM2(T, ZM) (p.tm == 4 ? TLQ_PANELM3(T, 4, ZM) : TLQ_PANELM3(T, 8, ZM))

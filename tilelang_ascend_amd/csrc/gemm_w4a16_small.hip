@@ -184,7 +184,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void w4a16_small_kernel(const
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const float zf = to_float(zv[rt]);
-          ok = ok && zf == __builtin_rintf(zf) && zf >= -256.0f && zf <= 256.0f;
+          ok = ok && zero_folds(zf);
         }
         if (__builtin_amdgcn_ballot_w64(ok) != ~0ull) return i;
       }
@@ -348,7 +348,7 @@ static int dispatch_small(const SmallArgs& a, const SmallTile& p) {
 int gemm_w4a16_small(const void* A, const void* Wp, const void* scales, const void* zeros, void* C, int64_t M, int64_t N, int64_t K, int64_t group,
                      float zero_scalar, int in_dtype, int out_dtype, int w_layout, const SmallTile& p, const char* what, hipStream_t st) {
   // An integer zero point shared by the whole matrix folds exactly into the unpack bias.
-  const bool fold = zeros == nullptr && zero_scalar == (float)(int)zero_scalar && zero_scalar >= -256.0f && zero_scalar <= 256.0f;
+  const bool fold = zeros == nullptr && zero_folds(zero_scalar);
   int gshift = 0;
   while (((int64_t)1 << gshift) < group) ++gshift;
   const SmallArgs a{A, Wp, scales, zeros, C, (int)M, (int)N, (int)K, gshift, zero_scalar, out_dtype, what, st};

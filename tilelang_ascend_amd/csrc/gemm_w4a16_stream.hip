@@ -351,7 +351,7 @@ __global__ __launch_bounds__(512, 2) void w4a16_stream_kernel(const T* __restric
           largest = __builtin_fmaxf(largest, __builtin_fabsf(zf));
         }
     }
-    const bool integral = fraction == 0 && largest <= 256.0f;
+    const bool integral = fraction == 0 && largest <= kFoldsWithin;
     return __builtin_amdgcn_ballot_w64(integral) == ~0ull;
   };
   // The steps of a window.  A wavefront's step is NU units of TB MFMAs (unit u: k-step u / 2 of its KT, weight tile u % 2): eight with two

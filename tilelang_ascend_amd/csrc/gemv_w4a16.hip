@@ -557,7 +557,7 @@ __device__ __forceinline__ void gemv_rows_body(const T* __restrict__ A, const ui
           zv[it] = has_z ? lds_z[lrow * groups + gsel[it]] : zs;
           sv[it] = ok[it] ? s0 : from_float<T>(0.0f);
           const float zf = to_float(zv[it]);
-          integral = integral && zf == __builtin_rintf(zf) && zf >= -256.0f && zf <= 256.0f;
+          integral = integral && zero_folds(zf);
         }
         if (__builtin_amdgcn_ballot_w64(integral) == ~0ull) {
 #pragma unroll
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(1024) void gemv_w4a16_ring_kernel(const T* __restri
 #pragma unroll
       for (int it = 0; it < ITERS; ++it) {
         const float zf = to_float(zv[it]);
-        integral = integral && zf == __builtin_rintf(zf) && zf >= -256.0f && zf <= 256.0f;
+        integral = integral && zero_folds(zf);
       }
       if (__builtin_amdgcn_ballot_w64(integral) == ~0ull) {
 #pragma unroll

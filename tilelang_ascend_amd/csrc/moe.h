@@ -47,7 +47,6 @@ __device__ __forceinline__ float4_t silu_times(const float4_t& x, const float4_t
   }
   return y;
 }
-__device__ __forceinline__ bool small_integer(float z) { return z == __builtin_rintf(z) && z >= -256.0f && z <= 256.0f; }
 
 // Gate / up (up = true) or down product of the tiles of 256 pairs (moe_w4a16_panel.hip).
 bool moe_panel_takes(const ExpertArgs& a, int64_t pairs, bool up);

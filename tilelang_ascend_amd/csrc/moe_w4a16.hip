@@ -406,7 +406,7 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
         for (int t = 0; t < NT; ++t) {
           sv[t] = a.scales ? ((const T*)sc)[sc_at[t] + g] : one;
           zv[t] = ANY && a.zeros ? ((const T*)zp)[sc_at[t] + g] : zs;
-          if (ANY && kFolds<T>) whole = whole && small_integer(to_float(zv[t]));
+          if (ANY && kFolds<T>) whole = whole && zero_folds(to_float(zv[t]));
         }
         if ((s * KSB + b) * 128 + 128 > a.K) {  // (uniform) behind K: zeros, not an infinite weight times zero
 #pragma unroll
@@ -708,7 +708,7 @@ __global__ __launch_bounds__(512, 4) void moe_few_kernel(const FewArgs a) {
         if constexpr (!kFolds<T>) {
           multiply(std::false_type{});
         } else if constexpr (ANY) {
-          if (__builtin_expect(__builtin_amdgcn_ballot_w64(small_integer(to_float(zv))) == ~0ull, 1)) multiply(std::true_type{});
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(zero_folds(to_float(zv))) == ~0ull, 1)) multiply(std::true_type{});
           else multiply(std::false_type{});
         } else {
           multiply(std::true_type{});
@@ -866,7 +866,7 @@ int launch_few(const char* what, const FewArgs& a, const FewPlan& p, hipStream_t
 
 template <bool UP>
 int run_few(const char* what, const ExpertArgs& x, const void* ids, int64_t pairs, int dtype, const FewPlan& p, hipStream_t st) {
-  const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
+  const bool whole = zero_folds(x.zero_scalar);
   const int units = x.group / 32;
   const int flags = (p.by_pair ? kFewByPair : 0) | (p.by_pair && pairs == x.top_k ? kFewOneToken : 0);
   const FewArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, (const int32_t*)ids, x.out, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
@@ -929,7 +929,7 @@ int run_tiles(const char* what, const ExpertArgs& x, const void* ids, int64_t pa
     const Plan plan{p.order, p.small, p.large, p.totals};
     if (moe_panel(what, x, plan, z.large, dtype, UP, st)) return 1;
   }
-  const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
+  const bool whole = zero_folds(x.zero_scalar);
   const int units = x.group / 32, window = units * 2 / KSB;  // steps of eight groups
   const TileArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, parts ? (void*)parts : x.out, p.small, p.order, (int)pairs, x.E, x.top_k, x.N, x.K, x.K / x.group,
                    make_group_of(units), x.zero_scalar, (int)n_groups, window, (int)chunk_steps};

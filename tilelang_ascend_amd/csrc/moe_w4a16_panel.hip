@@ -128,7 +128,7 @@ int moe_panel(const char* what, const ExpertArgs& x, const Plan& plan, int64_t m
   const int64_t n_groups = moe_panel_groups(x.N, up), grid = most_tiles * n_groups;
   TLQ_REQUIRE(grid <= kMostGroups, "%s: %lld work-groups: call it for fewer tokens at once", what, (long long)grid);
   const PanelArgs a{x.X, x.Wp, x.scales, x.zeros, x.weights, x.out, plan.order, plan.large, plan.totals + 1, x.top_k, x.N, x.K, gshift, (int)n_groups, x.zero_scalar};
-  const bool whole = x.zero_scalar == (float)(int)x.zero_scalar && x.zero_scalar >= -256.0f && x.zero_scalar <= 256.0f;
+  const bool whole = zero_folds(x.zero_scalar);
 #define TLQ_PANEL2(T, UP) (x.zeros ? launch_panel<T, UP, 0>(what, a, grid, st) : whole ? launch_panel<T, UP, 1>(what, a, grid, st) : launch_panel<T, UP, 2>(what, a, grid, st))
 #define TLQ_PANEL(T) (up ? TLQ_PANEL2(T, true) : TLQ_PANEL2(T, false))
   return dtype == TLQ_F16 ? TLQ_PANEL(half_t) : TLQ_PANEL(bf16_t);

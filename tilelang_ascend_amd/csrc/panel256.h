@@ -128,7 +128,7 @@ __device__ __forceinline__ void panel256_steps(uint8_t* smem, const T* __restric
       fract_bits |= bitcast<uint32_t>(__builtin_amdgcn_fractf(zf));
       max_abs = __builtin_fmaxf(max_abs, __builtin_fabsf(zf));
     }
-    return __builtin_amdgcn_ballot_w64(fract_bits == 0 && max_abs <= 256.0f) == ~0ull;
+    return __builtin_amdgcn_ballot_w64(fract_bits == 0 && max_abs <= kFoldsWithin) == ~0ull;
   };
 
 #pragma unroll

@@ -102,6 +102,11 @@ __device__ __forceinline__ NibbleMagic make_nibble_magic() {
 }
 __device__ __forceinline__ uint32_t bfi(uint32_t mask, uint32_t x, uint32_t y) { return (x & mask) | (y & ~mask); }
 
+// Whole zero points that the decoders fold into the unpacking's bias, with one rounding of (u - z) s: where u - z has at most the eight bits of
+// a bfloat16 for every u, 0 .. 15, so that rn(u - z) is u - z (-241 .. 256; by the magnitude, which is one comparison).
+constexpr float kFoldsWithin = 241.0f;
+__host__ __device__ __forceinline__ bool zero_folds(float z) { return z == __builtin_rintf(z) && z >= -kFoldsWithin && z <= kFoldsWithin; }
+
 // ---- 16-bit float helpers ----------------------------------------------------------------
 // bfloat16 <-> float.  The narrowing is round-to-nearest-even (what torch's .to(bfloat16)
 // and the reference's CAST_RINT do).

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void dequant_w4_vec8(const uint32_t* __restric
   auto group_of = [&](int64_t i) { return group_shift >= 0 ? i >> group_shift : i / group_words; };
   auto expand = [&](uint32_t x, T s, T z) {
     const float zf = to_float(z);
-    if (zf == __builtin_rintf(zf) && zf >= -256.0f && zf <= 256.0f) return Expand8<T, true, LAYOUT>(s, z, mg)(x);
+    if (zero_folds(zf)) return Expand8<T, true, LAYOUT>(s, z, mg)(x);
     return Expand8<T, false, LAYOUT>(s, z, mg)(x);
   };
   const int64_t stride = (int64_t)blocks * 512;
