@@ -452,3 +452,161 @@ def test_a_token_gets_the_same_bits_beside_other_tokens(M):  # (few pairs, tiles
         first = first or mine
         assert_bit_equal(mine[0], first[0], "hidden")
         assert_bit_equal(mine[1], first[1], "y")
+
+
+# ---- zero points, scales and inputs of every kind in every kernel -------------------------------------------------------------------
+# M, E, top_k, N, K, group: few pairs; tiles of 32, whole rows and K in parts; of 64, the same; of 256
+EVERY = [(3, 8, 2, 48, 256, 64, FEW), (12, 4, 2, 80, 224, 32, TILES32), (12, 4, 2, 48, 4096, 128, TILES32), (130, 4, 2, 80, 320, 64, TILES64), (60, 2, 2, 48, 4160, 32, TILES64),
+         (2047, 4, 2, 3088, 256, 64, TILES256)]
+
+
+def every_call(up, shape, dtype, scales, zeros, weights=None, x=None, ids=None, seed=121):
+    """-> (the output on the CPU, the oracle's value and bound), all in the tokens that are compared; `zeros` as the kernels take them, or a tensor."""
+    M, E, k, N, K, group, _ = shape
+    T = DT[dtype]
+    Wp, s, _ = make_experts(E, 2 * N if up else N, K, group, T, None, seed)
+    s = s if scales else None
+    z = zeros(s if scales else torch.empty(E, 2 * N if up else N, K // group, dtype=T)) if callable(zeros) else zeros
+    ids = make_ids(M, E, k, "spread", seed + 1) if ids is None else ids
+    some = torch.tensor(sorted({0, 1, 2, M // 2, M - 2, M - 1} & set(range(M))))
+    X = (torch.randn(M, K, generator=gen(seed + 2)) if up else torch.randn(M, k, K, generator=gen(seed + 2))) * (1 if scales else 0.02)
+    X = X.to(T) if x is None else x(X.to(T))
+    args = [X, ids, Wp] if up else [X, ids, torch.rand(M, k, generator=gen(seed + 3)) + 0.25 if weights is None else weights, Wp]
+    make = ops.moe_gate_up_w4a16 if up else ops.moe_down_w4a16
+    kernel = make(E, k, N, K, group, dtype, zeros=kernel_zeros(z), with_scales=scales, **({} if up else {"out_dtype": "float32"}))
+    got = kernel(*operands(*args, *([s] if scales else []), z)).cpu()
+    if up:
+        return got[some], ref.moe_gate_up(X[some], ids[some], Wp, s, z, group), some
+    return got[some], ref.moe_down(X[some], ids[some], args[2][some], Wp, s, z, group), some
+
+
+@pytest.mark.parametrize("shape", EVERY)
+def test_every_kernel_is_among_them(shape):
+    assert choice(True, *shape[:6], None)[0] == shape[6] and choice(False, *shape[:6], "tensor")[0] == shape[6]
+
+
+def whole_then_not(s):
+    """Zero points that are whole numbers in the first half of a row and not in the second."""
+    z = torch.randint(6, 10, s.shape, generator=gen(5)).to(s.dtype)
+    half = s.shape[2] // 2
+    z[:, :, half:] += 0.5
+    return z
+
+
+def large_whole(s):
+    return (torch.randint(0, 2, s.shape, generator=gen(6)) * 512 - 256).to(s.dtype)
+
+
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("shape", EVERY)
+def test_scales_and_zero_points_of_every_kind(shape, dtype, up):
+    for scales in (True, False):
+        for zeros in (None, 8, 7.5, whole_then_not):
+            got, want, _ = every_call(up, shape, dtype, scales, zeros)
+            assert_close64(got, *want, f"{shape} {dtype} up={up} scales={scales} zeros={zeros}")
+    # the ends of the zero points that bfloat16 folds into the unpacking, and those next to them: u - z rounds there
+    for zeros in (255, -255, 256, -256, 257, -258, large_whole):
+        got, want, _ = every_call(up, shape, dtype, True, zeros, x=lambda x: x * 0.02)
+        assert_close64(got, *want, f"{shape} {dtype} up={up} zeros={zeros}")
+
+
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("shape", EVERY)
+def test_tokens_that_are_no_numbers_leave_the_others_alone(shape, dtype, up):
+    M = shape[0]
+
+    def spoil(x):
+        x = x.clone()
+        x[1::3] = float("nan")
+        x[1::6] = float("inf")
+        return x
+
+    plain, want, some = every_call(up, shape, dtype, True, 8)
+    got, _, _ = every_call(up, shape, dtype, True, 8, x=spoil)
+    clean = (some % 3) != 1
+    assert_bit_equal(got[clean], plain[clean], "clean tokens")
+    assert not bool(torch.isfinite(got[~clean]).any())
+
+
+@gpu
+@pytest.mark.parametrize("shape", EVERY)
+def test_two_graphs_and_an_eager_call_of_the_same_weights(shape):
+    """Gate / up and down captured twice with inputs of their own, replayed in turn and on two streams at once, with eager calls in between."""
+    M, E, k, N, K, group, _ = shape
+    T = torch.bfloat16
+    w1, s1, z1 = operands(*make_experts(E, 2 * N, K, group, T, "int", 131))
+    w2, s2, _ = make_experts(E, K, N, N, T, None, 132) if N % 32 == 0 else make_experts(E, K, N + 16, N + 16, T, None, 132)
+    w2, s2 = w2.cuda(), s2.cuda()
+    N2 = w2.shape[2] * 2
+    up, down = ops.moe_gate_up_w4a16(E, k, N, K, group, "bfloat16", zeros="tensor"), ops.moe_down_w4a16(E, k, K, N2, N2, "bfloat16", "float32", zeros=8)
+
+    def layer(x, ids, weights):
+        h = up(x, ids, w1, s1, z1)
+        return down(torch.nn.functional.pad(h, (0, N2 - N)), ids, weights, w2, s2)
+
+    ins = [[torch.randn(M, K, generator=gen(140 + i)).to(T).cuda(), make_ids(M, E, k, "holes", 150 + i).cuda(), torch.rand(M, k, generator=gen(160 + i)).cuda()] for i in range(4)]
+    want = [layer(*a) for a in ins]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(*ins[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, slots, outs = [], [], []
+    for i in range(2):
+        slots.append([t.clone() for t in ins[i]])
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(layer(*slots[i]))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for rep in range(4):
+        for i in range(2):
+            for t, v in zip(slots[i], ins[(rep + 2 * i) % 4]):
+                t.copy_(v)
+            outs[i].fill_(float("nan"))
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        beside = layer(*ins[rep])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert_bit_equal(outs[i].cpu(), want[(rep + 2 * i) % 4].cpu(), f"graph {i}, replay {rep}")
+        assert_bit_equal(beside.cpu(), want[rep].cpu(), f"eager beside replay {rep}")
+
+
+@gpu
+def test_calls_from_several_threads():
+    import threading
+
+    shape = EVERY[2]
+    M, E, k, N, K, group, _ = shape
+    w, s, z = operands(*make_experts(E, 2 * N, K, group, torch.float16, "int", 171))
+    up = ops.moe_gate_up_w4a16(E, k, N, K, group, zeros="tensor")
+    ins = [(torch.randn(m, K, generator=gen(172 + m)).half().cuda(), make_ids(m, E, k, "spread", 173 + m).cuda()) for m in (1, 12, 70, 200)]
+    want = [up(*a, w, s, z) for a in ins]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in ins], []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(10):
+                    got[i].append(up(*ins[i], w, s, z))
+            st.synchronize()
+        except Exception as e:  # noqa: BLE001 (a thread's failure is the test's)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(ins))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for g, y in zip(got, want):
+        for one in g:
+            assert_bit_equal(one.cpu(), y.cpu(), "threads")
