@@ -387,8 +387,9 @@ int tlq_act_quant_i8(const void* X, void* Y, void* S, int64_t M, int64_t N, int 
  *   n_group > 1: the E experts are n_group runs of E / n_group; a run's value is the sum of its two largest v, and only the
  *   experts of the topk_group best runs may be chosen
  *   ids = the top_k experts with the largest v, largest first;  weights = p[ids], divided by their sum with renormalize, times scaling
- * Scores and what is compared are binary64, equal values go to the lowest index.  A logit or biased score of -infinity or NaN
- * masks its expert (p = 0); where fewer than top_k experts are left, the remaining ids are -1 with weight 0.  Logits of
+ * Scores and what is compared are binary64, equal values go to the lowest index.  A logit of -infinity or NaN masks its expert (p = 0,
+ * and the softmax is over the others); a biased score of either keeps its expert from being chosen (the softmax still counts
+ * it).  Where fewer than top_k experts are left, the remaining ids are -1 with weight 0.  Logits of
  * +infinity share the softmax among them.  Where the chosen scores add up to 0 the renormalised weights are 0.
  * logits [M, E] in_dtype (TLQ_F16, TLQ_BF16, TLQ_F32), bias fp32 [E] or NULL, weights fp32 [M, top_k], ids int32 [M, top_k].
  * E <= 1024, top_k <= 64, n_group <= 64. */
@@ -404,8 +405,8 @@ int tlq_moe_route(const void* logits, const void* bias, void* weights, void* ids
  * tlq_moe_down_w4a16:  Y[t, n] = rn_out( sum_j weights[t, j] * (H[t, j] . W[e, n]) ), fp32 sums; slots without an expert add nothing.
  *   H [M, top_k, K] in_dtype, weights fp32 [M, top_k], w_packed [E, N, K / 2], scales / zeros [E, N, K / group], Y [M, N] out_dtype.
  * W = rn_T(rn_T(T(u) - z) * s) as in tlq_dequant_w4 (scales NULL: 1; zeros NULL: zero_scalar); T = dtype: TLQ_F16 or TLQ_BF16.
- * N % 16 == 0, K % 32 == 0, N * K < 2^32, group a multiple of 32 that divides K, E <= 1024, top_k <= 64, M * top_k < 2^24.  X, H, Y, w_packed,
- * scales and zeros 16-byte aligned.  Results do not depend on timing: no floating-point sum is formed by atomic adds.
+ * N % 16 == 0, K % 32 == 0, N and K < 2^24, N * K < 2^32, group a multiple of 32 that divides K, E <= 1024, top_k <= 64, M * top_k < 2^24 (gate / up of
+ * very many outputs: of fewer tokens, said by the error).  X, H, Y, w_packed, scales and zeros 16-byte aligned.  Results do not depend on timing: no floating-point sum is formed by atomic adds.
  * The workspace (16-byte aligned, at least tlq_moe_*_workspace_bytes) holds nothing between calls; two calls that may run at the
  * same time need one each.  The size does not fall as M grows: that of a program's largest call does for its others of the same sizes. */
 int64_t tlq_moe_gate_up_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K);

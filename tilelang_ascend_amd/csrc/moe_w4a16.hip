@@ -207,8 +207,8 @@ constexpr bool kFolds = !std::is_same<T, half_t>::value;
 // two buffers a step ahead, the packed weights go straight into operand registers a step ahead -- lane (r16, q) has the 32 values 32 q ..
 // of each block of row r16, at MFMA k-step j the eight of word 4 q + j --, are expanded there and multiplied with all rows: a weight
 // is expanded once per 16 MAXMT pairs, an activation operand read once per NT tiles.  One barrier a step.
-//   64 pairs: fp16, zero points, 211 tokens on 2 of 8 experts of 14336 x 4096 (gate / up): 246 us; the vector units were busy for
-// 57 % of it, the matrix units for 26 %; the rest is the trip of a step's loads.  With 64 rows of W a wavefront in the
+//   64 pairs: fp16, zero points, 211 tokens on 2 of 8 experts of 14336 x 4096 (gate / up): 240 - 260 us; the vector units issue for
+// 60 % of it, the matrix units are busy for 25 %, 1.36 GB come from behind L2: every further tile of an expert reads its rows again.  With 64 rows of W a wavefront in the
 // place of 32 (NT = 4) 5 - 10 % slower -- fewer work-groups on a CU, coarser rounds --; with 128 pairs level where experts have 192 pairs and more, 10 - 30 % slower
 // below; tiles of an expert side by side on the same weight rows 3 - 6 % faster on matrices of 58 MB, 2 - 8 % slower on small ones.
 //   32 pairs: bf16, 48 tokens on 8 of 128 experts of 768 x 2048 (gate / up): 35 - 40 us for 199 MB, the rate of a large copy.
@@ -485,9 +485,9 @@ __global__ __launch_bounds__(256, ANY && kFolds<T> ? 3 : 4) void moe_tile_kernel
 //   A tile is 16 weight rows: 16 outputs, or 8 gate rows and the 8 up rows that go with them.  A block is 128 values of K of a tile.
 // Where tiles are few, `splits` wavefronts share one, each with a part of K; their sums meet in LDS and are added in the order of K.
 // Long rows of the down product are cut into `chunks` work-groups too, whose sums moe_combine_kernel adds.
-//   fp16, zero points: one token, 6 of 64 experts of 1408 x 2048, gate / up 10.3 us (18 MB), down 9.3; 2 of 8 of 4096 x 14336, down 21 us + 4 for the sums
-// (66 MB, 13.4 us at the rate of a large copy).  What is left is latency: ids, then rows and scales, then 28 KB of weights a wavefront, 4 KB at a time.  With
-// eight blocks asked for at once the kernel spills and takes 25 - 40 % more.
+//   fp16, zero points: one token, 6 of 64 experts of 1408 x 2048, gate / up 10.3 us (18 MB), down 9.3; 2 of 8 of 4096 x 14336, down 22 us + 4 for the sums
+// (66 MB, 13.4 us at the rate of a large copy).  What is left is latency: ids, then rows and scales, then the weights of a wavefront, 4 KB at a time: 8 KB in the
+// first case, 28 KB in the last.  With eight blocks asked for at once the kernel spills and takes 25 - 40 % more.
 constexpr int kFewPairs = 2048;
 constexpr int kFewGroup = 4;
 enum { kFewByPair = 1, kFewOneToken = 2 };

@@ -4,8 +4,9 @@
 // up rows, so that gate and up of an output meet in one lane.  down: 256 outputs, 64 a wavefront; weighted fp32 rows.
 // Work-groups in the order of the tiles, those of one tile next to each other, and every XCD a contiguous range of them: 32 at a time, that share
 // a few tiles' activation rows and one expert's weights in its L2.
-//   bf16, one zero point, 65536 pairs of 64 experts of 1024 x 2048 (gate / up): 523 us, 1.05 PFLOP/s of the pairs' own products; the rate of the step
-// loop alone is that of the dense product, 1.3 - 1.35 (power), the difference the rows that fill up an expert's last tile and the last round of work-groups.
+//   bf16, one zero point, 65536 pairs of 64 experts of 1024 x 2048 (gate / up): 519 - 549 us by the tracer on two boxes, 1.0 - 1.06 PFLOP/s of the pairs' own
+// products; the rate of the step loop alone is that of the dense product, 1.3 - 1.35 (power), the difference the rows that fill up an expert's last tile and
+// the last round of work-groups.
 #include "moe.h"
 #include "panel256.h"
 

@@ -7,7 +7,7 @@ weight matrix per expert, chosen on the device:
     hidden = moe_gate_up_w4a16(E, top_k, N, K, ...)(x, ids, w13, s13)        x [M, K] -> [M, top_k, N]
     y = moe_down_w4a16(E, top_k, K, N, ...)(hidden, ids, weights, w2, s2)    -> [M, K]
 
-Every kernel takes any number of tokens M.  Nothing is copied to the host: a step can be captured in a graph.  Weights are
+Routing takes any number of tokens M, the products any with M * top_k below 2^24.  Nothing is copied to the host: a step can be captured in a graph.  Weights are
 those of w4a16_gemm (uint8 [rows, K/2], low nibble first, W = rn(rn(u - z) * s) in the activations' type), the experts' matrices
 back to back; `gate` rows come before `up` rows.  An id outside 0 .. E - 1 is a slot without an expert here (another GPU's
 share, or an empty one): its hidden row is 0 and it adds nothing.  Results do not depend on timing.
@@ -39,7 +39,7 @@ def moe_route(E: int, top_k: int, scoring: str = "softmax", n_group: int = 1, to
     their weights are p of the chosen ones (the bias does not enter), divided by their sum with `renormalize`, times `scaling`.
     n_group > 1: only experts of the topk_group best of n_group runs of neighbouring experts are chosen, a run's value being
     the sum of its two largest p + bias.  What is compared is binary64.  A logit (or p + bias) of -infinity or NaN masks its
-    expert; slots for which no expert is left hold id -1 and weight 0."""
+    expert (a logit: in the softmax too); slots for which no expert is left hold id -1 and weight 0."""
     _check_experts(E, top_k)
     if scoring not in _SCORING:
         raise ValueError(f"scoring must be softmax or sigmoid, got {scoring}")
