@@ -116,7 +116,7 @@ int tlq_debug_check_gemv_ring_addressing(int64_t M, int64_t N, int64_t K, int64_
  * that share a tile, tiles of a wavefront, parts of K, bytes of LDS that the launch asks for, those that the kernel uses, work-groups of an expert.  0: sizes
  * that no call takes. */
 int tlq_debug_moe_choice(int up, int64_t M, int64_t E, int64_t top_k, int64_t N, int64_t K, int64_t group, int zeros, void* plan_out);
-/* The group of `group` values that the u-th 32 values of a row belong to, by the arithmetic of the experts' tiles. */
+/* The group of `group` values that the u-th 32 values of a row belong to, by the arithmetic of the experts' tiles.  -1: sizes that no row has. */
 int64_t tlq_debug_moe_group(int64_t group, int64_t u);
 
 /* Tuning hooks for benchmark sweeps and the autotuner (each sets a value of the CALLING THREAD, read by that thread's

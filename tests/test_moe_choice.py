@@ -74,6 +74,8 @@ def test_the_group_of_a_value_for_groups_of_any_size():
         for u in sorted({0, 1, longest - 1, *edges}):
             if 0 <= u < longest:
                 assert group_of(units * 32, u) == u // units, (units, u)
+    for group, u in ((0, 0), (31, 0), (33, 0), (-32, 0), (1 << 24, 0), (64, -1), (64, longest)):
+        assert group_of(group, u) == -1
 
 
 @gpu

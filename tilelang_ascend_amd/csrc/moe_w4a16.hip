@@ -1093,4 +1093,7 @@ extern "C" int tlq_debug_moe_choice(int up, int64_t M, int64_t E, int64_t top_k,
   return kernel;
 }
 
-extern "C" int64_t tlq_debug_moe_group(int64_t group, int64_t u) { return make_group_of((int)(group / 32))((int)u); }
+extern "C" int64_t tlq_debug_moe_group(int64_t group, int64_t u) {
+  if (group < 32 || group % 32 != 0 || group >= ((int64_t)1 << 24) || u < 0 || u >= ((int64_t)1 << 19)) return -1;
+  return make_group_of((int)(group / 32))((int)u);
+}
