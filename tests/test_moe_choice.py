@@ -612,3 +612,32 @@ def test_calls_from_several_threads():
     for g, y in zip(got, want):
         for one in g:
             assert_bit_equal(one.cpu(), y.cpu(), "threads")
+
+
+@gpu
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("shape", EVERY)
+def test_nothing_is_written_outside_of_the_output_and_the_workspace(shape, up):
+    """A workspace of exactly the size that is asked for, and 4 KB on either side of it and of the output."""
+    M, E, k, N, K, group, _ = shape
+    lib, P, side = _abi.load(), ctypes.c_void_p, 4096
+    T = torch.bfloat16
+    w, s, z = operands(*make_experts(E, 2 * N if up else N, K, group, T, "int", 181))
+    ids = make_ids(M, E, k, "holes", 182).cuda()
+    x = torch.randn(M, K, generator=gen(183)).to(T).cuda() if up else torch.randn(M, k, K, generator=gen(183)).to(T).cuda()
+    weights = torch.rand(M, k, generator=gen(184)).cuda()
+    size = (lib.tlq_moe_gate_up_workspace_bytes if up else lib.tlq_moe_down_workspace_bytes)(M, E, k, N, K)
+    out_size = M * (k if up else 1) * N * 2
+    ws = torch.full((size + 2 * side,), 0xAB, dtype=torch.uint8, device="cuda")
+    out = torch.full((out_size + 2 * side,), 0xFF, dtype=torch.uint8, device="cuda")
+    ws_at, out_at, st = P(ws.data_ptr() + side), P(out.data_ptr() + side), torch.cuda.current_stream().cuda_stream
+    if up:
+        rc = lib.tlq_moe_gate_up_w4a16(_abi.ptr(x), _abi.ptr(ids), _abi.ptr(w), _abi.ptr(s), _abi.ptr(z), out_at, ws_at, size, M, E, k, N, K, group, 0.0, _abi.BF16, st)
+    else:
+        rc = lib.tlq_moe_down_w4a16(_abi.ptr(x), _abi.ptr(ids), _abi.ptr(weights), _abi.ptr(w), _abi.ptr(s), _abi.ptr(z), out_at, ws_at, size, M, E, k, N, K, group, 0.0,
+                                    _abi.BF16, _abi.BF16, st)
+    _abi.check(rc)
+    torch.cuda.synchronize()
+    for buffer, n, fill in ((ws, size, 0xAB), (out, out_size, 0xFF)):
+        assert bool((buffer[:side] == fill).all()) and bool((buffer[side + n:] == fill).all())
+    assert bool(torch.isfinite(out[side:side + out_size].view(T)).all())  # (0xFFFF is a NaN: every output was written)
