@@ -377,6 +377,39 @@ int tlq_quantize_sym4(const void* W, void* q_minus8, void* scales, int64_t N, in
  * Its outputs are the A / scale_a operands of tlq_gemm_w8a8. */
 int tlq_act_quant_i8(const void* X, void* Y, void* S, int64_t M, int64_t N, int in_dtype, int round_scale, void* stream);
 
+/* Ahead of a projection: the residual's addition and the root-mean-square norm, with the outputs that the products take.  No counterpart in
+ * the reference.
+ *   h = rn_T(x + residual), written to H (residual NULL: h = x, H NULL);  y = h * w / sqrt(mean_n(h^2) + eps), fp32
+ *   Y = rn_T(y) (NULL: not wanted);  Q, S (both NULL: not wanted) as tlq_act_quant_i8 makes them, of y: S = max(max_n |y|, 1e-4) / 127
+ *   (round_scale: 2^ceil(log2)), Q = rint(clamp(y / S, -127, 127)).
+ * Where S is neither the floor nor rounded to a power of two, Q is decided exactly: rint(127 h w / max_n |h w|), half to even.
+ * A row with a NaN in it is NaN in Y; -127 and the floor's scale in Q and S, as the quantiser has it.  Sums of squares beyond fp32's range (bfloat16
+ * values from 1e19 on) make a row of 0.
+ * X, residual, H, Y [M, N] and weight [N] dtype (TLQ_F16 or TLQ_BF16), Q int8 [M, N], S fp32 [M]; any M and N (rows of a multiple of 8 values up
+ * to 32768, 16-byte aligned, Q 8-byte, are read once); 1e-12 <= eps <= 1.  H may be the residual or X, and Y may be X.  Y and Q are operands of
+ * tlq_gemm_w4a16, tlq_low_rank_update and tlq_gemm_w8a8. */
+int tlq_residual_rms_norm(const void* X, const void* residual, const void* weight, void* H, void* Y, void* Q, void* S, int64_t M,
+                          int64_t N, float eps, int dtype, int round_scale, void* stream);
+
+/* Between the products of an MLP: y = silu(g) * u, g = X[m, n], u = X[m, N + n], silu(g) = g / (1 + exp(-g)), fp32; Y, Q and S of it as above.
+ * X [M, 2 N], Y [M, N] dtype, Q int8 [M, N], S fp32 [M]; any M and N. */
+int tlq_gated_silu(const void* X, void* Y, void* Q, void* S, int64_t M, int64_t N, int dtype, int round_scale, void* stream);
+
+/* Low-rank adapters of many requests beside a projection (tlq_gemm_w4a16, tlq_gemm_w8a8, ...), whose outputs are one to three parts of n0, n1, n2
+ * values side by side (n1 = n2 = 0, n2 = 0: fewer), N = n0 + n1 + n2, each part with an A of its own:
+ *   out[m, n] = rn_out( Y[m, n] + scaling[l] * sum_j (sum_k X[m, k] * A[l, p * rank + j, k]) * B[l, n, j] ),  l = ids[m], p the part of n
+ * fp32 sums, rounded once.  An id outside 0 .. L - 1 is a row without an adapter: out = Y, and nothing of its X is looked at.  Results do not depend on timing, nor
+ * a row's on the other rows.
+ * X [M, K], A [L, parts * rank, K], B [L, N, rank] in_dtype (TLQ_F16 or TLQ_BF16), Y and out [M, N] out_dtype (in_dtype or TLQ_F32), ids
+ * int32 [M], scaling fp32 [L].  out may be Y.  rank 8, 16, 32, 64 or 128 (adapters of a lower rank: rows and columns of 0), K % 32 == 0,
+ * n0, n1, n2 % 16 == 0, L <= 4096, M < 2^24 (of very long rows fewer, said by the error); X, Y, A, B and out 16-byte aligned.
+ * The workspace (16-byte aligned, at least tlq_low_rank_update_workspace_bytes, which does not fall as M grows) holds nothing between calls;
+ * two calls that may run at the same time need one each. */
+int64_t tlq_low_rank_update_workspace_bytes(int64_t M, int64_t L, int64_t rank, int64_t parts, int64_t K);
+int tlq_low_rank_update(const void* X, const void* Y, const void* ids, const void* A, const void* B, const void* scaling, void* out,
+                        void* workspace, int64_t workspace_bytes, int64_t M, int64_t L, int64_t rank, int64_t n0, int64_t n1,
+                        int64_t n2, int64_t K, int in_dtype, int out_dtype, void* stream);
+
 /* A mixture-of-experts layer on packed 4-bit weights: the router's choice, the experts' first product with its gated activation,
  * the experts' second product with the weighted sum over a token's experts.  No counterpart in the reference, whose quantised
  * products are dense (examples/dequantize_gemm); weights, scales and zero points are those of tlq_gemm_w4a16, one matrix per

@@ -639,3 +639,75 @@ def moe_down(H, ids, weights, B_packed, scales=None, zeros=None, group=128):
     y = (dots * w[:, :, None]).sum(1)
     off = mags * (K + 8) * 2.0**-24
     return y, (w.abs()[:, :, None] * (off + (dots.abs() + off) * (k + 2) * 2.0**-24)).sum(1)
+
+
+# ------------------------------------------------------------------------------------------
+# between and beside the products of a block (no counterpart in the reference: the definitions of include/tlq.h, in 64 bits)
+# ------------------------------------------------------------------------------------------
+def _rounded_sum(x, residual):
+    """x + residual rounded to their type once: fp32 holds the sum of two such values to 24 bits, and rounding that again is innocuous (24 >= 2 p + 2)."""
+    return (x.float() + residual.float()).to(x.dtype)
+
+
+def residual_rms_norm(x, residual, weight, eps):
+    """-> (h in x's type, y float64 [M, N], v = h * weight float64: y over rstd)."""
+    x, weight = x.cpu(), weight.cpu()
+    h = x if residual is None else _rounded_sum(x, residual.cpu())
+    z = h.to(torch.float64)
+    v = z * weight.to(torch.float64)
+    return h, v / torch.sqrt((z * z).sum(1, keepdim=True) / z.shape[1] + eps), v
+
+
+def norm_codes(v):
+    """rint(127 v / max |v|) of each row, half to even, in whole numbers: v is a multiple of 2^-300 or so, and Python's fractions hold it."""
+    from fractions import Fraction
+
+    out = torch.zeros(v.shape, dtype=torch.int8)
+    for m, row in enumerate(v.tolist()):
+        top = max(abs(Fraction(e)) for e in row)
+        for n, e in enumerate(row):
+            out[m, n] = round(127 * Fraction(e) / top) if top else 0  # (round of a Fraction: half to even)
+    return out
+
+
+def gated_silu(x):
+    """-> y float64 [M, N]."""
+    g, u = x.cpu().to(torch.float64).chunk(2, 1)
+    return g / (1 + torch.exp(-g)) * u
+
+
+def row_scales(y, round_scale=False):
+    """-> S float64 [M]: of the quantiser, max(max |y|, 1e-4) / 127 or the next power of two."""
+    s = y.abs().amax(1).clamp(min=1e-4) / 127
+    return torch.exp2(torch.ceil(torch.log2(s))) if round_scale else s
+
+
+def low_rank_update(X, Y, ids, A, B, scaling, parts):
+    """-> (out, what it may be off by before its rounding) float64 [M, N], one row at a time.
+
+    fp32 sums of K and then rank products: (K + 16) 2^-24 of the first sums' magnitudes, and of the second's (rank + 16) 2^-24; the first
+    sums may be handed on in two pieces of the activations' type, the second's products round to fp32: 2^-15 (bfloat16: 16 bits) or 2^-20 (float16) of
+    the second sums' magnitudes; the scaling's product and the addition: 2^-23 of either side."""
+    X, Y, ids, A, B, scaling = (t.cpu() for t in (X, Y, ids, A, B, scaling))
+    M, K = X.shape
+    L, rows, _ = A.shape
+    r = rows // len(parts)
+    pieces = 2.0**-15 if X.dtype == torch.bfloat16 else 2.0**-20
+    out = Y.to(torch.float64).clone()
+    off = torch.zeros_like(out)
+    for m in range(M):
+        e = int(ids[m])
+        if not 0 <= e < L:
+            continue
+        x, a, s = X[m].to(torch.float64), A[e].to(torch.float64), float(scaling[e])
+        h, dh = a @ x, (a.abs() @ x.abs()) * (K + 16) * 2.0**-24
+        begin = 0
+        for p, n in enumerate(parts):
+            b = B[e, begin: begin + n].to(torch.float64)
+            hp, dp = h[p * r: (p + 1) * r], dh[p * r: (p + 1) * r]
+            delta = s * (b @ hp)
+            mags = abs(s) * (b.abs() @ (hp.abs() + dp))
+            off[m, begin: begin + n] = abs(s) * (b.abs() @ dp) + mags * ((r + 16) * 2.0**-24 + pieces) + (delta.abs() + out[m, begin: begin + n].abs()) * 2.0**-23
+            out[m, begin: begin + n] += delta
+            begin += n
+    return out, off

@@ -63,6 +63,10 @@ SIGNATURES = {
     "tlq_pack_int4": (_int, [_vp, _vp, _i64, _i64, _int, _vp]),
     "tlq_quantize_sym4": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
     "tlq_act_quant_i8": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "tlq_residual_rms_norm": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _int, _int, _vp]),
+    "tlq_gated_silu": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "tlq_low_rank_update_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "tlq_low_rank_update": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp]),
     "tlq_moe_route": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _int, _f32, _int, _vp]),
     "tlq_moe_gate_up_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "tlq_moe_down_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),

@@ -37,6 +37,8 @@ SOURCES = [
     "decode_i4.hip",
     "decode_lowbit.hip",
     "act_quant.hip",
+    "norm_act.hip",
+    "low_rank.hip",
     "repack.hip",
     "gemv_plain.hip",
     "gemv_w4a16.hip",

@@ -36,7 +36,7 @@ namespace {
   X(tlq_act_quant_i8) X(tlq_gemm_w4a8_ws) X(tlq_gemm_w4a8) X(tlq_gemm_i8) X(tlq_gemm_f16_ws) X(tlq_f16_workspace_bytes)          \
   X(tlq_gemm_f16_batched) X(tlq_gemv) X(tlq_gemm_f16_splitk) X(tlq_dequant_w4_layout) X(tlq_unpack_int4) X(tlq_pack_int4)        \
   X(tlq_quantize_sym4) X(tlq_moe_route) X(tlq_moe_gate_up_workspace_bytes) X(tlq_moe_down_workspace_bytes) X(tlq_moe_gate_up_w4a16)  \
-  X(tlq_moe_down_w4a16)
+  X(tlq_moe_down_w4a16) X(tlq_residual_rms_norm) X(tlq_gated_silu) X(tlq_low_rank_update) X(tlq_low_rank_update_workspace_bytes)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   TLQ_ENTRIES(X)
@@ -44,7 +44,7 @@ struct Entries {
 };
 Entries lib;
 
-enum Kind { kW4A16, kW8A8, kActQuant, kW4A8Ws, kW4A8, kI8, kF16, kF16Batched, kGemv, kSplitK, kMoeRoute, kMoeGateUp, kMoeDown };
+enum Kind { kW4A16, kW8A8, kActQuant, kW4A8Ws, kW4A8, kI8, kF16, kF16Batched, kGemv, kSplitK, kMoeRoute, kMoeGateUp, kMoeDown, kNorm, kGated, kLowRank };
 struct KindName {
   const char* name;
   Kind kind;
@@ -53,7 +53,8 @@ struct KindName {
 const KindName kKinds[] = {{"w4a16", kW4A16, 10, 3}, {"w8a8", kW8A8, 8, 4},  {"act_quant", kActQuant, 3, 3}, {"w4a8_ws", kW4A8Ws, 4, 4},
                            {"w4a8", kW4A8, 4, 3},    {"i8", kI8, 3, 3},      {"f16", kF16, 3, 3},            {"f16_batched", kF16Batched, 5, 3},
                            {"gemv", kGemv, 3, 3},    {"splitk", kSplitK, 5, 3},
-                           {"moe_route", kMoeRoute, 8, 3}, {"moe_gate_up", kMoeGateUp, 8, 4}, {"moe_down", kMoeDown, 9, 5}};
+                           {"moe_route", kMoeRoute, 8, 3}, {"moe_gate_up", kMoeGateUp, 8, 4}, {"moe_down", kMoeDown, 9, 5},
+                           {"norm", kNorm, 6, 3},    {"gated", kGated, 5, 2}, {"low_rank", kLowRank, 8, 7}};
 
 const int kMaxDims = 4, kMaxParams = 8, kMaxSymbols = 4;
 enum Role { kInput, kOutput, kWorkspace };
@@ -124,6 +125,8 @@ int launch(const PlanObject& p, const at::Tensor* const* t, int device, hipStrea
     ws_bytes = lib.tlq_moe_gate_up_workspace_bytes(t[0]->size(0), v[0], v[1], v[2], v[3]);
   } else if (p.kind == kMoeDown) {
     ws_bytes = lib.tlq_moe_down_workspace_bytes(t[0]->size(0), v[0], v[1], v[2], v[3]);
+  } else if (p.kind == kLowRank) {
+    ws_bytes = lib.tlq_low_rank_update_workspace_bytes(t[0]->size(0), v[0], v[1], v[3] == 0 ? 1 : v[4] == 0 ? 2 : 3, v[5]);
   }
   c10::DataPtr ws;  // the allocator's block alone: no tensor around it
   if (ws_bytes > 0) {
@@ -174,6 +177,24 @@ int launch(const PlanObject& p, const at::Tensor* const* t, int device, hipStrea
       return lib.tlq_moe_down_w4a16(ptr(t[0]), ptr(t[1]), ptr(t[2]), ptr(t[3]), ptr(s), ptr(z), ptr(t[i]), w, ws_bytes, t[0]->size(0), v[0], v[1], v[2],
                                     v[3], v[4], p.zero, (int)v[5], (int)v[8], stream);
     }
+    // v: N, type, round_scale, with a residual, with Y, with Q and S; p.zero: eps
+    case kNorm: {
+      int i = v[3] ? 3 : 2;
+      void* const h = v[3] ? ptr(t[i++]) : nullptr;
+      void* const y = v[4] ? ptr(t[i++]) : nullptr;
+      return lib.tlq_residual_rms_norm(ptr(t[0]), v[3] ? ptr(t[1]) : nullptr, ptr(t[v[3] ? 2 : 1]), h, y, v[5] ? ptr(t[i]) : nullptr,
+                                       v[5] ? ptr(t[i + 1]) : nullptr, t[0]->size(0), v[0], p.zero, (int)v[1], (int)v[2], stream);
+    }
+    // v: N, type, round_scale, with Y, with Q and S
+    case kGated: {
+      const int i = v[3] ? 2 : 1;
+      return lib.tlq_gated_silu(ptr(t[0]), v[3] ? ptr(t[1]) : nullptr, v[4] ? ptr(t[i]) : nullptr, v[4] ? ptr(t[i + 1]) : nullptr, t[0]->size(0), v[0],
+                                (int)v[1], (int)v[2], stream);
+    }
+    // v: L, rank, the three parts, K, input type, output type
+    case kLowRank:
+      return lib.tlq_low_rank_update(ptr(t[0]), ptr(t[1]), ptr(t[2]), ptr(t[3]), ptr(t[4]), ptr(t[5]), ptr(t[6]), w, ws_bytes, t[0]->size(0), v[0], v[1], v[2],
+                                     v[3], v[4], v[5], (int)v[6], (int)v[7], stream);
     case kSplitK: return lib.tlq_gemm_f16_splitk(ptr(t[0]), ptr(t[1]), ptr(t[2]), v[0], v[1], v[2], v[3], (int)v[4], TLQ_B_KN, stream);
   }
   return 1;
@@ -327,6 +348,8 @@ PyObject* plan_new(PyTypeObject* type, PyObject* args, PyObject*) {
   if (kn->kind == kW4A16) least += (p->v[8] != 0) + (p->v[9] != 0);
   if (kn->kind == kW8A8 || kn->kind == kMoeRoute) least += p->v[7] != 0;
   if (kn->kind == kMoeGateUp || kn->kind == kMoeDown) least += (p->v[6] != 0) + (p->v[7] != 0);
+  if (kn->kind == kNorm) least += 2 * (p->v[3] != 0) + (p->v[4] != 0) + 2 * (p->v[5] != 0) - 1;
+  if (kn->kind == kGated) least += (p->v[3] != 0) + 2 * (p->v[4] != 0) - 1;
   if (n > kMaxParams || n < least) return bad("wrong number of parameters");
   p->n_params = (int)n;
   std::vector<std::string> names;
