@@ -385,14 +385,14 @@ int tlq_act_quant_i8(const void* X, void* Y, void* S, int64_t M, int64_t N, int 
  * Where S is neither the floor nor rounded to a power of two, Q is decided exactly: rint(127 h w / max_n |h w|), half to even.
  * A row with a NaN in it is NaN in Y; -127 and the floor's scale in Q and S, as the quantiser has it.  Sums of squares beyond fp32's range (bfloat16
  * values from 1e19 on) make a row of 0.
- * X, residual, H, Y [M, N] and weight [N] dtype (TLQ_F16 or TLQ_BF16), Q int8 [M, N], S fp32 [M]; any M and N (rows of a multiple of 8 values up
- * to 32768, 16-byte aligned, Q 8-byte, are read once); 1e-12 <= eps <= 1.  H may be the residual or X, and Y may be X.  Y and Q are operands of
+ * X, residual, H, Y [M, N] and weight [N] dtype (TLQ_F16 or TLQ_BF16), Q int8 [M, N], S fp32 [M]; any M below 2^31 and N below 2^30 (fastest with rows of a
+ * multiple of 8 values, 16-byte aligned, Q 8-byte; beyond 32768 values a row is read twice); 1e-12 <= eps <= 1.  H may be the residual or X, and Y may be X.  Y and Q are operands of
  * tlq_gemm_w4a16, tlq_low_rank_update and tlq_gemm_w8a8. */
 int tlq_residual_rms_norm(const void* X, const void* residual, const void* weight, void* H, void* Y, void* Q, void* S, int64_t M,
                           int64_t N, float eps, int dtype, int round_scale, void* stream);
 
 /* Between the products of an MLP: y = silu(g) * u, g = X[m, n], u = X[m, N + n], silu(g) = g / (1 + exp(-g)), fp32; Y, Q and S of it as above.
- * X [M, 2 N], Y [M, N] dtype, Q int8 [M, N], S fp32 [M]; any M and N. */
+ * X [M, 2 N], Y [M, N] dtype, Q int8 [M, N], S fp32 [M]; M, N and alignment as above. */
 int tlq_gated_silu(const void* X, void* Y, void* Q, void* S, int64_t M, int64_t N, int dtype, int round_scale, void* stream);
 
 /* Low-rank adapters of many requests beside a projection (tlq_gemm_w4a16, tlq_gemm_w8a8, ...), whose outputs are one to three parts of n0, n1, n2
