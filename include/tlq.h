@@ -402,7 +402,7 @@ int tlq_gated_silu(const void* X, void* Y, void* Q, void* S, int64_t M, int64_t 
  * a row's on the other rows.
  * X [M, K], A [L, parts * rank, K], B [L, N, rank] in_dtype (TLQ_F16 or TLQ_BF16), Y and out [M, N] out_dtype (in_dtype or TLQ_F32), ids
  * int32 [M], scaling fp32 [L].  out may be Y.  rank 8, 16, 32, 64 or 128 (adapters of a lower rank: rows and columns of 0), K % 32 == 0,
- * n0, n1, n2 % 16 == 0, L <= 4096, M < 2^24 (of very long rows fewer, said by the error); X, Y, A, B and out 16-byte aligned.
+ * n0, n1, n2 % 16 == 0, L <= 4096, M < 2^24; X, Y, A, B and out 16-byte aligned.
  * The workspace (16-byte aligned, at least tlq_low_rank_update_workspace_bytes, which does not fall as M grows) holds nothing between calls;
  * two calls that may run at the same time need one each. */
 int64_t tlq_low_rank_update_workspace_bytes(int64_t M, int64_t L, int64_t rank, int64_t parts, int64_t K);

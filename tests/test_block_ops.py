@@ -413,6 +413,23 @@ def test_update_in_place_and_nothing_beside_its_outputs(M):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [5, 90])
+def test_update_infinities_stay_infinities(M, dtype):
+    """An infinity among the activations, beside weights of one sign: the row is infinite, the others are what they were."""
+    t = list(make_update(M, 2, 16, (64,), 64, dtype, "one", 4))
+    t[3], t[4], t[5] = t[3].abs() + 0.01, t[4].abs() + 0.01, t[5].abs() + 0.1
+    x = t[0].clone()
+    x[1, 3] = float("inf")
+    kernel = update_kernel(2, 16, (64,), 64, dtype)
+    rest = [v.cuda() for v in t[1:]]
+    got, was = kernel(x.cuda(), *rest).cpu(), kernel(t[0].cuda(), *rest).cpu()
+    assert (got[1] == float("inf")).all()
+    keep = torch.arange(M) != 1
+    assert_bit_equal(got[keep], was[keep])
+
+
+@gpu
 def test_update_offsets_beyond_32_bits():
     """Adapters whose matrices lie more than 4 GiB behind the first."""
     L, rank, K, N = 1200, 64, 14336, 14336
@@ -630,7 +647,7 @@ UPDATE_OK = dict(X=P16, Y=P16, ids=P16, A=P16, B=P16, scaling=P16, out=P16, ws=P
     ({"M": -1}, "bad shape"), ({"M": 1 << 24}, "bad shape"), ({"L": 0}, "bad shape"), ({"L": 4097}, "bad shape"), ({"rank": 24}, "bad shape"), ({"K": 48}, "bad shape"), ({"K": 0}, "bad shape"),
     ({"n0": 0}, "parts"), ({"n0": 24}, "parts"), ({"n2": 16}, "parts"), ({"n1": -16}, "parts"), ({"n1": 1 << 24}, "parts"), ({"in_dtype": _abi.F32}, "in_dtype"), ({"out_dtype": _abi.BF16}, "out_dtype"),
     ({"X": None}, "null"), ({"out": None}, "null"), ({"scaling": None}, "null"), ({"A": ctypes.c_void_p(24)}, "aligned"), ({"ids": ctypes.c_void_p(18)}, "aligned"), ({"ws": None}, "workspace"),
-    ({"ws_bytes": 16}, "workspace"), ({"ws": ctypes.c_void_p(8)}, "workspace"), ({"M": (1 << 24) - 1, "n0": (1 << 24) - 16}, "too many")])
+    ({"ws_bytes": 16}, "workspace"), ({"ws": ctypes.c_void_p(8)}, "workspace")])
 def test_update_entry_refuses(change, message):
     args = {**UPDATE_OK, **change}
     assert _abi.load().tlq_low_rank_update(*args.values()) != 0
