@@ -343,6 +343,28 @@ def test_update(M, L, rank, parts, K, kind, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("M,L,rank,parts,K,kind", [(8192, 3, 8, (48,), 64, "runs"), (8193, 4, 16, (32, 16), 32, "holes"), (9001, 700, 8, (32,), 64, "spread"), (20000, 2, 8, (16,), 32, "one"),
+                                                   (70001, 5, 8, (16,), 32, "runs"), (33000, 4096, 8, (16,), 32, "holes")])
+def test_update_many_rows(M, L, rank, parts, K, kind):
+    t = make_update(M, L, rank, parts, K, "bfloat16", kind, 3)
+    got = update_kernel(L, rank, parts, K, "bfloat16")(*[v.cuda() for v in t]).cpu()
+    some = torch.cat([torch.tensor([0, 1, 63, 64, M - 2, M - 1]), torch.randint(0, M, (300,), generator=gen(M))])
+    want, off = ref.low_rank_update(*[v[some] for v in t[:3]], *t[3:], parts)
+    assert_near(got[some], want, off, "many rows")
+    # all of them, in fp32 (the sums of both sides are off by what the oracle allows at most)
+    x, y, ids, a, b, s = t
+    begin, whole = 0, y.float().clone()
+    for e in torch.unique(ids).tolist():
+        if 0 <= e < L:
+            at = ids == e
+            h = x[at].float() @ a[e].float().T
+            for p, n in enumerate(parts):
+                begin = sum(parts[:p])
+                whole[at, begin: begin + n] += s[e] * (h[:, p * rank: (p + 1) * rank] @ b[e, begin: begin + n].float().T)
+    assert ((got.float() - whole).abs() <= 2.0**-8 * whole.abs() + 2.0**-10).all()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M", [4, 70, 400])
 def test_update_large_and_small_values(M, dtype):

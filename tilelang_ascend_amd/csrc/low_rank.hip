@@ -24,6 +24,13 @@ struct MmaOf<bf16_t> {
   typedef MmaBF16 type;
 };
 
+// Global -> LDS without registers: 16 bytes a lane, lane l's to lds + 16 l.
+__device__ __forceinline__ void direct16(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
+}
+typedef __attribute__((address_space(3))) uint8_t* lptr_t;
+__device__ __forceinline__ uint32_t lds_of(const void* p) { return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)p); }
+
 // ---- which rows ---------------------------------------------------------------------------------------------------------
 // A tile: `rows` rows of one adapter (L: rows without one), those of the plan's order from `first` on.
 struct RowTile {
@@ -36,8 +43,7 @@ struct Rows {
 };
 __host__ __device__ inline int64_t tiles_at(int64_t M) { return 64 + (M + 3) / 4 * 4; }  // (16-byte aligned)
 
-// Tile `no` as a wavefront sees it: its adapter, how many rows (0: no such tile), and the row in slot s < 16 MT (a row of the batch for an empty slot too).
-template <int MT>
+// Tile `no` as a wavefront sees it: its adapter, how many rows (0: no such tile), and the row in a slot (a row of the batch for an empty slot too).
 struct Tile {
   int adapter = 0, rows = 0;
   int own;  // without a plan: lane s has the row in slot s
@@ -67,52 +73,59 @@ struct Tile {
   __device__ __forceinline__ int row(const Rows& r, int slot) const { return r.plan ? order[slot < rows ? slot : rows - 1] : __shfl(own, slot); }
 };
 
-// One work-group.  Rows are counted by adapter, every adapter's are cut into tiles of 64, and the rows take their places: a run of one adapter with one
-// atomic addition a wavefront.  Which place of its adapter's a row gets may differ between runs; no value depends on it.
-__global__ __launch_bounds__(1024) void low_rank_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ plan, int M, int L) {
+// One work-group.  Rows are counted by adapter, every adapter's are cut into tiles of `tile_rows`, and the rows take their places: a run of one adapter with
+// one atomic addition a wavefront.  Which place of its adapter's a row gets may differ between runs; no value depends on it.  Up to 8192 rows (ONCE) ids and
+// places stay in registers.
+template <bool ONCE>
+__global__ __launch_bounds__(1024) void low_rank_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ plan, int M, int L, int tile_rows) {
   __shared__ int32_t count[kMaxAdapters + 1];
   __shared__ int32_t part[16][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int i = tid; i <= L; i += 1024) count[i] = 0;
-  __syncthreads();
-  // f(row, its adapter or L, what the rows of the wavefront before it with the same adapter are if all of them have one, whether so, whether there is a row)
+  constexpr int AHEAD = 8;
+  int id[AHEAD], place[AHEAD];
+  const auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (r0 + i * 1024 >= M) break;
+      const int r = r0 + i * 1024 + tid;
+      id[i] = ids[r < M ? r : M - 1];
+    }
+  };
   const auto add = [&](int key, bool there) __attribute__((always_inline)) {  // -> the place among the rows counted so far
     const int first = __builtin_amdgcn_readfirstlane(key);
     const uint64_t live = __builtin_amdgcn_ballot_w64(there);
-    if (__builtin_amdgcn_ballot_w64(there && key == first) == live && (live & 1)) {
+    if (__builtin_amdgcn_ballot_w64(there && key == first) == live && (live & 1)) {  // (rows that are there are the first lanes')
       int base = 0;
       if (lane == 0) base = atomicAdd(&count[first], __builtin_popcountll(live));
       return __builtin_amdgcn_readfirstlane(base) + lane;
     }
     return there ? atomicAdd(&count[key], 1) : 0;
   };
-  constexpr int AHEAD = 8;
-  const auto each = [&](auto&& f) __attribute__((always_inline)) {
-    for (int r0 = 0; r0 < M; r0 += 1024 * AHEAD) {
-      int id[AHEAD];
+  const auto place_all = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int r = r0 + i * 1024 + tid;
-        id[i] = ids[r < M ? r : M - 1];
-      }
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int r = r0 + i * 1024 + tid;
-        f(r, (uint32_t)id[i] < (uint32_t)L ? id[i] : L, r < M);
-      }
+    for (int i = 0; i < AHEAD; ++i) {
+      if (r0 + i * 1024 >= M) break;
+      id[i] = (uint32_t)id[i] < (uint32_t)L ? id[i] : L;
+      place[i] = add(id[i], r0 + i * 1024 + tid < M);
     }
   };
-  each([&](int, int key, bool there) __attribute__((always_inline)) { add(key, there); });
+  if (ONCE) load(0);
+  for (int i = tid; i <= L; i += 1024) count[i] = 0;
   __syncthreads();
-  // where every adapter's rows and tiles begin: five neighbouring adapters a lane
-  constexpr int PER = (kMaxAdapters + 1024) / 1024;
+  for (int r0 = 0; r0 < M; r0 += 1024 * AHEAD) {
+    if (!ONCE) load(r0);
+    place_all(r0);
+  }
+  __syncthreads();
+  // where every adapter's rows and tiles begin: neighbouring adapters a lane
+  const int per = (L + 1024) / 1024;
   int rows = 0, tiles = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int n = tid * PER + i <= L ? count[tid * PER + i] : 0;
-    rows += n, tiles += (n + 63) / 64;
+  for (int i = 0; i < per; ++i) {
+    const int n = tid * per + i <= L ? count[tid * per + i] : 0;
+    rows += n, tiles += (n + tile_rows - 1) / tile_rows;
   }
   int rows_to = rows, tiles_to = tiles;
+#pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int a = __shfl_up(rows_to, o), b = __shfl_up(tiles_to, o);
     if (lane >= o) rows_to += a, tiles_to += b;
@@ -120,25 +133,30 @@ __global__ __launch_bounds__(1024) void low_rank_plan_kernel(const int32_t* __re
   if (lane == 63) part[wave][0] = rows_to, part[wave][1] = tiles_to;
   __syncthreads();
   int row = rows_to - rows, tile = tiles_to - tiles;
-  for (int w = 0; w < 16; ++w) {
-    if (w < wave) row += part[w][0], tile += part[w][1];
-  }
-  RowTile* const out = (RowTile*)(plan + tiles_at(M));
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = tid * PER + i;
+  for (int w = 0; w < 16; ++w) row += w < wave ? part[w][0] : 0, tile += w < wave ? part[w][1] : 0;
+  RowTile* const out = (RowTile*)(plan + tiles_at(M));
+  for (int i = 0; i < per; ++i) {
+    const int e = tid * per + i;
     if (e > L) break;
     const int n = count[e];
-    for (int at = 0; at < n; at += 64) out[tile++] = RowTile{e, row + at, n - at < 64 ? n - at : 64, 0};
+    for (int at = 0; at < n; at += tile_rows) out[tile++] = RowTile{e, row + at, n - at < tile_rows ? n - at : tile_rows, 0};
     count[e] = row;
     row += n;
     if (e == L) plan[0] = tile;
   }
   __syncthreads();
-  each([&](int r, int key, bool there) __attribute__((always_inline)) {
-    const int place = add(key, there);
-    if (there) plan[64 + place] = r;
-  });
+  for (int r0 = 0; r0 < M; r0 += 1024 * AHEAD) {
+    if (!ONCE) {
+      load(r0);
+      place_all(r0);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int r = r0 + i * 1024 + tid;
+      if (r < M) plan[64 + place[i] + (ONCE ? count[id[i]] : 0)] = r;
+    }
+  }
 }
 
 // ---- the first product: sums[part][row][i] of h, parts of K -----------------------------------------------------------------
@@ -146,71 +164,115 @@ struct DownArgs {
   Rows r;
   const void *X, *A;
   float* sums;
-  int K, rows, part_k;  // rows: of an adapter's A; part_k: values of a part, a multiple of 256
+  int K, rows, part_k;  // rows: of an adapter's A; part_k: values of a part, a multiple of 64 (tiles of 16 rows: of kDownStep)
+  int groups, total;    // groups of rows of A of a tile, and tiles
+};
+// Work-group `no`: which of its tile's groups, and which tile.  (Numbers go to the XCDs in turn: the groups of a tile one after another on one of them.)
+struct DownPlace {
+  int group, tile;
+  __device__ __forceinline__ DownPlace(int no, int groups) {
+    const int turn = no >> 3;
+    group = turn % groups, tile = (turn / groups) * 8 + (no & 7);
+  }
 };
 
-// 16 MT rows x 16 NT rows of A on one part of K, which the four wavefronts share out in steps of 64 values; both operands straight into registers.
-template <typename T, int MT, int NT>
-__global__ __launch_bounds__(256) void low_rank_down_kernel(const DownArgs a) {
+// Tiles of 16 rows x 16 rows of A on one part of K, 64 values a wavefront and step, operands straight into registers; the wavefronts' sums meet in LDS.
+// The weights of many adapters, one trip to memory: latency counts, and more loads of a wavefront at once, more rows of A a work-group or fewer wavefronts
+// are slower (1 row, 4096 x rank 16, the whole call: 7.4 us, with four steps at once 10.2, with eight wavefronts 8.0; 64 rows of 48 adapters, K = 11008, 12.5 / 13.5 /
+// 13.6; 259 rows of 32 adapters of rank 64 on 2 x 11008 47.8 / 47.5 / 49, two rows of 16 of A 49).
+constexpr int kDownWaves = 16, kDownStep = 64 * kDownWaves;
+template <typename T>
+__global__ __launch_bounds__(64 * kDownWaves) void low_rank_down_kernel(const DownArgs a) {
   typedef typename MmaOf<T>::type Mma;
-  __shared__ float4_t red[4][MT * NT][64];
+  __shared__ float4_t red[kDownWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
-  const Tile<MT> tile(a.r, blockIdx.x, lane);
-  if (tile.rows == 0 || tile.adapter == a.r.L) return;
-  const int part = blockIdx.y, col0 = blockIdx.z * 16 * NT, frags = (tile.rows + 15) / 16;
-  int row[MT];
-  const T *x[MT], *w[NT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) row[t] = tile.row(a.r, t * 16 + r16), x[t] = (const T*)a.X + (int64_t)row[t] * a.K + q * 8;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int i = col0 + t * 16 + r16;
-    w[t] = (const T*)a.A + ((int64_t)tile.adapter * a.rows + (i < a.rows ? i : a.rows - 1)) * a.K + q * 8;
-  }
-  float4_t acc[MT][NT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int u = 0; u < NT; ++u) acc[t][u] = float4_t{0, 0, 0, 0};
+  const DownPlace at(blockIdx.x, a.groups);
+  const Tile tile(a.r, at.tile, lane);
+  if (at.tile >= a.total || tile.rows == 0 || tile.adapter == a.r.L) return;
+  const int part = blockIdx.y, col0 = at.group * 16;
+  const int64_t row = tile.row(a.r, r16);
+  const T* const x = (const T*)a.X + row * a.K + q * 8;
+  const T* const w = (const T*)a.A + ((int64_t)tile.adapter * a.rows + (col0 + r16 < a.rows ? col0 + r16 : a.rows - 1)) * a.K + q * 8;
+  float4_t acc = {0, 0, 0, 0};
   const int end = (part + 1) * a.part_k < a.K ? (part + 1) * a.part_k : a.K;
-  for (int k = part * a.part_k + wave * 64; k < end; k += 256) {
+  for (int k = part * a.part_k + wave * 64; k < end; k += kDownStep) {
     const bool both = k + 32 < a.K;  // (rows are multiples of 32 values)
-    uint4_t wf[NT][2], xf[MT][2];
+    uint4_t xf[2] = {*(const uint4_t*)(x + k), {0, 0, 0, 0}}, wf[2] = {*(const uint4_t*)(w + k), {0, 0, 0, 0}};
+    if (both) xf[1] = *(const uint4_t*)(x + k + 32), wf[1] = *(const uint4_t*)(w + k + 32);
+    acc = Mma::mma(wf[0], xf[0], acc);
+    acc = Mma::mma(wf[1], xf[1], acc);
+  }
+  red[wave][lane] = acc;
+  __syncthreads();
+  const int i = col0 + q * 4;
+  if (wave != 0 || r16 >= tile.rows || i >= a.rows) return;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      wf[u][0] = *(const uint4_t*)(w[u] + k);
-      wf[u][1] = both ? *(const uint4_t*)(w[u] + k + 32) : uint4_t{0, 0, 0, 0};
-    }
+  for (int v = 1; v < kDownWaves; ++v) acc += red[v][lane];
+  *(float4_t*)(a.sums + (part * (int64_t)a.r.M + row) * a.rows + i) = acc;
+}
+
+// Tiles of 64 rows x 16 NT rows of A: rows and weights come in stages of 64 values (128 bytes, a cache line, of a row), eight lanes a line, straight into
+// LDS, three stages ahead; a wavefront multiplies 16 rows.  (Operands read straight from memory -- 16 neighbouring lanes, 16 rows -- go through the cache at a
+// quarter of its rate.)  8192 rows, K = 4096, rank 32 bf16: 16 us where X is in the last-level cache, 27 behind a second product that has just written
+// 235 MB; five, seven stages ahead level.
+template <typename T, int NT>
+__global__ __launch_bounds__(256) void low_rank_down_tile_kernel(const DownArgs a) {
+  typedef typename MmaOf<T>::type Mma;
+  constexpr int DEPTH = 4, LINES = 64 + 16 * NT, W_LOADS = NT == 1 ? 1 : NT / 2, LOADS = 2 + W_LOADS;  // rows of a stage; loads of a wavefront
+  __shared__ uint4_t stages[DEPTH][LINES][8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
+  const DownPlace at(blockIdx.x, a.groups);
+  const Tile tile(a.r, at.tile, lane);
+  if (at.tile >= a.total || tile.rows == 0 || tile.adapter == a.r.L) return;
+  const int part = blockIdx.y, col0 = at.group * 16 * NT;
+  // chunk c of line r lies at place c ^ (r & 7): eight lines' chunks meet every bank once
+  const int line = lane >> 3, chunk = (lane & 7) ^ line;
+  const T* src[LOADS];
+  uint32_t to[LOADS];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (t >= frags) break;
-      xf[t][0] = *(const uint4_t*)(x[t] + k);
-      xf[t][1] = both ? *(const uint4_t*)(x[t] + k + 32) : uint4_t{0, 0, 0, 0};
-    }
+  for (int i = 0; i < 2; ++i) src[i] = (const T*)a.X + (int64_t)tile.row(a.r, wave * 16 + i * 8 + line) * a.K, to[i] = (wave * 16 + i * 8) * 128;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (t >= frags) break;
+  for (int i = 0; i < W_LOADS; ++i) {
+    const int first = (NT == 1 ? wave & 1 : wave * W_LOADS + i) * 8, col = col0 + first + line;  // (NT = 1: two wavefronts bring the same)
+    src[2 + i] = (const T*)a.A + ((int64_t)tile.adapter * a.rows + (col < a.rows ? col : a.rows - 1)) * a.K, to[2 + i] = (64 + first) * 128;
+  }
+  const uint32_t lds = lds_of(stages);
+  const int begin = part * a.part_k, end = begin + a.part_k < a.K ? begin + a.part_k : a.K, steps = (end - begin + 63) / 64;
+  const auto load = [&](int s) __attribute__((always_inline)) {
+    int k = begin + s * 64 + chunk * 8;
+    k = k < a.K ? k : a.K - 8;  // (rows are multiples of 32 values: the second half of the last stage may not be there)
+    const uint32_t stage = lds + (uint32_t)((s % DEPTH) * (LINES * 128));
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        acc[t][u] = Mma::mma(wf[u][0], xf[t][0], acc[t][u]);
-        acc[t][u] = Mma::mma(wf[u][1], xf[t][1], acc[t][u]);
-      }
+    for (int i = 0; i < LOADS; ++i) direct16(src[i] + k, stage + to[i]);
+  };
+  float4_t acc[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) acc[u] = float4_t{0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < DEPTH - 1; ++s)
+    if (s < steps) load(s);
+  for (int s = 0; s < steps; ++s) {
+    // this wavefront's loads of stage s have landed (DEPTH - 2 stages follow it; at the end all have), then everybody's, and nobody reads stage s - 1 any more
+    if (s + DEPTH - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + DEPTH - 1 < steps) load(s + DEPTH - 1);
+    const uint4_t(*const stage)[8] = stages[s % DEPTH];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half == 1 && begin + s * 64 + 32 >= a.K) break;
+      const int place = (half * 4 + q) ^ (r16 & 7);
+      const uint4_t x = stage[wave * 16 + r16][place];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) acc[u] = Mma::mma(stage[64 + u * 16 + r16][place], x, acc[u]);
     }
   }
+  if (wave * 16 + r16 >= tile.rows) return;
+  float* const out = a.sums + (part * (int64_t)a.r.M + tile.row(a.r, wave * 16 + r16)) * a.rows;
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int u = 0; u < NT; ++u) red[wave][t * NT + u][lane] = acc[t][u];
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int f = t * NT + u, i = col0 + u * 16 + q * 4;
-      if (f % 4 != wave || t * 16 + r16 >= tile.rows || i >= a.rows) continue;
-      const float4_t sum = (red[0][f][lane] + red[1][f][lane]) + (red[2][f][lane] + red[3][f][lane]);
-      *(float4_t*)(a.sums + ((int64_t)part * a.r.M + row[t]) * a.rows + i) = sum;
-    }
+  for (int u = 0; u < NT; ++u) {
+    const int i = col0 + u * 16 + q * 4;
+    if (i < a.rows) *(float4_t*)(out + i) = acc[u];
+  }
 }
 
 // ---- the second product, and the sum -----------------------------------------------------------------------------------------
@@ -219,9 +281,10 @@ struct UpArgs {
   const void *Y, *B;
   const float *scaling, *sums;
   void* out;
-  int N, rank, rows, parts;  // rows: of an adapter's A; parts: of K
-  int end0, end1;            // where the first and the second part of the outputs end
-  int per_group;             // blocks of 64 outputs of a work-group
+  int N, rows, parts;            // rows: of an adapter's A; parts: of K
+  int end0, end1;                // where the first and the second part of the outputs end
+  int per_group;                 // blocks of 128 outputs of a work-group
+  int groups, groups0, groups1;  // work-groups of a tile: all, those ahead of the second part of the outputs and of the third
 };
 
 // Two pieces of the operands' type for a value of h: bfloat16 holds 16 of its bits that way; float16 22, of h over a power of two that brings the row's
@@ -243,78 +306,90 @@ __device__ __forceinline__ void two_pieces(const float (&h)[8], uint4_t& high, u
   }
 }
 
-// 16 MT rows of a tile (which has `halves` times as many) x blocks of 64 outputs; RB blocks of 32 ranks.  Lane (m, q) has 16 neighbouring outputs of row m:
-// tile j of the four 16-row tiles of B holds rows 16 (i / 4) + 4 j + i % 4 of the block.
-template <typename T, typename TO, int MT, int RB>
-__global__ __launch_bounds__(256) void low_rank_up_kernel(const UpArgs a) {
+// Blocks of 128 outputs of one part of the outputs x 16 RW rows: RW wavefronts have 16 rows each and share a block's rows of B, 4 / RW (2: see kUpWaves)
+// blocks go at a time.  A block of B, RANK values a row, comes into LDS in whole cache lines; output n = 8 r + j belongs to column r of the j-th of eight
+// products of 16 x 16, so that 16 neighbouring lanes have 128 neighbouring outputs of one row of Y and out, 16 bytes each.
+template <int RW, int RANK>
+constexpr int kUpWaves = RW == 1 && RANK >= 64 ? 2 : 4;  // (32 KB of B for each wavefront)
+template <typename T, typename TO, int RW, int RANK>
+__global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(const UpArgs a) {
   typedef typename MmaOf<T>::type Mma;
-  constexpr int W = 16 * sizeof(TO) / 16;  // 16-byte pieces of a lane's outputs
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
-  const Tile<MT> tile(a.r, blockIdx.x, lane);
-  const int slot0 = blockIdx.z * 16 * MT, live = tile.rows - slot0;
-  if (live <= 0) return;
-  const int frags = (live + 15) / 16 < MT ? (live + 15) / 16 : MT;
-  int64_t row[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) row[t] = tile.row(a.r, slot0 + t * 16 + r16);
+  constexpr int CW = kUpWaves<RW, RANK> / RW, C = RANK / 8, RB = (RANK + 31) / 32, W = sizeof(TO) / 2, B_LOADS = 2 * C;  // chunks of a row of B, ..
+  __shared__ uint4_t tiles[CW][128 * C];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4, rw = wave % RW, cw = wave / RW;
+  // (work-groups that run at a time have neighbouring outputs of the same rows)
+  const int at = blockIdx.x / a.groups, no = blockIdx.x - at * a.groups;
+  const Tile tile(a.r, at, lane);
+  if (tile.rows == 0) return;
   const bool with = tile.adapter != a.r.L;
-  const float scaling = with ? a.scaling[tile.adapter] : 0.0f;
-  const int blocks0 = (a.end0 + 63) / 64, blocks1 = blocks0 + (a.end1 - a.end0 + 63) / 64, blocks = blocks1 + (a.N - a.end1 + 63) / 64;
-  int have = -1;  // the part of the outputs whose h is there
-  uint4_t high[MT][RB], low[MT][RB];
-  float back[MT];  // what the pieces' power of two takes back, times the scaling
-  for (int i = 0; i < a.per_group; i += 4) {
-    const int block = blockIdx.y * a.per_group + i + wave;
-    if (block >= blocks) break;
-    const int p = (block >= blocks0) + (block >= blocks1);
-    const int n0 = p == 0 ? block * 64 : p == 1 ? a.end0 + (block - blocks0) * 64 : a.end1 + (block - blocks1) * 64;
-    const int end = p == 0 ? a.end0 : p == 1 ? a.end1 : a.N;
-    const int n = n0 + q * 16;
-    const bool there = n < end;
-    uint4_t y[MT][W];
+  const int live = tile.rows - rw * 16;  // rows of this wavefront, if any
+  int64_t row[4];                        // rows 4 q + i of its 16
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (t >= frags) break;
+  for (int i = 0; i < 4; ++i) row[i] = tile.row(a.r, rw * 16 + q * 4 + i);
+  const int p = (no >= a.groups0) + (no >= a.groups1), begin = p == 0 ? 0 : p == 1 ? a.end0 : a.end1, end = p == 0 ? a.end0 : p == 1 ? a.end1 : a.N;
+  const int group = no - (p == 0 ? 0 : p == 1 ? a.groups0 : a.groups1);
+  // line l of a block in LDS is its row 8 (l % 16) + l / 16; chunk c of it lies at place c ^ turn(l): eight lines' chunks meet every bank once
+  const auto turn = [](int l) __attribute__((always_inline)) { return C == 1 ? 0 : C == 2 ? (l >> 2) & 1 : C == 4 ? (l >> 1) & 3 : l & 7; };
+  const T* const b0 = (const T*)a.B + ((int64_t)tile.adapter * a.N + begin) * RANK;
+  const uint32_t lds = lds_of(tiles[cw]);
+  uint4_t high[RB], low[RB];
+  float back[4];  // the scaling, times what the pieces' power of two takes back, of rows 4 q + i
+  for (int i = 0; i < a.per_group; i += CW) {
+    const int n0 = (group * a.per_group + i + cw) * 128;
+    if (begin + n0 >= end) break;
+    if (with) {
+      // (nobody reads the last block any more)
+      if (i > 0) {
+        if constexpr (RW > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
 #pragma unroll
-      for (int v = 0; v < W; ++v)
-        if (there && slot0 + t * 16 + r16 < tile.rows) y[t][v] = __builtin_nontemporal_load((const uint4_t*)((const TO*)a.Y + row[t] * a.N + n) + v);
+      for (int k = 0; k < (B_LOADS + RW - 1) / RW; ++k) {
+        const int load = k * RW + rw;
+        if (B_LOADS % RW != 0 && load >= B_LOADS) break;
+        const int l = (load * 64 + lane) / C, c = lane % C ^ turn(l);
+        int n = n0 + 8 * (l & 15) + (l >> 4);
+        n = n < end - begin ? n : end - begin - 1;
+        direct16(b0 + (int64_t)n * RANK + c * 8, lds + load * 1024);
+      }
     }
-    if (!with) {
+    const int n = begin + n0 + r16 * 8;
+    uint4_t y[4][W];
+    if (n < end) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
+      for (int m = 0; m < 4; ++m)
+        if (q * 4 + m < live)
 #pragma unroll
-        for (int v = 0; v < W; ++v)
-          if (there && slot0 + t * 16 + r16 < tile.rows) *((uint4_t*)((TO*)a.out + row[t] * a.N + n) + v) = y[t][v];
-      continue;
+          for (int v = 0; v < W; ++v) y[m][v] = __builtin_nontemporal_load((const uint4_t*)((const TO*)a.Y + row[m] * a.N + n) + v);
     }
-    uint4_t b[4][RB];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = n0 + 16 * (r16 >> 2) + 4 * j + (r16 & 3);
-      const T* const w = (const T*)a.B + ((int64_t)tile.adapter * a.N + (at < end ? at : n0)) * a.rank + q * 8;
-#pragma unroll
-      for (int c = 0; c < RB; ++c) b[j][c] = c * 32 + q * 8 < a.rank ? *(const uint4_t*)(w + c * 32) : uint4_t{0, 0, 0, 0};
-    }
-    if (p != have) {
-      have = p;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (t >= frags) break;
+    if (with) {
+      if (i == 0) {
         float h[RB][8];
+        const float* s = a.sums + (int64_t)tile.row(a.r, rw * 16 + r16) * a.rows + p * RANK + q * 8;
+        const int64_t step = (int64_t)a.r.M * a.rows;
 #pragma unroll
         for (int c = 0; c < RB; ++c) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) h[c][k] = 0.0f;
-          if (c * 32 + q * 8 < a.rank) {
-            const float* s = a.sums + row[t] * a.rows + p * a.rank + c * 32 + q * 8;
-            for (int part = 0; part < a.parts; ++part, s += (int64_t)a.r.M * a.rows) {
-              const float4_t u = *(const float4_t*)s, v = *(const float4_t*)(s + 4);
+          if (RANK >= 32 || q < C) {
+            constexpr int ONCE = RB == 1 ? 8 : 4;  // parts that are asked for at once
+            for (int part = 0; part < a.parts; part += ONCE) {
+              float4_t u[ONCE], v[ONCE];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) h[c][k] += u[k], h[c][4 + k] += v[k];
+              for (int o = 0; o < ONCE; ++o) {
+                const float* const from = s + (part + o < a.parts ? part + o : part) * step + c * 32;
+                u[o] = *(const float4_t*)from, v[o] = *(const float4_t*)(from + 4);
+              }
+#pragma unroll
+              for (int o = 0; o < ONCE; ++o) {
+                if (part + o >= a.parts) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h[c][k] += u[o][k], h[c][4 + k] += v[o][k];
+              }
             }
           }
         }
-        back[t] = scaling;
+        float scale = a.scaling[tile.adapter];
         if constexpr (std::is_same<T, half_t>::value) {
           float top = 0.0f;
 #pragma unroll
@@ -326,74 +401,86 @@ __global__ __launch_bounds__(256) void low_rank_up_kernel(const UpArgs a) {
           int e = (int)(bitcast<uint32_t>(top) >> 23) - 127;
           e = e < -100 ? -100 : e > 126 ? 126 : e;
           const float down = bitcast<float>((uint32_t)(127 - e) << 23), up = bitcast<float>((uint32_t)(127 + e) << 23);
-          back[t] *= up;
+          scale *= up;
 #pragma unroll
           for (int c = 0; c < RB; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k) h[c][k] *= down;
         }
 #pragma unroll
-        for (int c = 0; c < RB; ++c) two_pieces<T>(h[c], high[t][c], low[t][c]);
+        for (int c = 0; c < RB; ++c) two_pieces<T>(h[c], high[c], low[c]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) back[m] = __shfl(scale, q * 4 + m);
       }
-    }
+      if constexpr (RW > 1) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      float4_t acc[8];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (t >= frags) break;
-      float4_t acc[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         acc[j] = float4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < RB; ++c) acc[j] = Mma::mma(b[j][c], low[t][c], acc[j]);
-#pragma unroll
-        for (int c = 0; c < RB; ++c) acc[j] = Mma::mma(b[j][c], high[t][c], acc[j]);
-      }
-      if (!there || slot0 + t * 16 + r16 >= tile.rows) continue;
-      uint4_t* const o = (uint4_t*)((TO*)a.out + row[t] * a.N + n);
-      if constexpr (sizeof(TO) == 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float4_t z = bitcast<float4_t>(y[t][j]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) z[k] = __builtin_fmaf(back[t], acc[j][k], z[k]);
-          o[j] = bitcast<uint4_t>(z);
+        for (int c = 0; c < RB; ++c) {
+          // (a rank below 32: the lanes behind it have zeros for h, and a chunk of the same row of B)
+          const uint4_t b = tiles[cw][(j * 16 + r16) * C + ((C >= 4 ? c * 4 + q : q & (C - 1)) ^ turn(r16))];
+          acc[j] = Mma::mma(low[c], b, acc[j]);
+          acc[j] = Mma::mma(high[c], b, acc[j]);
         }
-      } else {
+      }
 #pragma unroll
-        for (int v = 0; v < W; ++v) {
-          uint4_t z;
+      for (int m = 0; m < 4; ++m) {
+        if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+          for (int v = 0; v < W; ++v) {
+            float4_t f = bitcast<float4_t>(y[m][v]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = __builtin_fmaf(back[m], acc[4 * v + k][m], f[k]);
+            y[m][v] = bitcast<uint4_t>(f);
+          }
+        } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t two = y[t][v][k];
+            const uint32_t two = y[m][0][k];
             float f[2];
             if constexpr (std::is_same<T, half_t>::value) f[0] = (float)bitcast<half2_t>(two)[0], f[1] = (float)bitcast<half2_t>(two)[1];
             else f[0] = bitcast<float>(two << 16), f[1] = bitcast<float>(two & 0xffff0000u);
-            const float4_t& s = acc[2 * v + (k >> 1)];
-            f[0] = __builtin_fmaf(back[t], s[2 * (k & 1)], f[0]), f[1] = __builtin_fmaf(back[t], s[2 * (k & 1) + 1], f[1]);
-            if constexpr (std::is_same<T, half_t>::value) z[k] = bitcast<uint32_t>(half2_t{(half_t)f[0], (half_t)f[1]});
-            else z[k] = pack_bf16x2(f[0], f[1]);
+            f[0] = __builtin_fmaf(back[m], acc[2 * k][m], f[0]), f[1] = __builtin_fmaf(back[m], acc[2 * k + 1][m], f[1]);
+            if constexpr (std::is_same<T, half_t>::value) y[m][0][k] = bitcast<uint32_t>(half2_t{(half_t)f[0], (half_t)f[1]});
+            else y[m][0][k] = pack_bf16x2(f[0], f[1]);
           }
-          o[v] = z;
         }
       }
+    }
+    if (n < end) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        if (q * 4 + m < live)
+#pragma unroll
+          for (int v = 0; v < W; ++v) *((uint4_t*)((TO*)a.out + row[m] * a.N + n) + v) = y[m][v];
     }
   }
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------
+constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;  // work-groups of 256 threads of a launch, which has fewer than 2^32 threads
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-inline int64_t most_tiles(int64_t M, int64_t L) { return M <= kInlineRows ? M : M / 64 + (L + 1 < M ? L + 1 : M); }
-int64_t plan_bytes(int64_t M, int64_t L) { return M <= kInlineRows ? 0 : align256((tiles_at(M) + 4 * most_tiles(M, L)) * 4); }
+// Tiles of 64 rows from 32 rows an adapter on average, of 16 below.
+inline int tile_rows_of(int64_t M, int64_t L) { return M <= kInlineRows || M < 32 * L ? 16 : 64; }
+inline int64_t most_tiles(int64_t M, int64_t L, int tile_rows) { return M <= kInlineRows ? M : M / tile_rows + (L + 1 < M ? L + 1 : M); }
+int64_t plan_bytes(int64_t M, int64_t L) { return M <= kInlineRows ? 0 : align256((tiles_at(M) + 4 * most_tiles(M, L, 16)) * 4); }
 int64_t most_parts(int64_t K) { return K >= 4096 ? 16 : (K + 255) / 256; }
-// parts * M is at most this for more than one part
-constexpr int64_t kPartRows = 32768;
-int64_t parts_of(int64_t M, int64_t L, int64_t groups, int64_t K) {
-  const int64_t tiles = most_tiles(M, L) * groups;
-  int64_t parts = (512 + tiles - 1) / tiles;
-  if (parts > most_parts(K)) parts = most_parts(K);
-  if (parts * M > kPartRows) parts = kPartRows / M;
-  return parts < 1 ? 1 : parts;
+// Parts of K: work-groups for the machine where there are few tiles (`want` of them), at most 16.  Every part costs a sum written and read: 8192 rows of rank 32 on 14336 outputs 136 us in one part, 139 in four, 145 in seven (tiles of 64 rows); 2048 of rank 16, three
+// projections, 31.2 for 128 work-groups, 33.4 for 256; tiles of 16 rows: 8 rows of 8 adapters, K = 11008, 9.9 us for 64 or more, 13.4 for 16.
+// With more than M / 64 (M / 16) tiles, parts * M is less than 64 * kTileGroups + M (16 * kFewGroups + M).
+constexpr int kTileGroups = 128, kFewGroups = 256;
+int64_t parts_of(int64_t tiles, int64_t K, int64_t want) {
+  const int64_t parts = (want + tiles - 1) / tiles;
+  return parts < most_parts(K) ? parts : most_parts(K);
 }
+int64_t sum_rows(int64_t M, int64_t K) {
+  const int64_t few = most_parts(K) * M, many = 64 * kTileGroups + M;
+  return few < many ? few : many;
+}
+static_assert(16 * kFewGroups <= 64 * kTileGroups, "sum_rows holds for both");
 
 struct Call {
   Rows r;
@@ -405,45 +492,60 @@ struct Call {
   int K, N, rank, rows, end0, end1;
 };
 
-template <typename T, int MT, int NT>
+// NT: 16 rows of A each that a work-group has; 0: tiles of 16 rows
+template <typename T, int NT>
 int run_down(const Call& c, int64_t tiles, int64_t* parts, hipStream_t st) {
-  const int groups = (c.rows + 16 * NT - 1) / (16 * NT);
-  int64_t want = parts_of(c.r.M, c.r.L, groups, c.K);
-  const int part_k = (int)((ceil_div(c.K, want) + 255) / 256 * 256);
+  const int groups = (c.rows + 16 * (NT ? NT : 1) - 1) / (16 * (NT ? NT : 1));
+  // (an adapter's last tile is half empty on average, and so counts as half of one)
+  const int64_t whole = NT ? tiles - (c.r.L + 1 < c.r.M ? c.r.L + 1 : c.r.M) / 2 : tiles, step = NT ? 64 : kDownStep;
+  const int part_k = (int)(ceil_div(ceil_div(c.K, parts_of(groups * whole, c.K, NT ? kTileGroups : kFewGroups)), step) * step);
   *parts = ceil_div(c.K, part_k);
-  const DownArgs a{c.r, c.X, c.A, c.sums, c.K, c.rows, part_k};
-  low_rank_down_kernel<T, MT, NT><<<dim3((unsigned)tiles, (unsigned)*parts, (unsigned)groups), 256, 0, st>>>(a);
-  return check_launch("tlq_low_rank_update", "low_rank_down_kernel") ? 0 : 1;
+  const DownArgs a{c.r, c.X, c.A, c.sums, c.K, c.rows, part_k, groups, (int)tiles};
+  const dim3 grid((unsigned)(ceil_div(tiles, (int64_t)8) * 8 * groups), (unsigned)*parts);
+  if constexpr (NT == 0) low_rank_down_kernel<T><<<grid, 64 * kDownWaves, 0, st>>>(a);
+  else low_rank_down_tile_kernel<T, NT><<<grid, 256, 0, st>>>(a);
+  return check_launch("tlq_low_rank_update", NT ? "low_rank_down_tile_kernel" : "low_rank_down_kernel") ? 0 : 1;
 }
 
-template <typename T, typename TO, int MT, int RB>
-int run_up(const Call& c, int64_t tiles, int64_t parts, int tile_rows, hipStream_t st) {
-  const int blocks = (c.end0 + 63) / 64 + (c.end1 - c.end0 + 63) / 64 + (c.N - c.end1 + 63) / 64;
-  int per_group = 4;
-  while (per_group < 64 && tiles * ceil_div(blocks, (int64_t)per_group) > 2048) per_group += 4;
-  while (ceil_div(blocks, (int64_t)per_group) > 65535) per_group *= 2;
-  const UpArgs a{c.r, c.Y, c.B, c.scaling, c.sums, c.out, c.N, c.rank, c.rows, (int)parts, c.end0, c.end1, per_group};
-  low_rank_up_kernel<T, TO, MT, RB><<<dim3((unsigned)tiles, (unsigned)ceil_div(blocks, (int64_t)per_group), (unsigned)(tile_rows / (16 * MT))), 256, 0, st>>>(a);
+template <typename T, typename TO, int RW, int RANK>
+int run_up(const Call& c, int64_t tiles, int64_t parts, hipStream_t st) {
+  constexpr int WAVES = kUpWaves<RW, RANK>, CW = WAVES / RW;
+  const int64_t blocks[3] = {(c.end0 + 127) / 128, (c.end1 - c.end0 + 127) / 128, (c.N - c.end1 + 127) / 128};
+  const auto groups = [&](int per) { return ceil_div(blocks[0], (int64_t)per) + ceil_div(blocks[1], (int64_t)per) + ceil_div(blocks[2], (int64_t)per); };
+  // h is made ready once a work-group: as many blocks for each as leave eight work-groups a CU (8192 rows of rank 32 on 14336 outputs bf16: 99 us; four a CU
+  // 117, sixteen 101; 259 rows of rank 64 on 2 x 11008, the whole call: 43.7 / 46.2 / 47.7)
+  int per_group = CW;
+  while ((per_group < 32 && tiles * groups(per_group) > 2048) || tiles * groups(per_group) > kMostGroups) per_group += per_group < 32 ? CW : per_group;
+  const int groups0 = (int)ceil_div(blocks[0], (int64_t)per_group), groups1 = groups0 + (int)ceil_div(blocks[1], (int64_t)per_group);
+  const UpArgs a{c.r, c.Y, c.B, c.scaling, c.sums, c.out, c.N, c.rows, (int)parts, c.end0, c.end1, per_group, (int)groups(per_group), groups0, groups1};
+  low_rank_up_kernel<T, TO, RW, RANK><<<(unsigned)(tiles * groups(per_group)), 64 * WAVES, 0, st>>>(a);
   return check_launch("tlq_low_rank_update", "low_rank_up_kernel") ? 0 : 1;
+}
+template <typename T, typename TO, int RW>
+int run_up(const Call& c, int64_t tiles, int64_t parts, hipStream_t st) {
+  switch (c.rank) {
+    case 8: return run_up<T, TO, RW, 8>(c, tiles, parts, st);
+    case 16: return run_up<T, TO, RW, 16>(c, tiles, parts, st);
+    case 32: return run_up<T, TO, RW, 32>(c, tiles, parts, st);
+    case 64: return run_up<T, TO, RW, 64>(c, tiles, parts, st);
+    default: return run_up<T, TO, RW, 128>(c, tiles, parts, st);
+  }
 }
 
 template <typename T, typename TO>
 int run_low_rank(Call c, hipStream_t st) {
-  const int64_t tiles = most_tiles(c.r.M, c.r.L);
+  const int tile_rows = tile_rows_of(c.r.M, c.r.L);
+  const int64_t tiles = most_tiles(c.r.M, c.r.L, tile_rows);
   int64_t parts = 1;
-  if (c.r.M <= kInlineRows) {
-    if (run_down<T, 1, 1>(c, tiles, &parts, st)) return 1;
-    if (c.rank <= 32) return run_up<T, TO, 1, 1>(c, tiles, parts, 16, st);
-    if (c.rank <= 64) return run_up<T, TO, 1, 2>(c, tiles, parts, 16, st);
-    return run_up<T, TO, 1, 4>(c, tiles, parts, 16, st);
+  if (c.r.M > kInlineRows) {
+    if (c.r.M <= 8192) low_rank_plan_kernel<true><<<1, 1024, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L, tile_rows);
+    else low_rank_plan_kernel<false><<<1, 1024, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L, tile_rows);
+    if (!check_launch("tlq_low_rank_update", "low_rank_plan_kernel")) return 1;
+    c.r.plan = c.plan;
   }
-  low_rank_plan_kernel<<<1, 1024, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L);
-  if (!check_launch("tlq_low_rank_update", "low_rank_plan_kernel")) return 1;
-  c.r.plan = c.plan;
-  if (c.rows <= 16 ? run_down<T, 4, 1>(c, tiles, &parts, st) : c.rows <= 32 ? run_down<T, 4, 2>(c, tiles, &parts, st) : run_down<T, 4, 4>(c, tiles, &parts, st)) return 1;
-  if (c.rank <= 32) return run_up<T, TO, 4, 1>(c, tiles, parts, 64, st);
-  if (c.rank <= 64) return run_up<T, TO, 2, 2>(c, tiles, parts, 64, st);
-  return run_up<T, TO, 2, 4>(c, tiles, parts, 64, st);
+  if (tile_rows == 16) return run_down<T, 0>(c, tiles, &parts, st) || run_up<T, TO, 1>(c, tiles, parts, st);
+  if (c.rows <= 16 ? run_down<T, 1>(c, tiles, &parts, st) : c.rows <= 32 ? run_down<T, 2>(c, tiles, &parts, st) : run_down<T, 4>(c, tiles, &parts, st)) return 1;
+  return run_up<T, TO, 4>(c, tiles, parts, st);
 }
 
 bool sizes_taken(int64_t M, int64_t L, int64_t rank, int64_t parts, int64_t K) {
@@ -458,8 +560,7 @@ using namespace tlq;
 
 extern "C" int64_t tlq_low_rank_update_workspace_bytes(int64_t M, int64_t L, int64_t rank, int64_t parts, int64_t K) {
   if (!sizes_taken(M, L, rank, parts, K)) return 0;
-  const int64_t few = most_parts(K) * M, many = M > kPartRows ? M : kPartRows;
-  return plan_bytes(M, L) + (few < many ? few : many) * parts * rank * 4;
+  return plan_bytes(M, L) + sum_rows(M, K) * parts * rank * 4;
 }
 
 extern "C" int tlq_low_rank_update(const void* X, const void* Y, const void* ids, const void* A, const void* B, const void* scaling, void* out,
