@@ -449,6 +449,18 @@ def test_update_infinities_stay_infinities(M, dtype):
     assert (got[1] == float("inf")).all()
     keep = torch.arange(M) != 1
     assert_bit_equal(got[keep], was[keep])
+    # an infinite weight in some places of a row of B: that output alone (an infinity, or NaN)
+    for rank in (8, 16, 32, 64):
+        t = make_update(M, 2, rank, (64,), 64, dtype, "one", 4)
+        kernel = update_kernel(2, rank, (64,), 64, dtype)
+        was = kernel(*[v.cuda() for v in t]).cpu()
+        for j in range(0, rank, 5):
+            b = t[4].clone()
+            b[1, 9, j] = float("inf")
+            got = kernel(*[v.cuda() for v in (*t[:4], b, t[5])]).cpu()
+            assert not torch.isfinite(got[:, 9]).any()
+            keep = torch.arange(64) != 9
+            assert_bit_equal(got[:, keep], was[:, keep])
 
 
 @gpu
