@@ -74,20 +74,21 @@ struct Tile {
 };
 
 // One work-group.  Rows are counted by adapter, every adapter's are cut into tiles of `tile_rows`, and the rows take their places: a run of one adapter with
-// one atomic addition a wavefront.  Which place of its adapter's a row gets may differ between runs; no value depends on it.  Up to 8192 rows (ONCE) ids and
-// places stay in registers.
-template <bool ONCE>
-__global__ __launch_bounds__(1024) void low_rank_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ plan, int M, int L, int tile_rows) {
+// one atomic addition a wavefront.  Which place of its adapter's a row gets may differ between runs; no value depends on it.  ONCE: up to AHEAD rows a lane, whose ids and places
+// stay in registers.
+template <bool ONCE, int THREADS, int AHEAD>
+__global__ __launch_bounds__(THREADS) void low_rank_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ plan, int M, int L, int tile_shift) {
+  constexpr int WAVES = THREADS / 64;
   __shared__ int32_t count[kMaxAdapters + 1];
-  __shared__ int32_t part[16][2];
+  __shared__ int32_t part[WAVES][2];
+  const int tile_rows = 1 << tile_shift;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int AHEAD = 8;
   int id[AHEAD], place[AHEAD];
   const auto load = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      if (r0 + i * 1024 >= M) break;
-      const int r = r0 + i * 1024 + tid;
+      if (r0 + i * THREADS >= M) break;
+      const int r = r0 + i * THREADS + tid;
       id[i] = ids[r < M ? r : M - 1];
     }
   };
@@ -104,25 +105,25 @@ __global__ __launch_bounds__(1024) void low_rank_plan_kernel(const int32_t* __re
   const auto place_all = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      if (r0 + i * 1024 >= M) break;
+      if (r0 + i * THREADS >= M) break;
       id[i] = (uint32_t)id[i] < (uint32_t)L ? id[i] : L;
-      place[i] = add(id[i], r0 + i * 1024 + tid < M);
+      place[i] = add(id[i], r0 + i * THREADS + tid < M);
     }
   };
   if (ONCE) load(0);
-  for (int i = tid; i <= L; i += 1024) count[i] = 0;
+  for (int i = tid; i <= L; i += THREADS) count[i] = 0;
   __syncthreads();
-  for (int r0 = 0; r0 < M; r0 += 1024 * AHEAD) {
+  for (int r0 = 0; r0 < M; r0 += THREADS * AHEAD) {
     if (!ONCE) load(r0);
     place_all(r0);
   }
   __syncthreads();
   // where every adapter's rows and tiles begin: neighbouring adapters a lane
-  const int per = (L + 1024) / 1024;
+  const int per = (L + THREADS) / THREADS;
   int rows = 0, tiles = 0;
   for (int i = 0; i < per; ++i) {
     const int n = tid * per + i <= L ? count[tid * per + i] : 0;
-    rows += n, tiles += (n + tile_rows - 1) / tile_rows;
+    rows += n, tiles += (n + tile_rows - 1) >> tile_shift;
   }
   int rows_to = rows, tiles_to = tiles;
 #pragma unroll
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(1024) void low_rank_plan_kernel(const int32_t* __re
   __syncthreads();
   int row = rows_to - rows, tile = tiles_to - tiles;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) row += w < wave ? part[w][0] : 0, tile += w < wave ? part[w][1] : 0;
+  for (int w = 0; w < WAVES; ++w) row += w < wave ? part[w][0] : 0, tile += w < wave ? part[w][1] : 0;
   RowTile* const out = (RowTile*)(plan + tiles_at(M));
   for (int i = 0; i < per; ++i) {
     const int e = tid * per + i;
@@ -146,14 +147,14 @@ __global__ __launch_bounds__(1024) void low_rank_plan_kernel(const int32_t* __re
     if (e == L) plan[0] = tile;
   }
   __syncthreads();
-  for (int r0 = 0; r0 < M; r0 += 1024 * AHEAD) {
+  for (int r0 = 0; r0 < M; r0 += THREADS * AHEAD) {
     if (!ONCE) {
       load(r0);
       place_all(r0);
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const int r = r0 + i * 1024 + tid;
+      const int r = r0 + i * THREADS + tid;
       if (r < M) plan[64 + place[i] + (ONCE ? count[id[i]] : 0)] = r;
     }
   }
@@ -538,8 +539,11 @@ int run_low_rank(Call c, hipStream_t st) {
   const int64_t tiles = most_tiles(c.r.M, c.r.L, tile_rows);
   int64_t parts = 1;
   if (c.r.M > kInlineRows) {
-    if (c.r.M <= 8192) low_rank_plan_kernel<true><<<1, 1024, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L, tile_rows);
-    else low_rank_plan_kernel<false><<<1, 1024, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L, tile_rows);
+    const int shift = tile_rows == 16 ? 4 : 6;
+    // (259 rows: four wavefronts 2.8 us, sixteen 4.4; 1003 level; 8192: sixteen 6.8, eight 8.5)
+    if (c.r.M <= 1024) low_rank_plan_kernel<true, 256, 4><<<1, 256, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L, shift);
+    else if (c.r.M <= 8192) low_rank_plan_kernel<true, 1024, 8><<<1, 1024, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L, shift);
+    else low_rank_plan_kernel<false, 1024, 8><<<1, 1024, 0, st>>>(c.r.ids, c.plan, c.r.M, c.r.L, shift);
     if (!check_launch("tlq_low_rank_update", "low_rank_plan_kernel")) return 1;
     c.r.plan = c.plan;
   }
