@@ -73,9 +73,9 @@ struct Tile {
   __device__ __forceinline__ int row(const Rows& r, int slot) const { return r.plan ? order[slot < rows ? slot : rows - 1] : __shfl(own, slot); }
 };
 
-// One work-group.  Rows are counted by adapter, every adapter's are cut into tiles of `tile_rows`, and the rows take their places: a run of one adapter with
-// one atomic addition a wavefront.  Which place of its adapter's a row gets may differ between runs; no value depends on it.  ONCE: up to AHEAD rows a lane, whose ids and places
-// stay in registers.
+// One work-group.  Rows are counted by adapter, every adapter's are cut into tiles of 2^tile_shift, and the rows take their places: a run of one adapter with
+// one atomic addition a wavefront.  Which place of its adapter's a row gets may differ between runs; no value depends on it.  ONCE: up to AHEAD rows a
+// lane, whose ids and places stay in registers.
 template <bool ONCE, int THREADS, int AHEAD>
 __global__ __launch_bounds__(THREADS) void low_rank_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ plan, int M, int L, int tile_shift) {
   constexpr int WAVES = THREADS / 64;

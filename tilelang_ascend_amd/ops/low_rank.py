@@ -3,7 +3,7 @@ rows of each request get what its own adapter adds to it:
 
     out = low_rank_update(L, rank, N, K)(x, w4a16_gemm(...)(x, ...), ids, A, B, scaling)
 
-Results do not depend on timing, nor a row's on the other rows of the batch; nothing is copied to the host: a step can be captured in a graph.
+Results do not depend on timing, nor a row's on what the other rows of the call hold; nothing is copied to the host: a step can be captured in a graph.
 """
 from __future__ import annotations
 
