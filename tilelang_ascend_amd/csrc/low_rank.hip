@@ -177,44 +177,70 @@ struct DownPlace {
   }
 };
 
-// Tiles of 16 rows x 16 rows of A on one part of K, 64 values a wavefront and step, operands straight into registers; the wavefronts' sums meet in LDS.
-// The weights of many adapters, one trip to memory: latency counts, and more loads of a wavefront at once, more rows of A a work-group or fewer wavefronts
-// are slower (1 row, 4096 x rank 16, the whole call: 7.4 us, with four steps at once 10.2, with eight wavefronts 8.0; 64 rows of 48 adapters, K = 11008, 12.5 / 13.5 /
-// 13.6; 259 rows of 32 adapters of rank 64 on 2 x 11008 47.8 / 47.5 / 49, two rows of 16 of A 49).
-constexpr int kDownWaves = 16, kDownStep = 64 * kDownWaves;
+// Tiles of 16 rows x 16 rows of A on one part of K: eight wavefronts take stages of 64 values (128 bytes, a cache line, of a row) in turn, each with a ring
+// of its own in LDS, which it fills two stages ahead, eight lanes a line, and nobody else looks at; the wavefronts' sums meet at the end.  Operands read
+// straight from memory -- 16 neighbouring lanes, 16 rows -- go through the cache at a quarter of its rate (13 bytes a clock and CU).  Whole calls, us, that
+// way / this: 1 row of 4096 x rank 16 7.4 / 6.9, K = 11008 9.1 / 7.7, 64 rows of 48 adapters, three projections 14.1 / 11.3, 512 rows of 128 21.2 / 18.4, 259
+// rows of 32 of rank 64 on 2 x 11008 44.1 / 41.2; four wavefronts, or four stages ahead: level to 0.2 behind.
+constexpr int kDownWaves = 8, kDownStep = 64 * kDownWaves;
 template <typename T>
 __global__ __launch_bounds__(64 * kDownWaves) void low_rank_down_kernel(const DownArgs a) {
   typedef typename MmaOf<T>::type Mma;
-  __shared__ float4_t red[kDownWaves][64];
+  constexpr int WAVES = kDownWaves, DEPTH = 2, LOADS = 4;
+  __shared__ uint4_t stages[WAVES][DEPTH][32][8];
+  __shared__ float4_t red[WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
   const DownPlace at(blockIdx.x, a.groups);
   const Tile tile(a.r, at.tile, lane);
   if (at.tile >= a.total || tile.rows == 0 || tile.adapter == a.r.L) return;
-  const int part = blockIdx.y, col0 = at.group * 16;
-  const int64_t row = tile.row(a.r, r16);
-  const T* const x = (const T*)a.X + row * a.K + q * 8;
-  const T* const w = (const T*)a.A + ((int64_t)tile.adapter * a.rows + (col0 + r16 < a.rows ? col0 + r16 : a.rows - 1)) * a.K + q * 8;
+  const int part = blockIdx.y, col0 = at.group * 16, line = lane >> 3, chunk = (lane & 7) ^ line;
+  const T* src[LOADS];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int col = col0 + i * 8 + line;
+    src[i] = (const T*)a.X + (int64_t)tile.row(a.r, i * 8 + line) * a.K;
+    src[2 + i] = (const T*)a.A + ((int64_t)tile.adapter * a.rows + (col < a.rows ? col : a.rows - 1)) * a.K;
+  }
+  const int begin = part * a.part_k, end = begin + a.part_k < a.K ? begin + a.part_k : a.K;
+  const int all = (end - begin + 63) / 64, steps = (all - wave + WAVES - 1) / WAVES;  // (this wavefront's: wave, wave + WAVES ..)
+  const uint32_t lds = lds_of(stages[wave]);
+  const auto load = [&](int s) __attribute__((always_inline)) {
+    int k = begin + (s * WAVES + wave) * 64 + chunk * 8;
+    k = k < a.K ? k : a.K - 8;  // (rows are multiples of 32 values: the second half of the last stage may not be there)
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) direct16(src[i] + k, lds + (uint32_t)((s % DEPTH) * 4096 + i * 1024));
+  };
   float4_t acc = {0, 0, 0, 0};
-  const int end = (part + 1) * a.part_k < a.K ? (part + 1) * a.part_k : a.K;
-  for (int k = part * a.part_k + wave * 64; k < end; k += kDownStep) {
-    const bool both = k + 32 < a.K;  // (rows are multiples of 32 values)
-    uint4_t xf[2] = {*(const uint4_t*)(x + k), {0, 0, 0, 0}}, wf[2] = {*(const uint4_t*)(w + k), {0, 0, 0, 0}};
-    if (both) xf[1] = *(const uint4_t*)(x + k + 32), wf[1] = *(const uint4_t*)(w + k + 32);
-    acc = Mma::mma(wf[0], xf[0], acc);
-    acc = Mma::mma(wf[1], xf[1], acc);
+#pragma unroll
+  for (int s = 0; s < DEPTH; ++s)
+    if (s < steps) load(s);
+  for (int s = 0; s < steps; ++s) {
+    if (s + DEPTH <= steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint4_t(*const stage)[8] = stages[wave][s % DEPTH];
+    const int k = begin + (s * WAVES + wave) * 64;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half == 1 && k + 32 >= a.K) break;
+      const int place = (half * 4 + q) ^ (r16 & 7);
+      acc = Mma::mma(stage[16 + r16][place], stage[r16][place], acc);
+    }
+    if (s + DEPTH < steps) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      load(s + DEPTH);
+    }
   }
   red[wave][lane] = acc;
   __syncthreads();
   const int i = col0 + q * 4;
   if (wave != 0 || r16 >= tile.rows || i >= a.rows) return;
 #pragma unroll
-  for (int v = 1; v < kDownWaves; ++v) acc += red[v][lane];
-  *(float4_t*)(a.sums + (part * (int64_t)a.r.M + row) * a.rows + i) = acc;
+  for (int v = 1; v < WAVES; ++v) acc += red[v][lane];
+  *(float4_t*)(a.sums + (part * (int64_t)a.r.M + tile.row(a.r, r16)) * a.rows + i) = acc;
 }
 
 // Tiles of 64 rows x 16 NT rows of A: rows and weights come in stages of 64 values (128 bytes, a cache line, of a row), eight lanes a line, straight into
-// LDS, three stages ahead; a wavefront multiplies 16 rows.  (Operands read straight from memory -- 16 neighbouring lanes, 16 rows -- go through the cache at a
-// quarter of its rate.)  8192 rows, K = 4096, rank 32 bf16: 16 us where X is in the last-level cache, 27 behind a second product that has just written
+// LDS, three stages ahead; a wavefront multiplies 16 rows.  8192 rows, K = 4096, rank 32 bf16: 16 us where X is in the last-level cache, 27 behind a second product that has just written
 // 235 MB; five, seven stages ahead level.
 template <typename T, int NT>
 __global__ __launch_bounds__(256) void low_rank_down_tile_kernel(const DownArgs a) {
@@ -468,14 +494,15 @@ inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 inline int tile_rows_of(int64_t M, int64_t L) { return M <= kInlineRows || M < 32 * L ? 16 : 64; }
 inline int64_t most_tiles(int64_t M, int64_t L, int tile_rows) { return M <= kInlineRows ? M : M / tile_rows + (L + 1 < M ? L + 1 : M); }
 int64_t plan_bytes(int64_t M, int64_t L) { return M <= kInlineRows ? 0 : align256((tiles_at(M) + 4 * most_tiles(M, L, 16)) * 4); }
-int64_t most_parts(int64_t K) { return K >= 4096 ? 16 : (K + 255) / 256; }
-// Parts of K: work-groups for the machine where there are few tiles (`want` of them), at most 16.  Every part costs a sum written and read: 8192 rows of rank 32 on 14336 outputs 136 us in one part, 139 in four, 145 in seven (tiles of 64 rows); 2048 of rank 16, three
-// projections, 31.2 for 128 work-groups, 33.4 for 256; tiles of 16 rows: 8 rows of 8 adapters, K = 11008, 9.9 us for 64 or more, 13.4 for 16.
+// Parts of K: work-groups for the machine where there are few tiles (`want` of them), at most 16, or 4 for tiles of 16 rows, whose eight wavefronts share K
+// already.  Every part costs a sum written and read: tiles of 64 rows: 8192 rows of rank 32 on 14336 outputs 136 us in one part, 139 in four, 145 in seven;
+// 2048 of rank 16, three projections, 31.2 for 128 work-groups, 33.4 for 256; tiles of 16: 1 row, K = 11008, 7.7 in four parts, 8.2 in sixteen.
 // With more than M / 64 (M / 16) tiles, parts * M is less than 64 * kTileGroups + M (16 * kFewGroups + M).
-constexpr int kTileGroups = 128, kFewGroups = 256;
-int64_t parts_of(int64_t tiles, int64_t K, int64_t want) {
-  const int64_t parts = (want + tiles - 1) / tiles;
-  return parts < most_parts(K) ? parts : most_parts(K);
+constexpr int kTileGroups = 128, kFewGroups = 192, kFewParts = 4;
+int64_t most_parts(int64_t K, int64_t most = 16) { return K >= 256 * most ? most : (K + 255) / 256; }
+int64_t parts_of(int64_t tiles, int64_t K, int64_t want, int64_t most) {
+  const int64_t parts = (want + tiles - 1) / tiles, can = most_parts(K, most);
+  return parts < can ? parts : can;
 }
 int64_t sum_rows(int64_t M, int64_t K) {
   const int64_t few = most_parts(K) * M, many = 64 * kTileGroups + M;
@@ -499,7 +526,7 @@ int run_down(const Call& c, int64_t tiles, int64_t* parts, hipStream_t st) {
   const int groups = (c.rows + 16 * (NT ? NT : 1) - 1) / (16 * (NT ? NT : 1));
   // (an adapter's last tile is half empty on average, and so counts as half of one)
   const int64_t whole = NT ? tiles - (c.r.L + 1 < c.r.M ? c.r.L + 1 : c.r.M) / 2 : tiles, step = NT ? 64 : kDownStep;
-  const int part_k = (int)(ceil_div(ceil_div(c.K, parts_of(groups * whole, c.K, NT ? kTileGroups : kFewGroups)), step) * step);
+  const int part_k = (int)(ceil_div(ceil_div(c.K, parts_of(groups * whole, c.K, NT ? kTileGroups : kFewGroups, NT ? 16 : kFewParts)), step) * step);
   *parts = ceil_div(c.K, part_k);
   const DownArgs a{c.r, c.X, c.A, c.sums, c.K, c.rows, part_k, groups, (int)tiles};
   const dim3 grid((unsigned)(ceil_div(tiles, (int64_t)8) * 8 * groups), (unsigned)*parts);
