@@ -71,16 +71,18 @@ for M, L, rank, parts, K in cases:
     what = (M, L, rank, parts, K)
     names = [n for n, _, _, _ in got]
     assert len(got) == (2 if M <= 64 else 3), what
-    tile_rows = 64 if any("down_tile" in n for n in names) else 16
-    result.add((len(got), tile_rows))
-    most = M if M <= 64 else M // tile_rows + min(L + 1, M)  # tiles, at most
     down, up = got[-2], got[-1]
-    ids, plan, m, l, x, a, sums, k, r, part_k, groups, total = struct.unpack("QQiiQQQiiiii", down[3][:68])
-    assert (ids, m, l, x, a, k, r, total) == (IDS, M, L, X, A, K, rows, most), what
+    ids, plan, m, l, x, a, sums, k, r, part_k, groups, total, subs = struct.unpack("QQiiQQQiiiiii", down[3][:72])
+    by_tiles = "down_tile" in down[0]
+    tile_rows = 64 if by_tiles else 16 * subs
+    result.add((len(got), tile_rows, by_tiles))
+    most = M if M <= 64 else M // tile_rows + min(L + 1, M)  # tiles, at most
+    assert (ids, m, l, x, a, k, r, total) == (IDS, M, L, X, A, K, rows, most * subs) and subs in ((1,) if by_tiles or M <= 64 else (1, 4)), what
+    assert ("Li4E" in up[0].split("up_kernel")[1].split("Li8E")[0].split("Li16E")[0].split("Li32E")[0].split("Li64E")[0].split("Li128E")[0]) == (tile_rows == 64), (what, up[0])
     cut = down[1][1]
     assert part_k % 64 == 0 and (cut - 1) * part_k < K <= cut * part_k, what
-    assert down[1][0] >= most * groups and down[1][0] >= (-(-most // 8)) * 8 * groups, what
-    per = 16 if tile_rows == 16 else 16 if "ILi1E" in down[0] or down[0].split("down_tile_kernel")[1].split("Li")[1][0] == "1" else 32 if "Li2E" in down[0] else 64
+    assert down[1][0] == (-(-total // 8)) * 8 * groups, what
+    per = 16 if not by_tiles else 16 * int(down[0].split("down_tile_kernel")[1].split("Li")[1][0])
     assert groups == -(-rows // per), (what, down[0], groups)
     assert sums % 16 == 0 and sums >= WS and sums + cut * M * rows * 4 <= WS + size, what
     if M > 64:
@@ -93,7 +95,7 @@ for M, L, rank, parts, K in cases:
     assert up[1][0] == most * all_groups, what
 result = sorted(result)
 """)
-    assert result == [[2, 16], [3, 16], [3, 64]]
+    assert result == [[2, 16, False], [3, 16, False], [3, 64, False], [3, 64, True]]
 
 
 def test_rows_have_work_groups(recorder):

@@ -331,6 +331,8 @@ UPDATES = [
     (256, 9, 16, (1040,), 96, "holes"), (257, 1, 32, (80,), 224, "one"), (300, 5, 64, (336, 16, 16), 416, "runs"), (40, 3, 16, (16,), 256, "none"), (700, 600, 8, (32,), 64, "spread"),
     (1030, 4, 16, (144,), 192, "runs"), (1100, 3, 128, (80, 48), 160, "holes"), (1500, 2, 32, (1088,), 64, "one"), (2, 4096, 8, (32,), 32, "spread"), (9, 2, 16, (32,), 16416, "spread"),
     (513, 2, 8, (16,), 8224, "holes"), (1025, 1025, 16, (48,), 32, "spread"), (600, 3, 16, (64,), 64, "none"),
+    # (tiles of 64 rows: the first product in runs of 16, and by whole tiles)
+    (1700, 2, 64, (80,), 416, "runs"), (900, 7, 128, (32,), 1120, "holes"), (2600, 3, 64, (48,), 352, "holes"), (5300, 2, 32, (32,), 288, "spread"), (10300, 2, 16, (16,), 160, "runs"),
 ]
 
 

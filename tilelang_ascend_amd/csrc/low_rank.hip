@@ -166,7 +166,8 @@ struct DownArgs {
   const void *X, *A;
   float* sums;
   int K, rows, part_k;  // rows: of an adapter's A; part_k: values of a part, a multiple of 64 (tiles of 16 rows: of kDownStep)
-  int groups, total;    // groups of rows of A of a tile, and tiles
+  int groups, total;    // groups of rows of A of a tile, and tiles (runs of 16 rows of them)
+  int subs;             // runs of 16 rows of a tile
 };
 // Work-group `no`: which of its tile's groups, and which tile.  (Numbers go to the XCDs in turn: the groups of a tile one after another on one of them.)
 struct DownPlace {
@@ -177,7 +178,7 @@ struct DownPlace {
   }
 };
 
-// Tiles of 16 rows x 16 rows of A on one part of K: eight wavefronts take stages of 64 values (128 bytes, a cache line, of a row) in turn, each with a ring
+// Tiles of 16 rows, or a tile of 64 in four runs, x 16 rows of A on one part of K: eight wavefronts take stages of 64 values (128 bytes, a cache line, of a row) in turn, each with a ring
 // of its own in LDS, which it fills two stages ahead, eight lanes a line, and nobody else looks at; the wavefronts' sums meet at the end.  Operands read
 // straight from memory -- 16 neighbouring lanes, 16 rows -- go through the cache at a quarter of its rate (13 bytes a clock and CU).  Whole calls, us, that
 // way / this: 1 row of 4096 x rank 16 7.4 / 6.9, K = 11008 9.1 / 7.7, 64 rows of 48 adapters, three projections 14.1 / 11.3, 512 rows of 128 21.2 / 18.4, 259
@@ -191,14 +192,15 @@ __global__ __launch_bounds__(64 * kDownWaves) void low_rank_down_kernel(const Do
   __shared__ float4_t red[WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
   const DownPlace at(blockIdx.x, a.groups);
-  const Tile tile(a.r, at.tile, lane);
-  if (at.tile >= a.total || tile.rows == 0 || tile.adapter == a.r.L) return;
+  const Tile tile(a.r, at.tile / a.subs, lane);
+  const int slot0 = at.tile % a.subs * 16, live = tile.rows - slot0;
+  if (at.tile >= a.total || live <= 0 || tile.adapter == a.r.L) return;
   const int part = blockIdx.y, col0 = at.group * 16, line = lane >> 3, chunk = (lane & 7) ^ line;
   const T* src[LOADS];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int col = col0 + i * 8 + line;
-    src[i] = (const T*)a.X + (int64_t)tile.row(a.r, i * 8 + line) * a.K;
+    src[i] = (const T*)a.X + (int64_t)tile.row(a.r, slot0 + i * 8 + line) * a.K;
     src[2 + i] = (const T*)a.A + ((int64_t)tile.adapter * a.rows + (col < a.rows ? col : a.rows - 1)) * a.K;
   }
   const int begin = part * a.part_k, end = begin + a.part_k < a.K ? begin + a.part_k : a.K;
@@ -233,15 +235,15 @@ __global__ __launch_bounds__(64 * kDownWaves) void low_rank_down_kernel(const Do
   red[wave][lane] = acc;
   __syncthreads();
   const int i = col0 + q * 4;
-  if (wave != 0 || r16 >= tile.rows || i >= a.rows) return;
+  if (wave != 0 || r16 >= live || i >= a.rows) return;
 #pragma unroll
   for (int v = 1; v < WAVES; ++v) acc += red[v][lane];
-  *(float4_t*)(a.sums + (part * (int64_t)a.r.M + tile.row(a.r, r16)) * a.rows + i) = acc;
+  *(float4_t*)(a.sums + (part * (int64_t)a.r.M + tile.row(a.r, slot0 + r16)) * a.rows + i) = acc;
 }
 
 // Tiles of 64 rows x 16 NT rows of A: rows and weights come in stages of 64 values (128 bytes, a cache line, of a row), eight lanes a line, straight into
-// LDS, three stages ahead; a wavefront multiplies 16 rows.  8192 rows, K = 4096, rank 32 bf16: 16 us where X is in the last-level cache, 27 behind a second product that has just written
-// 235 MB; five, seven stages ahead level.
+// LDS, three stages ahead; a wavefront multiplies 16 rows.  8192 rows, K = 4096, rank 32 bf16: 16 us where X is in the last-level
+// cache, 27 behind a second product that has just written 235 MB; five, seven stages ahead level.
 template <typename T, int NT>
 __global__ __launch_bounds__(256) void low_rank_down_tile_kernel(const DownArgs a) {
   typedef typename MmaOf<T>::type Mma;
@@ -490,8 +492,14 @@ __global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(
 // ---- launches ----------------------------------------------------------------------------------------------------------------
 constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;  // work-groups of 256 threads of a launch, which has fewer than 2^32 threads
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-// Tiles of 64 rows from 32 rows an adapter on average, of 16 below.
-inline int tile_rows_of(int64_t M, int64_t L) { return M <= kInlineRows || M < 32 * L ? 16 : 64; }
+// Tiles of 64 rows where an adapter has 32 or more on average and B is large enough to be worth sharing: the work-groups of a tile of 64 read it once,
+// those of 16 four times, and are twice as many.  Whole calls, us, K = 4096, tiles of 16 / 64 (first product by one_run_each): rank 16 on 4096 outputs, 1003 rows of 8
+// adapters 17.5 / 17.7, 4000 33.6 / 36.0, 8000 63.2 / 62.9; rank 64, 500 of 12 26.0 / 26.6, 1003 24.9 / 23.3, 1003 on 14336 outputs 47.8 / 38.6; rank 32 on
+// 14336, 8192 of 16 177 / 135.
+inline int tile_rows_of(int64_t M, int64_t L, int64_t rank) { return M > kInlineRows && M >= 32 * L && M * rank >= 50000 ? 64 : 16; }
+// Of tiles of 64 rows, the first product in runs of 16 (A read by each, but work-groups enough) or by whole tiles: 1003 rows, 64 rows of A 23.3 / 28.3, 128 28.6 /
+// 33.9; 2000, 128 82.8 / 77.6; 8192, 16 65.2 / 67.0, 32 136.9 / 135.5, 64 88.6 / 78.3.
+inline bool one_run_each(int64_t M, int64_t rows) { return M * rows <= 160000; }
 inline int64_t most_tiles(int64_t M, int64_t L, int tile_rows) { return M <= kInlineRows ? M : M / tile_rows + (L + 1 < M ? L + 1 : M); }
 int64_t plan_bytes(int64_t M, int64_t L) { return M <= kInlineRows ? 0 : align256((tiles_at(M) + 4 * most_tiles(M, L, 16)) * 4); }
 // Parts of K: work-groups for the machine where there are few tiles (`want` of them), at most 16, or 4 for tiles of 16 rows, whose eight wavefronts share K
@@ -520,16 +528,16 @@ struct Call {
   int K, N, rank, rows, end0, end1;
 };
 
-// NT: 16 rows of A each that a work-group has; 0: tiles of 16 rows
+// NT: 16 rows of A each that a work-group has; 0: runs of 16 rows, subs of them a tile
 template <typename T, int NT>
-int run_down(const Call& c, int64_t tiles, int64_t* parts, hipStream_t st) {
+int run_down(const Call& c, int64_t tiles, int subs, int64_t* parts, hipStream_t st) {
   const int groups = (c.rows + 16 * (NT ? NT : 1) - 1) / (16 * (NT ? NT : 1));
   // (an adapter's last tile is half empty on average, and so counts as half of one)
-  const int64_t whole = NT ? tiles - (c.r.L + 1 < c.r.M ? c.r.L + 1 : c.r.M) / 2 : tiles, step = NT ? 64 : kDownStep;
+  const int64_t whole = NT ? tiles - (c.r.L + 1 < c.r.M ? c.r.L + 1 : c.r.M) / 2 : tiles * subs, step = NT ? 64 : kDownStep;
   const int part_k = (int)(ceil_div(ceil_div(c.K, parts_of(groups * whole, c.K, NT ? kTileGroups : kFewGroups, NT ? 16 : kFewParts)), step) * step);
   *parts = ceil_div(c.K, part_k);
-  const DownArgs a{c.r, c.X, c.A, c.sums, c.K, c.rows, part_k, groups, (int)tiles};
-  const dim3 grid((unsigned)(ceil_div(tiles, (int64_t)8) * 8 * groups), (unsigned)*parts);
+  const DownArgs a{c.r, c.X, c.A, c.sums, c.K, c.rows, part_k, groups, (int)(tiles * subs), subs};
+  const dim3 grid((unsigned)(ceil_div(tiles * subs, (int64_t)8) * 8 * groups), (unsigned)*parts);
   if constexpr (NT == 0) low_rank_down_kernel<T><<<grid, 64 * kDownWaves, 0, st>>>(a);
   else low_rank_down_tile_kernel<T, NT><<<grid, 256, 0, st>>>(a);
   return check_launch("tlq_low_rank_update", NT ? "low_rank_down_tile_kernel" : "low_rank_down_kernel") ? 0 : 1;
@@ -562,7 +570,7 @@ int run_up(const Call& c, int64_t tiles, int64_t parts, hipStream_t st) {
 
 template <typename T, typename TO>
 int run_low_rank(Call c, hipStream_t st) {
-  const int tile_rows = tile_rows_of(c.r.M, c.r.L);
+  const int tile_rows = tile_rows_of(c.r.M, c.r.L, c.rank);
   const int64_t tiles = most_tiles(c.r.M, c.r.L, tile_rows);
   int64_t parts = 1;
   if (c.r.M > kInlineRows) {
@@ -574,9 +582,13 @@ int run_low_rank(Call c, hipStream_t st) {
     if (!check_launch("tlq_low_rank_update", "low_rank_plan_kernel")) return 1;
     c.r.plan = c.plan;
   }
-  if (tile_rows == 16) return run_down<T, 0>(c, tiles, &parts, st) || run_up<T, TO, 1>(c, tiles, parts, st);
-  if (c.rows <= 16 ? run_down<T, 1>(c, tiles, &parts, st) : c.rows <= 32 ? run_down<T, 2>(c, tiles, &parts, st) : run_down<T, 4>(c, tiles, &parts, st)) return 1;
-  return run_up<T, TO, 4>(c, tiles, parts, st);
+  const int rc = tile_rows == 16 ? run_down<T, 0>(c, tiles, 1, &parts, st)
+                 : one_run_each(c.r.M, c.rows) ? run_down<T, 0>(c, tiles, 4, &parts, st)
+                 : c.rows <= 16 ? run_down<T, 1>(c, tiles, 1, &parts, st)
+                 : c.rows <= 32 ? run_down<T, 2>(c, tiles, 1, &parts, st)
+                                : run_down<T, 4>(c, tiles, 1, &parts, st);
+  if (rc) return rc;
+  return tile_rows == 16 ? run_up<T, TO, 1>(c, tiles, parts, st) : run_up<T, TO, 4>(c, tiles, parts, st);
 }
 
 bool sizes_taken(int64_t M, int64_t L, int64_t rank, int64_t parts, int64_t K) {
