@@ -383,7 +383,7 @@ int tlq_act_quant_i8(const void* X, void* Y, void* S, int64_t M, int64_t N, int 
  *   Y = rn_T(y) (NULL: not wanted);  Q, S (both NULL: not wanted) as tlq_act_quant_i8 makes them, of y: S = max(max_n |y|, 1e-4) / 127
  *   (round_scale: 2^ceil(log2)), Q = rint(clamp(y / S, -127, 127)).
  * Where S is neither the floor nor rounded to a power of two, Q is decided exactly: rint(127 h w / max_n |h w|), half to even.
- * A row with a NaN in it is NaN in Y; -127 and the floor's scale in Q and S, as the quantiser has it.  Sums of squares beyond fp32's range (bfloat16
+ * NaN in h makes a row NaN in Y, -127 in Q with the floor's scale; an infinity is NaN there and the row's other values 0.  Sums of squares beyond fp32's range (bfloat16
  * values from 1e19 on) make a row of 0.
  * X, residual, H, Y [M, N] and weight [N] dtype (TLQ_F16 or TLQ_BF16), Q int8 [M, N], S fp32 [M]; any M below 2^31 and N below 2^30 (fastest with rows of a
  * multiple of 8 values, 16-byte aligned, Q 8-byte; beyond 32768 values a row is read twice); 1e-12 <= eps <= 1.  H may be the residual or X, and Y may be X.  Y and Q are operands of
@@ -392,7 +392,8 @@ int tlq_residual_rms_norm(const void* X, const void* residual, const void* weigh
                           int64_t N, float eps, int dtype, int round_scale, void* stream);
 
 /* Between the products of an MLP: y = silu(g) * u, g = X[m, n], u = X[m, N + n], silu(g) = g / (1 + exp(-g)), fp32; Y, Q and S of it as above.
- * X [M, 2 N], Y [M, N] dtype, Q int8 [M, N], S fp32 [M]; M, N and alignment as above. */
+ * A NaN has code -127 and no part in S; an infinity makes S infinite, its own code -127 and the others 0.
+ * X [M, 2 N], Y [M, N] dtype (not in X's place), Q int8 [M, N], S fp32 [M]; M, N and alignment as above. */
 int tlq_gated_silu(const void* X, void* Y, void* Q, void* S, int64_t M, int64_t N, int dtype, int round_scale, void* stream);
 
 /* Low-rank adapters of many requests beside a projection (tlq_gemm_w4a16, tlq_gemm_w8a8, ...), whose outputs are one to three parts of n0, n1, n2

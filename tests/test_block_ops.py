@@ -268,6 +268,8 @@ def test_gated_far_gates_and_not_finite_values(N, dtype):
     assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y[torch.isinf(want)].double(), want[torch.isinf(want)])
     assert_near(y[at], want[at], gated_off(x, want)[at] + torch.finfo(torch.float32).tiny, "beside")
     assert (q[torch.isnan(want)] == -127).all()
+    # an infinity: its row's scale, -127 in its place and 0 elsewhere
+    assert torch.isinf(s[3]) and (q[3][torch.isinf(want[3]) | torch.isnan(want[3])] == -127).all() and (q[3][at[3]] == 0).all() and torch.isinf(want[3]).any()
     for m in (4, 5):  # NaN alone: the scale of the others
         rest = torch.where(at[m], want[m], 0.0)
         check_codes(torch.where(at[m], q[m], 0)[None], s[m: m + 1], rest[None], rel, "beside NaN")
@@ -415,6 +417,12 @@ def test_update_rows_do_not_depend_on_each_other():
     assert_bit_equal(moved, whole[perm], "rows in another order")
     for _ in range(3):
         assert_bit_equal(kernel(*gpu_t), whole, "again")
+
+
+@gpu
+def test_update_of_no_row():
+    t = make_update(0, 3, 16, (64,), 32, "float16", "one", 1)
+    assert update_kernel(3, 16, (64,), 32, "float16")(*[v.cuda() for v in t]).shape == (0, 64)
 
 
 @gpu

@@ -26,6 +26,10 @@ __device__ __forceinline__ int code_exact(float v, float t, float amax) {
   return v < 0.0f ? -n : n;
 }
 
+// What quant1 divides by in a row of this scale.  A row with an infinity has an infinite scale, whose reciprocal is 0: over 0 its finite values get code 0, and
+// the infinity, as NaN does, -127.
+__device__ __forceinline__ float divisor(float scale) { return scale < __builtin_inff() ? scale : 0.0f; }
+
 struct NormArgs {
   const void *X, *R, *W;  // R: null without a residual
   void *H, *Y;            // H: null without a residual; Y, or Q and S: null if not wanted
@@ -203,7 +207,7 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(const NormArgs a) {
     const RowCodes codes = row_codes(amax, rstd, a.round_scale);
     if (live && at == 0) a.S[m] = codes.scale;
     if (!live) continue;
-    const float rcp = 1.0f / codes.scale;
+    const float rcp = 1.0f / codes.scale, over = divisor(codes.scale);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = c * LANES + at;
@@ -226,7 +230,7 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(const NormArgs a) {
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = quant1(value_of<T>(h[c], k) * value_of<T>(w[c], k) * rstd, codes.scale, rcp);
+        for (int k = 0; k < 8; ++k) q[k] = quant1(value_of<T>(h[c], k) * value_of<T>(w[c], k) * rstd, over, rcp);
       }
       store_codes<ANY>(a.Q + row + i * 8, pack_codes(q), a.N - i * 8);
     }
@@ -260,14 +264,14 @@ __global__ __launch_bounds__(256) void norm_long_kernel(const NormArgs a) {
     amax = fmaxf(fmaxf(part[it][1][0], part[it][1][1]), fmaxf(part[it][1][2], part[it][1][3]));
     const float rstd = 1.0f / sqrtf(ss / (float)N + a.eps);
     const RowCodes c = row_codes(amax, rstd, a.round_scale);
-    const float rcp = 1.0f / c.scale;
+    const float rcp = 1.0f / c.scale, over = divisor(c.scale);
     if (a.S && tid == 0) a.S[m] = c.scale;
     const T* const from = a.R ? h : x;
     for (int n = tid; n < N; n += 256) {
       const float v = to_float(from[n]) * to_float(w[n]), y = v * rstd;
       if (a.Q) {
         const float t = v * c.mul;
-        a.Q[m * N + n] = (int8_t)(c.mul == 0.0f ? quant1(y, c.scale, rcp) : code_near(t) ? (uint32_t)code_exact(v, t, amax) : quant1(t, 1.0f, 1.0f));
+        a.Q[m * N + n] = (int8_t)(c.mul == 0.0f ? quant1(y, over, rcp) : code_near(t) ? (uint32_t)code_exact(v, t, amax) : quant1(t, 1.0f, 1.0f));
       }
       if (a.Y) ((T*)a.Y)[m * N + n] = from_float<T>(y);
     }
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(THREADS) void gated_rows_kernel(const GatedArgs a) 
 #pragma unroll
       for (int k = 0; k < WPR; ++k) amax = fmaxf(amax, part[it][first + k]);
     }
-    const float scale = row_scale(amax, a.round_scale), rcp = 1.0f / scale;
+    const float scale = row_scale(amax, a.round_scale), rcp = 1.0f / scale, over = divisor(scale);
     if (!live) continue;
     if (at == 0) a.S[m] = scale;
 #pragma unroll
@@ -358,7 +362,7 @@ __global__ __launch_bounds__(THREADS) void gated_rows_kernel(const GatedArgs a) 
       if (i >= chunks) break;
       uint32_t q[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) q[k] = quant1(y[c][k], scale, rcp);
+      for (int k = 0; k < 8; ++k) q[k] = quant1(y[c][k], over, rcp);
       store_codes<ANY>(a.Q + m * a.N + i * 8, pack_codes(q), a.N - i * 8);
     }
   }
@@ -386,9 +390,9 @@ __global__ __launch_bounds__(256) void gated_long_kernel(const GatedArgs a) {
     if ((tid & 63) == 0) part[it][tid >> 6] = amax;
     __syncthreads();
     amax = fmaxf(fmaxf(part[it][0], part[it][1]), fmaxf(part[it][2], part[it][3]));
-    const float scale = row_scale(amax, a.round_scale), rcp = 1.0f / scale;
+    const float scale = row_scale(amax, a.round_scale), rcp = 1.0f / scale, over = divisor(scale);
     if (tid == 0) a.S[m] = scale;
-    for (int n = tid; n < N; n += 256) a.Q[m * N + n] = (int8_t)quant1(value(n), scale, rcp);
+    for (int n = tid; n < N; n += 256) a.Q[m * N + n] = (int8_t)quant1(value(n), over, rcp);
   }
 }
 

@@ -7,6 +7,7 @@ Results do not depend on timing, nor a row's on what the other rows of the call 
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Sequence, Union
 
 from ..jit import ABI_DTYPE, TORCH_DTYPES, KernelSpec, NativeCall, Param, PassConfigKey, jit
@@ -31,7 +32,7 @@ def low_rank_update(L: int, rank: int, N: Union[int, Sequence[int]], K: int, in_
     id lies outside 0 .. L - 1 is Y.  N: the projection's outputs, or those of up to three projections side by side (queries, keys and values;
     gate and up), which are the parts p, each with `rank` rows of A.  rank: 8, 16, 32, 64 or 128; an adapter of a lower rank has zeros in the
     rows and columns that it lacks.  X, A and B are in_dtype, Y and out out_dtype: in_dtype (the default) or float32."""
-    parts = (N,) if isinstance(N, int) else tuple(int(n) for n in N)
+    parts = tuple(operator.index(n) for n in (N if isinstance(N, (tuple, list)) else (N,)))
     if not 1 <= len(parts) <= 3:
         raise ValueError(f"N must be one to three sizes (got {N})")
     for n in parts:
