@@ -335,6 +335,12 @@ UPDATES = [
     (513, 2, 8, (16,), 8224, "holes"), (1025, 1025, 16, (48,), 32, "spread"), (600, 3, 16, (64,), 64, "none"),
     # (tiles of 64 rows: the first product in runs of 16, and by whole tiles)
     (1700, 2, 64, (80,), 416, "runs"), (900, 7, 128, (32,), 1120, "holes"), (2600, 3, 64, (48,), 352, "holes"), (5300, 2, 32, (32,), 288, "spread"), (10300, 2, 16, (16,), 160, "runs"),
+    # (tiles of 16 rows: sizes beyond what single rows are for)
+    (1, 1, 8, (16,), 16416, "one"), (3, 2, 64, (80, 16, 32), 2080, "holes"), (17, 1, 16, (112,), 8224, "one"), (33, 40, 8, (256, 64, 64), 16416, "spread"), (64, 1, 32, (48,), 4128, "one"),
+    (63, 9, 128, (96, 32), 1056, "spread"), (40, 3, 16, (16,), 8224, "none"), (2, 4096, 16, (32,), 8224, "spread"), (100, 100, 16, (208,), 8224, "spread"), (700, 600, 32, (32,), 352, "spread"),
+    # (single rows: every rank, runs of more than one block, K that ends inside of a stage)
+    (1, 2, 64, (2000,), 2048, "spread"), (1, 3, 128, (48, 4096, 16), 992, "holes"), (16, 16, 32, (4112, 32), 1120, "spread"), (2, 2, 32, (22016, 16), 4096, "runs"), (600, 40, 8, (16, 1040), 736, "holes"),
+    (64, 5, 8, (8208, 48), 2080, "spread"), (9, 2, 8, (528,), 16384, "spread"),
 ]
 
 
@@ -348,7 +354,9 @@ def test_update(M, L, rank, parts, K, kind, dtype):
 
 @gpu
 @pytest.mark.parametrize("M,L,rank,parts,K,kind", [(8192, 3, 8, (48,), 64, "runs"), (8193, 4, 16, (32, 16), 32, "holes"), (9001, 700, 8, (32,), 64, "spread"), (20000, 2, 8, (16,), 32, "one"),
-                                                   (70001, 5, 8, (16,), 32, "runs"), (33000, 4096, 8, (16,), 32, "holes")])
+                                                   (70001, 5, 8, (16,), 32, "runs"), (33000, 4096, 8, (16,), 32, "holes"),
+                                                   (8192, 3, 32, (48,), 64, "runs"), (8193, 4, 32, (32, 16), 32, "holes"), (9001, 700, 32, (32,), 64, "spread"), (20000, 2, 16, (16,), 64, "one"),
+                                                   (33000, 4096, 16, (16,), 32, "holes")])
 def test_update_many_rows(M, L, rank, parts, K, kind):
     t = make_update(M, L, rank, parts, K, "bfloat16", kind, 3)
     got = update_kernel(L, rank, parts, K, "bfloat16")(*[v.cuda() for v in t]).cpu()
@@ -370,10 +378,10 @@ def test_update_many_rows(M, L, rank, parts, K, kind):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M", [4, 70, 400])
-def test_update_large_and_small_values(M, dtype):
+@pytest.mark.parametrize("M,rank,K", [(4, 16, 128), (70, 16, 128), (400, 16, 128), (4, 32, 4128), (70, 32, 4128), (800, 64, 2080)])
+def test_update_large_and_small_values(M, rank, K, dtype):
     """First sums far outside float16's range, and far below its normal numbers, that the second product brings back."""
-    K, rank, parts, L = 128, 16, (64,), 3
+    parts, L = (64,), 3
     x, y, ids, a, b, scaling = make_update(M, L, rank, parts, K, "float16", "spread", 5)
     T = DT[dtype]
     a[0] = (a[0].float() * 2000).half()
@@ -389,17 +397,18 @@ def test_update_large_and_small_values(M, dtype):
 
 
 @gpu
-def test_update_rows_do_not_depend_on_each_other():
+@pytest.mark.parametrize("M,rank,K", [(300, 16, 512), (300, 64, 2080), (420, 128, 1056), (60, 32, 4128)])
+def test_update_rows_do_not_depend_on_each_other(M, rank, K):
     """A row alone, in a small batch, in a large one, beside rows of NaN: the values that it has by itself, but for sums formed in another order."""
-    L, rank, parts, K = 6, 16, (96, 32), 512
-    t = make_update(300, L, rank, parts, K, "bfloat16", "spread", 8)
+    L, parts = 6, (96, 32)
+    t = make_update(M, L, rank, parts, K, "bfloat16", "spread", 8)
     kernel = update_kernel(L, rank, parts, K, "bfloat16")
     gpu_t = [v.cuda() for v in t]
     whole = kernel(*gpu_t)
     bad = gpu_t[0].clone()
     bad[::3] = float("nan")
     beside = kernel(bad, *gpu_t[1:])
-    keep = torch.arange(300) % 3 != 0
+    keep = torch.arange(M) % 3 != 0
     assert_bit_equal(beside.cpu()[keep], whole.cpu()[keep], "beside NaN")
     want, off = ref.low_rank_update(*t, parts)
     for rows in (slice(7, 8), slice(40, 57), slice(0, 100)):
@@ -412,7 +421,7 @@ def test_update_rows_do_not_depend_on_each_other():
     assert_bit_equal(other.cpu()[keep], whole.cpu()[keep], "beside an adapter of NaN")
     assert torch.isnan(other.cpu()[~keep]).all()
     # the order of the rows
-    perm = torch.randperm(300, generator=gen(2)).cuda()
+    perm = torch.randperm(M, generator=gen(2)).cuda()
     moved = kernel(*[v[perm].contiguous() for v in gpu_t[:3]], *gpu_t[3:])
     assert_bit_equal(moved, whole[perm], "rows in another order")
     for _ in range(3):
@@ -426,9 +435,9 @@ def test_update_of_no_row():
 
 
 @gpu
-@pytest.mark.parametrize("M", [20, 400])
-def test_update_in_place_and_nothing_beside_its_outputs(M):
-    L, rank, parts, K = 4, 32, (80, 16), 256
+@pytest.mark.parametrize("M,rank,K", [(20, 32, 256), (400, 32, 256), (20, 32, 4128), (900, 64, 288)])
+def test_update_in_place_and_nothing_beside_its_outputs(M, rank, K):
+    L, parts = 4, (80, 16)
     N = sum(parts)
     t = [v.cuda() for v in make_update(M, L, rank, parts, K, "float16", "holes", 3)]
     want = update_kernel(L, rank, parts, K, "float16")(*t)
@@ -446,14 +455,15 @@ def test_update_in_place_and_nothing_beside_its_outputs(M):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M", [5, 90])
-def test_update_infinities_stay_infinities(M, dtype):
+@pytest.mark.parametrize("M,times", [(5, 0), (90, 0), (5, 1), (90, 1)])
+def test_update_infinities_stay_infinities(M, times, dtype):
     """An infinity among the activations, beside weights of one sign: the row is infinite, the others are what they were."""
-    t = list(make_update(M, 2, 16, (64,), 64, dtype, "one", 4))
+    K = 64 + times * 8160  # (the longer rows: for tiles)
+    t = list(make_update(M, 2, 16, (64,), K, dtype, "one", 4))
     t[3], t[4], t[5] = t[3].abs() + 0.01, t[4].abs() + 0.01, t[5].abs() + 0.1
     x = t[0].clone()
     x[1, 3] = float("inf")
-    kernel = update_kernel(2, 16, (64,), 64, dtype)
+    kernel = update_kernel(2, 16, (64,), K, dtype)
     rest = [v.cuda() for v in t[1:]]
     got, was = kernel(x.cuda(), *rest).cpu(), kernel(t[0].cuda(), *rest).cpu()
     assert (got[1] == float("inf")).all()
@@ -461,8 +471,9 @@ def test_update_infinities_stay_infinities(M, dtype):
     assert_bit_equal(got[keep], was[keep])
     # an infinite weight in some places of a row of B: that output alone (an infinity, or NaN)
     for rank in (8, 16, 32, 64):
-        t = make_update(M, 2, rank, (64,), 64, dtype, "one", 4)
-        kernel = update_kernel(2, rank, (64,), 64, dtype)
+        K = 64 + times * (131072 // rank)
+        t = make_update(M, 2, rank, (64,), K, dtype, "one", 4)
+        kernel = update_kernel(2, rank, (64,), K, dtype)
         was = kernel(*[v.cuda() for v in t]).cpu()
         for j in range(0, rank, 5):
             b = t[4].clone()
@@ -494,6 +505,23 @@ def test_update_offsets_beyond_32_bits():
         rows = [0, 1, M - 1]
         want, off = ref.low_rank_update(x[rows], y[rows], ids[rows] // (L - 1), torch.stack([a[0], a[L - 1]]), torch.stack([b[0], b[L - 1]]), scaling[:2], (N, N))
         assert_near(got[rows], want, off, "far adapters")
+
+
+@gpu
+def test_update_single_rows_offsets_beyond_32_bits():
+    L, rank, K, N = 4096, 64, 2048, 2752
+    g = torch.Generator(device="cuda").manual_seed(2)
+    a = torch.zeros(L, 3 * rank, K, dtype=torch.bfloat16, device="cuda")
+    b = torch.zeros(L, 3 * N, rank, dtype=torch.bfloat16, device="cuda")
+    assert (L - 1) * 3 * rank * K * 2 > 2**31 and (L - 1) * 3 * N * rank * 2 > 2**32
+    a[L - 1] = (torch.randn(3 * rank, K, generator=g, device="cuda") * K**-0.5).to(torch.bfloat16)
+    b[L - 1] = (torch.randn(3 * N, rank, generator=g, device="cuda") * 0.2).to(torch.bfloat16)
+    x, y = torch.randn(2, K, generator=g, device="cuda").to(torch.bfloat16), torch.randn(2, 3 * N, generator=g, device="cuda").to(torch.bfloat16)
+    ids = torch.tensor([L - 1, 0], dtype=torch.int32, device="cuda")
+    got = ops.low_rank_update(L, rank, (N, N, N), K, in_dtype="bfloat16")(x, y, ids, a, b, torch.ones(L, device="cuda"))
+    want, off = ref.low_rank_update(x[:1], y[:1], torch.zeros(1, dtype=torch.int32), a[L - 1:], b[L - 1:], torch.ones(1), (N, N, N))
+    assert_near(got[:1], want, off, "far adapter")
+    assert_bit_equal(got[1], y[1], "an adapter of zeros")
 
 
 # ---- together ---------------------------------------------------------------------------------------------------------------------
@@ -549,18 +577,18 @@ def block_inputs(M, hidden, L, dtype, seed):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M", [1, 21, 300])
-def test_a_block_of_them(M, dtype):
-    steps, check = make_block(M, 256, 384, 5, 16, dtype, 1)
+@pytest.mark.parametrize("M,rank", [(1, 16), (21, 16), (300, 16), (21, 128), (300, 128), (500, 128)])
+def test_a_block_of_them(M, rank, dtype):
+    steps, check = make_block(M, 256, 384, 5, rank, dtype, 1)
     x, r, ids = block_inputs(M, 256, 5, dtype, 2)
     check(x, r, ids, steps(x, r, ids))
 
 
 @gpu
-@pytest.mark.parametrize("M", [4, 300])
-def test_a_block_captured_and_replayed(M):
+@pytest.mark.parametrize("M,rank", [(4, 16), (300, 16), (21, 128), (500, 128)])
+def test_a_block_captured_and_replayed(M, rank):
     """Two graphs of the same weights, with eager calls between their replays and new inputs for each."""
-    steps, _ = make_block(M, 256, 384, 5, 16, "bfloat16", 1)
+    steps, _ = make_block(M, 256, 384, 5, rank, "bfloat16", 1)
     graphs = []
     for seed in (3, 4):
         ins = block_inputs(M, 256, 5, "bfloat16", seed)
@@ -585,8 +613,9 @@ def test_a_block_captured_and_replayed(M):
 
 
 @gpu
-def test_on_other_streams_and_from_several_threads():
-    steps, _ = make_block(30, 256, 384, 5, 16, "float16", 1)
+@pytest.mark.parametrize("rank", [16, 128])
+def test_on_other_streams_and_from_several_threads(rank):
+    steps, _ = make_block(30, 256, 384, 5, rank, "float16", 1)
     ins = [block_inputs(M, 256, 5, "float16", M) for M in (30, 1, 280, 64)]
     want = [steps(*i) for i in ins]
     torch.cuda.synchronize()

@@ -2,9 +2,9 @@
 //   out[m, n] = rn(Y[m, n] + scaling[l] * sum_j h[m, p r + j] * B[l, n, j]),  h[m, i] = sum_k X[m, k] * A[l, i, k]
 // l = ids[m], p the part that n lies in, r the rank; a row whose id names no adapter is out = Y.  h and the sums are fp32, rounded once, at the end.
 //
-// Memory bound: Y and out, X, and the weights of the adapters that some row names, each once.  Rows are gathered by adapter into tiles of 16 or 64, which
-// meet their adapter's weights on the matrix units: the first product writes fp32 sums of parts of K (few tiles: many parts), the second adds the parts
-// as it reads them.  A row's values do not depend on its tile or its place there.
+// Memory bound: Y and out, X, and the weights of the adapters that some row names, each once.  Few rows of low rank take one launch, a work-group a row and run of
+// outputs.  More are gathered by adapter into tiles of 16 or 64, which meet their adapter's weights on the matrix units: the first product writes fp32 sums of
+// parts of K (few tiles: many parts), the second adds the parts as it reads them.  A row's values do not depend on its tile or its place there.
 #include "gemm_core.h"
 
 namespace tlq {
@@ -181,7 +181,7 @@ struct DownPlace {
 // Tiles of 16 rows, or a tile of 64 in four runs, x 16 rows of A on one part of K: eight wavefronts take stages of 64 values (128 bytes, a cache line, of a row) in turn, each with a ring
 // of its own in LDS, which it fills two stages ahead, eight lanes a line, and nobody else looks at; the wavefronts' sums meet at the end.  Operands read
 // straight from memory -- 16 neighbouring lanes, 16 rows -- go through the cache at a quarter of its rate (13 bytes a clock and CU).  Whole calls, us, that
-// way / this: 1 row of 4096 x rank 16 7.4 / 6.9, K = 11008 9.1 / 7.7, 64 rows of 48 adapters, three projections 14.1 / 11.3, 512 rows of 128 21.2 / 18.4, 259
+// way / this: 1 row of rank 16, K = 11008, 9.1 / 7.7, 64 rows of 48 adapters, three projections 14.1 / 11.3, 512 rows of 128 21.2 / 18.4, 259
 // rows of 32 of rank 64 on 2 x 11008 44.1 / 41.2; four wavefronts, or four stages ahead: level to 0.2 behind.
 constexpr int kDownWaves = 8, kDownStep = 64 * kDownWaves;
 template <typename T>
@@ -351,6 +351,7 @@ __global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(
   const Tile tile(a.r, at, lane);
   if (tile.rows == 0) return;
   const bool with = tile.adapter != a.r.L;
+  if (!with && a.Y == a.out) return;
   const int live = tile.rows - rw * 16;  // rows of this wavefront, if any
   int64_t row[4];                        // rows 4 q + i of its 16
 #pragma unroll
@@ -489,6 +490,121 @@ __global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(
   }
 }
 
+// ---- single rows: both products in one launch ---------------------------------------------------------------------------------
+struct RowArgs {
+  const int32_t* ids;
+  const void *X, *Y, *A, *B;
+  const float* scaling;
+  void* out;
+  int L, N, K, rows, end0, end1;  // as above
+  int per_group, groups, groups0, groups1;
+};
+template <typename T>
+__device__ __forceinline__ float value8(const uint4_t& v, int k) {
+  if constexpr (std::is_same<T, half_t>::value) return (float)bitcast<half2_t>(v[k / 2])[k % 2];
+  else return bitcast<float>(k % 2 ? v[k / 2] & 0xffff0000u : v[k / 2] << 16);
+}
+
+// A row and blocks of 4096 / RANK outputs of one part of the outputs a work-group, which forms the part's RANK values of h for itself: CL lanes have a run of
+// 8 CL values of each of H rows of A, the wavefronts take K in turn, and their sums meet in LDS; X, A and the first block's B and Y are asked for at once.
+// Bounded by latency and by A through the CU (rank 16, K = 4096: 128 KB, about 1 us of 3.9).  More code costs more than loads it has in flight: a row of rank 8,
+// K = 4096, with 8 / 16 / 32 loads of A at a time 3.3 / 3.9 / 5.3 us; sixteen wavefronts 4.6.  CL = 16 reads X less often, 8 has fewer sums a lane, us, 16 / 8: rank
+// 32 5.9 / 5.1, 64 10.6 / 7.9, 8 on K = 11008 4.7 / 5.2.
+constexpr int kRowWaves = 8;
+template <typename T, typename TO, int RANK>
+__global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowArgs a) {
+  constexpr int WAVES = kRowWaves, CL = RANK >= 32 ? 8 : 16, LINES = 64 / CL, STAGE = CL * 8, H = RANK / LINES, AHEAD = H >= 8 ? 1 : 8 / H;
+  constexpr int C = RANK / 8, OUT = 64 * WAVES / C;  // chunks of a row of B, outputs of a block
+  __shared__ float4_t sums[WAVES][RANK / 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x / a.groups, no = blockIdx.x - row * a.groups;
+  const int p = (no >= a.groups0) + (no >= a.groups1), begin = p == 0 ? 0 : p == 1 ? a.end0 : a.end1, end = p == 0 ? a.end0 : p == 1 ? a.end1 : a.N;
+  const int first = begin + (no - (p == 0 ? 0 : p == 1 ? a.groups0 : a.groups1)) * a.per_group * OUT, n_end = end - first < a.per_group * OUT ? end - first : a.per_group * OUT;
+  const int adapter = a.ids[row];
+  const TO* const y_row = (const TO*)a.Y + (int64_t)row * a.N + first;
+  TO* const out_row = (TO*)a.out + (int64_t)row * a.N + first;
+  if ((uint32_t)adapter >= (uint32_t)a.L) {
+    if (a.Y != a.out)
+      for (int n = tid; n < n_end; n += 64 * kRowWaves) out_row[n] = y_row[n];
+    return;
+  }
+  const uint4_t* const b_row = (const uint4_t*)((const T*)a.B + ((int64_t)adapter * a.N + first) * RANK);
+  const int place = tid % C;
+  uint4_t b;
+  TO y;
+  const auto load = [&](int n0) __attribute__((always_inline)) {
+    int n = n0 + tid / C;
+    n = n < n_end ? n : n_end - 1;
+    b = b_row[(int64_t)n * C + place], y = y_row[n];
+  };
+  load(0);
+  const float scale = a.scaling[adapter];
+  const int chunk = lane % CL, line = lane / CL;
+  const T* const x = (const T*)a.X + (int64_t)row * a.K;
+  const T* const w = (const T*)a.A + ((int64_t)adapter * a.rows + p * RANK + line) * a.K;
+  float h[H];
+#pragma unroll
+  for (int j = 0; j < H; ++j) h[j] = 0.0f;
+  for (int k0 = wave * STAGE + chunk * 8; k0 - chunk * 8 < a.K; k0 += AHEAD * STAGE * WAVES) {
+    uint4_t xs[AHEAD], ws[AHEAD][H];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = k0 + u * STAGE * WAVES < a.K ? k0 + u * STAGE * WAVES : a.K - 8;
+      xs[u] = *(const uint4_t*)(x + k);
+#pragma unroll
+      for (int j = 0; j < H; ++j) ws[u][j] = *(const uint4_t*)(w + (int64_t)j * LINES * a.K + k);
+    }
+    asm volatile("" ::: "memory");  // (all loads ahead of the first value's use)
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (k0 + u * STAGE * WAVES >= a.K) break;
+#pragma unroll
+      for (int j = 0; j < H; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[j] = __builtin_fmaf(value8<T>(xs[u], k), value8<T>(ws[u][j], k), h[j]);
+    }
+  }
+  // sums over a run's lanes: of two values a lane has, it keeps one and hands over the other, while there are two
+  int at = 0;
+#pragma unroll
+  for (int o = CL / 2, n = H; o >= 1; o /= 2) {
+    if (n > 1) {
+      n /= 2;
+      const bool upper = chunk & o;
+      at += upper ? n : 0;
+#pragma unroll
+      for (int j = 0; j < H / 2; ++j)
+        if (j < n) h[j] = (upper ? h[j + n] : h[j]) + __shfl_xor(upper ? h[j] : h[j + n], o);
+    } else {
+      h[0] += __shfl_xor(h[0], o);
+    }
+  }
+  constexpr int KEPT = H > CL ? H / CL : 1;
+#pragma unroll
+  for (int j = 0; j < KEPT; ++j) ((float*)sums[wave])[(at + j) * LINES + line] = h[j];
+  __syncthreads();
+  float4_t low = sums[0][place * 2], high = sums[0][place * 2 + 1];
+#pragma unroll
+  for (int v = 1; v < WAVES; ++v) low += sums[v][place * 2], high += sums[v][place * 2 + 1];
+  for (int n0 = 0; n0 < n_end; n0 += OUT) {
+    float f = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f = __builtin_fmaf(value8<T>(b, k), low[k], f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f = __builtin_fmaf(value8<T>(b, 4 + k), high[k], f);
+    const TO from = y;
+    if (n0 + OUT < n_end) load(n0 + OUT);
+#pragma unroll
+    for (int o = 1; o < C; o *= 2) f += __shfl_xor(f, o);
+    const int n = n0 + tid / C;
+    if (place == 0 && n < n_end) {
+      if constexpr (sizeof(TO) == 4) out_row[n] = __builtin_fmaf(scale, f, from);
+      else if constexpr (std::is_same<TO, half_t>::value) out_row[n] = (half_t)__builtin_fmaf(scale, f, (float)from);
+      else ((uint16_t*)out_row)[n] = (uint16_t)pack_bf16x2(__builtin_fmaf(scale, f, bitcast<float>((uint32_t)bitcast<uint16_t>(from) << 16)), 0.0f);
+    }
+  }
+}
+
 // ---- launches ----------------------------------------------------------------------------------------------------------------
 constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;  // work-groups of 256 threads of a launch, which has fewer than 2^32 threads
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -517,6 +633,17 @@ int64_t sum_rows(int64_t M, int64_t K) {
   return few < many ? few : many;
 }
 static_assert(16 * kFewGroups <= 64 * kTileGroups, "sum_rows holds for both");
+
+// Single rows where it is not too much that all work-groups of a row read its part of A (2 rank K bytes; there are N rank / 4096 of them): neither a plan nor a
+// second launch.  Whole calls, us, with them / this, bf16: 1 row of rank 16, K = N = 4096, 7.0 / 3.9, 16 rows 8.0 / 4.5, 32 of as many adapters 7.8 / 8.0; 64, K =
+// 11008, N = 22016, 17.6 / 27.0; 1 row of rank 64, N = 4096, 9.1 / 8.4, N = 22016 9.1 / 10.0, two of K = 11008 10.2 / 18.7; rank 8, K = N = 4096, 64 rows of as many
+// adapters 8.5 / 5.9, 128 11.8 / 6.8, 192 on 14336 outputs 13.9 / 15.4; 1 row of rank 128, K = 1024, 9.9 / 8.2; 2500 rows of rank 16, 64 -> 256, 11.3 / 7.4; rank 8, 5000,
+// 256 -> 256, 15.6 / 15.6, 10000, 64 -> 256, 21.0 / 22.3.
+inline bool single_rows(int64_t M, int64_t rank, int64_t K, int64_t N) {
+  return M <= 4096 && rank * K <= (int64_t)1 << 17 && M * rank * rank * (4 * K + N) <= (M <= kInlineRows ? (int64_t)2 << 27 : (int64_t)3 << 27);
+}
+// (512: 16 rows of rank 32 on 14336 outputs 15.2 us, 256 10.5; 128: 64 rows of rank 16, three projections, 12.3, 256 9.7)
+constexpr int kRowGroups = 256;
 
 struct Call {
   Rows r;
@@ -568,8 +695,32 @@ int run_up(const Call& c, int64_t tiles, int64_t parts, hipStream_t st) {
   }
 }
 
+template <typename T, typename TO, int RANK>
+int run_rows(const Call& c, hipStream_t st) {
+  constexpr int OUT = 512 * kRowWaves / RANK;
+  const int64_t blocks[3] = {(c.end0 + OUT - 1) / OUT, (c.end1 - c.end0 + OUT - 1) / OUT, (c.N - c.end1 + OUT - 1) / OUT};
+  const auto groups = [&](int64_t per) { return ceil_div(blocks[0], per) + ceil_div(blocks[1], per) + ceil_div(blocks[2], per); };
+  int per_group = 1;
+  while (c.r.M * groups(per_group) > kRowGroups && per_group < 1 << 20) per_group *= 2;
+  const int groups0 = (int)ceil_div(blocks[0], (int64_t)per_group), groups1 = groups0 + (int)ceil_div(blocks[1], (int64_t)per_group);
+  const RowArgs a{c.r.ids, c.X, c.Y, c.A, c.B, c.scaling, c.out, c.r.L, c.N, c.K, c.rows, c.end0, c.end1, per_group, (int)groups(per_group), groups0, groups1};
+  low_rank_row_kernel<T, TO, RANK><<<(unsigned)(c.r.M * groups(per_group)), 64 * kRowWaves, 0, st>>>(a);
+  return check_launch("tlq_low_rank_update", "low_rank_row_kernel") ? 0 : 1;
+}
+template <typename T, typename TO>
+int run_rows(const Call& c, hipStream_t st) {
+  switch (c.rank) {
+    case 8: return run_rows<T, TO, 8>(c, st);
+    case 16: return run_rows<T, TO, 16>(c, st);
+    case 32: return run_rows<T, TO, 32>(c, st);
+    case 64: return run_rows<T, TO, 64>(c, st);
+    default: return run_rows<T, TO, 128>(c, st);
+  }
+}
+
 template <typename T, typename TO>
 int run_low_rank(Call c, hipStream_t st) {
+  if (single_rows(c.r.M, c.rank, c.K, c.N)) return run_rows<T, TO>(c, st);
   const int tile_rows = tile_rows_of(c.r.M, c.r.L, c.rank);
   const int64_t tiles = most_tiles(c.r.M, c.r.L, tile_rows);
   int64_t parts = 1;
