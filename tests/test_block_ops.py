@@ -341,6 +341,11 @@ UPDATES = [
     # (single rows: every rank, runs of more than one block, K that ends inside of a stage)
     (1, 2, 64, (2000,), 2048, "spread"), (1, 3, 128, (48, 4096, 16), 992, "holes"), (16, 16, 32, (4112, 32), 1120, "spread"), (2, 2, 32, (22016, 16), 4096, "runs"), (600, 40, 8, (16, 1040), 736, "holes"),
     (64, 5, 8, (8208, 48), 2080, "spread"), (9, 2, 8, (528,), 16384, "spread"),
+    # (longer rows, for tiles again)
+    (1, 1, 8, (16,), 32800, "one"), (3, 2, 64, (80, 16, 32), 4128, "holes"), (17, 1, 16, (112,), 16416, "one"), (33, 40, 8, (256, 64, 64), 32800, "spread"), (64, 1, 32, (48,), 8224, "one"),
+    (63, 9, 128, (96, 32), 2080, "spread"), (40, 3, 16, (16,), 16416, "none"), (5, 300, 32, (32,), 8224, "spread"), (100, 100, 16, (208,), 16416, "spread"), (700, 600, 64, (32,), 352, "spread"),
+    # (single rows that have more than four blocks of outputs each)
+    (60, 7, 16, (22016,), 96, "holes"), (4096, 9, 8, (272,), 64, "spread"), (200, 3, 32, (2048, 48), 1504, "runs"),
 ]
 
 
@@ -378,7 +383,7 @@ def test_update_many_rows(M, L, rank, parts, K, kind):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,rank,K", [(4, 16, 128), (70, 16, 128), (400, 16, 128), (4, 32, 4128), (70, 32, 4128), (800, 64, 2080)])
+@pytest.mark.parametrize("M,rank,K", [(4, 16, 128), (70, 16, 128), (400, 16, 128), (4, 32, 4128), (70, 32, 4128), (800, 64, 2080), (4, 32, 8224), (70, 32, 8224), (900, 64, 4128)])
 def test_update_large_and_small_values(M, rank, K, dtype):
     """First sums far outside float16's range, and far below its normal numbers, that the second product brings back."""
     parts, L = (64,), 3
@@ -397,7 +402,7 @@ def test_update_large_and_small_values(M, rank, K, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("M,rank,K", [(300, 16, 512), (300, 64, 2080), (420, 128, 1056), (60, 32, 4128)])
+@pytest.mark.parametrize("M,rank,K", [(300, 16, 512), (300, 64, 2080), (420, 128, 1056), (60, 32, 4128), (300, 64, 4128), (60, 32, 8224)])
 def test_update_rows_do_not_depend_on_each_other(M, rank, K):
     """A row alone, in a small batch, in a large one, beside rows of NaN: the values that it has by itself, but for sums formed in another order."""
     L, parts = 6, (96, 32)
@@ -435,7 +440,7 @@ def test_update_of_no_row():
 
 
 @gpu
-@pytest.mark.parametrize("M,rank,K", [(20, 32, 256), (400, 32, 256), (20, 32, 4128), (900, 64, 288)])
+@pytest.mark.parametrize("M,rank,K", [(20, 32, 256), (400, 32, 256), (20, 32, 4128), (900, 64, 288), (20, 32, 8224), (400, 32, 8224)])
 def test_update_in_place_and_nothing_beside_its_outputs(M, rank, K):
     L, parts = 4, (80, 16)
     N = sum(parts)
@@ -455,7 +460,7 @@ def test_update_in_place_and_nothing_beside_its_outputs(M, rank, K):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,times", [(5, 0), (90, 0), (5, 1), (90, 1)])
+@pytest.mark.parametrize("M,times", [(5, 0), (90, 0), (5, 1), (90, 1), (5, 3), (90, 3)])
 def test_update_infinities_stay_infinities(M, times, dtype):
     """An infinity among the activations, beside weights of one sign: the row is infinite, the others are what they were."""
     K = 64 + times * 8160  # (the longer rows: for tiles)
@@ -577,7 +582,7 @@ def block_inputs(M, hidden, L, dtype, seed):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,rank", [(1, 16), (21, 16), (300, 16), (21, 128), (300, 128), (500, 128)])
+@pytest.mark.parametrize("M,rank", [(1, 16), (21, 16), (300, 16), (21, 128), (60, 128), (300, 128), (500, 128)])
 def test_a_block_of_them(M, rank, dtype):
     steps, check = make_block(M, 256, 384, 5, rank, dtype, 1)
     x, r, ids = block_inputs(M, 256, 5, dtype, 2)
@@ -585,7 +590,7 @@ def test_a_block_of_them(M, rank, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("M,rank", [(4, 16), (300, 16), (21, 128), (500, 128)])
+@pytest.mark.parametrize("M,rank", [(4, 16), (300, 16), (21, 128), (60, 128), (500, 128)])
 def test_a_block_captured_and_replayed(M, rank):
     """Two graphs of the same weights, with eager calls between their replays and new inputs for each."""
     steps, _ = make_block(M, 256, 384, 5, rank, "bfloat16", 1)

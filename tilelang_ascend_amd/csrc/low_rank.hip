@@ -181,7 +181,7 @@ struct DownPlace {
 // Tiles of 16 rows, or a tile of 64 in four runs, x 16 rows of A on one part of K: eight wavefronts take stages of 64 values (128 bytes, a cache line, of a row) in turn, each with a ring
 // of its own in LDS, which it fills two stages ahead, eight lanes a line, and nobody else looks at; the wavefronts' sums meet at the end.  Operands read
 // straight from memory -- 16 neighbouring lanes, 16 rows -- go through the cache at a quarter of its rate (13 bytes a clock and CU).  Whole calls, us, that
-// way / this: 1 row of rank 16, K = 11008, 9.1 / 7.7, 64 rows of 48 adapters, three projections 14.1 / 11.3, 512 rows of 128 21.2 / 18.4, 259
+// way / this: 512 rows of 128 21.2 / 18.4, 259
 // rows of 32 of rank 64 on 2 x 11008 44.1 / 41.2; four wavefronts, or four stages ahead: level to 0.2 behind.
 constexpr int kDownWaves = 8, kDownStep = 64 * kDownWaves;
 template <typename T>
@@ -506,14 +506,15 @@ __device__ __forceinline__ float value8(const uint4_t& v, int k) {
 }
 
 // A row and blocks of 4096 / RANK outputs of one part of the outputs a work-group, which forms the part's RANK values of h for itself: CL lanes have a run of
-// 8 CL values of each of H rows of A, the wavefronts take K in turn, and their sums meet in LDS; X, A and the first block's B and Y are asked for at once.
+// 8 CL values of each of H rows of A, the wavefronts take K in turn, and their sums meet in LDS; X, A and the first four blocks' B and Y are asked for at once.
 // Bounded by latency and by A through the CU (rank 16, K = 4096: 128 KB, about 1 us of 3.9).  More code costs more than loads it has in flight: a row of rank 8,
 // K = 4096, with 8 / 16 / 32 loads of A at a time 3.3 / 3.9 / 5.3 us; sixteen wavefronts 4.6.  CL = 16 reads X less often, 8 has fewer sums a lane, us, 16 / 8: rank
-// 32 5.9 / 5.1, 64 10.6 / 7.9, 8 on K = 11008 4.7 / 5.2.
+// 32 5.9 / 5.1, 64 10.6 / 7.9, 8 on K = 11008 4.7 / 5.2.  One / two / four / eight blocks at a time: 16 rows of rank 16 on 22016 outputs 9.7 / 8.0 / 7.4 / 7.2, 64 of
+// 48 adapters on 6144 11.0 / 9.2 / 8.6 / 8.5, 16 of rank 32 on 14336 11.8 / 10.1 / 9.4 / 10.5.
 constexpr int kRowWaves = 8;
 template <typename T, typename TO, int RANK>
 __global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowArgs a) {
-  constexpr int WAVES = kRowWaves, CL = RANK >= 32 ? 8 : 16, LINES = 64 / CL, STAGE = CL * 8, H = RANK / LINES, AHEAD = H >= 8 ? 1 : 8 / H;
+  constexpr int WAVES = kRowWaves, CL = RANK >= 32 ? 8 : 16, LINES = 64 / CL, STAGE = CL * 8, H = RANK / LINES, AHEAD = H >= 8 ? 1 : 8 / H, BLOCKS = 4;
   constexpr int C = RANK / 8, OUT = 64 * WAVES / C;  // chunks of a row of B, outputs of a block
   __shared__ float4_t sums[WAVES][RANK / 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -530,12 +531,16 @@ __global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowA
   }
   const uint4_t* const b_row = (const uint4_t*)((const T*)a.B + ((int64_t)adapter * a.N + first) * RANK);
   const int place = tid % C;
-  uint4_t b;
-  TO y;
+  uint4_t b[BLOCKS];
+  TO y[BLOCKS];
   const auto load = [&](int n0) __attribute__((always_inline)) {
-    int n = n0 + tid / C;
-    n = n < n_end ? n : n_end - 1;
-    b = b_row[(int64_t)n * C + place], y = y_row[n];
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      if (n0 + u * OUT >= n_end) break;
+      int n = n0 + u * OUT + tid / C;
+      n = n < n_end ? n : n_end - 1;
+      b[u] = b_row[(int64_t)n * C + place], y[u] = y_row[n];
+    }
   };
   load(0);
   const float scale = a.scaling[adapter];
@@ -586,21 +591,24 @@ __global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowA
   float4_t low = sums[0][place * 2], high = sums[0][place * 2 + 1];
 #pragma unroll
   for (int v = 1; v < WAVES; ++v) low += sums[v][place * 2], high += sums[v][place * 2 + 1];
-  for (int n0 = 0; n0 < n_end; n0 += OUT) {
-    float f = 0.0f;
+  for (int n0 = 0; n0 < n_end; n0 += BLOCKS * OUT) {
+    if (n0 > 0) load(n0);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) f = __builtin_fmaf(value8<T>(b, k), low[k], f);
+    for (int u = 0; u < BLOCKS; ++u) {
+      if (n0 + u * OUT >= n_end) break;
+      float f = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) f = __builtin_fmaf(value8<T>(b, 4 + k), high[k], f);
-    const TO from = y;
-    if (n0 + OUT < n_end) load(n0 + OUT);
+      for (int k = 0; k < 4; ++k) f = __builtin_fmaf(value8<T>(b[u], k), low[k], f);
 #pragma unroll
-    for (int o = 1; o < C; o *= 2) f += __shfl_xor(f, o);
-    const int n = n0 + tid / C;
-    if (place == 0 && n < n_end) {
-      if constexpr (sizeof(TO) == 4) out_row[n] = __builtin_fmaf(scale, f, from);
-      else if constexpr (std::is_same<TO, half_t>::value) out_row[n] = (half_t)__builtin_fmaf(scale, f, (float)from);
-      else ((uint16_t*)out_row)[n] = (uint16_t)pack_bf16x2(__builtin_fmaf(scale, f, bitcast<float>((uint32_t)bitcast<uint16_t>(from) << 16)), 0.0f);
+      for (int k = 0; k < 4; ++k) f = __builtin_fmaf(value8<T>(b[u], 4 + k), high[k], f);
+#pragma unroll
+      for (int o = 1; o < C; o *= 2) f += __shfl_xor(f, o);
+      const int n = n0 + u * OUT + tid / C;
+      if (place == 0 && n < n_end) {
+        if constexpr (sizeof(TO) == 4) out_row[n] = __builtin_fmaf(scale, f, y[u]);
+        else if constexpr (std::is_same<TO, half_t>::value) out_row[n] = (half_t)__builtin_fmaf(scale, f, (float)y[u]);
+        else ((uint16_t*)out_row)[n] = (uint16_t)pack_bf16x2(__builtin_fmaf(scale, f, bitcast<float>((uint32_t)bitcast<uint16_t>(y[u]) << 16)), 0.0f);
+      }
     }
   }
 }
@@ -634,15 +642,16 @@ int64_t sum_rows(int64_t M, int64_t K) {
 }
 static_assert(16 * kFewGroups <= 64 * kTileGroups, "sum_rows holds for both");
 
-// Single rows where it is not too much that all work-groups of a row read its part of A (2 rank K bytes; there are N rank / 4096 of them): neither a plan nor a
-// second launch.  Whole calls, us, with them / this, bf16: 1 row of rank 16, K = N = 4096, 7.0 / 3.9, 16 rows 8.0 / 4.5, 32 of as many adapters 7.8 / 8.0; 64, K =
-// 11008, N = 22016, 17.6 / 27.0; 1 row of rank 64, N = 4096, 9.1 / 8.4, N = 22016 9.1 / 10.0, two of K = 11008 10.2 / 18.7; rank 8, K = N = 4096, 64 rows of as many
-// adapters 8.5 / 5.9, 128 11.8 / 6.8, 192 on 14336 outputs 13.9 / 15.4; 1 row of rank 128, K = 1024, 9.9 / 8.2; 2500 rows of rank 16, 64 -> 256, 11.3 / 7.4; rank 8, 5000,
-// 256 -> 256, 15.6 / 15.6, 10000, 64 -> 256, 21.0 / 22.3.
+// Single rows where it is not too much that all work-groups of a row read its part of A (2 rank K bytes; there are up to N rank / 4096 of them) and all rows their
+// adapter's B, which tiles share: neither a plan nor a second launch.  Whole calls, us, with them / this: 1 row of rank 16, K = N = 4096, 7.0 / 3.9; rank 64, K
+// = 4096 9.1 / 8.5, K = 11008 10.2 / 18.7.  Rank 16, 16 rows 8.0 / 5.1, 64 of 48 adapters on 6144 outputs 10.0 / 8.6, 52 of 200, K = 4352, on 19056 16.1 / 15.4, 47 of one
+// on 22224 10.6 / 12.5; rank 32, 22 on 9600 9.1 / 9.4, K = 2976, 27 on 16640 8.9 / 11.0; rank 8, K = 8000, 336 on 21104 28.9 / 27.4, 753 on 15248 24.4 / 21.6, K = 1568,
+// 1977 on 13536 44.0 / 65.5; rank 16, K = 736, 219 on 18352 14.2 / 20.9; rank 128, K = 768, 2 on 5456 9.8 / 7.5, K = 1312, 5 on 2384 11.5 / 11.6; rank 8, 256 -> 256,
+// 5000 15.6 / 15.6, 64 -> 256, 10000 21.0 / 22.3.  (730 sizes: 1.32 times as fast as without, the better of the two 1.34.)
 inline bool single_rows(int64_t M, int64_t rank, int64_t K, int64_t N) {
-  return M <= 4096 && rank * K <= (int64_t)1 << 17 && M * rank * rank * (4 * K + N) <= (M <= kInlineRows ? (int64_t)2 << 27 : (int64_t)3 << 27);
+  return M <= 4096 && rank * K <= (int64_t)1 << 18 && M * rank * rank * (K + N) <= (int64_t)(M <= kInlineRows ? 3 : 6) << 27;
 }
-// (512: 16 rows of rank 32 on 14336 outputs 15.2 us, 256 10.5; 128: 64 rows of rank 16, three projections, 12.3, 256 9.7)
+// (384 / 256 / 192: rank 16, 64 rows of 48 adapters on 6144 outputs 10.6 / 8.6 / 8.5 us, of one on 14336 7.2 / 7.2 / 9.4, 8 on 22016 6.7 / 5.3 / 5.5)
 constexpr int kRowGroups = 256;
 
 struct Call {
