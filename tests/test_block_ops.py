@@ -345,7 +345,7 @@ UPDATES = [
     (1, 1, 8, (16,), 32800, "one"), (3, 2, 64, (80, 16, 32), 4128, "holes"), (17, 1, 16, (112,), 16416, "one"), (33, 40, 8, (256, 64, 64), 32800, "spread"), (64, 1, 32, (48,), 8224, "one"),
     (63, 9, 128, (96, 32), 2080, "spread"), (40, 3, 16, (16,), 16416, "none"), (5, 300, 32, (32,), 8224, "spread"), (100, 100, 16, (208,), 16416, "spread"), (700, 600, 64, (32,), 352, "spread"),
     # (single rows that have more than four blocks of outputs each)
-    (60, 7, 16, (22016,), 96, "holes"), (4096, 9, 8, (272,), 64, "spread"), (200, 3, 32, (2048, 48), 1504, "runs"),
+    (60, 7, 16, (22016,), 96, "holes"), (4096, 9, 8, (272,), 64, "spread"), (200, 3, 32, (2048, 48), 1504, "runs"), (2, 2, 64, (4112, 16), 1952, "holes"),
 ]
 
 

@@ -178,11 +178,10 @@ struct DownPlace {
   }
 };
 
-// Tiles of 16 rows, or a tile of 64 in four runs, x 16 rows of A on one part of K: eight wavefronts take stages of 64 values (128 bytes, a cache line, of a row) in turn, each with a ring
-// of its own in LDS, which it fills two stages ahead, eight lanes a line, and nobody else looks at; the wavefronts' sums meet at the end.  Operands read
+// Tiles of 16 rows, or a tile of 64 in four runs, x 16 rows of A on one part of K: eight wavefronts take stages of 64 values (128 bytes, a cache line, of a row) in
+// turn, each with a ring of its own in LDS, which it fills two stages ahead, eight lanes a line, and nobody else looks at; the wavefronts' sums meet at the end.  Operands read
 // straight from memory -- 16 neighbouring lanes, 16 rows -- go through the cache at a quarter of its rate (13 bytes a clock and CU).  Whole calls, us, that
-// way / this: 512 rows of 128 21.2 / 18.4, 259
-// rows of 32 of rank 64 on 2 x 11008 44.1 / 41.2; four wavefronts, or four stages ahead: level to 0.2 behind.
+// way / this: 512 rows of 128 adapters 21.2 / 18.4, 259 of 32 of rank 64 on 2 x 11008 44.1 / 41.2; four wavefronts, or four stages ahead: level to 0.2 behind.
 constexpr int kDownWaves = 8, kDownStep = 64 * kDownWaves;
 template <typename T>
 __global__ __launch_bounds__(64 * kDownWaves) void low_rank_down_kernel(const DownArgs a) {
@@ -398,24 +397,26 @@ __global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(
         const float* s = a.sums + (int64_t)tile.row(a.r, rw * 16 + r16) * a.rows + p * RANK + q * 8;
         const int64_t step = (int64_t)a.r.M * a.rows;
 #pragma unroll
-        for (int c = 0; c < RB; ++c) {
+        for (int c = 0; c < RB; ++c)
 #pragma unroll
           for (int k = 0; k < 8; ++k) h[c][k] = 0.0f;
-          if (RANK >= 32 || q < C) {
-            constexpr int ONCE = RB == 1 ? 8 : 4;  // parts that are asked for at once
-            for (int part = 0; part < a.parts; part += ONCE) {
-              float4_t u[ONCE], v[ONCE];
+        if (RANK >= 32 || q < C) {
+          constexpr int ONCE = RB == 1 ? 8 : 2;  // parts that are asked for at once
+          for (int part = 0; part < a.parts; part += ONCE) {
+            float4_t u[ONCE][RB], v[ONCE][RB];
 #pragma unroll
-              for (int o = 0; o < ONCE; ++o) {
-                const float* const from = s + (part + o < a.parts ? part + o : part) * step + c * 32;
-                u[o] = *(const float4_t*)from, v[o] = *(const float4_t*)(from + 4);
-              }
+            for (int o = 0; o < ONCE; ++o) {
+              const float* const from = s + (part + o < a.parts ? part + o : part) * step;
 #pragma unroll
-              for (int o = 0; o < ONCE; ++o) {
-                if (part + o >= a.parts) break;
+              for (int c = 0; c < RB; ++c) u[o][c] = *(const float4_t*)(from + c * 32), v[o][c] = *(const float4_t*)(from + c * 32 + 4);
+            }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) h[c][k] += u[o][k], h[c][4 + k] += v[o][k];
-              }
+            for (int o = 0; o < ONCE; ++o) {
+              if (part + o >= a.parts) break;
+#pragma unroll
+              for (int c = 0; c < RB; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h[c][k] += u[o][c][k], h[c][4 + k] += v[o][c][k];
             }
           }
         }
@@ -509,12 +510,13 @@ __device__ __forceinline__ float value8(const uint4_t& v, int k) {
 // 8 CL values of each of H rows of A, the wavefronts take K in turn, and their sums meet in LDS; X, A and the first four blocks' B and Y are asked for at once.
 // Bounded by latency and by A through the CU (rank 16, K = 4096: 128 KB, about 1 us of 3.9).  More code costs more than loads it has in flight: a row of rank 8,
 // K = 4096, with 8 / 16 / 32 loads of A at a time 3.3 / 3.9 / 5.3 us; sixteen wavefronts 4.6.  CL = 16 reads X less often, 8 has fewer sums a lane, us, 16 / 8: rank
-// 32 5.9 / 5.1, 64 10.6 / 7.9, 8 on K = 11008 4.7 / 5.2.  One / two / four / eight blocks at a time: 16 rows of rank 16 on 22016 outputs 9.7 / 8.0 / 7.4 / 7.2, 64 of
+// 32 5.9 / 5.1, 64 10.6 / 7.9, 8, K = 11008, 4.7 / 5.2.  One / two / four / eight blocks at a time: 16 rows of rank 16 on 22016 outputs 9.7 / 8.0 / 7.4 / 7.2, 64 of
 // 48 adapters on 6144 11.0 / 9.2 / 8.6 / 8.5, 16 of rank 32 on 14336 11.8 / 10.1 / 9.4 / 10.5.
 constexpr int kRowWaves = 8;
 template <typename T, typename TO, int RANK>
 __global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowArgs a) {
-  constexpr int WAVES = kRowWaves, CL = RANK >= 32 ? 8 : 16, LINES = 64 / CL, STAGE = CL * 8, H = RANK / LINES, AHEAD = H >= 8 ? 1 : 8 / H, BLOCKS = 4;
+  constexpr int WAVES = kRowWaves, CL = RANK >= 32 ? 8 : 16, LINES = 64 / CL, STAGE = CL * 8, H = RANK / LINES, AHEAD = 8 / H, BLOCKS = 4;
+  static_assert(H <= 8 && H <= CL, "the sums of a run of lanes end as one a lane");
   constexpr int C = RANK / 8, OUT = 64 * WAVES / C;  // chunks of a row of B, outputs of a block
   __shared__ float4_t sums[WAVES][RANK / 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -584,9 +586,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowA
       h[0] += __shfl_xor(h[0], o);
     }
   }
-  constexpr int KEPT = H > CL ? H / CL : 1;
-#pragma unroll
-  for (int j = 0; j < KEPT; ++j) ((float*)sums[wave])[(at + j) * LINES + line] = h[j];
+  ((float*)sums[wave])[at * LINES + line] = h[0];
   __syncthreads();
   float4_t low = sums[0][place * 2], high = sums[0][place * 2 + 1];
 #pragma unroll
@@ -628,7 +628,8 @@ inline int64_t most_tiles(int64_t M, int64_t L, int tile_rows) { return M <= kIn
 int64_t plan_bytes(int64_t M, int64_t L) { return M <= kInlineRows ? 0 : align256((tiles_at(M) + 4 * most_tiles(M, L, 16)) * 4); }
 // Parts of K: work-groups for the machine where there are few tiles (`want` of them), at most 16, or 4 for tiles of 16 rows, whose eight wavefronts share K
 // already.  Every part costs a sum written and read: tiles of 64 rows: 8192 rows of rank 32 on 14336 outputs 136 us in one part, 139 in four, 145 in seven;
-// 2048 of rank 16, three projections, 31.2 for 128 work-groups, 33.4 for 256; tiles of 16: 1 row, K = 11008, 7.7 in four parts, 8.2 in sixteen.
+// 2048 of rank 16, three projections, 31.2 for 128 work-groups, 33.4 for 256; tiles of 16: 1 row of rank 32, K = 11008, 8.8 in two, 8.5 in
+// four, 9.1 in eight, 9.7 in sixteen; 8 rows of rank 16, K = 28672, 13.2, 10.8, 10.5, 11.7.
 // With more than M / 64 (M / 16) tiles, parts * M is less than 64 * kTileGroups + M (16 * kFewGroups + M).
 constexpr int kTileGroups = 128, kFewGroups = 192, kFewParts = 4;
 int64_t most_parts(int64_t K, int64_t most = 16) { return K >= 256 * most ? most : (K + 255) / 256; }
@@ -643,15 +644,16 @@ int64_t sum_rows(int64_t M, int64_t K) {
 static_assert(16 * kFewGroups <= 64 * kTileGroups, "sum_rows holds for both");
 
 // Single rows where it is not too much that all work-groups of a row read its part of A (2 rank K bytes; there are up to N rank / 4096 of them) and all rows their
-// adapter's B, which tiles share: neither a plan nor a second launch.  Whole calls, us, with them / this: 1 row of rank 16, K = N = 4096, 7.0 / 3.9; rank 64, K
-// = 4096 9.1 / 8.5, K = 11008 10.2 / 18.7.  Rank 16, 16 rows 8.0 / 5.1, 64 of 48 adapters on 6144 outputs 10.0 / 8.6, 52 of 200, K = 4352, on 19056 16.1 / 15.4, 47 of one
-// on 22224 10.6 / 12.5; rank 32, 22 on 9600 9.1 / 9.4, K = 2976, 27 on 16640 8.9 / 11.0; rank 8, K = 8000, 336 on 21104 28.9 / 27.4, 753 on 15248 24.4 / 21.6, K = 1568,
-// 1977 on 13536 44.0 / 65.5; rank 16, K = 736, 219 on 18352 14.2 / 20.9; rank 128, K = 768, 2 on 5456 9.8 / 7.5, K = 1312, 5 on 2384 11.5 / 11.6; rank 8, 256 -> 256,
-// 5000 15.6 / 15.6, 64 -> 256, 10000 21.0 / 22.3.  (730 sizes: 1.32 times as fast as without, the better of the two 1.34.)
+// adapter's B, which tiles share: neither a plan nor a second launch.  Whole calls, us, with them / this.  Rank 16: K = N = 4096, 1 row 7.0 / 3.9, 16 8.0 / 5.1; 64 of 48
+// adapters on 6144 outputs 10.0 / 8.4, 52 of 200, K = 4352, on 19056 16.1 / 15.4, 47 of one on 22224 10.6 / 12.5; K = 736, 219 on 18352 14.2 / 20.9.  Rank 32: 22, K = 4672,
+// on 9600 9.1 / 9.4, 27, K = 2976, on 16640 8.9 / 11.0.  Rank 64: 1 row, K = 2080, 7.4 / 6.0, 4, K = 1184, on 16832 7.8 / 7.8, K = 3392 8.5 / 10.2, 8, K = 3424,
+// on 784 8.2 / 10.9.  Rank 128: 4, K = 512, on 2224 8.4 / 7.3, 2, K = 1312, on 2528 8.6 / 9.2: left to tiles.  Rank 8: K = 8000, 336 on 21104 28.9 / 27.4, K = 7360,
+// 753 on 15248 24.4 / 21.6, K = 1568, 1977 on 13536 44.0 / 65.5; 256 -> 256, 5000 15.6 / 15.6, 64 -> 256, 10000 21.0 / 22.3.
 inline bool single_rows(int64_t M, int64_t rank, int64_t K, int64_t N) {
-  return M <= 4096 && rank * K <= (int64_t)1 << 18 && M * rank * rank * (K + N) <= (int64_t)(M <= kInlineRows ? 3 : 6) << 27;
+  return M <= 4096 && rank <= 64 && rank * K <= (int64_t)1 << 18 && rank * rank * K <= (int64_t)1 << 23 &&
+         M * rank * rank * (K + N) <= (int64_t)(M <= kInlineRows ? 3 : 6) << 27;
 }
-// (384 / 256 / 192: rank 16, 64 rows of 48 adapters on 6144 outputs 10.6 / 8.6 / 8.5 us, of one on 14336 7.2 / 7.2 / 9.4, 8 on 22016 6.7 / 5.3 / 5.5)
+// (384 / 256 / 192: rank 16, 64 rows of 48 adapters on 6144 outputs 10.6 / 8.6 / 8.5, of one on 14336 7.2 / 7.2 / 9.4, 8 on 22016 6.7 / 5.3 / 5.5)
 constexpr int kRowGroups = 256;
 
 struct Call {
@@ -722,8 +724,7 @@ int run_rows(const Call& c, hipStream_t st) {
     case 8: return run_rows<T, TO, 8>(c, st);
     case 16: return run_rows<T, TO, 16>(c, st);
     case 32: return run_rows<T, TO, 32>(c, st);
-    case 64: return run_rows<T, TO, 64>(c, st);
-    default: return run_rows<T, TO, 128>(c, st);
+    default: return run_rows<T, TO, 64>(c, st);
   }
 }
 
