@@ -74,10 +74,11 @@ for M, L, rank, parts, K in cases:
         name, g, threads, data = got[0]
         x, y, a, b = struct.unpack("QQQQ", data[8:40])
         l, n, k, r, end0, end1, per_group, all_groups, groups0, groups1 = struct.unpack("iiiiiiiiii", data[56:96])
+        assert struct.unpack("i", data[96:100]) == (M,), what
         assert "low_rank_row_kernel" in name and (x, y, a, b) == (X, Y, A, B) and (l, n, k, r, end0, end1) == (L, N, K, rows, parts[0], sum(parts[:2])), what
         outputs = 512 * 8 // rank * per_group
         need = [-(-n // outputs) for n in parts] + [0, 0]
-        assert threads == 512 and g[0] == M * all_groups and (groups0, groups1 - groups0, all_groups - groups1) == tuple(need[:3]) and 512 * per_group < 2**31, what
+        assert threads == 512 and g[0] == (M if M < 8 else -(-M // 8) * 8) * all_groups and (groups0, groups1 - groups0, all_groups - groups1) == tuple(need[:3]) and 512 * per_group < 2**31, what
         result.add((1, 0, False))
         continue
     assert len(got) == (2 if M <= 64 else 3), what

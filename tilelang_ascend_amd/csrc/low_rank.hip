@@ -498,7 +498,7 @@ struct RowArgs {
   const float* scaling;
   void* out;
   int L, N, K, rows, end0, end1;  // as above
-  int per_group, groups, groups0, groups1;
+  int per_group, groups, groups0, groups1, M;
 };
 template <typename T>
 __device__ __forceinline__ float value8(const uint4_t& v, int k) {
@@ -510,9 +510,12 @@ __device__ __forceinline__ float value8(const uint4_t& v, int k) {
 // 8 CL values of each of H rows of A, the wavefronts take K in turn, and their sums meet in LDS; X, A and the first four blocks' B and Y are asked for at once.
 // Bounded by latency and by A through the CU (rank 16, K = 4096: 128 KB, about 1 us of 3.9).  More code costs more than loads it has in flight: a row of rank 8,
 // K = 4096, with 8 / 16 / 32 loads of A at a time 3.3 / 3.9 / 5.3 us; sixteen wavefronts 4.6.  CL = 16 reads X less often, 8 has fewer sums a lane, us, 16 / 8: rank
-// 32 5.9 / 5.1, 64 10.6 / 7.9, 8, K = 11008, 4.7 / 5.2.  One / two / four / eight blocks at a time: 16 rows of rank 16 on 22016 outputs 9.7 / 8.0 / 7.4 / 7.2, 64 of
-// 48 adapters on 6144 11.0 / 9.2 / 8.6 / 8.5, 16 of rank 32 on 14336 11.8 / 10.1 / 9.4 / 10.5.
+// 32 5.9 / 5.1, 64 10.6 / 7.9, 8, K = 11008, 4.7 / 5.2.  One / two / four / eight blocks at a time (work-groups spread over the XCDs): 16 rows of
+// rank 16 on 22016 outputs 9.7 / 8.0 / 7.4 / 7.2, 64 of 48 adapters on 6144 11.0 / 9.2 / 8.6 / 8.5, 16 of rank 32 on 14336 11.8 / 10.1 / 9.4 / 10.5.
 constexpr int kRowWaves = 8;
+// From so many rows on a row's work-groups go to one XCD, whose L2 reads the row's A once; fewer would leave XCDs without work.  Spread / together, us, rank 16, K = 4096:
+// 4 rows on 22016 outputs 4.2 / 6.0, 8 5.3 / 4.8, 8 on 4096 4.0 / 4.2, 32 7.0 / 5.0, 64 of 48 adapters on 6144 8.5 / 7.3; rank 8, K = 11008, 64 9.5 / 6.2.
+constexpr int kTogether = 8;
 template <typename T, typename TO, int RANK>
 __global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowArgs a) {
   constexpr int WAVES = kRowWaves, CL = RANK >= 32 ? 8 : 16, LINES = 64 / CL, STAGE = CL * 8, H = RANK / LINES, AHEAD = 8 / H, BLOCKS = 4;
@@ -520,7 +523,12 @@ __global__ __launch_bounds__(64 * kRowWaves) void low_rank_row_kernel(const RowA
   constexpr int C = RANK / 8, OUT = 64 * WAVES / C;  // chunks of a row of B, outputs of a block
   __shared__ float4_t sums[WAVES][RANK / 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = blockIdx.x / a.groups, no = blockIdx.x - row * a.groups;
+  int row = blockIdx.x / a.groups, no = blockIdx.x - row * a.groups;
+  if (a.M >= kTogether) {
+    const DownPlace at(blockIdx.x, a.groups);
+    row = at.tile, no = at.group;
+    if (row >= a.M) return;
+  }
   const int p = (no >= a.groups0) + (no >= a.groups1), begin = p == 0 ? 0 : p == 1 ? a.end0 : a.end1, end = p == 0 ? a.end0 : p == 1 ? a.end1 : a.N;
   const int first = begin + (no - (p == 0 ? 0 : p == 1 ? a.groups0 : a.groups1)) * a.per_group * OUT, n_end = end - first < a.per_group * OUT ? end - first : a.per_group * OUT;
   const int adapter = a.ids[row];
@@ -644,16 +652,16 @@ int64_t sum_rows(int64_t M, int64_t K) {
 static_assert(16 * kFewGroups <= 64 * kTileGroups, "sum_rows holds for both");
 
 // Single rows where it is not too much that all work-groups of a row read its part of A (2 rank K bytes; there are up to N rank / 4096 of them) and all rows their
-// adapter's B, which tiles share: neither a plan nor a second launch.  Whole calls, us, with them / this.  Rank 16: K = N = 4096, 1 row 7.0 / 3.9, 16 8.0 / 5.1; 64 of 48
-// adapters on 6144 outputs 10.0 / 8.4, 52 of 200, K = 4352, on 19056 16.1 / 15.4, 47 of one on 22224 10.6 / 12.5; K = 736, 219 on 18352 14.2 / 20.9.  Rank 32: 22, K = 4672,
-// on 9600 9.1 / 9.4, 27, K = 2976, on 16640 8.9 / 11.0.  Rank 64: 1 row, K = 2080, 7.4 / 6.0, 4, K = 1184, on 16832 7.8 / 7.8, K = 3392 8.5 / 10.2, 8, K = 3424,
-// on 784 8.2 / 10.9.  Rank 128: 4, K = 512, on 2224 8.4 / 7.3, 2, K = 1312, on 2528 8.6 / 9.2: left to tiles.  Rank 8: K = 8000, 336 on 21104 28.9 / 27.4, K = 7360,
-// 753 on 15248 24.4 / 21.6, K = 1568, 1977 on 13536 44.0 / 65.5; 256 -> 256, 5000 15.6 / 15.6, 64 -> 256, 10000 21.0 / 22.3.
+// adapter's B, which tiles share: neither a plan nor a second launch.  Whole calls, us, with them / this.  Rank 16: K = N = 4096, 1 row 7.0 / 3.9, 16 8.0 / 4.5; 64 of 48
+// adapters on 6144 outputs 10.0 / 7.3, 52 of 200, K = 4352, on 19056 15.8 / 14.3, 47 of one on 22224 10.8 / 11.8; K = 736, 219 on 18352 14.2 / 20.8.  Rank 32: 22, K = 4672,
+// on 9600 9.3 / 9.4, 27, K = 2976, on 16640 9.6 / 13.4.  Rank 64: 1 row, K = 2080, 7.4 / 6.0, 4, K = 1184, on 16832 7.8 / 7.8, K = 3392 8.5 / 10.1, 8, K = 3424,
+// on 784 8.2 / 7.5.  Rank 128: 4, K = 512, on 2224 8.4 / 7.3, 2, K = 1312, on 2528 8.6 / 9.2: left to tiles.  Rank 8: K = 8000, 336 on 21104 28.9 / 27.4, K = 7360,
+// 753 on 15248 24.8 / 21.7, K = 1568, 1977 on 13536 44.7 / 65.3; 256 -> 256, 5000 15.6 / 15.6, 64 -> 256, 10000 21.0 / 22.3.
 inline bool single_rows(int64_t M, int64_t rank, int64_t K, int64_t N) {
   return M <= 4096 && rank <= 64 && rank * K <= (int64_t)1 << 18 && rank * rank * K <= (int64_t)1 << 23 &&
          M * rank * rank * (K + N) <= (int64_t)(M <= kInlineRows ? 3 : 6) << 27;
 }
-// (384 / 256 / 192: rank 16, 64 rows of 48 adapters on 6144 outputs 10.6 / 8.6 / 8.5, of one on 14336 7.2 / 7.2 / 9.4, 8 on 22016 6.7 / 5.3 / 5.5)
+// (384 / 256 / 192, spread over the XCDs: rank 16, 64 rows of 48 adapters on 6144 outputs 10.6 / 8.6 / 8.5, of one on 14336 7.2 / 7.2 / 9.4, 8 on 22016 6.7 / 5.3 / 5.5)
 constexpr int kRowGroups = 256;
 
 struct Call {
@@ -714,8 +722,8 @@ int run_rows(const Call& c, hipStream_t st) {
   int per_group = 1;
   while (c.r.M * groups(per_group) > kRowGroups && per_group < 1 << 20) per_group *= 2;
   const int groups0 = (int)ceil_div(blocks[0], (int64_t)per_group), groups1 = groups0 + (int)ceil_div(blocks[1], (int64_t)per_group);
-  const RowArgs a{c.r.ids, c.X, c.Y, c.A, c.B, c.scaling, c.out, c.r.L, c.N, c.K, c.rows, c.end0, c.end1, per_group, (int)groups(per_group), groups0, groups1};
-  low_rank_row_kernel<T, TO, RANK><<<(unsigned)(c.r.M * groups(per_group)), 64 * kRowWaves, 0, st>>>(a);
+  const RowArgs a{c.r.ids, c.X, c.Y, c.A, c.B, c.scaling, c.out, c.r.L, c.N, c.K, c.rows, c.end0, c.end1, per_group, (int)groups(per_group), groups0, groups1, c.r.M};
+  low_rank_row_kernel<T, TO, RANK><<<(unsigned)((c.r.M >= kTogether ? ceil_div(c.r.M, 8) * 8 : c.r.M) * groups(per_group)), 64 * kRowWaves, 0, st>>>(a);
   return check_launch("tlq_low_rank_update", "low_rank_row_kernel") ? 0 : 1;
 }
 template <typename T, typename TO>
