@@ -247,13 +247,14 @@ struct RowLoaderDirect {
   // outstanding the compiler turns every LDS wait into a wait for everything (it must assume the load
   // may also return through the LDS counter), which serialises the operand reads and LDS stores of the
   // whole stage.  The kernel waits for them by hand (wait_direct) before the barrier that publishes
-  // the buffer.
+  // the buffer.  Between the write of M0 and the load that reads it the hardware wants one wait state (s_nop), which the
+  // compiler inserts behind its builtins alone.
   __device__ __forceinline__ const uint8_t* stage_src(int kt) const { return uniform_ptr(base + (int64_t)kt * kStageBytes); }
   __device__ __forceinline__ uint32_t stage_dst(uint8_t* lds) const {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave_off);
   }
   __device__ __forceinline__ void load_one(int j, const uint8_t* src, uint32_t dst) const {  // of the PER_WAVE loads of a stage
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst + addr::direct_lds_off(0, 0, j, WAVES)), "v"(voff[j]), "s"(src)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(dst + addr::direct_lds_off(0, 0, j, WAVES)), "v"(voff[j]), "s"(src)
                  : "memory");
   }
   template <bool TAIL>
@@ -343,7 +344,7 @@ struct I8KNLoaderDirect {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave_off);
   }
   __device__ __forceinline__ void load_one(int j, const uint8_t* src, uint32_t dst) const {  // of the PER_WAVE loads of a stage
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst + addr::direct_lds_off(0, 0, j, WAVES)), "v"(voff[j]), "s"(src)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(dst + addr::direct_lds_off(0, 0, j, WAVES)), "v"(voff[j]), "s"(src)
                  : "memory");
   }
   template <bool TAIL>
@@ -417,7 +418,7 @@ struct H16KNLoaderDirect {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave_off);
   }
   __device__ __forceinline__ void load_one(int j, const uint8_t* src, uint32_t dst) const {  // of the PER_WAVE loads of a stage
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst + addr::direct_lds_off(0, 0, j, WAVES)), "v"(voff[j]), "s"(src)
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(dst + addr::direct_lds_off(0, 0, j, WAVES)), "v"(voff[j]), "s"(src)
                  : "memory");
   }
   template <bool TAIL>

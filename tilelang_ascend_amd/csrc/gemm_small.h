@@ -110,7 +110,7 @@ __global__ __launch_bounds__(RT* MT <= 4 ? 1024 : 512) void gemm_small_kernel(Sm
                   (uint32_t)(n_base * (W == kSmallKN8 ? 1 : 2));
   }
   auto dma16 = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   auto issue = [&](int s, int slot) {
     const uint8_t* asb = uniform_ptr(a_base + (int64_t)s * 128);

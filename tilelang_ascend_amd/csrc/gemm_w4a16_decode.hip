@@ -108,14 +108,14 @@ __global__ __launch_bounds__(1024) void w4a16_decode_kernel(const T* __restrict_
     const uint32_t sc_off = addr::dec_sc_off(last ? sc_e_last : sc_e0 + (int64_t)t * 16 * groups);
     const uint32_t so = has_s ? sc_off : 0u, zo = has_z ? sc_off : 0u;
     if (sc_lane) {
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(l0 + 2048u), "v"(so), "s"(s_src) : "memory");
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(l0 + 2304u), "v"(zo), "s"(z_src) : "memory");
+      asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(l0 + 2048u), "v"(so), "s"(s_src) : "memory");
+      asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(l0 + 2304u), "v"(zo), "s"(z_src) : "memory");
     }
     const uint8_t* wsb = uniform_ptr(Wp + addr::dec_w_base(t, K, k0));
     const uint32_t voff = last ? w_lane_last : w_lane;
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(l0), "v"(voff), "s"(wsb) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(l0), "v"(voff), "s"(wsb) : "memory");
     // the instruction offset moves the LDS side as well as the global side: M0 is set 64 bytes low to land on l0 + 1024
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 offset:64" ::"s"(l0 + 1024u - 64u), "v"(voff), "s"(wsb) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:64" ::"{m0}"(l0 + 1024u - 64u), "v"(voff), "s"(wsb) : "memory");
   };
 
   // ---- activations of this wavefront's K slice -> MFMA operands in registers ----
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(1024) void w4a16_decode_kernel(const T* __restrict_
         const uint32_t voff = (uint32_t)(addr::dec_a_off(lane, mt, kb, i, M, K, k0) - (k0 + kb * 128) * 2);
         // rows past M are not fetched: what the staging area holds for them only reaches output rows that are never stored
         if (mt * 16 + 4 * i + (lane >> 4) < M)
-          asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(mine_lds + STG + (uint32_t)(i * 1024)), "v"(voff), "s"(asb)
+          asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(mine_lds + STG + (uint32_t)(i * 1024)), "v"(voff), "s"(asb)
                        : "memory");
       }
     };

@@ -118,7 +118,7 @@ __global__ __launch_bounds__(512, 1) void w4a16_panel_kernel(const T* __restrict
   const uint8_t* const w_base = Wp + (int64_t)step0 * 64;
   const uint8_t* const a_base = (const uint8_t*)A + (int64_t)step0 * 256;
   auto dma16 = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   // the loads of step s of this slice into ring slot s % 2: the shared activation tile one step ahead of its use, the
   // wavefront's own packed weights two steps ahead (their slot is free once the words of step s - 2 have been read)

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256, 1) void w4a16_panelm_kernel(const T* __restric
   const uint8_t* const w_base = Wp + (int64_t)step0 * 64;
   const uint8_t* const a_base = (const uint8_t*)A + (int64_t)step0 * 256;
   auto dma16 = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   auto clamp_step = [&](int s) { return s < steps ? s : steps - 1; };  // past the end: the last step again, into a slot nobody reads
   auto a_src = [&](int s) { return uniform_ptr(a_base + (int64_t)clamp_step(s) * 256); };

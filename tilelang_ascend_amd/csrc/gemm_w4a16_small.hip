@@ -92,7 +92,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void w4a16_small_kernel(const
   for (int j = 0; j < 4; ++j) fo_a[j] = (uint32_t)(RT * 1024) + addr::sa_frag_off(lane, 0, j);
 
   auto dma16 = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   auto issue_kb = [&](int kb, int slot) {
     const uint8_t* wsb = uniform_ptr(Wp + (int64_t)kb * 64);
@@ -111,11 +111,11 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void w4a16_small_kernel(const
       const uint64_t e2 = addr::smallw_sc_elem(lane, base, row_g[rt], groups) * 2u;
       if (has_s) {
         const uint64_t a = ((uint64_t)(uintptr_t)scales + e2) & ~(uint64_t)3;
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(l0 + (rt * 2 + 0) * 256), "v"(a) : "memory");
+        asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(l0 + (rt * 2 + 0) * 256), "v"(a) : "memory");
       }
       if (has_z) {
         const uint64_t a = ((uint64_t)(uintptr_t)zeros + e2) & ~(uint64_t)3;
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(l0 + (rt * 2 + 1) * 256), "v"(a) : "memory");
+        asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(l0 + (rt * 2 + 1) * 256), "v"(a) : "memory");
       }
     }
   };

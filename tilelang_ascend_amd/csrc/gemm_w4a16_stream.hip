@@ -180,10 +180,10 @@ __global__ __launch_bounds__(512, 2) void w4a16_stream_kernel(const T* __restric
   const uint8_t* const w_base = Wp + (int64_t)step0 * 64;
   const uint8_t* const a_base = (const uint8_t*)A + (int64_t)step0 * 256;
   auto dma16 = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   auto dma4 = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   // load i (of L) of step s of this slice into ring slot `slot`: the activation tile's, then the packed weights'.  Loads of
   // steps past `end` are issued with no lane active: they move nothing, but every step is L loads and the loop has no branch
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(512, 2) void w4a16_stream_kernel(const T* __restric
     const uint8_t* const src = i < LA ? uniform_ptr(a_base + (int64_t)s * 256) : uniform_ptr(w_base + (int64_t)s * 64);
     const uint32_t from = voff[i];
     const int lanes = __builtin_amdgcn_readfirstlane((s - end) >> 31);  // -1 or 0
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
-                 ::"s"(l0), "v"(from), "s"(src), "s"(lanes)
+    asm volatile("s_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+                 ::"{m0}"(l0), "v"(from), "s"(src), "s"(lanes)
                  : "memory");
   };
 

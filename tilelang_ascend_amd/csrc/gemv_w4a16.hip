@@ -627,12 +627,12 @@ __global__ __launch_bounds__(1024) void gemv_w4a16_ring_kernel(const T* __restri
   const addr::RingLayout L = addr::ring_layout(nwaves, D, ITERS, K, rows_per_block, groups, MT);
   const bool has_s = scales != nullptr, has_z = zeros != nullptr;
   auto dma16 = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   // the packed weights are read once: non-temporal, so that they do not displace what the caches hold for later
   // (single launch of 22.5 MB: 6.46 instead of 7.18 us)
   auto dma16_once = [&](uint32_t lds_addr, uint32_t voff, const uint8_t* sbase) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_addr), "v"(voff), "s"(sbase) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"{m0}"(lds_addr), "v"(voff), "s"(sbase) : "memory");
   };
   auto wait_vm = [&](int outstanding) {  // a wavefront-uniform count, 0 .. ITERS * D
     static_assert(ITERS * D <= 6, "cases below");

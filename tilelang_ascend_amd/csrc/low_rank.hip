@@ -24,9 +24,10 @@ struct MmaOf<bf16_t> {
   typedef MmaBF16 type;
 };
 
-// Global -> LDS without registers: 16 bytes a lane, lane l's to lds + 16 l.
+// Global -> LDS without registers: 16 bytes a lane, lane l's to lds + 16 l.  (Between the write of M0 and the load that reads it
+// the hardware wants a wait state, which the compiler inserts behind its builtins alone: s_nop.)
 __device__ __forceinline__ void direct16(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(lds), "v"(src) : "memory");
 }
 typedef __attribute__((address_space(3))) uint8_t* lptr_t;
 __device__ __forceinline__ uint32_t lds_of(const void* p) { return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lptr_t)p); }

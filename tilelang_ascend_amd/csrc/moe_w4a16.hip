@@ -186,13 +186,13 @@ struct MmaOf<bf16_t> {
 
 // Global -> LDS without registers: 16 or 4 bytes per lane, lane l to lds + 16 l or 4 l (lanes that are switched off: nothing).
 __device__ __forceinline__ void direct16(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(lds), "v"(src) : "memory");
 }
 __device__ __forceinline__ void direct16_at(uint32_t off, const uint8_t* base, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void direct4(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(lds), "v"(src) : "memory");
 }
 
 // A zero point that is a small integer can be folded into the unpacking's bias.  In bfloat16 that is worth it (gate / up of 64 experts of 1408 x 2048,
