@@ -1,0 +1,52 @@
+"""What the block operators' sums hold: first sums of adapters that are small beside their row's largest."""
+import pytest
+import torch
+
+from helpers import DT, gen
+from oracle import ref
+from tilelang_ascend_amd import ops
+
+gpu = pytest.mark.gpu
+TYPES = ["float16", "bfloat16"]
+
+
+def update(L, rank, parts, K, dtype, out_dtype):
+    return ops.low_rank_update(L, rank, parts, K, in_dtype=dtype, out_dtype=out_dtype)
+
+
+def not_more(got, want, off, what):
+    got = got.cpu()
+    fi = torch.finfo(got.dtype)
+    assert torch.isfinite(got).all(), what
+    worst = ((got.double() - want).abs() - off - (want.abs() + off).clamp_min(fi.tiny) * (fi.eps / 2)).max().item()
+    assert worst <= 0, f"{what}: {worst:.3e} more than allowed"
+
+
+# M, L, rank, parts, K: single rows; tiles of 16 rows without and with a plan, of 64 in runs of 16 and whole
+SIZES = [(3, 2, 16, (64,), 256), (20, 3, 32, (64,), 8224), (20, 3, 128, (64, 32), 512), (300, 3, 16, (48,), 16416), (500, 3, 128, (48,), 256), (900, 3, 64, (64,), 4128), (5300, 2, 32, (32,), 288), (6400, 3, 8, (32,), 64)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("quiet", [12, 20, 28])
+@pytest.mark.parametrize("M,L,rank,parts,K", SIZES)
+def test_first_sums_far_below_their_rows_largest(M, L, rank, parts, K, quiet, dtype):
+    """Every other row of A is 2^-quiet of the others, and half of the outputs have weights of 0 for the loud ones: they are made of the quiet sums alone, and are
+    as exact as any."""
+    T, g, N = DT[dtype], gen(quiet + M), sum(parts)
+    x = torch.randn(M, K, generator=g).to(T)
+    a = torch.randn(L, len(parts) * rank, K, generator=g)
+    a[:, 0::2] *= 2.0 ** (quiet // 2 - 4)
+    a[:, 1::2] *= 2.0 ** (quiet // 2 - 4 - quiet)
+    b = torch.randn(L, N, rank, generator=g)
+    b[:, : N // 2, 0::2] = 0
+    b[:, N // 2:, 0::2] *= 2.0**-6
+    a, b = a.to(T), b.to(T)
+    scaling = torch.rand(L, generator=g) + 0.5
+    ids = torch.randint(0, L, (M,), generator=g, dtype=torch.int32)
+    some = torch.arange(M) if M <= 100 else torch.cat([torch.tensor([0, M - 1]), torch.randint(0, M, (40,), generator=g)])
+    for out in (dtype, "float32"):
+        y = torch.zeros(M, N, dtype=DT[out])
+        got = update(L, rank, parts, K, dtype, out)(*[v.cuda() for v in (x, y, ids, a, b, scaling)])
+        want, off = ref.low_rank_update(x[some], y[some], ids[some], a, b, scaling, parts)
+        not_more(got[some.cuda()], want, off, f"quiet sums {out}")
