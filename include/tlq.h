@@ -401,7 +401,8 @@ int tlq_gated_silu(const void* X, void* Y, void* Q, void* S, int64_t M, int64_t 
  *   out[m, n] = rn_out( Y[m, n] + scaling[l] * sum_j (sum_k X[m, k] * A[l, p * rank + j, k]) * B[l, n, j] ),  l = ids[m], p the part of n
  * fp32 sums, rounded once.  An id outside 0 .. L - 1 is a row without an adapter: out = Y, and nothing of its X is looked at.  Results do not depend on timing, nor
  * a row's on what the other rows of the call hold.  An infinite weight in B makes its output NaN or an infinity.
- * float16, where rows share work: first sums enter the second product with 22 bits down to 2^-29 of the row's largest; smaller ones may be off by 2^-51 of it.
+ * Where rows share work, the first sums enter the second product in pieces of in_dtype: bfloat16 16 bits of each for an output in bfloat16, all 24 for one in
+ * fp32; float16 22 bits down to 2^-29 of the row's largest (smaller ones may be off by 2^-51 of it).
  * X [M, K], A [L, parts * rank, K], B [L, N, rank] in_dtype (TLQ_F16 or TLQ_BF16), Y and out [M, N] out_dtype (in_dtype or TLQ_F32), ids
  * int32 [M], scaling fp32 [L].  out may be Y.  rank 8, 16, 32, 64 or 128 (adapters of a lower rank: rows and columns of 0), K % 32 == 0,
  * n0, n1, n2 % 16 == 0, L <= 4096, M < 2^24; X, Y, A, B and out 16-byte aligned.

@@ -1,4 +1,4 @@
-"""What the block operators' sums hold: first sums of adapters that are small beside their row's largest."""
+"""What the block operators' sums hold: first sums of adapters that are small beside their row's largest, and their last bits."""
 import pytest
 import torch
 
@@ -50,3 +50,33 @@ def test_first_sums_far_below_their_rows_largest(M, L, rank, parts, K, quiet, dt
         got = update(L, rank, parts, K, dtype, out)(*[v.cuda() for v in (x, y, ids, a, b, scaling)])
         want, off = ref.low_rank_update(x[some], y[some], ids[some], a, b, scaling, parts)
         not_more(got[some.cuda()], want, off, f"quiet sums {out}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,L,rank,parts,K", SIZES)
+def test_first_sums_enter_the_second_product_whole(M, L, rank, parts, K, dtype):
+    """Whole numbers whose first sums fp32 holds exactly, in any order (below 2^24), and one power of two a row of B: fp32 sums rounded once are those sums, bit for
+    bit; of float16 22 bits are handed on, each piece rounded to 11 (2^-11 of what it is made of)."""
+    T, g, N = DT[dtype], gen(M), sum(parts)
+    top = min(2047 if T == torch.float16 else 255, int((2**24 / K) ** 0.5))
+    x = torch.randint(0, top + 1, (M, K), generator=g).to(T)
+    a = torch.randint(-top, top + 1, (L, len(parts) * rank, K), generator=g).to(T)
+    a[:, ::2] = a[:, ::2].abs()
+    chosen = torch.randint(0, rank, (L, N), generator=g)
+    b = torch.zeros(L, N, rank).scatter_(2, chosen[:, :, None], torch.randint(-8, 5, (L, N, 1), generator=g).float().exp2()).to(T)
+    scaling = torch.randint(-3, 4, (L,), generator=g).float().exp2()
+    ids = torch.randint(0, L, (M,), generator=g, dtype=torch.int32)
+    y = torch.zeros(M, N)
+    got = update(L, rank, parts, K, dtype, "float32")(*[v.cuda() for v in (x, y, ids, a, b, scaling)]).cpu()
+    want = torch.zeros(M, N, dtype=torch.float64)
+    for e in range(L):
+        rows, begin = ids == e, 0
+        h = x[rows].double() @ a[e].double().T
+        assert h.abs().max() < 2**24
+        for p, n in enumerate(parts):
+            want[rows, begin: begin + n] = scaling[e].double() * (h[:, p * rank: (p + 1) * rank] @ b[e, begin: begin + n].double().T)
+            begin += n
+    assert (want.abs() > 2**16).any()
+    off = want.abs() * (2.0**-22 + 2.0**-24) if T == torch.float16 else 0
+    assert ((got.double() - want).abs() <= off).all(), f"{((got.double() - want).abs() / want.abs().clamp_min(2.0**-30)).max().item():.3e}"

@@ -316,26 +316,33 @@ struct UpArgs {
   int groups, groups0, groups1;  // work-groups of a tile: all, those ahead of the second part of the outputs and of the third
 };
 
-// Two pieces of the operands' type for a value of h: bfloat16 holds 16 of its bits that way; float16 22, of h times a power of two that brings the row's
-// largest to 2^14 or above, below 2^15 (h itself may lie outside of float16's range).  float16's steps end at 2^-24, so its second piece is what the first leaves over times
-// kPieceStep (2^15 at most again), with a sum of products of its own that is divided by that: values down to 2^-29 of the row's largest have 22 bits, smaller
-// ones are off by 2^-51 of the largest.  (Without the step, 8192 rows of rank 32 on 14336 outputs take 145 us, with it 141; 500 rows of 40 adapters on 4096 outputs 16.5 / 16.7.)
-// One piece would round h to the operands' type: as much error as the output's own rounding.  (Beside an infinity the second piece is 0.)
+// Pieces of the operands' type for a value of h: one would round h to it, as much error as the output's own rounding.  Two of bfloat16 hold 16 of its 24 bits, 2^-8 of a
+// step of the 16-bit output; three all of them, for an output in fp32 (8192 rows of rank 32 on 14336 outputs: 271 us either way; with a 16-bit output 139 / 146, of
+// rank 64 150 / 170).  Two of float16 hold 22, of h times a power of two that brings the row's largest to 2^14 or above, below 2^15 (h itself may lie outside of float16's
+// range).  float16's steps end at 2^-24, so its second piece is what the first leaves over times kPieceStep (2^15 at most again), with a sum of products of its own that
+// is divided by that: values down to 2^-29 of the row's largest have 22 bits, smaller ones are off by 2^-51 of the largest.  (Without the step, the same rows take
+// 145 us, with it 141; 500 rows of 40 adapters on 4096 outputs 16.5 / 16.7.)  (Beside an infinity the further pieces are 0.)
+template <typename T, typename TO>
+constexpr int kPieces = std::is_same<T, half_t>::value || sizeof(TO) == 2 ? 2 : 3;
 constexpr float kPieceStep = 4096.0f;
 __device__ __forceinline__ float rest(float h, float piece) { return fabsf(piece) < __builtin_inff() ? h - piece : 0.0f; }
-template <typename T>
-__device__ __forceinline__ void two_pieces(const float (&h)[8], uint4_t& high, uint4_t& low) {
+template <typename T, int PIECES>
+__device__ __forceinline__ void pieces_of(float (&h)[8], uint4_t (&piece)[PIECES]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same<T, half_t>::value) {
-      const half2_t p = {(half_t)h[2 * i], (half_t)h[2 * i + 1]};
-      high[i] = bitcast<uint32_t>(p);
-      low[i] = bitcast<uint32_t>(half2_t{(half_t)(rest(h[2 * i], (float)p[0]) * kPieceStep), (half_t)(rest(h[2 * i + 1], (float)p[1]) * kPieceStep)});
-    } else {
-      high[i] = pack_bf16x2(h[2 * i], h[2 * i + 1]);
-      low[i] = pack_bf16x2(rest(h[2 * i], bitcast<float>(high[i] << 16)), rest(h[2 * i + 1], bitcast<float>(high[i] & 0xffff0000u)));
+  for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float first, second;
+      if constexpr (std::is_same<T, half_t>::value) {
+        const half2_t p = {(half_t)h[2 * i], (half_t)h[2 * i + 1]};
+        piece[n][i] = bitcast<uint32_t>(p), first = (float)p[0], second = (float)p[1];
+      } else {
+        piece[n][i] = pack_bf16x2(h[2 * i], h[2 * i + 1]);
+        first = bitcast<float>(piece[n][i] << 16), second = bitcast<float>(piece[n][i] & 0xffff0000u);
+      }
+      h[2 * i] = rest(h[2 * i], first), h[2 * i + 1] = rest(h[2 * i + 1], second);
+      if constexpr (std::is_same<T, half_t>::value) h[2 * i] *= kPieceStep, h[2 * i + 1] *= kPieceStep;
     }
-  }
 }
 
 // Blocks of 128 outputs of one part of the outputs x 16 RW rows: RW wavefronts have 16 rows each and share a block's rows of B, 4 / RW (2: see kUpWaves)
@@ -365,7 +372,8 @@ __global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(
   const auto turn = [](int l) __attribute__((always_inline)) { return C == 1 ? 0 : C == 2 ? (l >> 2) & 1 : C == 4 ? (l >> 1) & 3 : l & 7; };
   const T* const b0 = (const T*)a.B + ((int64_t)tile.adapter * a.N + begin) * RANK;
   const uint32_t lds = lds_of(tiles[cw]);
-  uint4_t high[RB], low[RB];
+  constexpr int PIECES = kPieces<T, TO>;
+  uint4_t pieces[RB][PIECES];
   float back[4];  // the scaling, times what the pieces' power of two takes back, of rows 4 q + i
   for (int i = 0; i < a.per_group; i += CW) {
     const int n0 = (group * a.per_group + i + cw) * 128;
@@ -443,7 +451,7 @@ __global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(
             for (int k = 0; k < 8; ++k) h[c][k] *= down;
         }
 #pragma unroll
-        for (int c = 0; c < RB; ++c) two_pieces<T>(h[c], high[c], low[c]);
+        for (int c = 0; c < RB; ++c) pieces_of<T>(h[c], pieces[c]);
 #pragma unroll
         for (int m = 0; m < 4; ++m) back[m] = __shfl(scale, q * 4 + m);
       }
@@ -458,9 +466,12 @@ __global__ __launch_bounds__((64 * kUpWaves<RW, RANK>)) void low_rank_up_kernel(
         for (int c = 0; c < RB; ++c) {
           // (a rank below 32: the lanes behind it have zeros for h, and a chunk of the same row of B)
           const uint4_t b = tiles[cw][(j * 16 + r16) * C + ((C >= 4 ? c * 4 + q : q & (C - 1)) ^ turn(r16))];
-          if constexpr (std::is_same<T, half_t>::value) less = Mma::mma(low[c], b, less);
-          else acc[j] = Mma::mma(low[c], b, acc[j]);
-          acc[j] = Mma::mma(high[c], b, acc[j]);
+#pragma unroll
+          for (int of = PIECES - 1; of > 0; --of) {
+            if constexpr (std::is_same<T, half_t>::value) less = Mma::mma(pieces[c][of], b, less);
+            else acc[j] = Mma::mma(pieces[c][of], b, acc[j]);
+          }
+          acc[j] = Mma::mma(pieces[c][0], b, acc[j]);
         }
         if constexpr (std::is_same<T, half_t>::value)
 #pragma unroll

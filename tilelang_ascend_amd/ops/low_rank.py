@@ -31,7 +31,9 @@ def low_rank_update(L: int, rank: int, N: Union[int, Sequence[int]], K: int, in_
     out[m, n] = Y[m, n] + scaling[l] * sum_j (X[m] . A[l, p * rank + j]) * B[l, n, j] with l = ids[m], fp32 sums, rounded once; a row whose
     id lies outside 0 .. L - 1 is Y.  N: the projection's outputs, or those of up to three projections side by side (queries, keys and values;
     gate and up), which are the parts p, each with `rank` rows of A.  rank: 8, 16, 32, 64 or 128; an adapter of a lower rank has zeros in the
-    rows and columns that it lacks.  X, A and B are in_dtype, Y and out out_dtype: in_dtype (the default) or float32."""
+    rows and columns that it lacks.  X, A and B are in_dtype, Y and out out_dtype: in_dtype (the default) or float32.
+
+    Where rows share work, the first sums enter the second product with 16 bits (bfloat16; 24 with a float32 output) or 22 (float16)."""
     parts = tuple(operator.index(n) for n in (N if isinstance(N, (tuple, list)) else (N,)))
     if not 1 <= len(parts) <= 3:
         raise ValueError(f"N must be one to three sizes (got {N})")
