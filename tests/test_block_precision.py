@@ -1,4 +1,4 @@
-"""What the block operators' sums hold: first sums of adapters that are small beside their row's largest, and their last bits."""
+"""What the block operators' sums hold: first sums of adapters that are small beside their row's largest, and their last bits; squares of very long rows."""
 import pytest
 import torch
 
@@ -80,3 +80,20 @@ def test_first_sums_enter_the_second_product_whole(M, L, rank, parts, K, dtype):
     assert (want.abs() > 2**16).any()
     off = want.abs() * (2.0**-22 + 2.0**-24) if T == torch.float16 else 0
     assert ((got.double() - want).abs() <= off).all(), f"{((got.double() - want).abs() / want.abs().clamp_min(2.0**-30)).max().item():.3e}"
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [32769 + 7, (1 << 22) + 5, 1 << 24])
+@pytest.mark.parametrize("value", [1.1, 0.7])
+def test_norm_of_very_long_rows(N, value, dtype):
+    """Equal values, whose squares all round a growing sum the same way: sums of at most 64 in fp32, those in more, a tree of 256."""
+    x = torch.full((2, N), value).to(DT[dtype])
+    x[1, ::3] *= -0.5
+    w = torch.ones(N, dtype=DT[dtype])
+    y, q, s = ops.residual_rms_norm(N, outputs="both", with_residual=False, in_dtype=dtype)(x.cuda(), w.cuda())
+    _, want, _ = ref.residual_rms_norm(x, None, w, 1e-6)
+    rel = ((64 + 16) / 2 + 8) * 2.0**-24
+    not_more(y, want, want.abs() * rel, "y")
+    assert ((s.cpu().double() - ref.row_scales(want)).abs() <= ref.row_scales(want) * (rel + 2.0**-22)).all(), (s, ref.row_scales(want))
+    assert (q[0] == 127).all() and (q[1, ::3].abs() == 64).all()  # (127 / 2: the even one)

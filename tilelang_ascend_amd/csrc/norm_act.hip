@@ -238,7 +238,9 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(const NormArgs a) {
 }
 
 // Longer rows: a work-group a row, one value per lane and step, the row read twice (with a residual the sum is read back from H by the lane that wrote
-// it: H may be the residual itself).
+// it: H may be the residual itself).  A lane has up to 2^22 squares: sums of kRun of them in fp32, those in binary64 (one sum in fp32 was 0.3 % off for equal values
+// in rows of 2^26, and 3 % in the longest).
+constexpr int kRun = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void norm_long_kernel(const NormArgs a) {
   __shared__ float part[2][2][4];
@@ -247,17 +249,23 @@ __global__ __launch_bounds__(256) void norm_long_kernel(const NormArgs a) {
   for (int64_t m = blockIdx.x; m < a.M; m += a.blocks, it ^= 1) {
     const T *x = (const T*)a.X + m * N, *r = (const T*)a.R + m * N, *w = (const T*)a.W;
     T* const h = (T*)a.H + m * N;
-    float ss = 0.0f, amax = 0.0f;
-    for (int n = tid; n < N; n += 256) {
-      float z = to_float(x[n]);
-      if (a.R) {
-        const T sum = from_float<T>(z + to_float(r[n]));
-        h[n] = sum, z = to_float(sum);
+    float amax = 0.0f;
+    double all = 0.0;
+    for (int n0 = tid; n0 < N; n0 += kRun * 256) {
+      float run = 0.0f;
+      for (int n = n0; n < N && n < n0 + kRun * 256; n += 256) {
+        float z = to_float(x[n]);
+        if (a.R) {
+          const T sum = from_float<T>(z + to_float(r[n]));
+          h[n] = sum, z = to_float(sum);
+        }
+        run += z * z;
+        amax = fmaxf(amax, fabsf(z * to_float(w[n])));
       }
-      ss += z * z;
-      amax = fmaxf(amax, fabsf(z * to_float(w[n])));
+      all += (double)run;
     }
-    ss = wave_sum(ss), amax = wave_max(amax);
+    float ss = wave_sum((float)all);
+    amax = wave_max(amax);
     if ((tid & 63) == 0) part[it][0][tid >> 6] = ss, part[it][1][tid >> 6] = amax;
     __syncthreads();  // (part[] alternates: one barrier a row)
     ss = (part[it][0][0] + part[it][0][1]) + (part[it][0][2] + part[it][0][3]);
