@@ -386,7 +386,7 @@ int tlq_act_quant_i8(const void* X, void* Y, void* S, int64_t M, int64_t N, int 
  * NaN in h makes a row NaN in Y, -127 in Q with the floor's scale; an infinity is NaN there and the row's other values 0.  Sums of squares beyond fp32's range (bfloat16
  * values from 1e19 on) make a row of 0.
  * X, residual, H, Y [M, N] and weight [N] dtype (TLQ_F16 or TLQ_BF16), Q int8 [M, N], S fp32 [M]; any M below 2^31 and N below 2^30 (fastest with rows of a
- * multiple of 8 values, 16-byte aligned, Q 8-byte; beyond 32768 values a row is read twice); 1e-12 <= eps <= 1.  H may be the residual or X, and Y may be X.  Y and Q are operands of
+ * multiple of 8 values, 16-byte aligned, Q 8-byte; beyond 32768 values a row is read twice); 1e-12 <= eps <= 1.  H may be the residual or X, and Y may be X (one of them).  Y and Q are operands of
  * tlq_gemm_w4a16, tlq_low_rank_update and tlq_gemm_w8a8. */
 int tlq_residual_rms_norm(const void* X, const void* residual, const void* weight, void* H, void* Y, void* Q, void* S, int64_t M,
                           int64_t N, float eps, int dtype, int round_scale, void* stream);

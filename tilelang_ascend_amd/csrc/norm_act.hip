@@ -512,6 +512,7 @@ extern "C" int tlq_residual_rms_norm(const void* X, const void* residual, const 
   TLQ_REQUIRE(!residual == !H, "%s: a residual and H are wanted together", what);
   TLQ_REQUIRE((((uintptr_t)X | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)H) & 1) == 0, "%s: misaligned pointer", what);
   if (check_outputs(what, Y, Q, S)) return 1;
+  TLQ_REQUIRE(!H || H != Y, "%s: H and Y are two outputs (X's place is for one of them)", what);
   const NormArgs a{X, residual, weight, H, Y, (int8_t*)Q, (float*)S, M, (int)N, round_scale != 0, 0, eps};
   return dtype == TLQ_F16 ? run_norm<half_t>(a, (hipStream_t)stream) : run_norm<bf16_t>(a, (hipStream_t)stream);
 }
