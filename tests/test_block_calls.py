@@ -1,12 +1,13 @@
-"""Calls of the block operators that their documentation allows or refuses, beside those of test_block_ops.py: more rows than the machine takes at
-once, and refusals.  Tolerances as there (gated: gates up to 8 here)."""
+"""Calls of the block operators that their documentation allows or refuses, beside those of test_block_ops.py: more rows than the machine takes at once, more
+blocks of outputs than a work-group takes at once, and refusals.  Tolerances as there (gated: gates up to 8 here)."""
 import ctypes
 
 import pytest
 import torch
 
-from helpers import DT, assert_bit_equal
+from helpers import DT, assert_bit_equal, gen
 from oracle import ref
+from test_block_launches import ask, recorder  # noqa: F401
 from tilelang_ascend_amd import _abi, ops
 
 gpu = pytest.mark.gpu
@@ -80,3 +81,55 @@ def test_gated_of_more_rows_than_work_groups(N, rows, dtype):
     assert ((whole[0][some].cpu().double() - yw).abs() <= yw.abs() * (12 * 2.0**-22 + torch.finfo(DT[dtype]).eps / 2) + 2.0**-25).all()
     assert ((whole[2][some].cpu().double() - scale).abs() <= scale * (12 + 1) * 2.0**-22).all()
     assert ((whole[1][some].cpu().double() - yw / scale[:, None]).abs() <= 0.5 + 127 * (2 * 12 + 4) * 2.0**-22).all()
+
+
+# ---- more blocks of outputs than a work-group of the second product takes at once -------------------------------------------------------
+# M, L, rank, N, K: tiles of 64 rows, then of 16; no size of these goes to single rows, nor does a part of its outputs
+BLOCKS = [(6400, 3, 8, 4112, 64), (4200, 3, 16, 4368, 64), (1700, 2, 32, 9232, 8224), (900, 3, 64, 15376, 2080), (500, 3, 128, 25616, 96),
+          (6000, 200, 8, 2064, 64), (5000, 200, 16, 2576, 64), (600, 300, 32, 3600, 8224), (300, 40, 64, 9232, 2080), (300, 100, 128, 4624, 96)]
+
+
+def test_blocks_reach_the_second_pass(recorder):  # noqa: F811
+    result = ask(recorder, f"""
+result = []
+for M, L, rank, N, K in {BLOCKS}:
+    size = lib.tlq_low_rank_update_workspace_bytes(M, L, rank, 1, K)
+    per = []
+    for n in (N, 1024):
+        got = launches(lambda: lib.tlq_low_rank_update(X, Y, IDS, A, B, S, H, WS, size, M, L, rank, n, 0, 0, K, 1, 1, None))
+        assert "up_kernel" in got[-1][0], (M, n)
+        per.append((struct.unpack("i", got[-1][3][84:88])[0], got[-1][2] // 64 // (4 if "Li4ELi" in got[-1][0] else 1)))
+    result.append(per)
+""")
+    for case, ((per, at_a_time), (per_part, _)) in zip(BLOCKS, result):
+        assert per > at_a_time >= 1 and (per_part <= at_a_time or per_part < per), (case, per, at_a_time, per_part)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,L,rank,N,K", BLOCKS)
+def test_update_of_several_blocks_a_work_group(M, L, rank, N, K, dtype):
+    """What calls on 1024 of the outputs give, bit for bit, with 16-bit outputs and fp32 ones, and in place."""
+    T, g = DT[dtype], torch.Generator(device="cuda").manual_seed(M + N)
+    x = torch.randn(M, K, generator=g, device="cuda").to(T)
+    a = (torch.randn(L, rank, K, generator=g, device="cuda") * K**-0.5).to(T)
+    b = (torch.randn(L, N, rank, generator=g, device="cuda") * 0.3).to(T)
+    scaling = torch.rand(L, generator=g, device="cuda") + 0.5
+    ids = torch.randint(-1, L, (M,), generator=g, device="cuda", dtype=torch.int32)
+    some = torch.randint(0, M, (12,), generator=gen(M))
+    for out in (dtype, "float32"):
+        y = torch.randn(M, N, generator=g, device="cuda").to(DT[out])
+        whole = ops.low_rank_update(L, rank, N, K, in_dtype=dtype, out_dtype=out)(x, y, ids, a, b, scaling)
+        for n in range(0, N, 1024):
+            part = slice(n, min(n + 1024, N))
+            got = ops.low_rank_update(L, rank, part.stop - n, K, in_dtype=dtype, out_dtype=out)(x, y[:, part].contiguous(), ids, a, b[:, part].contiguous(), scaling)
+            assert torch.equal(got, whole[:, part]), (out, n)
+        want, off = ref.low_rank_update(x[some.cuda()], y[some.cuda()], ids[some.cuda()], a, b, scaling, (N,))
+        assert ((whole[some.cuda()].cpu().double() - want).abs() <= off + (want.abs() + off) * (torch.finfo(DT[out]).eps / 2) + torch.finfo(DT[out]).tiny).all()
+        P, lib = _abi.ptr, _abi.load()
+        bytes_ = lib.tlq_low_rank_update_workspace_bytes(M, L, rank, 1, K)
+        ws = torch.empty(bytes_, dtype=torch.uint8, device="cuda")
+        code = _abi.F16 if dtype == "float16" else _abi.BF16
+        _abi.check(lib.tlq_low_rank_update(P(x), P(y), P(ids), P(a), P(b), P(scaling), P(y), P(ws), bytes_, M, L, rank, N, 0, 0, K, code, _abi.F32 if out == "float32" else code,
+                                           torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(y, whole), "in place"
