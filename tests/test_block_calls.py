@@ -1,5 +1,5 @@
 """Calls of the block operators that their documentation allows or refuses, beside those of test_block_ops.py: more rows than the machine takes at once, more
-blocks of outputs than a work-group takes at once, and refusals.  Tolerances as there (gated: gates up to 8 here)."""
+blocks of outputs than a work-group takes at once, both types through every launch, and refusals.  Tolerances as there (gated: gates up to 8 here)."""
 import ctypes
 
 import pytest
@@ -133,3 +133,30 @@ def test_update_of_several_blocks_a_work_group(M, L, rank, N, K, dtype):
         _abi.check(lib.tlq_low_rank_update(P(x), P(y), P(ids), P(a), P(b), P(scaling), P(y), P(ws), bytes_, M, L, rank, N, 0, 0, K, code, _abi.F32 if out == "float32" else code,
                                            torch.cuda.current_stream().cuda_stream))
         assert torch.equal(y, whole), "in place"
+
+
+# ---- both types through every launch ------------------------------------------------------------------------------------------------
+def test_update_launches_the_kernels_of_its_types(recorder):  # noqa: F811
+    result = ask(recorder, """
+rng, result = random.Random(7), set()
+log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))
+for _ in range(2000):
+    M, L, rank, parts, K = log(1, rng.choice([64, 2000, 1 << 24])), log(1, 4096), rng.choice([8, 16, 32, 64, 128]), tuple(16 * log(1, 4096) for _ in range(rng.randint(1, 3))), 32 * log(1, 2048)
+    t = rng.choice([0, 1])
+    out = rng.choice([t, 2])
+    size = lib.tlq_low_rank_update_workspace_bytes(M, L, rank, len(parts), K)
+    of_in, of_out = ("DF16_", "DF16b")[t], ("DF16_", "DF16b", "f")[out]
+    for name, g, threads, data in launches(lambda: lib.tlq_low_rank_update(X, Y, IDS, A, B, S, H, WS, size, M, L, rank, *parts, *[0] * (3 - len(parts)), K, t, out, None)):
+        kind = [k for k in ("row", "up", "down_tile", "down", "plan") if "low_rank_" + k + "_kernel" in name][0]
+        if kind in ("row", "up"):
+            assert "_kernelI" + of_in + of_out + "Li" in name, (t, out, name)
+        elif kind != "plan":
+            assert "_kernelI" + of_in in name and "_kernelI" + of_in + "D" not in name, (t, out, name)
+        if kind in ("row", "up"):
+            assert name.split("Li")[-1].startswith(str(rank) + "E"), (rank, name)
+        result.add((kind, t, out if kind in ("row", "up") else -1))
+result = sorted(result)
+""")
+    pairs = [(0, 0), (0, 2), (1, 1), (1, 2)]
+    want = {("plan", t, -1) for t in (0, 1)} | {(k, t, -1) for k in ("down", "down_tile") for t in (0, 1)} | {(k, *p) for k in ("row", "up") for p in pairs}
+    assert {tuple(r) for r in result} == want
