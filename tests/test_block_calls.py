@@ -2,6 +2,7 @@
 blocks of outputs than a work-group takes at once, both types through every launch, and refusals.  Tolerances as there (gated: gates up to 8 here)."""
 import ctypes
 
+import numpy
 import pytest
 import torch
 
@@ -20,6 +21,16 @@ def test_norm_refuses_one_place_for_two_outputs():
     args = dict(X=HERE, residual=THERE, weight=THERE, H=HERE, Y=HERE, Q=None, S=None, M=4, N=64, eps=1e-6, dtype=_abi.F16, round_scale=0, stream=None)
     assert _abi.load().tlq_residual_rms_norm(*args.values()) != 0
     assert "two outputs" in _abi.last_error()
+
+
+@pytest.mark.parametrize("make", [lambda n: ops.residual_rms_norm(n), lambda n: ops.gated_silu(n), lambda n: ops.low_rank_update(n, 16, 64, 64), lambda n: ops.low_rank_update(4, n, 64, 64),
+                                  lambda n: ops.low_rank_update(4, 16, n, 64), lambda n: ops.low_rank_update(4, 16, 64, n)])
+def test_factories_refuse_sizes_that_are_no_whole_numbers(make):
+    """A kernel for 64 is not what a call for 64.5 asked for."""
+    for n in (64.5, 64.0, "64", None):
+        with pytest.raises(TypeError):
+            make(n)
+    assert make(numpy.int64(64)).params[0].name == "X"
 
 
 # ---- rows beyond the machine's work-groups ------------------------------------------------------------------------------------------

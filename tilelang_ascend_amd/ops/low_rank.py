@@ -34,6 +34,7 @@ def low_rank_update(L: int, rank: int, N: Union[int, Sequence[int]], K: int, in_
     rows and columns that it lacks.  X, A and B are in_dtype, Y and out out_dtype: in_dtype (the default) or float32.
 
     Where rows share work, the first sums enter the second product with 16 bits (bfloat16; 24 with a float32 output) or 22 (float16)."""
+    L, rank, K = operator.index(L), operator.index(rank), operator.index(K)
     parts = tuple(operator.index(n) for n in (N if isinstance(N, (tuple, list)) else (N,)))
     if not 1 <= len(parts) <= 3:
         raise ValueError(f"N must be one to three sizes (got {N})")

@@ -10,6 +10,8 @@ beside an int8 product take Y).  Q is made of the fp32 values, not of Y.  Any nu
 """
 from __future__ import annotations
 
+import operator
+
 from ..jit import ABI_DTYPE, TORCH_DTYPES, KernelSpec, NativeCall, Param, PassConfigKey, jit
 
 _PASS_CONFIGS = {PassConfigKey.TL_ASCEND_AUTO_SYNC: True, PassConfigKey.TL_ASCEND_MEMORY_PLANNING: True}
@@ -64,11 +66,11 @@ def residual_rms_norm(N: int, eps: float = 1e-6, outputs: str = "float", with_re
     H = X + residual in their type (without a residual: X, and no H);  y = H * weight / sqrt(mean(H^2) + eps) in fp32;  Y = y rounded once;
     S = max(max|y|, 1e-4) / 127 (round_scale: the next power of two), Q = int8(rint(clamp(y / S, -127, 127))).  Without round_scale, and where S
     is not the floor, Q is decided exactly: it does not depend on how the sum of squares was formed."""
-    return _norm[_OUTPUTS.get(outputs, 1) + bool(with_residual)](N, eps, outputs, bool(with_residual), bool(round_scale), in_dtype)
+    return _norm[_OUTPUTS.get(outputs, 1) + bool(with_residual)](operator.index(N), eps, outputs, bool(with_residual), bool(round_scale), in_dtype)
 
 
 def gated_silu(N: int, outputs: str = "float", round_scale: bool = False, in_dtype: str = "bfloat16"):
     """kernel(X [M, 2N]) -> [[Y,] [Q int8 [M, N], S float32 [M]]] (the tensor itself where it is one).
 
     y = silu(X[:, :N]) * X[:, N:] in fp32, the gates first; Y, Q and S of it as residual_rms_norm makes them."""
-    return _gated[_OUTPUTS.get(outputs, 1)](N, outputs, bool(round_scale), in_dtype)
+    return _gated[_OUTPUTS.get(outputs, 1)](operator.index(N), outputs, bool(round_scale), in_dtype)
