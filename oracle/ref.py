@@ -686,13 +686,13 @@ def low_rank_update(X, Y, ids, A, B, scaling, parts):
     """-> (out, what it may be off by before its rounding) float64 [M, N], one row at a time.
 
     fp32 sums of K and then rank products: (K + 16) 2^-24 of the first sums' magnitudes, and of the second's (rank + 16) 2^-24; the first
-    sums may be handed on in two pieces of the activations' type, the second's products round to fp32: 2^-15 (bfloat16: 16 bits) or 2^-20 (float16) of
-    the second sums' magnitudes; the scaling's product and the addition: 2^-23 of either side."""
+    sums may be handed on in two pieces of the activations' type, each rounded to it: 2^-16 (bfloat16; in three, all of an fp32 sum, for an output in fp32) or
+    2^-22 (float16) of the second sums' magnitudes; the scaling's product and the addition: 2^-23 of either side."""
     X, Y, ids, A, B, scaling = (t.cpu() for t in (X, Y, ids, A, B, scaling))
     M, K = X.shape
     L, rows, _ = A.shape
     r = rows // len(parts)
-    pieces = 2.0**-15 if X.dtype == torch.bfloat16 else 2.0**-20
+    pieces = 2.0**-22 if X.dtype == torch.float16 else 0.0 if Y.dtype == torch.float32 else 2.0**-16
     out = Y.to(torch.float64).clone()
     off = torch.zeros_like(out)
     for m in range(M):
