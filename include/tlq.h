@@ -392,7 +392,8 @@ int tlq_residual_rms_norm(const void* X, const void* residual, const void* weigh
                           int64_t N, float eps, int dtype, int round_scale, void* stream);
 
 /* Between the products of an MLP: y = silu(g) * u, g = X[m, n], u = X[m, N + n], silu(g) = g / (1 + exp(-g)), fp32; Y, Q and S of it as above.
- * A NaN has code -127 and no part in S; an infinity makes S infinite, its own code -127 and the others 0.
+ * A NaN has code -127 and no part in S; an infinity makes S infinite, its own code -127 and the others 0.  Gates below -174 count as 0 (fp32 holds exp(g / 2) no more; the
+ * exact value is below its normal numbers for all |u| < 2^118).
  * X [M, 2 N], Y [M, N] dtype (not in X's place), Q int8 [M, N], S fp32 [M]; M, N and alignment as above. */
 int tlq_gated_silu(const void* X, void* Y, void* Q, void* S, int64_t M, int64_t N, int dtype, int round_scale, void* stream);
 

@@ -677,6 +677,8 @@ static_assert(16 * kFewGroups <= 64 * kTileGroups, "sum_rows holds for both");
 // on 9600 9.3 / 9.4, 27, K = 2976, on 16640 9.6 / 13.4.  Rank 64: 1 row, K = 2080, 7.4 / 6.0, 4, K = 1184, on 16832 7.8 / 7.8, K = 3392 8.5 / 10.1, 8, K = 3424,
 // on 784 8.2 / 7.5.  Rank 128: 4, K = 512, on 2224 8.4 / 7.3, 2, K = 1312, on 2528 8.6 / 9.2: left to tiles.  Rank 8: K = 8000, 336 on 21104 28.9 / 27.4, K = 7360,
 // 753 on 15248 24.8 / 21.7, K = 1568, 1977 on 13536 44.7 / 65.3; 256 -> 256, 5000 15.6 / 15.6, 64 -> 256, 10000 21.0 / 22.3.
+// A bound on sizes alone, and not the best one: of these it takes the slower way, by 9 to 23 %, for the 47 rows of one adapter (tiles share its B; how many adapters the
+// rows have is not among its arguments), for 1 and 8 rows of rank 64 with K = 2080 and 3424, for the 753 of rank 8 and, for want of that kernel, for the 4 of rank 128.
 inline bool single_rows(int64_t M, int64_t rank, int64_t K, int64_t N) {
   return M <= 4096 && rank <= 64 && rank * K <= (int64_t)1 << 18 && rank * rank * K <= (int64_t)1 << 23 &&
          M * rank * rank * (K + N) <= (int64_t)(M <= kInlineRows ? 3 : 6) << 27;

@@ -239,7 +239,8 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(const NormArgs a) {
 
 // Longer rows: a work-group a row, one value per lane and step, the row read twice (with a residual the sum is read back from H by the lane that wrote
 // it: H may be the residual itself).  A lane has up to 2^22 squares: sums of kRun of them in fp32, those in binary64 (one sum in fp32 was 0.3 % off for equal values
-// in rows of 2^26, and 3 % in the longest).
+// in rows of 2^26, and 3 % in the longest).  Bounded by the latency of two-byte loads and by the second reading: rows of 53248 bf16 with a residual, us, 16 bits / codes:
+// 1 97 / 109, 64 142 / 148, 2000 486 / 470 (852 and 745 MB: 1.8 and 1.6 TB/s).
 constexpr int kRun = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void norm_long_kernel(const NormArgs a) {
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(THREADS) void gated_rows_kernel(const GatedArgs a) 
   }
 }
 
-// Longer rows with codes: a work-group a row, one value per lane and step; codes are made of a second look at the row.
+// Longer rows with codes: a work-group a row, one value per lane and step; codes are made of a second look at the row.  (Rows of 53248 bf16: 1 78 us, 64 118, 2000 296 for 533 MB.)
 template <typename T>
 __global__ __launch_bounds__(256) void gated_long_kernel(const GatedArgs a) {
   __shared__ float part[2][4];
@@ -473,6 +474,9 @@ int run_gated(GatedArgs a, hipStream_t st) {
     if (any) gated_rows_kernel<T, CH, WPR, THREADS, true><<<a.blocks, THREADS, 0, st>>>(a);  \
     else gated_rows_kernel<T, CH, WPR, THREADS, false><<<a.blocks, THREADS, 0, st>>>(a);     \
   } while (0)
+  // the norm's table: codes alone, bf16, us, fewer wavefronts a row (four to 8192 values) / this / more (eight to 4096, sixteen to 16384): 67 x 14336 4.3 / 4.3 / 4.4, 2048 x 14336
+  // 25.7 / 25.8 / 27.5, 512 x 11008 7.1 / 7.2 / 7.4, 512 x 8192 5.6 / 5.4 / 5.5, 4096 x 8192 28.0 / 27.7 / 31.2, 1024 x 4096 5.4 / 5.6 / 5.6, 4096 x 2048 9.1 / 9.1 / 12.9, 4096 x 1024
+  // 7.5 / 5.3 / 11.5; four are faster where many rows have up to 4096 values (8192 x 4096 27.3 / 30.2 / 30.5)
   if (a.N <= 512) TLQ_GATED(1, 1, 256);
   else if (a.N <= 1024) TLQ_GATED(2, 1, 256);
   else if (a.N <= 2048) TLQ_GATED(1, 4, 256);
